@@ -71,24 +71,24 @@ def draw(rng):
     case = dict(op=op, heads=rng.randrange(1, 17), d=d, k_bits=bits[0], v_bits=bits[1],
                 page=rng.choice((16, 32, 64, 128)))
     if op == "attend":
-        # Up to about the largest listed case's codes.
+        # Up to about the largest listed cases' codes and products.
         group = rng.choice((1, 2, 4, 5, 7, 8, 12, 16))
         case["heads"] = max(1, min(case["heads"], 64 // group))
         row = d * (bits[0] + bits[1]) / 8 + 8
-        most = 220e6 / (row * case["heads"])
+        most = min(200e6 / (row * case["heads"]), 2.5e9 / (case["heads"] * group * d))
         batch = _log(rng, 1, min(64, most / 32))
         longest = _log(rng, 1, min(200000, most / batch))
         case.update(batch=batch, group=group, dtype=rng.choice(("bf16", "bf16", "fp16", "f32")), longest=max(1, longest),
                     ragged=batch > 2 and rng.random() < 0.7, accumulate=rng.random() < 0.3, lse=rng.random() < 0.3)
     elif op == "append":
-        most = 24576 * 8 * 128 * 0.7 / (case["heads"] * max(d, 64) * (2 if d > 128 else 1))
-        case.update(tokens=_log(rng, 1, most), dtype=rng.choice(("bf16", "bf16", "fp16", "f32")),
-                    padded=rng.random() < 0.4)
+        dtype = rng.choice(("bf16", "bf16", "fp16", "f32"))
+        most = 24576 * 8 * 128 * (0.45 if dtype == "f32" else 0.7) / (case["heads"] * max(d, 64) * (2 if d > 128 else 1))
+        case.update(tokens=_log(rng, 1, most), dtype=dtype, padded=rng.random() < 0.4)
     else:
         batch, prompt = _log(rng, 1, 8), rng.random() < 0.5
         rows = batch * case["heads"]
-        longest = _log(rng, 2, min(100000, (2.5e6 if prompt else 1.1e5) / rows))
-        budget = max(1, min(longest, int(longest * rng.uniform(0.02, 0.98)), int(1.1e5 / rows)))
+        longest = _log(rng, 2, min(100000, (2e6 if prompt else 8e4) / rows))
+        budget = max(1, min(longest, int(longest * rng.uniform(0.02, 0.98)), int(8e4 / rows)))
         if not prompt:  # the new tokens cost as an append does
             budget = max(budget, longest - int(2e4 / rows) - 1)
         case.update(batch=batch, longest=longest, budget=budget, recent=rng.randrange(0, budget + 1) // 4,

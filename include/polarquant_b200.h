@@ -335,6 +335,107 @@ int pq_repack(const uint8_t* packed, int64_t ldb, int64_t n, int d, int bits, in
 int pq_pack_codes(const uint8_t* codes, int64_t n, int d, int bits, uint8_t* out, int64_t ldb,
                   void* stream);
 
+/* ---------------------------------------------------------------------------
+ * Compressed key-value cache of a language model's attention (no counterpart
+ * in the reference).  Every token's key and value of every key-value head is
+ * one packed row of Lloyd-Max codes of the rotated unit vector (the rows that
+ * pq_encode writes) and its f32 norm, in pages of page_size tokens:
+ *   rows      [pages][heads][page_size][ldb]  uint8
+ *   norms     [pages][heads][page_size]       f32
+ *   positions [pages][heads][page_size]       int32, the token's place in its
+ *             sequence (slots move when tokens are evicted)
+ *   weights   [pages][heads][page_size]       f32, accumulated attention
+ * A slot is page * page_size + offset.  A sequence is a row of a page table
+ * (int32, table_width entries, row stride table_stride) and a length: its
+ * token i lies in page table[i / page_size] at offset i % page_size, for every
+ * head.  Entries behind the length are not read.  Lengths are taken as at most
+ * table_width * page_size and at least 0; a token on a page outside
+ * [0, pages) is not there (attention passes over it, nothing is written).
+ * Calls that write a page (append, evict, attend with `accumulate`) are
+ * ordered by the caller against others that use it.
+ *
+ * d <= 256; k_bits and v_bits are 2, 4 or 8, on their own; page_size is a
+ * power of two, 16 .. 1024; rows are 16-byte aligned, ldb a multiple of 16 and
+ * at least the packed bytes of a row.  dtype: 0 = f32, 1 = f16, 2 = bf16.
+ * The descriptor and its fields' sizes are host memory, read during the call.
+ * ------------------------------------------------------------------------- */
+#define PQ_KV_F32 0
+#define PQ_KV_F16 1
+#define PQ_KV_BF16 2
+#define PQ_KV_MAX_D 256
+
+typedef struct pq_kv_cache {
+  uint8_t* k_rows;
+  uint8_t* v_rows;
+  float* k_norms;
+  float* v_norms;
+  int32_t* positions;
+  float* weights;
+  const void* k_codec; /* written by pq_kv_prepare_codec */
+  const void* v_codec;
+  int64_t k_ldb;
+  int64_t v_ldb;
+  int32_t pages;
+  int32_t heads;
+  int32_t page_size;
+  int32_t d;
+  int32_t k_bits;
+  int32_t v_bits;
+} pq_kv_cache;
+
+/* Lays out one side's tables once: rotation R (d x d f32), boundaries
+ * (2^bits - 1 f32, ascending) and centroids (2^bits f32), all on the device. */
+size_t pq_kv_codec_bytes(int d, int bits);
+int pq_kv_prepare_codec(const float* R, const float* boundaries, const float* centroids, int d,
+                        int bits, void* codec, size_t codec_bytes, void* stream);
+
+/* Writes n tokens: k and v are [n][heads][d] of `dtype` with the given strides
+ * (elements; the last is 1); token i goes to slots[i], or nowhere when that is
+ * outside [0, pages * page_size); the slots named have to differ.  codes,
+ * norms: as pq_encode's, the codes those of the exact product.  positions:
+ * [n] int32.  weights: [n][heads] f32 or NULL for zeros. */
+int pq_kv_append(const pq_kv_cache* cache, const void* k, const void* v, int dtype, int64_t n,
+                 int64_t k_stride_n, int64_t k_stride_h, int64_t v_stride_n, int64_t v_stride_h,
+                 const int64_t* slots, const int32_t* positions, const float* weights,
+                 void* stream);
+
+/* Reads n slots as the vectors they stand for, in rotated coordinates: norm *
+ * centroid[code], [n][heads][d] of `dtype`.  Slots outside the pool give 0. */
+int pq_kv_read(const pq_kv_cache* cache, const int64_t* slots, int64_t n, void* k, void* v,
+               int dtype, void* stream);
+
+/* Attention of one token of each sequence over its cache: q [batch][q_heads][d]
+ * (strides in elements, the last 1), query head h reads key-value head
+ * h / (q_heads / heads); scores are scale * q . k; out [batch][q_heads][d] of
+ * the same dtype; lse (or NULL) [batch][q_heads] f32, the natural logarithm of
+ * the softmax's sum.  A sequence without tokens gives 0 and -inf.  accumulate:
+ * adds every token's softmax weights, summed over its head's query heads, to
+ * `weights`. */
+size_t pq_kv_attend_workspace_bytes(const pq_kv_cache* cache, int batch, int q_heads,
+                                    int table_width, int accumulate);
+int pq_kv_attend(const pq_kv_cache* cache, const void* q, int dtype, int64_t q_stride_b,
+                 int64_t q_stride_h, const int32_t* table, int64_t table_stride, int table_width,
+                 const int32_t* lengths, int batch, int q_heads, float scale, void* out,
+                 float* lse, int accumulate, void* ws, size_t ws_bytes, void* stream);
+
+/* Keeps `budget` tokens of every longer sequence, for each head its own: those
+ * of a position below `sinks` or among the last `recent` positions first, then
+ * the heaviest, ties to the lowest slot (a NaN weight counts as the lightest).
+ * Kept tokens behind the budget move into the places of evicted ones before
+ * it, the first into the first; all others stay where they are.  With
+ * prompt_weights ([batch][heads], strides in elements, prompt_width tokens
+ * each, at least the lengths) the tokens are a prompt's: token i has position
+ * i and that weight, and the kept ones' positions and weights are written.
+ * new_lengths: [batch], min(length, budget).  A page may be in one sequence
+ * only. */
+size_t pq_kv_evict_workspace_bytes(const pq_kv_cache* cache, int batch, int table_width,
+                                   int budget);
+int pq_kv_evict(const pq_kv_cache* cache, const int32_t* table, int64_t table_stride,
+                int table_width, const int32_t* lengths, int batch, int budget, int recent,
+                int sinks, const float* prompt_weights, int64_t prompt_stride_b,
+                int64_t prompt_stride_h, int prompt_width, int32_t* new_lengths, void* ws,
+                size_t ws_bytes, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

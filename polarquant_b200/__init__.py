@@ -10,6 +10,7 @@ import warnings
 
 from .core import CompressedVectors, PackedVectors, Quantizer
 from .ivf import IVFCoarseIndex
+from .kvcache import KVCache, KVCodec
 from .packing import pack, packed_nbytes, unpack
 from .params import lloyd_max_codebook, nested_codebooks
 from .pq_format import load_pq, save_params, save_pq
@@ -19,6 +20,7 @@ __all__ = [
     "Quantizer", "CompressedVectors", "PackedVectors",
     "PolarQuantizer",
     "IVFCoarseIndex",
+    "KVCache", "KVCodec",
     "lloyd_max_codebook", "nested_codebooks",
     "pack", "unpack", "packed_nbytes",
     "save_pq", "load_pq", "save_params",

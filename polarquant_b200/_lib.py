@@ -20,6 +20,7 @@ _P = ctypes.c_void_p
 _I = ctypes.c_int
 _L = ctypes.c_int64
 _Z = ctypes.c_size_t
+_F = ctypes.c_float
 
 # name -> (restype, argtypes); must list every symbol of the public header.
 SIGNATURES = {
@@ -65,7 +66,26 @@ SIGNATURES = {
     "pq_unpack_at": (_I, [_P, _L, _P, _L, _I, _I, _I, _P, _P]),
     "pq_repack": (_I, [_P, _L, _L, _I, _I, _I, _P, _L, _P]),
     "pq_pack_codes": (_I, [_P, _L, _I, _I, _P, _L, _P]),
+    "pq_kv_codec_bytes": (_Z, [_I, _I]),
+    "pq_kv_prepare_codec": (_I, [_P, _P, _P, _I, _I, _P, _Z, _P]),
+    "pq_kv_append": (_I, [_P, _P, _P, _I, _L, _L, _L, _L, _L, _P, _P, _P, _P]),
+    "pq_kv_read": (_I, [_P, _P, _L, _P, _P, _I, _P]),
+    "pq_kv_attend_workspace_bytes": (_Z, [_P, _I, _I, _I, _I]),
+    "pq_kv_attend": (_I, [_P, _P, _I, _L, _L, _P, _L, _I, _P, _I, _I, _F, _P, _P, _I, _P, _Z,
+                          _P]),
+    "pq_kv_evict_workspace_bytes": (_Z, [_P, _I, _I, _I]),
+    "pq_kv_evict": (_I, [_P, _P, _L, _I, _P, _I, _I, _I, _I, _P, _L, _L, _I, _P, _P, _Z, _P]),
 }
+
+class KVCacheDesc(ctypes.Structure):
+    """pq_kv_cache of the public header."""
+
+    _fields_ = ([(n, _P) for n in ("k_rows", "v_rows", "k_norms", "v_norms", "positions",
+                                   "weights", "k_codec", "v_codec")] +
+                [(n, _L) for n in ("k_ldb", "v_ldb")] +
+                [(n, ctypes.c_int32) for n in ("pages", "heads", "page_size", "d", "k_bits",
+                                               "v_bits")])
+
 
 _lock = threading.Lock()
 _lib = None

@@ -1,0 +1,138 @@
+// Shared parts of the compressed key-value cache's kernels: argument checks,
+// the tables of a codec, and the addresses of a page's rows.
+#pragma once
+#include <cuda_bf16.h>
+
+#include "common.cuh"
+
+namespace pqb {
+namespace kv {
+
+// One side's tables as pq_kv_prepare_codec lays them out.
+struct Codec {
+  const float* R;       // d x d
+  const float* RT;      // its transpose
+  const float* bounds;  // 2^bits - 1
+  const float* cent;    // 2^bits
+};
+
+inline size_t codec_bytes(int d, int /*bits*/) {
+  return (size_t)2 * align_up((size_t)d * d * sizeof(float), 256) + 2 * 256 * sizeof(float);
+}
+
+inline Codec codec_of(const void* tables, int d) {
+  const char* b = (const char*)tables;
+  const size_t m = align_up((size_t)d * d * sizeof(float), 256);
+  return Codec{(const float*)b, (const float*)(b + m), (const float*)(b + 2 * m),
+               (const float*)(b + 2 * m + 1024)};
+}
+
+// One side of the pool.
+struct Side {
+  uint8_t* rows;
+  float* norms;
+  int64_t ldb;
+  int bits;
+  Codec c;
+};
+
+inline Side side_k(const pq_kv_cache& c) {
+  return Side{c.k_rows, c.k_norms, c.k_ldb, c.k_bits, codec_of(c.k_codec, c.d)};
+}
+inline Side side_v(const pq_kv_cache& c) {
+  return Side{c.v_rows, c.v_norms, c.v_ldb, c.v_bits, codec_of(c.v_codec, c.d)};
+}
+
+inline bool bits_ok(int b) { return b == 2 || b == 4 || b == 8; }
+
+inline int check_cache(const pq_kv_cache* c) {
+  PQ_CHECK_ARG(c, "null cache");
+  PQ_CHECK_ARG(c->d >= 1 && c->d <= PQ_KV_MAX_D, "d must be in [1, %d] (got %d)", PQ_KV_MAX_D,
+               c->d);
+  PQ_CHECK_ARG(bits_ok(c->k_bits) && bits_ok(c->v_bits),
+               "k_bits and v_bits must be 2, 4 or 8 (got %d and %d)", c->k_bits, c->v_bits);
+  PQ_CHECK_ARG(c->heads >= 1, "heads must be at least 1 (got %d)", c->heads);
+  PQ_CHECK_ARG(c->pages >= 0, "pages must be at least 0 (got %d)", c->pages);
+  PQ_CHECK_ARG(c->page_size >= 16 && c->page_size <= 1024 &&
+                   (c->page_size & (c->page_size - 1)) == 0,
+               "page_size must be a power of two from 16 to 1024 (got %d)", c->page_size);
+  PQ_CHECK_ARG((int64_t)c->pages * c->page_size < (1ll << 31) &&
+                   (int64_t)c->pages * c->heads < (1ll << 31),
+               "a pool has fewer than 2^31 slots");
+  PQ_CHECK_ARG(c->k_ldb % 16 == 0 && c->k_ldb >= row_bytes(c->d, c->k_bits) &&
+                   c->v_ldb % 16 == 0 && c->v_ldb >= row_bytes(c->d, c->v_bits),
+               "k_ldb and v_ldb must be multiples of 16 that hold a row (got %lld and %lld)",
+               (long long)c->k_ldb, (long long)c->v_ldb);
+  PQ_CHECK_ARG(c->k_codec && c->v_codec, "null codec");
+  PQ_CHECK_ARG(c->pages == 0 || (c->k_rows && c->v_rows && c->k_norms && c->v_norms &&
+                                 c->positions && c->weights),
+               "null pool pointer");
+  PQ_CHECK_ARG(((uintptr_t)c->k_rows | (uintptr_t)c->v_rows) % 16 == 0,
+               "rows must be 16-byte aligned");
+  return PQ_OK;
+}
+
+inline int check_dtype(int dtype) {
+  PQ_CHECK_ARG(dtype == PQ_KV_F32 || dtype == PQ_KV_F16 || dtype == PQ_KV_BF16,
+               "dtype must be 0 (f32), 1 (f16) or 2 (bf16) (got %d)", dtype);
+  return PQ_OK;
+}
+
+inline int check_sequences(const int32_t* table, int table_width, const int32_t* lengths,
+                           int batch, int page_size) {
+  PQ_CHECK_ARG(table_width >= 0 && (int64_t)table_width * page_size < (1ll << 31),
+               "a sequence has fewer than 2^31 tokens");
+  PQ_CHECK_ARG((table || table_width == 0) && lengths, "null table or lengths");
+  PQ_CHECK_ARG(batch >= 0, "batch must be at least 0");
+  return PQ_OK;
+}
+
+template <class T>
+__device__ __forceinline__ float to_f32(T x);
+template <>
+__device__ __forceinline__ float to_f32<float>(float x) { return x; }
+template <>
+__device__ __forceinline__ float to_f32<__half>(__half x) { return __half2float(x); }
+template <>
+__device__ __forceinline__ float to_f32<__nv_bfloat16>(__nv_bfloat16 x) {
+  return __bfloat162float(x);
+}
+
+template <class T>
+__device__ __forceinline__ T from_f32(float x);
+template <>
+__device__ __forceinline__ float from_f32<float>(float x) { return x; }
+template <>
+__device__ __forceinline__ __half from_f32<__half>(float x) { return __float2half_rn(x); }
+template <>
+__device__ __forceinline__ __nv_bfloat16 from_f32<__nv_bfloat16>(float x) {
+  return __float2bfloat16_rn(x);
+}
+
+// Runs the statement with T_ as the element type of `dtype`.
+#define PQ_KV_DISPATCH_T(dtype, ...)      \
+  do {                                    \
+    if ((dtype) == PQ_KV_F32) {           \
+      using T_ = float;                   \
+      __VA_ARGS__;                        \
+    } else if ((dtype) == PQ_KV_F16) {    \
+      using T_ = __half;                  \
+      __VA_ARGS__;                        \
+    } else {                              \
+      using T_ = __nv_bfloat16;           \
+      __VA_ARGS__;                        \
+    }                                     \
+  } while (0)
+
+// Code j of a packed row (first code in the highest bits of a byte).
+__device__ __forceinline__ uint32_t code_at(const uint8_t* row, int j, int bits) {
+  const uint32_t bit = (uint32_t)j * (uint32_t)bits;
+  return (row[bit >> 3] >> (8 - bits - (int)(bit & 7u))) & ((1u << bits) - 1u);
+}
+
+__device__ __forceinline__ int clamp_length(int len, int table_width, int page_size) {
+  return max(0, min(len, table_width * page_size));
+}
+
+}  // namespace kv
+}  // namespace pqb

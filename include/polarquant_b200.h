@@ -348,7 +348,8 @@ int pq_pack_codes(const uint8_t* codes, int64_t n, int d, int bits, uint8_t* out
  * A slot is page * page_size + offset.  A sequence is a row of a page table
  * (int32, table_width entries, row stride table_stride) and a length: its
  * token i lies in page table[i / page_size] at offset i % page_size, for every
- * head.  Entries behind the length are not read.  Lengths are taken as at most
+ * head.  Entries behind the length are not read; table_width * page_size is at most
+ * 2^30.  Lengths are taken as at most
  * table_width * page_size and at least 0; a token on a page outside
  * [0, pages) is not there (attention passes over it, nothing is written).
  * Calls that write a page (append, evict, attend with `accumulate`) are

@@ -10,21 +10,30 @@ namespace kv {
 
 // One side's tables as pq_kv_prepare_codec lays them out.
 struct Codec {
-  const float* R;       // d x d
-  const float* RT;      // its transpose
-  const float* bounds;  // 2^bits - 1
-  const float* cent;    // 2^bits
+  const float* R;         // d x d
+  const float* RT;        // its transpose
+  const float* bounds;    // 2^bits - 1
+  const float* cent;      // 2^bits
+  const uint32_t* pairs;  // [2][256] centroids * 2^exponent for decoding in f16
+                          // 4 bits: both of a byte's, hi parts; then lo parts
+                          // 8 bits: hi and lo part of the byte's
+                          // 2 bits: bytes 0 and 1 of the four hi parts, of the lo parts
+  const int* exponent;    // the largest centroid * 2^exponent lies in [2^13, 2^14)
 };
 
 inline size_t codec_bytes(int d, int /*bits*/) {
-  return (size_t)2 * align_up((size_t)d * d * sizeof(float), 256) + 2 * 256 * sizeof(float);
+  return (size_t)2 * align_up((size_t)d * d * sizeof(float), 256) + 4 * 1024 + 256;
 }
 
 inline Codec codec_of(const void* tables, int d) {
   const char* b = (const char*)tables;
   const size_t m = align_up((size_t)d * d * sizeof(float), 256);
-  return Codec{(const float*)b, (const float*)(b + m), (const float*)(b + 2 * m),
-               (const float*)(b + 2 * m + 1024)};
+  return Codec{(const float*)b,
+               (const float*)(b + m),
+               (const float*)(b + 2 * m),
+               (const float*)(b + 2 * m + 1024),
+               (const uint32_t*)(b + 2 * m + 2048),
+               (const int*)(b + 2 * m + 4096)};
 }
 
 // One side of the pool.
@@ -80,8 +89,8 @@ inline int check_dtype(int dtype) {
 
 inline int check_sequences(const int32_t* table, int table_width, const int32_t* lengths,
                            int batch, int page_size) {
-  PQ_CHECK_ARG(table_width >= 0 && (int64_t)table_width * page_size < (1ll << 31),
-               "a sequence has fewer than 2^31 tokens");
+  PQ_CHECK_ARG(table_width >= 0 && (int64_t)table_width * page_size <= (1ll << 30),
+               "a sequence has at most 2^30 tokens");
   PQ_CHECK_ARG((table || table_width == 0) && lengths, "null table or lengths");
   PQ_CHECK_ARG(batch >= 0, "batch must be at least 0");
   return PQ_OK;

@@ -5,214 +5,933 @@
 // and the output Rv^T (sum_j p_j vn_j c[vcode_j]), p = softmax(s): neither side
 // of the cache is turned back, only the query and the output.
 //
-// rotate_kernel turns the queries; attend_kernel takes kSplit tokens of one
-// key-value head and up to eight of its query heads and leaves their maximum,
-// sum and unnormalised output; join_kernel puts a row's splits together and
-// turns the output back; weights_kernel adds the softmax weights.
+// Three launches, each let in early by the one before it (programmatic
+// dependent launch):
+//  1. kv_query_kernel turns the queries (f32), splits each into f16 hi + lo
+//     planes of a power-of-two scale and one block sums up the sequences' units
+//     of work.
+//  2. kv_attend_kernel: persistent blocks take equal runs of units (a unit: 8
+//     warps' steps of one key-value head and up to eight of its query heads),
+//     so ragged batches and single long sequences fill the GPU alike.  One pass
+//     with running maximum and sum; a block leaves one partial result for every
+//     head that its run touches.
+//  3. kv_join_kernel puts a head's partials together in order (no atomics: the
+//     same call gives the same bits) and turns the output back.
+// With `accumulate`, 2 also leaves the scores and a fourth kernel turns them
+// into softmax weights.
+//
+// The step.  A warp takes 16 tokens at a time through mma.m16n8k16: keys are
+// the A operand (16 tokens x 16 coordinates), the eight queries B, so S^T has
+// tokens in rows; values transposed are A (16 coordinates x 16 tokens) and P^T
+// is B, made from S^T's registers by movmatrix.  Operand registers are made in
+// place from the packed codes: every lane's 16-byte load of a row holds the
+// coordinates of its own operand registers, because the order of coordinates
+// is free as long as the queries have the same one.  A packed byte is decoded
+// by one shared-memory lookup that gives both of its centroids as an f16 pair
+// (4 bits; at 8 bits one centroid as f16 hi + lo), from a table with a copy for
+// each lane, 256 bytes per entry with keys in the lower and values in the
+// upper half: no bank conflicts, and the address is a single byte permute.  2
+// bits are decoded by byte permutes on a table of four in registers.
+//
+// What bounds it: at 4 bits and d = 128 a token and head is 136 bytes, 128
+// lookups of the 32 a cycle that an SM's shared memory gives, 160 byte
+// permutes of 64 a cycle and 16 matrix instructions of 0.46 a cycle; at HBM
+// rate that is 67 %, 50 % and 36 % of these.
+//
+// Roundings.  Centroids and queries are taken times powers of two that put the
+// largest at 2^13; f16 hi has 11 bits, hi + lo 22.  Softmax weights times value
+// norms (relative to a power of two near the largest so far) are rounded to
+// f16 for the product.  Precision levels (kPrec):
+//   0 (bf16 out): hi alone everywhere: errors of 2^-12 next to the output's 2^-9
+//   1 (f16 out): queries and weights hi + lo, centroids hi
+//   2 (lse or accumulated weights are asked for, in f32): keys hi + lo too
+//   3 (f32): values hi + lo too
+// Maxima, sums and accumulators are f32.
+#include <float.h>
+
 #include "kv.cuh"
 
 namespace pqb {
 namespace kv {
 
-constexpr int kSplit = 512;   // tokens of one block
-constexpr int kTile = 32;     // tokens dequantised at a time
-constexpr int kHeadsPer = 8;  // query heads of one block
+constexpr int kHeadsPer = 8;    // query heads of one block: the width of an mma
+constexpr int kAttWarps = 8;
 constexpr float kLog2e = 1.4426950408889634f;
+constexpr float kLn2 = 0.6931471805599453f;
+constexpr float kRescale = 8.f;  // the running maximum follows when exceeded by 2^8
 
-// Queries in rotated coordinates, times scale * log2(e) (scores are powers of 2).
-template <class T>
-__global__ void __launch_bounds__(PQ_KV_MAX_D)
-rotate_kernel(const T* __restrict__ q, int64_t sb, int64_t sh, int hq, int d,
-              const float* __restrict__ RT, float scale, float* __restrict__ out) {
-  __shared__ float sq[PQ_KV_MAX_D];
-  const int b = blockIdx.x / hq, h = blockIdx.x % hq, j = threadIdx.x;
-  if (j < d) sq[j] = to_f32<T>(q[b * sb + h * sh + j]);
-  __syncthreads();
-  if (j >= d) return;
-  float y = 0.f;
-  for (int i = 0; i < d; ++i) y = fmaf(sq[i], RT[i * d + j], y);
-  out[(int64_t)blockIdx.x * d + j] = y * (scale * kLog2e);
+__device__ __forceinline__ void pdl_wait() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
+__device__ __forceinline__ void pdl_next() {
+  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
 }
 
-__global__ void __launch_bounds__(128)
-attend_kernel(Side sk, Side sv, int heads, int group, int d, int pages, int page_size,
-              const float* __restrict__ qrot, const int32_t* __restrict__ table,
-              int64_t table_stride, int table_width, const int32_t* __restrict__ lengths,
-              int splits, float* __restrict__ part_o, float2* __restrict__ part_ml,
-              float* __restrict__ scores, int64_t score_width) {
-  extern __shared__ float sm[];
-  float* sq = sm;                            // kHeadsPer x d
-  float* tile = sq + kHeadsPer * d;          // kTile x (d + 1)
-  float* sp = tile + kTile * (d + 1);        // kHeadsPer x kTile
-  float* cent_k = sp + kHeadsPer * kTile;    // 256
-  float* cent_v = cent_k + 256;              // 256
-  __shared__ float s_m[kHeadsPer], s_l[kHeadsPer], s_c[kHeadsPer];
-  const int split = blockIdx.x, b = blockIdx.y / heads, h = blockIdx.y % heads;
-  const int hq = heads * group, g0 = blockIdx.z * kHeadsPer, ng = min(kHeadsPer, group - g0);
-  const int len = clamp_length(lengths[b], table_width, page_size);
-  const int t0 = split * kSplit, t1 = min(len, t0 + kSplit);
-  const int64_t row0 = (int64_t)b * hq + (int64_t)h * group + g0;
+__device__ __forceinline__ void mma16816(float (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2,
+                                         uint32_t a3, uint32_t b0, uint32_t b1) {
+  asm volatile(
+      "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, "
+      "{%0,%1,%2,%3};"
+      : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
+      : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+}
+
+__device__ __forceinline__ uint32_t transpose8(uint32_t x) {
+  uint32_t y;
+  asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(y) : "r"(x));
+  return y;
+}
+
+__device__ __forceinline__ uint32_t pack_half2(float a, float b) {
+  const __half2 h = __floats2half2_rn(a, b);
+  return *reinterpret_cast<const uint32_t*>(&h);
+}
+
+__device__ __forceinline__ float2 unpack_half2(uint32_t x) {
+  return __half22float2(*reinterpret_cast<const __half2*>(&x));
+}
+
+__device__ __forceinline__ float ex2(float x) {
+  float y;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+
+// B bytes (2, 4, 8 or 16) of a row; streamed, so not kept in L1.  Zeros without `in`.
+template <int B>
+__device__ __forceinline__ void load_bytes(const uint8_t* p, bool in, uint32_t* w) {
+  if constexpr (B == 16) {
+    w[0] = w[1] = w[2] = w[3] = 0u;
+    if (in)
+      asm volatile("ld.global.L1::no_allocate.v4.b32 {%0,%1,%2,%3}, [%4];"
+                   : "=r"(w[0]), "=r"(w[1]), "=r"(w[2]), "=r"(w[3])
+                   : "l"(p));
+  } else if constexpr (B == 8) {
+    w[0] = w[1] = 0u;
+    if (in)
+      asm volatile("ld.global.L1::no_allocate.v2.b32 {%0,%1}, [%2];"
+                   : "=r"(w[0]), "=r"(w[1])
+                   : "l"(p));
+  } else if constexpr (B == 4) {
+    w[0] = 0u;
+    if (in) asm volatile("ld.global.L1::no_allocate.b32 %0, [%1];" : "=r"(w[0]) : "l"(p));
+  } else {
+    uint16_t h = 0;
+    if (in) asm volatile("ld.global.L1::no_allocate.b16 %0, [%1];" : "=h"(h) : "l"(p));
+    w[0] = h;
+  }
+}
+
+__device__ __forceinline__ float load_norm(const float* p, bool in) {
+  float x = 0.f;
+  if (in) asm volatile("ld.global.L1::no_allocate.f32 %0, [%1];" : "=f"(x) : "l"(p));
+  return x;
+}
+
+// How a row of D coordinates is dealt to L lanes: lane i holds bytes
+// [u * L * UB + i * UB, + UB) of it for each unit u, CU codes a unit.
+template <int D, int BITS, int L>
+struct Deal {
+  static constexpr int bytes = D * BITS / 8 / L;
+  static constexpr int UB = bytes < 16 ? bytes : 16;
+  static constexpr int units = bytes / UB;
+  static constexpr int words = (bytes + 3) / 4;
+  static constexpr int CU = UB * 8 / BITS;
+  // Coordinate of the lane's code n.
+  static __device__ __forceinline__ int dim(int lane, int n) {
+    return (n / CU) * L * CU + lane * CU + n % CU;
+  }
+  static __device__ __forceinline__ void load(const uint8_t* row, int64_t ldb, int lane, bool in,
+                                              uint32_t (&w)[words]) {
+#pragma unroll
+    for (int u = 0; u < units; ++u) {
+      const int off = u * L * UB + lane * UB;
+      load_bytes<UB>(row + off, in && off < ldb, &w[u * UB / 4]);
+    }
+  }
+};
+
+// Decoding.  Tables in shared memory as described above; `lane_off` is the
+// lane's offset in an entry.  lo: offset of the 4-bit tables' lo parts.
+constexpr uint32_t kTableBytes = 65536;
+
+__device__ __forceinline__ uint32_t lookup(const uint8_t* table, uint32_t lane_off, uint32_t w,
+                                           int byte) {
+  return *reinterpret_cast<const uint32_t*>(table +
+                                            __byte_perm(w, lane_off, 0x5504u | (byte << 4)));
+}
+
+// The four codes that a lane gives to one K step: pairs a (first operand
+// register) and b (third), hi and lo.  2 bits: the pairs are codes (2, 0) and
+// (3, 1) of the byte, else (0, 1) and (2, 3).
+template <int BITS, bool LO, int W>
+__device__ __forceinline__ void decode_key(const uint32_t (&w)[W], int s, const uint8_t* table,
+                                           uint32_t lane_off, const uint32_t (&reg)[4],
+                                           uint32_t& ah, uint32_t& bh, uint32_t& al, uint32_t& bl) {
+  if constexpr (BITS == 4) {
+    const uint32_t x = w[s >> 1];
+    const int b = (s & 1) * 2;
+    ah = lookup(table, lane_off, x, b);
+    bh = lookup(table, lane_off, x, b + 1);
+    if constexpr (LO) {
+      al = lookup(table + kTableBytes, lane_off, x, b);
+      bl = lookup(table + kTableBytes, lane_off, x, b + 1);
+    }
+  } else if constexpr (BITS == 8) {
+    const uint32_t x = w[s];
+    const uint32_t e0 = lookup(table, lane_off, x, 0), e1 = lookup(table, lane_off, x, 1);
+    const uint32_t e2 = lookup(table, lane_off, x, 2), e3 = lookup(table, lane_off, x, 3);
+    ah = __byte_perm(e0, e1, 0x5410);
+    bh = __byte_perm(e2, e3, 0x5410);
+    if constexpr (LO) {
+      al = __byte_perm(e0, e1, 0x7632);
+      bl = __byte_perm(e2, e3, 0x7632);
+    }
+  } else {
+    const uint32_t x = w[s >> 2] >> (8 * (s & 3));
+    const uint32_t sel = (x & 0x33u) << 8 | ((x >> 2) & 0x33u);  // codes 2, 0, 3, 1
+    const uint32_t l = __byte_perm(reg[0], reg[1], sel);
+    const uint32_t h = __byte_perm(reg[0], reg[1], sel | 0x4444u);
+    ah = __byte_perm(l, h, 0x5140);
+    bh = __byte_perm(l, h, 0x7362);
+    if constexpr (LO) {
+      const uint32_t l2 = __byte_perm(reg[2], reg[3], sel);
+      const uint32_t h2 = __byte_perm(reg[2], reg[3], sel | 0x4444u);
+      al = __byte_perm(l2, h2, 0x5140);
+      bl = __byte_perm(l2, h2, 0x7362);
+    }
+  }
+}
+
+// Codes 2m and 2m + 1 of two tokens' rows: the pairs (x's, y's) of either code.
+template <int BITS, bool LO, int W>
+__device__ __forceinline__ void decode_value(const uint32_t (&x)[W], const uint32_t (&y)[W], int m,
+                                             const uint8_t* table, uint32_t lane_off,
+                                             const uint32_t (&reg)[4], uint32_t& eh, uint32_t& oh,
+                                             uint32_t& el, uint32_t& ol) {
+  if constexpr (BITS == 4) {
+    const uint32_t p = lookup(table, lane_off, x[m >> 2], m & 3);
+    const uint32_t q = lookup(table, lane_off, y[m >> 2], m & 3);
+    eh = __byte_perm(p, q, 0x5410);
+    oh = __byte_perm(p, q, 0x7632);
+    if constexpr (LO) {
+      const uint32_t r = lookup(table + kTableBytes, lane_off, x[m >> 2], m & 3);
+      const uint32_t t = lookup(table + kTableBytes, lane_off, y[m >> 2], m & 3);
+      el = __byte_perm(r, t, 0x5410);
+      ol = __byte_perm(r, t, 0x7632);
+    }
+  } else if constexpr (BITS == 8) {
+    const int b = 2 * (m & 1);
+    const uint32_t p0 = lookup(table, lane_off, x[m >> 1], b);
+    const uint32_t p1 = lookup(table, lane_off, x[m >> 1], b + 1);
+    const uint32_t q0 = lookup(table, lane_off, y[m >> 1], b);
+    const uint32_t q1 = lookup(table, lane_off, y[m >> 1], b + 1);
+    eh = __byte_perm(p0, q0, 0x5410);
+    oh = __byte_perm(p1, q1, 0x5410);
+    if constexpr (LO) {
+      el = __byte_perm(p0, q0, 0x7632);
+      ol = __byte_perm(p1, q1, 0x7632);
+    }
+  } else {
+    // The byte of both tokens: codes 0, 1 (m even) or 2, 3 of it.
+    const uint32_t z = __byte_perm(x[m >> 3], y[m >> 3],
+                                   ((m >> 1) & 3) | (((m >> 1) & 3) + 4) << 4) & 0xffffu;
+    const uint32_t n = (m & 1) ? z : z >> 4;
+    // nibbles: odd code of x, even of x, odd of y, even of y
+    const uint32_t sel = (n & 0x0303u) | ((n & 0x0c0cu) << 2);
+    const uint32_t l = __byte_perm(reg[0], reg[1], sel);
+    const uint32_t h = __byte_perm(reg[0], reg[1], sel | 0x4444u);
+    oh = __byte_perm(l, h, 0x6240);
+    eh = __byte_perm(l, h, 0x7351);
+    if constexpr (LO) {
+      const uint32_t l2 = __byte_perm(reg[2], reg[3], sel);
+      const uint32_t h2 = __byte_perm(reg[2], reg[3], sel | 0x4444u);
+      ol = __byte_perm(l2, h2, 0x6240);
+      el = __byte_perm(l2, h2, 0x7351);
+    }
+  }
+}
+
+// ---------------------------------------------------------------------------
+// Work: the units of all (sequence, key-value head, block of query heads), in
+// that order; segment = the units of one of them.
+// ---------------------------------------------------------------------------
+
+struct Work {
+  const int32_t* table;
+  int64_t table_stride;
+  int table_width;
+  const int32_t* lengths;
+  int batch, heads, group, blocks;  // blocks of query heads per key-value head
+  int unit;                         // tokens of a unit
+  const int* first;                 // [batch + 1] first unit of each sequence
+
+  __device__ int units_of(int len) const { return (len + unit - 1) / unit; }
+};
+
+// Worker of a unit: worker w of n takes units [w * total / n, (w + 1) * total / n).
+__device__ __forceinline__ int worker_of(int64_t u, int n, int total) {
+  return (int)(((u + 1) * n - 1) / total);
+}
+
+struct QueryOut {
+  __half *hi, *lo;  // [segment][8][D]
+  float* factor;    // [segment][8]: score = factor * key norm * product, in log2
+};
+
+template <class T, int D>
+__global__ void __launch_bounds__(256)
+kv_query_kernel(const T* __restrict__ q, int64_t sb, int64_t sh, int d, int page_size,
+                const float* __restrict__ RT, const int* __restrict__ exponent, float scale,
+                Work wk, QueryOut out, int* __restrict__ first) {
+  __shared__ float sq[kHeadsPer][D], red[256 / (D < 256 ? D : 256)][kHeadsPer][D];
+  __shared__ int s_part[8];
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
-  if (t0 >= t1) {
-    if (tid < ng) part_ml[(row0 + tid) * splits + split] = make_float2(-INFINITY, 0.f);
+  pdl_next();
+  const int per = wk.heads * wk.blocks;
+  if (blockIdx.x == wk.batch * per) {
+    // First units: a running sum over the sequences.
+    int base = 0;
+    for (int b0 = 0; b0 < wk.batch; b0 += 256) {
+      const int b = b0 + tid;
+      const int n = b < wk.batch
+                        ? per * wk.units_of(clamp_length(wk.lengths[b], wk.table_width, page_size))
+                        : 0;
+      int v = n;
+#pragma unroll
+      for (int o = 1; o < 32; o <<= 1) {
+        const int y = __shfl_up_sync(0xffffffffu, v, o);
+        if (lane >= o) v += y;
+      }
+      if (lane == 31) s_part[warp] = v;
+      __syncthreads();
+      int before = 0, all = 0;
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        if (i < warp) before += s_part[i];
+        all += s_part[i];
+      }
+      if (b < wk.batch) first[b] = base + before + v - n;
+      base += all;
+      __syncthreads();
+    }
+    if (tid == 0) first[wk.batch] = base;
     return;
   }
-  for (int i = tid; i < ng * d; i += blockDim.x) sq[i] = qrot[row0 * d + i];
-  for (int i = tid; i < 256; i += blockDim.x) {
-    cent_k[i] = sk.c.cent[i];
-    cent_v[i] = sv.c.cent[i];
+  const int b = blockIdx.x / per, h = blockIdx.x % per / wk.blocks, hb = blockIdx.x % wk.blocks;
+  const int ng = min(kHeadsPer, wk.group - hb * kHeadsPer);
+  const T* src = q + b * sb + ((int64_t)h * wk.group + hb * kHeadsPer) * sh;
+  for (int i = tid; i < kHeadsPer * D; i += 256) {
+    const int g = i / D, j = i % D;
+    sq[g][j] = g < ng && j < d ? to_f32<T>(src[g * sh + j]) : 0.f;
   }
-  if (tid < kHeadsPer) {
-    s_m[tid] = -INFINITY;
-    s_l[tid] = 0.f;
-  }
-  float acc[2][kHeadsPer];
+  __syncthreads();
+  // Column j of R^T, rows split over 256 / D parts.
+  constexpr int parts = 256 / D;
+  const int j = tid % D, part = tid / D;
+  float acc[kHeadsPer];
 #pragma unroll
-  for (int g = 0; g < kHeadsPer; ++g) acc[0][g] = acc[1][g] = 0.f;
-  for (int base = t0; base < t1; base += kTile) {
-    // Each thread's token of the tile, for norms and rows.
-    auto place = [&](int i, bool& in) -> int64_t {
-      const int t = base + i;
-      in = t < t1;
-      const int pg = in ? table[b * table_stride + t / page_size] : -1;
-      in = pg >= 0 && pg < pages;
-      return in ? ((int64_t)pg * heads + h) * page_size + t % page_size : 0;
-    };
+  for (int g = 0; g < kHeadsPer; ++g) acc[g] = 0.f;
+  if (j < d) {
+    const int i0 = d * part / parts, i1 = d * (part + 1) / parts;
+#pragma unroll 8
+    for (int i = i0; i < i1; ++i) {
+      const float r = __ldg(RT + i * d + j);
+#pragma unroll
+      for (int g = 0; g < kHeadsPer; ++g) acc[g] = fmaf(sq[g][i], r, acc[g]);
+    }
+  }
+#pragma unroll
+  for (int g = 0; g < kHeadsPer; ++g) red[part][g][j] = acc[g];
+  __syncthreads();
+  // A warp per head: scale to a largest of [2^13, 2^14) and split.
+  float y[D / 32], mx = 0.f;
+#pragma unroll
+  for (int i = 0; i < D / 32; ++i) {
+    y[i] = 0.f;
+#pragma unroll
+    for (int p = 0; p < parts; ++p) y[i] += red[p][warp][lane + 32 * i];
+    mx = fmaxf(mx, fabsf(y[i]));
+  }
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, o));
+  const int e = mx > 0.f && mx < INFINITY ? max(-100, min(100, 13 - ilogbf(mx))) : 0;
+  const int64_t row = (int64_t)blockIdx.x * kHeadsPer + warp;
+#pragma unroll
+  for (int i = 0; i < D / 32; ++i) {
+    const float v = ldexpf(y[i], e);
+    const __half hi = __float2half_rn(v);
+    out.hi[row * D + lane + 32 * i] = hi;
+    out.lo[row * D + lane + 32 * i] = __float2half_rn(v - __half2float(hi));
+  }
+  if (lane == 0) out.factor[row] = ldexpf(scale * kLog2e, -e - *exponent);
+}
+
+struct Parts {
+  float* o;    // [slot][8][D]
+  float2* ml;  // [slot][8]: maximum (log2), sum
+};
+
+template <int D, int KB, int VB, int PREC>
+struct AttendShape {
+  // Steps of 32 tokens where the registers hold them, else of 16.
+  static constexpr int MT = D == 256 || (PREC >= 2 && (KB == 8 || VB == 8)) ? 1 : 2;
+  static constexpr bool tables = KB != 2 || VB != 2;
+  static constexpr bool lo_tables = (PREC >= 2 && KB == 4) || (PREC == 3 && VB == 4);
+  static constexpr int unit = kAttWarps * 16 * MT;
+  static constexpr size_t table_bytes =
+      tables ? (lo_tables ? 2 * (size_t)kTableBytes : (size_t)kTableBytes) : 0;
+  static constexpr int ostride = D + 8;
+  static constexpr size_t smem =
+      table_bytes + sizeof(float) * ((size_t)kAttWarps * kHeadsPer * ostride + 3 * 64);
+  static constexpr int ctas = D <= 128 && smem <= 110 * 1024 && PREC < 2 ? 2 : 1;
+};
+
+template <int D, int KB, int VB, int PREC>
+__global__ void __launch_bounds__(32 * kAttWarps, AttendShape<D, KB, VB, PREC>::ctas)
+kv_attend_kernel(Side sk, Side sv, int d, int pages, int page_size, Work wk, QueryOut qo,
+                 Parts parts, float* __restrict__ scores, int64_t score_width) {
+  using Shape = AttendShape<D, KB, VB, PREC>;
+  constexpr int MT = Shape::MT;
+  constexpr bool QLO = PREC >= 1, KLO = PREC >= 2, VLO = PREC >= 3;
+  using KD = Deal<D, KB, 4>;
+  using VD = Deal<D, VB, 8>;
+  constexpr int KS = D / 16;  // K steps of a score, and pairs of coordinates of a value
+  extern __shared__ __align__(16) uint8_t smem[];
+  const uint8_t* table = smem;
+  float* so = reinterpret_cast<float*>(smem + Shape::table_bytes);
+  float* s_m = so + kAttWarps * kHeadsPer * Shape::ostride;  // [warp][head]
+  float* s_l = s_m + 64;
+  float* s_f = s_l + 64;
+  __shared__ int s_b;
+  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, g = lane >> 2, t = lane & 3;
+  pdl_next();
+
+  // Tables, from the codec's entries (set-up data: not written by the kernel
+  // before).  Thread i copies entry i to the 32 lanes' places.
+  if constexpr (Shape::tables) {
+#pragma unroll
     for (int side = 0; side < 2; ++side) {
-      const Side& s = side ? sv : sk;
-      const float* cent = side ? cent_v : cent_k;
-      __syncthreads();
-      for (int i = warp; i < kTile; i += 4) {
-        bool in;
-        const int64_t at = place(i, in);
-        const float nrm = in ? s.norms[at] : 0.f;
-        for (int j = lane; j < d; j += 32)
-          tile[i * (d + 1) + j] = in ? nrm * cent[code_at(s.rows + at * s.ldb, j, s.bits)] : 0.f;
-      }
-      __syncthreads();
-      if (side == 0) {
-        bool in;
-        place(lane, in);
-        for (int g = warp; g < ng; g += 4) {
-          float y = 0.f;
-          for (int j = 0; j < d; ++j) y = fmaf(sq[g * d + j], tile[lane * (d + 1) + j], y);
-          if (!in) y = -INFINITY;
-          if (scores && base + lane < t1)
-            scores[(row0 + g) * score_width + base + lane] = y;
-          float mx = y;
+      const Codec& c = side ? sv.c : sk.c;
+      if ((side ? VB : KB) == 2) continue;
 #pragma unroll
-          for (int o = 16; o > 0; o >>= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, o));
-          const float m = fmaxf(s_m[g], mx);
-          const float mm = m == -INFINITY ? 0.f : m;
-          const float p = exp2f(y - mm);
-          float l = p;
+      for (int part = 0; part < (Shape::lo_tables ? 2 : 1); ++part) {
+        const uint32_t e = c.pairs[part * 256 + tid];
+        const uint4 v = make_uint4(e, e, e, e);
 #pragma unroll
-          for (int o = 16; o > 0; o >>= 1) l += __shfl_xor_sync(0xffffffffu, l, o);
-          sp[g * kTile + lane] = p;
-          __syncwarp();
-          if (lane == 0) {
-            s_c[g] = exp2f(s_m[g] - mm);
-            s_l[g] = s_l[g] * s_c[g] + l;
-            s_m[g] = m;
-          }
-        }
-      } else {
-#pragma unroll
-        for (int u = 0; u < 2; ++u) {
-          const int j = tid + 128 * u;
-          if (j >= d) continue;
-#pragma unroll
-          for (int g = 0; g < kHeadsPer; ++g) {
-            if (g >= ng) break;
-            float a = acc[u][g] * s_c[g];
-            for (int i = 0; i < kTile; ++i) a = fmaf(sp[g * kTile + i], tile[i * (d + 1) + j], a);
-            acc[u][g] = a;
-          }
-        }
+        for (int i = 0; i < 8; ++i)
+          *reinterpret_cast<uint4*>(smem + part * kTableBytes + tid * 256 + side * 128 +
+                                    ((i + tid) & 7) * 16) = v;
       }
     }
   }
+  uint32_t kreg[4], vreg[4];
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    kreg[i] = KB == 2 ? sk.c.pairs[i] : 0u;
+    vreg[i] = VB == 2 ? sv.c.pairs[i] : 0u;
+  }
+  const uint32_t koff = lane * 4, voff = 128 + lane * 4;
+  pdl_wait();
+
+  const int per = wk.heads * wk.blocks;
+  const int total = wk.first[wk.batch];
+  const int n = min((int)gridDim.x, total);
+  if ((int)blockIdx.x >= n) return;
+  int64_t u = (int64_t)blockIdx.x * total / n;
+  const int64_t uend = ((int64_t)blockIdx.x + 1) * total / n;
+  for (int i = tid; i < wk.batch; i += 32 * kAttWarps)
+    if (wk.first[i] <= u && u < wk.first[i + 1]) s_b = i;
   __syncthreads();
+  int b = s_b;
+
+  while (u < uend) {
+    // The segment of unit u and this block's share of it.
+    while (u >= wk.first[b + 1]) ++b;
+    const int len = clamp_length(wk.lengths[b], wk.table_width, page_size);
+    const int nu = wk.units_of(len);
+    const int r = (int)(u - wk.first[b]), seg_in = r / nu, u0 = r % nu;
+    const int u1 = (int)min((int64_t)nu, u0 + (uend - u));
+    const int h = seg_in / wk.blocks, hb = seg_in % wk.blocks;
+    const int seg = b * per + seg_in;
+    const int t0 = u0 * Shape::unit, t1 = min(len, u1 * Shape::unit);
+    const int32_t* trow = wk.table + b * wk.table_stride;
+
+    // The queries as B operands: lane (g, t) holds head g.
+    uint32_t qh[KS][2], ql[QLO ? KS : 1][2];
+    {
+      const __half* hi = qo.hi + ((int64_t)seg * kHeadsPer + g) * D;
+      const __half* lo = qo.lo + ((int64_t)seg * kHeadsPer + g) * D;
 #pragma unroll
-  for (int u = 0; u < 2; ++u)
+      for (int s = 0; s < KS; ++s) {
+        const int dim = KD::dim(t, 4 * s);
+        uint2 x = *reinterpret_cast<const uint2*>(hi + dim);
+        if (KB == 2)
+          x = make_uint2(__byte_perm(x.x, x.y, 0x1054), __byte_perm(x.x, x.y, 0x3276));
+        qh[s][0] = x.x;
+        qh[s][1] = x.y;
+        if constexpr (QLO) {
+          x = *reinterpret_cast<const uint2*>(lo + dim);
+          if (KB == 2)
+            x = make_uint2(__byte_perm(x.x, x.y, 0x1054), __byte_perm(x.x, x.y, 0x3276));
+          ql[s][0] = x.x;
+          ql[s][1] = x.y;
+        }
+      }
+    }
+    const float f0 = qo.factor[(int64_t)seg * kHeadsPer + 2 * t];
+    const float f1 = qo.factor[(int64_t)seg * kHeadsPer + 2 * t + 1];
+
+    float o[KS][4];
 #pragma unroll
-    for (int g = 0; g < kHeadsPer; ++g)
-      if (g < ng && tid + 128 * u < d)
-        part_o[((row0 + g) * splits + split) * d + tid + 128 * u] = acc[u][g];
-  if (tid < ng) part_ml[(row0 + tid) * splits + split] = make_float2(s_m[tid], s_l[tid]);
+    for (int m = 0; m < KS; ++m) o[m][0] = o[m][1] = o[m][2] = o[m][3] = 0.f;
+    float m0 = -FLT_MAX, m1 = -FLT_MAX, l0 = 0.f, l1 = 0.f;
+    float vinv = 0.f, vlim = 0.f, vref = 0.f;  // value norms are taken times vinv = 1 / vref
+
+    uint32_t kw[MT][2][KD::words], vw[MT][4][VD::words];
+    float kn[MT][2], vn[MT][2];
+    int pid[MT], pid_next[MT];
+    // Page of 16-token group i of the step at token `base`; -1 behind the end.
+    auto page_of = [&](int base, int i) {
+      const int tok = base + 16 * i;
+      int p = -1;
+      if (tok < t1) {
+        p = __ldg(trow + tok / page_size);
+        if (p >= pages) p = -1;
+      }
+      return p;
+    };
+    // First row of the group, and which of its rows are tokens.
+    auto row_of = [&](int p, int base, int i) {
+      return ((int64_t)p * wk.heads + h) * page_size + ((base + 16 * i) & (page_size - 1));
+    };
+    auto load_keys = [&](int base) {
+#pragma unroll
+      for (int i = 0; i < MT; ++i) {
+        const int64_t row = row_of(pid[i], base, i);
+#pragma unroll
+        for (int e = 0; e < 2; ++e) {
+          const int x = g + 8 * e;
+          const bool in = pid[i] >= 0 && base + 16 * i + x < t1;
+          KD::load(sk.rows + (row + x) * sk.ldb, sk.ldb, t, in, kw[i][e]);
+          kn[i][e] = load_norm(sk.norms + row + x, in);
+        }
+      }
+    };
+    auto load_values = [&](int base) {
+#pragma unroll
+      for (int i = 0; i < MT; ++i) {
+        const int64_t row = row_of(pid[i], base, i);
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          const int x = 2 * t + (e & 1) + 8 * (e >> 1);
+          const bool in = pid[i] >= 0 && base + 16 * i + x < t1;
+          VD::load(sv.rows + (row + x) * sv.ldb, sv.ldb, g, in, vw[i][e]);
+        }
+#pragma unroll
+        for (int e = 0; e < 2; ++e) {
+          const int x = g + 8 * e;
+          vn[i][e] = load_norm(sv.norms + row + x, pid[i] >= 0 && base + 16 * i + x < t1);
+        }
+      }
+    };
+
+    constexpr int stride = Shape::unit;
+    int base = t0 + warp * 16 * MT;
+#pragma unroll
+    for (int i = 0; i < MT; ++i) {
+      pid[i] = page_of(base, i);
+      pid_next[i] = page_of(base + stride, i);
+    }
+    if (base < t1) {
+      load_keys(base);
+      load_values(base);
+    }
+    for (; base < t1; base += stride) {
+      // Scores: S^T, tokens g and g + 8, heads 2t and 2t + 1.
+      float s[MT][4];
+#pragma unroll
+      for (int i = 0; i < MT; ++i) {
+        s[i][0] = s[i][1] = s[i][2] = s[i][3] = 0.f;
+#pragma unroll
+        for (int k = 0; k < KS; ++k) {
+          uint32_t a0, a1, a2, a3, c0 = 0, c1 = 0, c2 = 0, c3 = 0;
+          decode_key<KB, KLO>(kw[i][0], k, table, koff, kreg, a0, a2, c0, c2);
+          decode_key<KB, KLO>(kw[i][1], k, table, koff, kreg, a1, a3, c1, c3);
+          mma16816(s[i], a0, a1, a2, a3, qh[k][0], qh[k][1]);
+          if constexpr (QLO) mma16816(s[i], a0, a1, a2, a3, ql[k][0], ql[k][1]);
+          if constexpr (KLO) mma16816(s[i], c0, c1, c2, c3, qh[k][0], qh[k][1]);
+        }
+      }
+      float mx0 = -FLT_MAX, mx1 = -FLT_MAX, vmx = 0.f;
+#pragma unroll
+      for (int i = 0; i < MT; ++i)
+#pragma unroll
+        for (int e = 0; e < 2; ++e) {
+          const int tok = base + 16 * i + g + 8 * e;
+          const bool in = pid[i] >= 0 && tok < t1;
+          float& x = s[i][2 * e];
+          float& y = s[i][2 * e + 1];
+          x = in ? x * (kn[i][e] * f0) : -INFINITY;
+          y = in ? y * (kn[i][e] * f1) : -INFINITY;
+          if (PREC >= 2 && scores && tok < t1) {
+            float* to = scores + (((int64_t)b * wk.heads + h) * score_width + tok) * wk.group +
+                        hb * kHeadsPer + 2 * t;
+            if (hb * kHeadsPer + 2 * t < wk.group) to[0] = x;
+            if (hb * kHeadsPer + 2 * t + 1 < wk.group) to[1] = y;
+          }
+          mx0 = fmaxf(mx0, x);
+          mx1 = fmaxf(mx1, y);
+          vmx = fmaxf(vmx, vn[i][e]);
+        }
+      float vnow[MT][2];
+#pragma unroll
+      for (int i = 0; i < MT; ++i) {
+        vnow[i][0] = vn[i][0];
+        vnow[i][1] = vn[i][1];
+      }
+      // The next step's keys.
+#pragma unroll
+      for (int i = 0; i < MT; ++i) pid[i] = pid_next[i];
+      const bool more = base + stride < t1;
+      if (more) load_keys(base + stride);
+#pragma unroll
+      for (int i = 0; i < MT; ++i) pid_next[i] = page_of(base + 2 * stride, i);
+
+      if (__any_sync(0xffffffffu, mx0 > m0 + kRescale || mx1 > m1 + kRescale || vmx > vlim)) {
+#pragma unroll
+        for (int w = 4; w < 32; w <<= 1) {
+          mx0 = fmaxf(mx0, __shfl_xor_sync(0xffffffffu, mx0, w));
+          mx1 = fmaxf(mx1, __shfl_xor_sync(0xffffffffu, mx1, w));
+          vmx = fmaxf(vmx, __shfl_xor_sync(0xffffffffu, vmx, w));
+        }
+        mx0 = fmaxf(mx0, m0);
+        mx1 = fmaxf(mx1, m1);
+        float e0 = ex2(m0 - mx0), e1 = ex2(m1 - mx1);
+        m0 = mx0;
+        m1 = mx1;
+        l0 *= e0;
+        l1 *= e1;
+        if (vmx > vlim) {
+          const int ex = vmx < INFINITY ? max(-100, min(100, ilogbf(vmx) + 1)) : 100;
+          const float now = ldexpf(1.f, ex);
+          e0 *= vref / now;
+          e1 *= vref / now;
+          vref = now;
+          vinv = 1.f / now;
+          vlim = 16.f * now;
+        }
+#pragma unroll
+        for (int m = 0; m < KS; ++m) {
+          o[m][0] *= e0;
+          o[m][1] *= e1;
+          o[m][2] *= e0;
+          o[m][3] *= e1;
+        }
+      }
+      // P^T as B operands: tokens 2t, 2t + 1 (and + 8), head g.
+      uint32_t ph[MT][2], pl[MT][2];
+#pragma unroll
+      for (int i = 0; i < MT; ++i)
+#pragma unroll
+        for (int e = 0; e < 2; ++e) {
+          const float p0 = ex2(s[i][2 * e] - m0), p1 = ex2(s[i][2 * e + 1] - m1);
+          l0 += p0;
+          l1 += p1;
+          const float w = vnow[i][e] * vinv;
+          const float x = p0 * w, y = p1 * w;
+          const uint32_t hi = pack_half2(x, y);
+          ph[i][e] = transpose8(hi);
+          if constexpr (QLO) {
+            const float2 f = unpack_half2(hi);
+            pl[i][e] = transpose8(pack_half2(x - f.x, y - f.y));
+          }
+        }
+#pragma unroll
+      for (int i = 0; i < MT; ++i) {
+#pragma unroll
+        for (int m = 0; m < KS; ++m) {
+          uint32_t a0, a1, a2, a3, c0 = 0, c1 = 0, c2 = 0, c3 = 0;
+          decode_value<VB, VLO>(vw[i][0], vw[i][1], m, table, voff, vreg, a0, a1, c0, c1);
+          decode_value<VB, VLO>(vw[i][2], vw[i][3], m, table, voff, vreg, a2, a3, c2, c3);
+          mma16816(o[m], a0, a1, a2, a3, ph[i][0], ph[i][1]);
+          if constexpr (QLO) mma16816(o[m], a0, a1, a2, a3, pl[i][0], pl[i][1]);
+          if constexpr (VLO) mma16816(o[m], c0, c1, c2, c3, ph[i][0], ph[i][1]);
+        }
+      }
+      if (more) load_values(base + stride);
+    }
+
+    // The block's partial result: warps joined in order.
+#pragma unroll
+    for (int w = 4; w < 32; w <<= 1) {
+      l0 += __shfl_xor_sync(0xffffffffu, l0, w);
+      l1 += __shfl_xor_sync(0xffffffffu, l1, w);
+    }
+    if (g == 0) {
+      s_m[warp * 8 + 2 * t] = m0;
+      s_m[warp * 8 + 2 * t + 1] = m1;
+      s_l[warp * 8 + 2 * t] = l0;
+      s_l[warp * 8 + 2 * t + 1] = l1;
+    }
+    if (lane == 0) s_f[warp] = vref;
+    const int active = min(kAttWarps, (t1 - t0 + 16 * MT - 1) / (16 * MT));
+    if (warp < active) {
+      float* dst = so + (warp * kHeadsPer + 2 * t) * Shape::ostride;
+#pragma unroll
+      for (int m = 0; m < KS; ++m) {
+        const int dim = VD::dim(g, 2 * m);
+        *reinterpret_cast<float2*>(dst + dim) = make_float2(o[m][0], o[m][2]);
+        *reinterpret_cast<float2*>(dst + Shape::ostride + dim) = make_float2(o[m][1], o[m][3]);
+      }
+    }
+    __syncthreads();
+    const int64_t slot = (int64_t)blockIdx.x + seg;
+    const int ng = min(kHeadsPer, wk.group - hb * kHeadsPer);
+    for (int i = tid; i < ng * D; i += 32 * kAttWarps) {
+      const int hd = i / D, j = i % D;
+      float mm = -FLT_MAX;
+      for (int w = 0; w < active; ++w) mm = fmaxf(mm, s_m[w * 8 + hd]);
+      float sum = 0.f, l = 0.f;
+      for (int w = 0; w < active; ++w) {
+        const float f = ex2(s_m[w * 8 + hd] - mm);
+        sum = fmaf(so[(w * kHeadsPer + hd) * Shape::ostride + j], f * s_f[w], sum);
+        l = fmaf(s_l[w * 8 + hd], f, l);
+      }
+      parts.o[slot * kHeadsPer * D + i] = sum;
+      if (j == 0) parts.ml[slot * kHeadsPer + hd] = make_float2(mm, l);
+    }
+    __syncthreads();
+    u += u1 - u0;
+  }
 }
 
-template <class T>
-__global__ void __launch_bounds__(PQ_KV_MAX_D)
-join_kernel(const float* __restrict__ part_o, const float2* __restrict__ part_ml, int splits, int d,
-            const float* __restrict__ R, T* __restrict__ out, float* __restrict__ lse,
-            float* __restrict__ lse2) {
-  __shared__ float so[PQ_KV_MAX_D];
-  const int64_t row = blockIdx.x;
-  const int j = threadIdx.x;
-  float m = -INFINITY;
-  for (int s = 0; s < splits; ++s) m = fmaxf(m, part_ml[row * splits + s].x);
-  const float mm = m == -INFINITY ? 0.f : m;
-  float l = 0.f, o = 0.f;
-  for (int s = 0; s < splits; ++s) {
-    const float2 ml = part_ml[row * splits + s];
-    if (ml.y == 0.f) continue;
-    const float c = exp2f(ml.x - mm);
-    l = fmaf(ml.y, c, l);
-    if (j < d) o = fmaf(part_o[(row * splits + s) * d + j], c, o);
-  }
-  if (j < d) so[j] = l > 0.f ? o / l : (l == 0.f ? 0.f : l);
-  __syncthreads();
-  if (j == 0) {
-    const float l2 = l > 0.f ? mm + log2f(l) : (l == 0.f ? -INFINITY : l);
-    if (lse) lse[row] = l2 / kLog2e;
-    if (lse2) lse2[row] = l2;
-  }
-  if (j >= d) return;
-  float y = 0.f;
-  for (int i = 0; i < d; ++i) y = fmaf(so[i], R[i * d + j], y);
-  out[row * d + j] = from_f32<T>(y);
-}
-
+// One block per segment: its partials in order, 1 / sum, the values' scale,
+// and the rotation back.
+template <class T, int D>
 __global__ void __launch_bounds__(256)
-weights_kernel(const float* __restrict__ scores, const float* __restrict__ lse2, int heads,
-               int group, int pages, int page_size, const int32_t* __restrict__ table,
-               int64_t table_stride, int table_width, const int32_t* __restrict__ lengths,
-               int64_t width, float* __restrict__ weights) {
-  const int b = blockIdx.y / heads, h = blockIdx.y % heads;
-  const int len = clamp_length(lengths[b], table_width, page_size);
-  const int t = blockIdx.x * blockDim.x + threadIdx.x;
-  if (t >= len) return;
-  const int pg = table[b * table_stride + t / page_size];
-  if (pg < 0 || pg >= pages) return;
-  const int64_t row0 = ((int64_t)b * heads + h) * group;
-  float w = 0.f;
-  for (int g = 0; g < group; ++g) w += exp2f(scores[(row0 + g) * width + t] - lse2[row0 + g]);
-  atomicAdd(weights + ((int64_t)pg * heads + h) * page_size + t % page_size, w);
+kv_join_kernel(Parts parts, Work wk, int workers, int d, int page_size,
+               const float* __restrict__ R, const int* __restrict__ exponent, T* __restrict__ out,
+               float* __restrict__ lse, float* __restrict__ lse2) {
+  __shared__ float so[kHeadsPer][D], red[256 / D][kHeadsPer][D];
+  const int tid = threadIdx.x;
+  const int per = wk.heads * wk.blocks, seg = blockIdx.x;
+  const int b = seg / per, seg_in = seg % per, h = seg_in / wk.blocks, hb = seg_in % wk.blocks;
+  const int ng = min(kHeadsPer, wk.group - hb * kHeadsPer);
+  const int64_t row0 = ((int64_t)b * wk.heads + h) * wk.group + hb * kHeadsPer;
+  pdl_next();
+  pdl_wait();
+  const int len = clamp_length(wk.lengths[b], wk.table_width, page_size);
+  const int nu = wk.units_of(len), total = wk.first[wk.batch];
+  int w0 = 0, w1 = -1;
+  if (nu) {
+    const int n = min(workers, total);
+    const int64_t u0 = wk.first[b] + (int64_t)seg_in * nu;
+    w0 = worker_of(u0, n, total);
+    w1 = worker_of(u0 + nu - 1, n, total);
+  }
+  const float vscale = ldexpf(1.f, -*exponent);
+  for (int i = tid; i < ng * D; i += 256) {
+    const int hd = i / D;
+    float m = -FLT_MAX;
+    for (int w = w0; w <= w1; ++w)
+      m = fmaxf(m, parts.ml[((int64_t)w + seg) * kHeadsPer + hd].x);
+    float l = 0.f, x = 0.f;
+    for (int w = w0; w <= w1; ++w) {
+      const int64_t slot = (int64_t)w + seg;
+      const float2 ml = parts.ml[slot * kHeadsPer + hd];
+      const float f = ex2(ml.x - m);
+      l = fmaf(ml.y, f, l);
+      x = fmaf(parts.o[slot * kHeadsPer * D + i], f, x);
+    }
+    so[hd][i % D] = l == 0.f ? 0.f : x / l * vscale;
+    if (i % D == 0) {
+      const float l2 = l == 0.f ? -INFINITY : m + log2f(l);
+      if (lse) lse[row0 + hd] = l2 * kLn2;
+      if (lse2) lse2[row0 + hd] = l2;
+    }
+  }
+  __syncthreads();
+  constexpr int splits = 256 / D;
+  const int j = tid % D, part = tid / D;
+  float acc[kHeadsPer];
+#pragma unroll
+  for (int g = 0; g < kHeadsPer; ++g) acc[g] = 0.f;
+  if (j < d) {
+    const int i0 = d * part / splits, i1 = d * (part + 1) / splits;
+#pragma unroll 8
+    for (int i = i0; i < i1; ++i) {
+      const float r = __ldg(R + i * d + j);
+#pragma unroll
+      for (int g = 0; g < kHeadsPer; ++g) acc[g] = fmaf(so[g][i], r, acc[g]);
+    }
+  }
+#pragma unroll
+  for (int g = 0; g < kHeadsPer; ++g) red[part][g][j] = acc[g];
+  __syncthreads();
+  for (int i = tid; i < ng * D; i += 256) {
+    const int hd = i / D, jj = i % D;
+    if (jj >= d) continue;
+    float y = 0.f;
+#pragma unroll
+    for (int p = 0; p < splits; ++p) y += red[p][hd][jj];
+    out[(row0 + hd) * d + jj] = from_f32<T>(y);
+  }
 }
+
+// weights += sum over the key-value head's queries of 2^(score - lse2).
+__global__ void __launch_bounds__(256)
+kv_weights_kernel(const float* __restrict__ scores, const float* __restrict__ lse2, Work wk,
+                  int pages, int page_size, int64_t width, float* __restrict__ weights) {
+  const int64_t bh = blockIdx.y + (int64_t)blockIdx.z * gridDim.y;
+  if (bh >= (int64_t)wk.batch * wk.heads) return;
+  const int b = (int)(bh / wk.heads), h = (int)(bh % wk.heads);
+  pdl_wait();
+  const int len = clamp_length(wk.lengths[b], wk.table_width, page_size);
+  for (int t = blockIdx.x * blockDim.x + threadIdx.x; t < len; t += gridDim.x * blockDim.x) {
+    const int pg = wk.table[b * wk.table_stride + t / page_size];
+    if (pg < 0 || pg >= pages) continue;
+    const float* s = scores + (bh * width + t) * wk.group;
+    const float* l = lse2 + bh * wk.group;
+    float w = 0.f;
+    for (int g = 0; g < wk.group; ++g) w += ex2(s[g] - __ldg(l + g));
+    atomicAdd(weights + ((int64_t)pg * wk.heads + h) * page_size + t % page_size, w);
+  }
+}
+
+// ---------------------------------------------------------------------------
+// Host
+// ---------------------------------------------------------------------------
 
 struct AttendPlan {
-  int splits;
+  int D, blocks, segments, workers;
   int64_t rows, width;
   size_t bytes;
-  float *qrot, *part_o, *lse2, *scores;
-  float2* part_ml;
+  QueryOut q;
+  Parts parts;
+  int* first;
+  float *lse2, *scores;
 };
 
 inline AttendPlan attend_plan(const pq_kv_cache& c, int batch, int q_heads, int table_width,
                               int accumulate, void* ws, size_t ws_bytes) {
   AttendPlan p;
+  p.D = c.d <= 64 ? 64 : c.d <= 128 ? 128 : 256;
+  const int group = q_heads / c.heads;
+  p.blocks = (group + kHeadsPer - 1) / kHeadsPer;
   p.rows = (int64_t)batch * q_heads;
   p.width = (int64_t)table_width * c.page_size;
-  p.splits = (int)max((int64_t)1, (p.width + kSplit - 1) / kSplit);
+  const int64_t segments = (int64_t)batch * c.heads * p.blocks;
+  p.segments = (int)segments;
+  // Two blocks an SM where their shared memory allows it, never more than the
+  // units (of at least 128 tokens) that the table has room for.
+  const int64_t units = segments * ((p.width + 127) / 128);
+  p.workers = (int)max((int64_t)1, min(units, (int64_t)2 * num_sms()));
   Carve cv(ws, ws_bytes);
-  p.qrot = cv.take<float>(p.rows * c.d);
-  p.part_o = cv.take<float>(p.rows * p.splits * c.d);
-  p.part_ml = cv.take<float2>(p.rows * p.splits);
+  p.q.hi = cv.take<__half>(segments * kHeadsPer * p.D);
+  p.q.lo = cv.take<__half>(segments * kHeadsPer * p.D);
+  p.q.factor = cv.take<float>(segments * kHeadsPer);
+  p.first = cv.take<int>(batch + 1);
+  p.parts.o = cv.take<float>((segments + p.workers) * kHeadsPer * p.D);
+  p.parts.ml = cv.take<float2>((segments + p.workers) * kHeadsPer);
   p.lse2 = cv.take<float>(p.rows);
   p.scores = accumulate ? cv.take<float>(p.rows * p.width) : nullptr;
   p.bytes = cv.off;
   return p;
+}
+
+template <class... KArgs, class... Args>
+inline int launch_pdl(void (*kernel)(KArgs...), dim3 grid, int threads, size_t smem,
+                      cudaStream_t st, bool early, Args... args) {
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = grid;
+  cfg.blockDim = dim3(threads);
+  cfg.dynamicSmemBytes = smem;
+  cfg.stream = st;
+  cudaLaunchAttribute at;
+  at.id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  at.val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = &at;
+  cfg.numAttrs = early ? 1 : 0;
+  PQ_CUDA_TRY(cudaLaunchKernelEx(&cfg, kernel, KArgs(args)...));
+  PQ_LAUNCH_CHECK("kv attend");
+  return PQ_OK;
+}
+
+template <int D, int KB, int VB, int PREC>
+int launch_attend(const pq_kv_cache& c, Work wk, const AttendPlan& p, int workers,
+                  cudaStream_t st) {
+  using Shape = AttendShape<D, KB, VB, PREC>;
+  auto kern = kv_attend_kernel<D, KB, VB, PREC>;
+  PQ_CUDA_TRY(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                                   (int)Shape::smem));
+  return launch_pdl(kern, dim3(workers), 32 * kAttWarps, Shape::smem, st, true, side_k(c),
+                    side_v(c), c.d, c.pages, c.page_size, wk, p.q, p.parts, p.scores, p.width);
+}
+
+// Calls f with the kernel's template arguments.
+template <int D, int KB, int VB, class F>
+int with_prec(int prec, F f) {
+  switch (prec) {
+    case 0: return f.template operator()<D, KB, VB, 0>();
+    case 1: return f.template operator()<D, KB, VB, 1>();
+    case 2: return f.template operator()<D, KB, VB, 2>();
+    default: return f.template operator()<D, KB, VB, 3>();
+  }
+}
+template <int D, int KB, class F>
+int with_v(int vb, int prec, F f) {
+  return vb == 2 ? with_prec<D, KB, 2>(prec, f)
+                 : vb == 4 ? with_prec<D, KB, 4>(prec, f) : with_prec<D, KB, 8>(prec, f);
+}
+template <int D, class F>
+int with_k(int kb, int vb, int prec, F f) {
+  return kb == 2 ? with_v<D, 2>(vb, prec, f)
+                 : kb == 4 ? with_v<D, 4>(vb, prec, f) : with_v<D, 8>(vb, prec, f);
+}
+template <class F>
+int with_shape(int D, int kb, int vb, int prec, F f) {
+  return D == 64 ? with_k<64>(kb, vb, prec, f)
+                 : D == 128 ? with_k<128>(kb, vb, prec, f) : with_k<256>(kb, vb, prec, f);
+}
+
+struct UnitOf {
+  template <int D, int KB, int VB, int PREC>
+  int operator()() const {
+    return AttendShape<D, KB, VB, PREC>::unit;
+  }
+};
+struct CtasOf {
+  template <int D, int KB, int VB, int PREC>
+  int operator()() const {
+    return AttendShape<D, KB, VB, PREC>::ctas;
+  }
+};
+struct LaunchAttend {
+  const pq_kv_cache& c;
+  Work wk;
+  const AttendPlan& p;
+  int workers;
+  cudaStream_t st;
+  template <int D, int KB, int VB, int PREC>
+  int operator()() const {
+    return launch_attend<D, KB, VB, PREC>(c, wk, p, workers, st);
+  }
+};
+
+template <class T, int D>
+int launch_query(const pq_kv_cache& c, const void* q, int64_t sb, int64_t sh, float scale, Work wk,
+                 const AttendPlan& p, cudaStream_t st) {
+  const Codec k = codec_of(c.k_codec, c.d);
+  return launch_pdl(kv_query_kernel<T, D>, dim3(p.segments + 1), 256, 0, st, false, (const T*)q, sb,
+                    sh, c.d, c.page_size, k.RT, k.exponent, scale, wk, p.q, p.first);
+}
+
+template <class T, int D>
+int launch_join(const pq_kv_cache& c, Work wk, const AttendPlan& p, int workers, void* out,
+                float* lse, int accumulate, cudaStream_t st) {
+  const Codec v = codec_of(c.v_codec, c.d);
+  return launch_pdl(kv_join_kernel<T, D>, dim3(p.segments), 256, 0, st, true, p.parts, wk, workers,
+                    c.d, c.page_size, v.R, v.exponent, (T*)out, lse,
+                    accumulate ? p.lse2 : (float*)nullptr);
 }
 
 }  // namespace kv
@@ -224,7 +943,7 @@ extern "C" {
 
 size_t pq_kv_attend_workspace_bytes(const pq_kv_cache* cache, int batch, int q_heads,
                                     int table_width, int accumulate) {
-  if (!cache || batch <= 0 || q_heads <= 0 || table_width < 0) return 256;
+  if (!cache || batch <= 0 || q_heads <= 0 || table_width < 0 || cache->heads <= 0) return 256;
   return kv::attend_plan(*cache, batch, q_heads, table_width, accumulate, nullptr, 0).bytes;
 }
 
@@ -244,38 +963,54 @@ int pq_kv_attend(const pq_kv_cache* cache, const void* q, int dtype, int64_t q_s
   PQ_CHECK_ARG(isfinite(scale), "scale must be finite");
   if (batch == 0) return PQ_OK;
   PQ_CHECK_ARG(q && out, "null pointer argument");
-  PQ_CHECK_ARG((int64_t)batch * q_heads < 65536, "batch * q_heads must be below 65536");
+  const int64_t widest = ((int64_t)table_width * c.page_size + 127) / 128;
+  PQ_CHECK_ARG((int64_t)batch * q_heads < (1ll << 28) &&
+                   (int64_t)batch * q_heads * max(widest, (int64_t)1) < (1ll << 31),
+               "a call takes fewer than 2^28 query rows and 2^31 pieces of 128 tokens");
   const kv::AttendPlan p =
       kv::attend_plan(c, batch, q_heads, table_width, accumulate, ws, ws_bytes);
   if (!ws || ws_bytes < p.bytes)
     return fail(PQ_ERR_WORKSPACE, "pq_kv_attend needs %zu workspace bytes, got %zu", p.bytes,
                 ws_bytes);
   const cudaStream_t st = (cudaStream_t)stream;
-  const kv::Side sk = kv::side_k(c), sv = kv::side_v(c);
-  const int group = q_heads / c.heads;
+  const int prec = dtype == PQ_KV_F32 ? 3 : (lse || accumulate) ? 2 : dtype == PQ_KV_F16 ? 1 : 0;
+  kv::Work wk;
+  wk.table = table;
+  wk.table_stride = table_stride;
+  wk.table_width = table_width;
+  wk.lengths = lengths;
+  wk.batch = batch;
+  wk.heads = c.heads;
+  wk.group = q_heads / c.heads;
+  wk.blocks = p.blocks;
+  wk.first = p.first;
+  wk.unit = kv::with_shape(p.D, c.k_bits, c.v_bits, prec, kv::UnitOf{});
+  const int workers =
+      min(p.workers, num_sms() * kv::with_shape(p.D, c.k_bits, c.v_bits, prec, kv::CtasOf{}));
   PQ_KV_DISPATCH_T(dtype, {
-    kv::rotate_kernel<T_><<<(unsigned)p.rows, PQ_KV_MAX_D, 0, st>>>(
-        (const T_*)q, q_stride_b, q_stride_h, q_heads, c.d, sk.c.RT, scale, p.qrot);
+    rc = p.D == 64 ? kv::launch_query<T_, 64>(c, q, q_stride_b, q_stride_h, scale, wk, p, st)
+                   : p.D == 128
+                         ? kv::launch_query<T_, 128>(c, q, q_stride_b, q_stride_h, scale, wk, p, st)
+                         : kv::launch_query<T_, 256>(c, q, q_stride_b, q_stride_h, scale, wk, p, st);
   });
-  PQ_LAUNCH_CHECK("kv::rotate_kernel");
-  const size_t smem = sizeof(float) * ((size_t)kv::kHeadsPer * c.d + kv::kTile * (c.d + 1) +
-                                       kv::kHeadsPer * kv::kTile + 512);
-  const dim3 grid(p.splits, batch * c.heads, (group + kv::kHeadsPer - 1) / kv::kHeadsPer);
-  kv::attend_kernel<<<grid, 128, smem, st>>>(sk, sv, c.heads, group, c.d, c.pages, c.page_size,
-                                             p.qrot, table, table_stride, table_width, lengths,
-                                             p.splits, p.part_o, p.part_ml, p.scores, p.width);
-  PQ_LAUNCH_CHECK("kv::attend_kernel");
+  if (rc) return rc;
+  rc = kv::with_shape(p.D, c.k_bits, c.v_bits, prec, kv::LaunchAttend{c, wk, p, workers, st});
+  if (rc) return rc;
   PQ_KV_DISPATCH_T(dtype, {
-    kv::join_kernel<T_><<<(unsigned)p.rows, PQ_KV_MAX_D, 0, st>>>(
-        p.part_o, p.part_ml, p.splits, c.d, sv.c.R, (T_*)out, lse, p.lse2);
+    rc = p.D == 64 ? kv::launch_join<T_, 64>(c, wk, p, workers, out, lse, accumulate, st)
+                   : p.D == 128
+                         ? kv::launch_join<T_, 128>(c, wk, p, workers, out, lse, accumulate, st)
+                         : kv::launch_join<T_, 256>(c, wk, p, workers, out, lse, accumulate, st);
   });
-  PQ_LAUNCH_CHECK("kv::join_kernel");
+  if (rc) return rc;
   if (accumulate && p.width) {
-    const dim3 wg((unsigned)((p.width + 255) / 256), batch * c.heads);
-    kv::weights_kernel<<<wg, 256, 0, st>>>(p.scores, p.lse2, c.heads, group, c.pages, c.page_size,
-                                           table, table_stride, table_width, lengths, p.width,
-                                           c.weights);
-    PQ_LAUNCH_CHECK("kv::weights_kernel");
+    const int64_t bh = (int64_t)batch * c.heads;
+    const int gy = (int)min(bh, (int64_t)32768);
+    const int64_t gx = min((p.width + 255) / 256, max((int64_t)1, (int64_t)16 * num_sms() / bh));
+    rc = kv::launch_pdl(kv::kv_weights_kernel, dim3((unsigned)gx, gy, (unsigned)((bh + gy - 1) / gy)),
+                        256, 0, st, true, p.scores, p.lse2, wk, c.pages, c.page_size, p.width,
+                        c.weights);
+    if (rc) return rc;
   }
   return PQ_OK;
 }

@@ -9,7 +9,8 @@ namespace kv {
 __global__ void prepare_codec_kernel(const float* __restrict__ R, const float* __restrict__ bounds,
                                      const float* __restrict__ cent, int d, int bits,
                                      float* __restrict__ oR, float* __restrict__ oRT,
-                                     float* __restrict__ ob, float* __restrict__ oc) {
+                                     float* __restrict__ ob, float* __restrict__ oc,
+                                     uint32_t* __restrict__ pairs, int* __restrict__ exponent) {
   const int t = blockIdx.x * blockDim.x + threadIdx.x;
   for (int i = t; i < d * d; i += gridDim.x * blockDim.x) {
     const float v = R[i];
@@ -20,6 +21,37 @@ __global__ void prepare_codec_kernel(const float* __restrict__ R, const float* _
     ob[t] = t < (1 << bits) - 1 ? bounds[t] : INFINITY;
     oc[t] = t < (1 << bits) ? cent[t] : 0.f;
   }
+  if (blockIdx.x) return;
+  __shared__ uint32_t s_half[256];  // hi | lo << 16
+  __shared__ int s_mx;
+  if (threadIdx.x == 0) s_mx = 0;
+  __syncthreads();
+  const float c = threadIdx.x < (1 << bits) ? cent[threadIdx.x] : 0.f;
+  atomicMax(&s_mx, __float_as_int(fabsf(c)));  // ordered as the floats are
+  __syncthreads();
+  const float mx = __int_as_float(s_mx);
+  const int e = mx > 0.f ? max(-100, min(100, 13 - ilogbf(mx))) : 0;
+  const float x = ldexpf(c, e);
+  const __half hi = __float2half_rn(x), lo = __float2half_rn(x - __half2float(hi));
+  s_half[threadIdx.x] = __half_as_ushort(hi) | (uint32_t)__half_as_ushort(lo) << 16;
+  __syncthreads();
+  const int i = threadIdx.x;
+  uint32_t p0, p1;
+  if (bits == 4) {
+    const uint32_t a = s_half[i >> 4], b = s_half[i & 15];
+    p0 = __byte_perm(a, b, 0x5410);
+    p1 = __byte_perm(a, b, 0x7632);
+  } else if (bits == 8) {
+    p0 = s_half[i];
+    p1 = 0u;
+  } else {
+    p0 = p1 = 0u;
+    if (i < 4)  // byte i of the four 32-bit hi | lo words
+      for (int k = 0; k < 4; ++k) p0 |= ((s_half[k] >> (8 * i)) & 255u) << (8 * k);
+  }
+  pairs[i] = p0;
+  pairs[256 + i] = p1;
+  if (i == 0) *exponent = e;
 }
 
 // Append.  x -> norm = f32(sqrt(sum_f64 x^2)), u = x / max(norm, 1e-8) in f32,
@@ -136,7 +168,7 @@ int pq_kv_prepare_codec(const float* R, const float* boundaries, const float* ce
   const kv::Codec c = kv::codec_of(codec, d);
   kv::prepare_codec_kernel<<<64, 256, 0, (cudaStream_t)stream>>>(
       R, boundaries, centroids, d, bits, (float*)c.R, (float*)c.RT, (float*)c.bounds,
-      (float*)c.cent);
+      (float*)c.cent, (uint32_t*)c.pairs, (int*)c.exponent);
   PQ_LAUNCH_CHECK("prepare_codec_kernel");
   return PQ_OK;
 }

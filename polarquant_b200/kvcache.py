@@ -61,6 +61,8 @@ class KVCodec:
         self.centroids = to_device_f32(centroids, self.device)
         if not bool((self.boundaries[1:] >= self.boundaries[:-1]).all()):
             raise ValueError("boundaries must ascend")
+        if not bool(self.rotation.isfinite().all() & self.centroids.isfinite().all()):
+            raise ValueError("rotation and centroids must be finite")
         nbytes = _lib.query("pq_kv_codec_bytes", self.d, self.bits)
         self.tables = workspace(nbytes, self.device)
         with torch.cuda.device(self.device):
@@ -220,8 +222,8 @@ class KVCache:
             raise ValueError("table's last dimension must be contiguous")
         if batch > 1 and lengths.stride(0) != 1:
             raise ValueError("lengths must be contiguous")
-        if table.shape[1] * self.page_size >= 1 << 31:
-            raise ValueError("a sequence has fewer than 2^31 tokens")
+        if table.shape[1] * self.page_size > 1 << 30:
+            raise ValueError("a sequence has at most 2^30 tokens")
         return batch
 
     def _slots(self, slots) -> int:

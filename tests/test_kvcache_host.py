@@ -60,8 +60,9 @@ def test_abi_refuses_bad_arguments(lib):
         (lib.pq_kv_attend, (c, 16, 0, 1, 1, 0, 4, 4, 16, 1, 2, 1.0, 16, 0, 0, 16, big, None), b"null"),
         (lib.pq_kv_attend, (c, 16, 0, 1, 1, 16, 4, 4, 0, 1, 2, 1.0, 16, 0, 0, 16, big, None), b"null"),
         (lib.pq_kv_attend, (c, 16, 0, 1, 1, 16, 4, 4, 16, 1, 2, float("nan"), 16, 0, 0, 16, big, None), b"finite"),
-        (lib.pq_kv_attend, (c, 16, 0, 1, 1, 16, 4, -1, 16, 1, 2, 1.0, 16, 0, 0, 16, big, None), b"2^31"),
-        (lib.pq_kv_attend, (c, 16, 0, 1, 1, 16, 4, 1 << 27, 16, 1, 2, 1.0, 16, 0, 0, 16, big, None), b"2^31"),
+        (lib.pq_kv_attend, (c, 16, 0, 1, 1, 16, 4, -1, 16, 1, 2, 1.0, 16, 0, 0, 16, big, None), b"2^30"),
+        (lib.pq_kv_attend, (c, 16, 0, 1, 1, 16, 4, 1 << 27, 16, 1, 2, 1.0, 16, 0, 0, 16, big, None), b"2^30"),
+        (lib.pq_kv_attend, (c, 16, 0, 1, 1, 16, 4, 1 << 26, 16, 64, 32, 1.0, 16, 0, 0, 16, big, None), b"2^31"),
         (lib.pq_kv_evict, (c, 16, 4, 4, 16, 1, -1, 0, 0, 0, 0, 0, 0, 16, 16, big, None), b"budget"),
         (lib.pq_kv_evict, (c, 16, 4, 4, 16, 1, 5, -1, 0, 0, 0, 0, 0, 16, 16, big, None), b"recent"),
         (lib.pq_kv_evict, (c, 16, 4, 4, 16, 1, 5, 0, 0, 16, 0, 0, -1, 16, 16, big, None), b"prompt_width"),

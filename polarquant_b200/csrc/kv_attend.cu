@@ -56,9 +56,15 @@ namespace kv {
 
 constexpr int kHeadsPer = 8;    // query heads of one block: the width of an mma
 constexpr int kAttWarps = 8;
+constexpr int kMaxWorkers = 384;  // blocks of the attention kernel
 constexpr float kLog2e = 1.4426950408889634f;
 constexpr float kLn2 = 0.6931471805599453f;
-constexpr float kRescale = 8.f;  // the running maximum follows when exceeded by 2^8
+// Softmax weights relative to the running maximum reach 2^3 before that follows,
+// value norms 2^2 of their reference before it does, and their product is taken
+// times 2^10: at most 2^15 in f16, with 11 bits down to 2^-24 of the largest.
+constexpr float kRescale = 3.f;
+constexpr float kNormRoom = 4.f;
+constexpr float kWeightScale = 1024.f;
 
 __device__ __forceinline__ void pdl_wait() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
 __device__ __forceinline__ void pdl_next() {
@@ -95,35 +101,34 @@ __device__ __forceinline__ float ex2(float x) {
   return y;
 }
 
-// B bytes (2, 4, 8 or 16) of a row; streamed, so not kept in L1.  Zeros without `in`.
+// B bytes (2, 4, 8 or 16) of a row; streamed, so not kept in L1.
 template <int B>
-__device__ __forceinline__ void load_bytes(const uint8_t* p, bool in, uint32_t* w) {
-  if constexpr (B == 16) {
-    w[0] = w[1] = w[2] = w[3] = 0u;
-    if (in)
-      asm volatile("ld.global.L1::no_allocate.v4.b32 {%0,%1,%2,%3}, [%4];"
-                   : "=r"(w[0]), "=r"(w[1]), "=r"(w[2]), "=r"(w[3])
-                   : "l"(p));
-  } else if constexpr (B == 8) {
-    w[0] = w[1] = 0u;
-    if (in)
-      asm volatile("ld.global.L1::no_allocate.v2.b32 {%0,%1}, [%2];"
-                   : "=r"(w[0]), "=r"(w[1])
-                   : "l"(p));
-  } else if constexpr (B == 4) {
-    w[0] = 0u;
-    if (in) asm volatile("ld.global.L1::no_allocate.b32 %0, [%1];" : "=r"(w[0]) : "l"(p));
-  } else {
-    uint16_t h = 0;
-    if (in) asm volatile("ld.global.L1::no_allocate.b16 %0, [%1];" : "=h"(h) : "l"(p));
-    w[0] = h;
-  }
+__device__ __forceinline__ void load_bytes(const uint8_t* p, uint32_t* w) {
+  if constexpr (B == 16)
+    asm volatile("ld.global.L1::no_allocate.v4.b32 {%0,%1,%2,%3}, [%4];"
+                 : "=r"(w[0]), "=r"(w[1]), "=r"(w[2]), "=r"(w[3])
+                 : "l"(p));
+  else if constexpr (B == 8)
+    asm volatile("ld.global.L1::no_allocate.v2.b32 {%0,%1}, [%2];"
+                 : "=r"(w[0]), "=r"(w[1])
+                 : "l"(p));
+  else if constexpr (B == 4)
+    asm volatile("ld.global.L1::no_allocate.b32 %0, [%1];" : "=r"(w[0]) : "l"(p));
+  else
+    asm volatile("{\n\t.reg .b16 h;\n\tld.global.L1::no_allocate.b16 h, [%1];\n\tcvt.u32.u16 %0, h;\n\t}"
+                 : "=r"(w[0])
+                 : "l"(p));
 }
 
-__device__ __forceinline__ float load_norm(const float* p, bool in) {
-  float x = 0.f;
-  if (in) asm volatile("ld.global.L1::no_allocate.f32 %0, [%1];" : "=f"(x) : "l"(p));
+__device__ __forceinline__ float load_norm(const float* p) {
+  float x;
+  asm volatile("ld.global.L1::no_allocate.f32 %0, [%1];" : "=f"(x) : "l"(p));
   return x;
+}
+
+// Asks for `bytes` (a multiple of 16) at p to be brought into L2.
+__device__ __forceinline__ void prefetch_l2(const void* p, uint32_t bytes) {
+  asm volatile("cp.async.bulk.prefetch.L2.global [%0], %1;" ::"l"(p), "r"(bytes) : "memory");
 }
 
 // How a row of D coordinates is dealt to L lanes: lane i holds bytes
@@ -139,13 +144,20 @@ struct Deal {
   static __device__ __forceinline__ int dim(int lane, int n) {
     return (n / CU) * L * CU + lane * CU + n % CU;
   }
-  static __device__ __forceinline__ void load(const uint8_t* row, int64_t ldb, int lane, bool in,
-                                              uint32_t (&w)[words]) {
+  // The lane's place in a row.  A row shorter than D coordinates ends before
+  // some lanes' places: these read its start, as codes of coordinates that meet
+  // zeros in the queries and are dropped from the values.
+  static __device__ __forceinline__ void places(int ldb, int lane, int (&off)[units]) {
 #pragma unroll
     for (int u = 0; u < units; ++u) {
-      const int off = u * L * UB + lane * UB;
-      load_bytes<UB>(row + off, in && off < ldb, &w[u * UB / 4]);
+      off[u] = u * L * UB + lane * UB;
+      if (off[u] >= ldb) off[u] = 0;
     }
+  }
+  static __device__ __forceinline__ void load(const uint8_t* row, const int (&off)[units],
+                                              uint32_t (&w)[words]) {
+#pragma unroll
+    for (int u = 0; u < units; ++u) load_bytes<UB>(row + off[u], &w[u * UB / 4]);
   }
 };
 
@@ -277,20 +289,44 @@ struct QueryOut {
   float* factor;    // [segment][8]: score = factor * key norm * product, in log2
 };
 
+// Blocks that turn rows by a D x D matrix: kRotParts threads a column share its
+// products, so that few blocks have many loads of the matrix in flight (64 KB
+// from L2 at D = 128; one row of loads after another took 16 us).
+constexpr int kRotParts = 4;
+
+// acc[g] = sum over this thread's rows i of x[g][i] * M[i][j].
+template <int D>
+__device__ __forceinline__ void turn(const float (&x)[kHeadsPer][D], const float* __restrict__ M,
+                                     int d, int j, int part, float (&acc)[kHeadsPer]) {
+#pragma unroll
+  for (int g = 0; g < kHeadsPer; ++g) acc[g] = 0.f;
+  constexpr int rows = D / kRotParts, chunk = rows < 32 ? rows : 32;
+  for (int i0 = part * rows; i0 < (part + 1) * rows; i0 += chunk) {
+    float r[chunk];
+#pragma unroll
+    for (int i = 0; i < chunk; ++i) r[i] = i0 + i < d && j < d ? __ldg(M + (i0 + i) * d + j) : 0.f;
+#pragma unroll
+    for (int i = 0; i < chunk; ++i)
+#pragma unroll
+      for (int g = 0; g < kHeadsPer; ++g) acc[g] = fmaf(x[g][i0 + i], r[i], acc[g]);
+  }
+}
+
 template <class T, int D>
-__global__ void __launch_bounds__(256)
+__global__ void __launch_bounds__(kRotParts * D)
 kv_query_kernel(const T* __restrict__ q, int64_t sb, int64_t sh, int d, int page_size,
                 const float* __restrict__ RT, const int* __restrict__ exponent, float scale,
                 Work wk, QueryOut out, int* __restrict__ first) {
-  __shared__ float sq[kHeadsPer][D], red[256 / (D < 256 ? D : 256)][kHeadsPer][D];
-  __shared__ int s_part[8];
+  constexpr int threads = kRotParts * D, warps = threads / 32;
+  __shared__ float sq[kHeadsPer][D], red[kRotParts][kHeadsPer][D];
+  __shared__ int s_part[warps];
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   pdl_next();
   const int per = wk.heads * wk.blocks;
   if (blockIdx.x == wk.batch * per) {
     // First units: a running sum over the sequences.
     int base = 0;
-    for (int b0 = 0; b0 < wk.batch; b0 += 256) {
+    for (int b0 = 0; b0 < wk.batch; b0 += threads) {
       const int b = b0 + tid;
       const int n = b < wk.batch
                         ? per * wk.units_of(clamp_length(wk.lengths[b], wk.table_width, page_size))
@@ -304,8 +340,7 @@ kv_query_kernel(const T* __restrict__ q, int64_t sb, int64_t sh, int d, int page
       if (lane == 31) s_part[warp] = v;
       __syncthreads();
       int before = 0, all = 0;
-#pragma unroll
-      for (int i = 0; i < 8; ++i) {
+      for (int i = 0; i < warps; ++i) {
         if (i < warp) before += s_part[i];
         all += s_part[i];
       }
@@ -319,45 +354,34 @@ kv_query_kernel(const T* __restrict__ q, int64_t sb, int64_t sh, int d, int page
   const int b = blockIdx.x / per, h = blockIdx.x % per / wk.blocks, hb = blockIdx.x % wk.blocks;
   const int ng = min(kHeadsPer, wk.group - hb * kHeadsPer);
   const T* src = q + b * sb + ((int64_t)h * wk.group + hb * kHeadsPer) * sh;
-  for (int i = tid; i < kHeadsPer * D; i += 256) {
-    const int g = i / D, j = i % D;
-    sq[g][j] = g < ng && j < d ? to_f32<T>(src[g * sh + j]) : 0.f;
-  }
-  __syncthreads();
-  // Column j of R^T, rows split over 256 / D parts.
-  constexpr int parts = 256 / D;
   const int j = tid % D, part = tid / D;
+#pragma unroll
+  for (int g = part; g < kHeadsPer; g += kRotParts)
+    sq[g][j] = g < ng && j < d ? to_f32<T>(src[g * sh + j]) : 0.f;
+  __syncthreads();
   float acc[kHeadsPer];
-#pragma unroll
-  for (int g = 0; g < kHeadsPer; ++g) acc[g] = 0.f;
-  if (j < d) {
-    const int i0 = d * part / parts, i1 = d * (part + 1) / parts;
-#pragma unroll 8
-    for (int i = i0; i < i1; ++i) {
-      const float r = __ldg(RT + i * d + j);
-#pragma unroll
-      for (int g = 0; g < kHeadsPer; ++g) acc[g] = fmaf(sq[g][i], r, acc[g]);
-    }
-  }
+  turn<D>(sq, RT, d, j, part, acc);
 #pragma unroll
   for (int g = 0; g < kHeadsPer; ++g) red[part][g][j] = acc[g];
   __syncthreads();
   // A warp per head: scale to a largest of [2^13, 2^14) and split.
+  if (warp >= kHeadsPer) return;
   float y[D / 32], mx = 0.f;
 #pragma unroll
   for (int i = 0; i < D / 32; ++i) {
     y[i] = 0.f;
 #pragma unroll
-    for (int p = 0; p < parts; ++p) y[i] += red[p][warp][lane + 32 * i];
+    for (int p = 0; p < kRotParts; ++p) y[i] += red[p][warp][lane + 32 * i];
     mx = fmaxf(mx, fabsf(y[i]));
   }
 #pragma unroll
   for (int o = 16; o > 0; o >>= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, o));
   const int e = mx > 0.f && mx < INFINITY ? max(-100, min(100, 13 - ilogbf(mx))) : 0;
   const int64_t row = (int64_t)blockIdx.x * kHeadsPer + warp;
+  const float up = ldexpf(1.f, e);
 #pragma unroll
   for (int i = 0; i < D / 32; ++i) {
-    const float v = ldexpf(y[i], e);
+    const float v = y[i] * up;
     const __half hi = __float2half_rn(v);
     out.hi[row * D + lane + 32 * i] = hi;
     out.lo[row * D + lane + 32 * i] = __float2half_rn(v - __half2float(hi));
@@ -387,8 +411,8 @@ struct AttendShape {
 
 template <int D, int KB, int VB, int PREC>
 __global__ void __launch_bounds__(32 * kAttWarps, AttendShape<D, KB, VB, PREC>::ctas)
-kv_attend_kernel(Side sk, Side sv, int d, int pages, int page_size, Work wk, QueryOut qo,
-                 Parts parts, float* __restrict__ scores, int64_t score_width) {
+kv_attend_kernel(Side sk, Side sv, int pages, int page_shift, Work wk, QueryOut qo, Parts parts,
+                 float* __restrict__ scores, int64_t score_width) {
   using Shape = AttendShape<D, KB, VB, PREC>;
   constexpr int MT = Shape::MT;
   constexpr bool QLO = PREC >= 1, KLO = PREC >= 2, VLO = PREC >= 3;
@@ -430,6 +454,10 @@ kv_attend_kernel(Side sk, Side sv, int d, int pages, int page_size, Work wk, Que
     vreg[i] = VB == 2 ? sv.c.pairs[i] : 0u;
   }
   const uint32_t koff = lane * 4, voff = 128 + lane * 4;
+  const int kld = (int)sk.ldb, vld = (int)sv.ldb;
+  int kplace[KD::units], vplace[VD::units];
+  KD::places(kld, t, kplace);
+  VD::places(vld, g, vplace);
   pdl_wait();
 
   const int per = wk.heads * wk.blocks;
@@ -446,7 +474,7 @@ kv_attend_kernel(Side sk, Side sv, int d, int pages, int page_size, Work wk, Que
   while (u < uend) {
     // The segment of unit u and this block's share of it.
     while (u >= wk.first[b + 1]) ++b;
-    const int len = clamp_length(wk.lengths[b], wk.table_width, page_size);
+    const int len = clamp_length(wk.lengths[b], wk.table_width, 1 << page_shift);
     const int nu = wk.units_of(len);
     const int r = (int)(u - wk.first[b]), seg_in = r / nu, u0 = r % nu;
     const int u1 = (int)min((int64_t)nu, u0 + (uend - u));
@@ -484,52 +512,62 @@ kv_attend_kernel(Side sk, Side sv, int d, int pages, int page_size, Work wk, Que
 #pragma unroll
     for (int m = 0; m < KS; ++m) o[m][0] = o[m][1] = o[m][2] = o[m][3] = 0.f;
     float m0 = -FLT_MAX, m1 = -FLT_MAX, l0 = 0.f, l1 = 0.f;
-    float vinv = 0.f, vlim = 0.f, vref = 0.f;  // value norms are taken times vinv = 1 / vref
+    float vinv = 0.f, vlim = 0.f, vref = 0.f;  // value norms are taken times vinv = 2^10 / vref
 
     uint32_t kw[MT][2][KD::words], vw[MT][4][VD::words];
     float kn[MT][2], vn[MT][2];
-    int pid[MT], pid_next[MT];
-    // Page of 16-token group i of the step at token `base`; -1 behind the end.
+    int pid[MT], pid1[MT], pid2[MT];  // pages of this step's groups and of the next ones
+    // Page of 16-token group i of the step at token `base`; -1 for none.
     auto page_of = [&](int base, int i) {
       const int tok = base + 16 * i;
       int p = -1;
       if (tok < t1) {
-        p = __ldg(trow + tok / page_size);
+        p = __ldg(trow + (tok >> page_shift));
         if (p >= pages) p = -1;
       }
       return p;
     };
-    // First row of the group, and which of its rows are tokens.
+    // First row of the group.  Groups without a page read page 0: what tokens
+    // that are not there decode to is finite, and meets a weight of 0.
     auto row_of = [&](int p, int base, int i) {
-      return ((int64_t)p * wk.heads + h) * page_size + ((base + 16 * i) & (page_size - 1));
+      return (((int64_t)max(p, 0) * wk.heads + h) << page_shift) +
+             ((base + 16 * i) & ((1 << page_shift) - 1));
     };
     auto load_keys = [&](int base) {
 #pragma unroll
       for (int i = 0; i < MT; ++i) {
-        const int64_t row = row_of(pid[i], base, i);
-#pragma unroll
-        for (int e = 0; e < 2; ++e) {
-          const int x = g + 8 * e;
-          const bool in = pid[i] >= 0 && base + 16 * i + x < t1;
-          KD::load(sk.rows + (row + x) * sk.ldb, sk.ldb, t, in, kw[i][e]);
-          kn[i][e] = load_norm(sk.norms + row + x, in);
-        }
+        const int64_t row = row_of(pid[i], base, i) + g;
+        const uint8_t* p = sk.rows + row * kld;
+        KD::load(p, kplace, kw[i][0]);
+        KD::load(p + 8 * kld, kplace, kw[i][1]);
+        kn[i][0] = load_norm(sk.norms + row);
+        kn[i][1] = load_norm(sk.norms + row + 8);
       }
     };
     auto load_values = [&](int base) {
 #pragma unroll
       for (int i = 0; i < MT; ++i) {
         const int64_t row = row_of(pid[i], base, i);
-#pragma unroll
-        for (int e = 0; e < 4; ++e) {
-          const int x = 2 * t + (e & 1) + 8 * (e >> 1);
-          const bool in = pid[i] >= 0 && base + 16 * i + x < t1;
-          VD::load(sv.rows + (row + x) * sv.ldb, sv.ldb, g, in, vw[i][e]);
-        }
-#pragma unroll
-        for (int e = 0; e < 2; ++e) {
-          const int x = g + 8 * e;
-          vn[i][e] = load_norm(sv.norms + row + x, pid[i] >= 0 && base + 16 * i + x < t1);
+        const uint8_t* p = sv.rows + (row + 2 * t) * vld;
+        VD::load(p, vplace, vw[i][0]);
+        VD::load(p + vld, vplace, vw[i][1]);
+        VD::load(p + 8 * vld, vplace, vw[i][2]);
+        VD::load(p + 9 * vld, vplace, vw[i][3]);
+        vn[i][0] = load_norm(sv.norms + row + g);
+        vn[i][1] = load_norm(sv.norms + row + g + 8);
+      }
+    };
+    auto prefetch = [&](const int (&p)[MT], int base) {
+      if (lane < 2 * MT) {
+        const int i = lane >> 1;
+        int pg = p[0];
+        if (MT > 1 && i) pg = p[MT - 1];
+        if (pg >= 0) {
+          const int64_t row = row_of(pg, base, i);
+          if (lane & 1)
+            prefetch_l2(sv.rows + row * vld, 16 * vld);
+          else
+            prefetch_l2(sk.rows + row * kld, 16 * kld);
         }
       }
     };
@@ -539,11 +577,13 @@ kv_attend_kernel(Side sk, Side sv, int d, int pages, int page_size, Work wk, Que
 #pragma unroll
     for (int i = 0; i < MT; ++i) {
       pid[i] = page_of(base, i);
-      pid_next[i] = page_of(base + stride, i);
+      pid1[i] = page_of(base + stride, i);
+      pid2[i] = page_of(base + 2 * stride, i);
     }
     if (base < t1) {
       load_keys(base);
       load_values(base);
+      prefetch(pid1, base + stride);
     }
     for (; base < t1; base += stride) {
       // Scores: S^T, tokens g and g + 8, heads 2t and 2t + 1.
@@ -561,40 +601,60 @@ kv_attend_kernel(Side sk, Side sv, int d, int pages, int page_size, Work wk, Que
           if constexpr (KLO) mma16816(s[i], c0, c1, c2, c3, qh[k][0], qh[k][1]);
         }
       }
+      bool there = base + 16 * MT <= t1;
+#pragma unroll
+      for (int i = 0; i < MT; ++i) there = there && pid[i] >= 0;
       float mx0 = -FLT_MAX, mx1 = -FLT_MAX, vmx = 0.f;
 #pragma unroll
       for (int i = 0; i < MT; ++i)
 #pragma unroll
         for (int e = 0; e < 2; ++e) {
-          const int tok = base + 16 * i + g + 8 * e;
-          const bool in = pid[i] >= 0 && tok < t1;
-          float& x = s[i][2 * e];
-          float& y = s[i][2 * e + 1];
-          x = in ? x * (kn[i][e] * f0) : -INFINITY;
-          y = in ? y * (kn[i][e] * f1) : -INFINITY;
-          if (PREC >= 2 && scores && tok < t1) {
-            float* to = scores + (((int64_t)b * wk.heads + h) * score_width + tok) * wk.group +
-                        hb * kHeadsPer + 2 * t;
-            if (hb * kHeadsPer + 2 * t < wk.group) to[0] = x;
-            if (hb * kHeadsPer + 2 * t + 1 < wk.group) to[1] = y;
+          s[i][2 * e] *= kn[i][e] * f0;
+          s[i][2 * e + 1] *= kn[i][e] * f1;
+        }
+      if (!there) {
+#pragma unroll
+        for (int i = 0; i < MT; ++i)
+#pragma unroll
+          for (int e = 0; e < 2; ++e)
+            if (pid[i] < 0 || base + 16 * i + g + 8 * e >= t1) {
+              s[i][2 * e] = s[i][2 * e + 1] = -INFINITY;
+              vn[i][e] = 0.f;
+            }
+      }
+      float vnow[MT][2];
+#pragma unroll
+      for (int i = 0; i < MT; ++i)
+#pragma unroll
+        for (int e = 0; e < 2; ++e) {
+          const float x = s[i][2 * e], y = s[i][2 * e + 1];
+          if (PREC >= 2 && scores) {
+            const int tok = base + 16 * i + g + 8 * e;
+            if (tok < t1) {
+              float* to = scores + (((int64_t)b * wk.heads + h) * score_width + tok) * wk.group +
+                          hb * kHeadsPer + 2 * t;
+              if (hb * kHeadsPer + 2 * t < wk.group) to[0] = x;
+              if (hb * kHeadsPer + 2 * t + 1 < wk.group) to[1] = y;
+            }
           }
           mx0 = fmaxf(mx0, x);
           mx1 = fmaxf(mx1, y);
           vmx = fmaxf(vmx, vn[i][e]);
+          vnow[i][e] = vn[i][e];
         }
-      float vnow[MT][2];
+      // The next step's keys, and into L2 what the one after it reads.
 #pragma unroll
       for (int i = 0; i < MT; ++i) {
-        vnow[i][0] = vn[i][0];
-        vnow[i][1] = vn[i][1];
+        pid[i] = pid1[i];
+        pid1[i] = pid2[i];
       }
-      // The next step's keys.
-#pragma unroll
-      for (int i = 0; i < MT; ++i) pid[i] = pid_next[i];
       const bool more = base + stride < t1;
-      if (more) load_keys(base + stride);
+      if (more) {
+        load_keys(base + stride);
+        prefetch(pid1, base + 2 * stride);
+      }
 #pragma unroll
-      for (int i = 0; i < MT; ++i) pid_next[i] = page_of(base + 2 * stride, i);
+      for (int i = 0; i < MT; ++i) pid2[i] = page_of(base + 3 * stride, i);
 
       if (__any_sync(0xffffffffu, mx0 > m0 + kRescale || mx1 > m1 + kRescale || vmx > vlim)) {
 #pragma unroll
@@ -616,8 +676,8 @@ kv_attend_kernel(Side sk, Side sv, int d, int pages, int page_size, Work wk, Que
           e0 *= vref / now;
           e1 *= vref / now;
           vref = now;
-          vinv = 1.f / now;
-          vlim = 16.f * now;
+          vinv = kWeightScale / now;
+          vlim = kNormRoom * now;
         }
 #pragma unroll
         for (int m = 0; m < KS; ++m) {
@@ -707,74 +767,89 @@ kv_attend_kernel(Side sk, Side sv, int d, int pages, int page_size, Work wk, Que
 // One block per segment: its partials in order, 1 / sum, the values' scale,
 // and the rotation back.
 template <class T, int D>
-__global__ void __launch_bounds__(256)
+__global__ void __launch_bounds__(kRotParts * D)
 kv_join_kernel(Parts parts, Work wk, int workers, int d, int page_size,
                const float* __restrict__ R, const int* __restrict__ exponent, T* __restrict__ out,
                float* __restrict__ lse, float* __restrict__ lse2) {
-  __shared__ float so[kHeadsPer][D], red[256 / D][kHeadsPer][D];
-  const int tid = threadIdx.x;
+  __shared__ float so[kHeadsPer][D], s_l[kHeadsPer];
+  // The partials' factors [worker][head], then the parts' sums [part][head][D].
+  constexpr int room = kRotParts > kMaxWorkers / D ? kRotParts : kMaxWorkers / D;
+  __shared__ float red[room][kHeadsPer][D];
+  float* fac = &red[0][0][0];
+  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, j = tid % D, part = tid / D;
   const int per = wk.heads * wk.blocks, seg = blockIdx.x;
   const int b = seg / per, seg_in = seg % per, h = seg_in / wk.blocks, hb = seg_in % wk.blocks;
   const int ng = min(kHeadsPer, wk.group - hb * kHeadsPer);
   const int64_t row0 = ((int64_t)b * wk.heads + h) * wk.group + hb * kHeadsPer;
+  const float vscale = ldexpf(1.f / kWeightScale, -*exponent);
   pdl_next();
   pdl_wait();
   const int len = clamp_length(wk.lengths[b], wk.table_width, page_size);
   const int nu = wk.units_of(len), total = wk.first[wk.batch];
-  int w0 = 0, w1 = -1;
+  int w0 = 0, nw = 0;
   if (nu) {
     const int n = min(workers, total);
     const int64_t u0 = wk.first[b] + (int64_t)seg_in * nu;
     w0 = worker_of(u0, n, total);
-    w1 = worker_of(u0 + nu - 1, n, total);
+    nw = worker_of(u0 + nu - 1, n, total) - w0 + 1;
   }
-  const float vscale = ldexpf(1.f, -*exponent);
-  for (int i = tid; i < ng * D; i += 256) {
-    const int hd = i / D;
-    float m = -FLT_MAX;
-    for (int w = w0; w <= w1; ++w)
-      m = fmaxf(m, parts.ml[((int64_t)w + seg) * kHeadsPer + hd].x);
-    float l = 0.f, x = 0.f;
-    for (int w = w0; w <= w1; ++w) {
-      const int64_t slot = (int64_t)w + seg;
-      const float2 ml = parts.ml[slot * kHeadsPer + hd];
+  const int64_t slot0 = (int64_t)w0 + seg;
+  if (warp < kHeadsPer) {
+    float m = -FLT_MAX, l = 0.f;
+    for (int w = lane; w < nw; w += 32)
+      m = fmaxf(m, parts.ml[(slot0 + w) * kHeadsPer + warp].x);
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
+    for (int w = lane; w < nw; w += 32) {
+      const float2 ml = parts.ml[(slot0 + w) * kHeadsPer + warp];
       const float f = ex2(ml.x - m);
       l = fmaf(ml.y, f, l);
-      x = fmaf(parts.o[slot * kHeadsPer * D + i], f, x);
+      fac[w * kHeadsPer + warp] = f;
     }
-    so[hd][i % D] = l == 0.f ? 0.f : x / l * vscale;
-    if (i % D == 0) {
-      const float l2 = l == 0.f ? -INFINITY : m + log2f(l);
-      if (lse) lse[row0 + hd] = l2 * kLn2;
-      if (lse2) lse2[row0 + hd] = l2;
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) l += __shfl_xor_sync(0xffffffffu, l, o);
+    if (lane == 0) {
+      s_l[warp] = l;
+      if (warp < ng) {
+        const float l2 = l == 0.f ? -INFINITY : m + log2f(l);
+        if (lse) lse[row0 + warp] = l2 * kLn2;
+        if (lse2) lse2[row0 + warp] = l2;
+      }
     }
   }
   __syncthreads();
-  constexpr int splits = 256 / D;
-  const int j = tid % D, part = tid / D;
   float acc[kHeadsPer];
 #pragma unroll
   for (int g = 0; g < kHeadsPer; ++g) acc[g] = 0.f;
-  if (j < d) {
-    const int i0 = d * part / splits, i1 = d * (part + 1) / splits;
-#pragma unroll 8
-    for (int i = i0; i < i1; ++i) {
-      const float r = __ldg(R + i * d + j);
+#pragma unroll 4
+  for (int w = part; w < nw; w += kRotParts) {
+    const float* o = parts.o + (slot0 + w) * kHeadsPer * D + j;
 #pragma unroll
-      for (int g = 0; g < kHeadsPer; ++g) acc[g] = fmaf(so[g][i], r, acc[g]);
-    }
+    for (int g = 0; g < kHeadsPer; ++g)
+      if (g < ng) acc[g] = fmaf(o[g * D], fac[w * kHeadsPer + g], acc[g]);
   }
+  __syncthreads();
 #pragma unroll
   for (int g = 0; g < kHeadsPer; ++g) red[part][g][j] = acc[g];
   __syncthreads();
-  for (int i = tid; i < ng * D; i += 256) {
-    const int hd = i / D, jj = i % D;
-    if (jj >= d) continue;
-    float y = 0.f;
+  for (int g = part; g < kHeadsPer; g += kRotParts) {
+    float x = 0.f;
 #pragma unroll
-    for (int p = 0; p < splits; ++p) y += red[p][hd][jj];
-    out[(row0 + hd) * d + jj] = from_f32<T>(y);
+    for (int p = 0; p < kRotParts; ++p) x += red[p][g][j];
+    so[g][j] = g >= ng || s_l[g] == 0.f ? 0.f : x / s_l[g] * vscale;
   }
+  __syncthreads();
+  turn<D>(so, R, d, j, part, acc);
+#pragma unroll
+  for (int g = 0; g < kHeadsPer; ++g) red[part][g][j] = acc[g];
+  __syncthreads();
+  if (j < d)
+    for (int g = part; g < ng; g += kRotParts) {
+      float y = 0.f;
+#pragma unroll
+      for (int p = 0; p < kRotParts; ++p) y += red[p][g][j];
+      out[(row0 + g) * d + j] = from_f32<T>(y);
+    }
 }
 
 // weights += sum over the key-value head's queries of 2^(score - lse2).
@@ -824,7 +899,7 @@ inline AttendPlan attend_plan(const pq_kv_cache& c, int batch, int q_heads, int 
   // Two blocks an SM where their shared memory allows it, never more than the
   // units (of at least 128 tokens) that the table has room for.
   const int64_t units = segments * ((p.width + 127) / 128);
-  p.workers = (int)max((int64_t)1, min(units, (int64_t)2 * num_sms()));
+  p.workers = (int)max((int64_t)1, min(units, (int64_t)min(2 * num_sms(), kMaxWorkers)));
   Carve cv(ws, ws_bytes);
   p.q.hi = cv.take<__half>(segments * kHeadsPer * p.D);
   p.q.lo = cv.take<__half>(segments * kHeadsPer * p.D);
@@ -861,10 +936,12 @@ int launch_attend(const pq_kv_cache& c, Work wk, const AttendPlan& p, int worker
                   cudaStream_t st) {
   using Shape = AttendShape<D, KB, VB, PREC>;
   auto kern = kv_attend_kernel<D, KB, VB, PREC>;
+  int page_shift = 4;
+  while ((1 << page_shift) < c.page_size) ++page_shift;
   PQ_CUDA_TRY(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize,
                                    (int)Shape::smem));
   return launch_pdl(kern, dim3(workers), 32 * kAttWarps, Shape::smem, st, true, side_k(c),
-                    side_v(c), c.d, c.pages, c.page_size, wk, p.q, p.parts, p.scores, p.width);
+                    side_v(c), c.pages, page_shift, wk, p.q, p.parts, p.scores, p.width);
 }
 
 // Calls f with the kernel's template arguments.
@@ -921,7 +998,7 @@ template <class T, int D>
 int launch_query(const pq_kv_cache& c, const void* q, int64_t sb, int64_t sh, float scale, Work wk,
                  const AttendPlan& p, cudaStream_t st) {
   const Codec k = codec_of(c.k_codec, c.d);
-  return launch_pdl(kv_query_kernel<T, D>, dim3(p.segments + 1), 256, 0, st, false, (const T*)q, sb,
+  return launch_pdl(kv_query_kernel<T, D>, dim3(p.segments + 1), kRotParts * D, 0, st, false, (const T*)q, sb,
                     sh, c.d, c.page_size, k.RT, k.exponent, scale, wk, p.q, p.first);
 }
 
@@ -929,7 +1006,7 @@ template <class T, int D>
 int launch_join(const pq_kv_cache& c, Work wk, const AttendPlan& p, int workers, void* out,
                 float* lse, int accumulate, cudaStream_t st) {
   const Codec v = codec_of(c.v_codec, c.d);
-  return launch_pdl(kv_join_kernel<T, D>, dim3(p.segments), 256, 0, st, true, p.parts, wk, workers,
+  return launch_pdl(kv_join_kernel<T, D>, dim3(p.segments), kRotParts * D, 0, st, true, p.parts, wk, workers,
                     c.d, c.page_size, v.R, v.exponent, (T*)out, lse,
                     accumulate ? p.lse2 : (float*)nullptr);
 }
@@ -977,7 +1054,7 @@ int pq_kv_attend(const pq_kv_cache* cache, const void* q, int dtype, int64_t q_s
   kv::Work wk;
   wk.table = table;
   wk.table_stride = table_stride;
-  wk.table_width = table_width;
+  wk.table_width = c.pages ? table_width : 0;  // without a pool every sequence is empty
   wk.lengths = lengths;
   wk.batch = batch;
   wk.heads = c.heads;

@@ -66,18 +66,20 @@ inline int check_cache(const pq_kv_cache* c) {
                    (c->page_size & (c->page_size - 1)) == 0,
                "page_size must be a power of two from 16 to 1024 (got %d)", c->page_size);
   PQ_CHECK_ARG((int64_t)c->pages * c->page_size < (1ll << 31) &&
+                   (int64_t)c->pages * c->heads * c->page_size < (1ll << 32) &&
                    (int64_t)c->pages * c->heads < (1ll << 31),
-               "a pool has fewer than 2^31 slots");
-  PQ_CHECK_ARG(c->k_ldb % 16 == 0 && c->k_ldb >= row_bytes(c->d, c->k_bits) &&
-                   c->v_ldb % 16 == 0 && c->v_ldb >= row_bytes(c->d, c->v_bits),
-               "k_ldb and v_ldb must be multiples of 16 that hold a row (got %lld and %lld)",
+               "a pool has fewer than 2^31 slots and 2^32 rows");
+  PQ_CHECK_ARG(c->k_ldb == (int64_t)align_up(row_bytes(c->d, c->k_bits), 16) &&
+                   c->v_ldb == (int64_t)align_up(row_bytes(c->d, c->v_bits), 16),
+               "k_ldb and v_ldb must be a row's packed bytes rounded up to 16 (got %lld and %lld)",
                (long long)c->k_ldb, (long long)c->v_ldb);
   PQ_CHECK_ARG(c->k_codec && c->v_codec, "null codec");
   PQ_CHECK_ARG(c->pages == 0 || (c->k_rows && c->v_rows && c->k_norms && c->v_norms &&
                                  c->positions && c->weights),
                "null pool pointer");
-  PQ_CHECK_ARG(((uintptr_t)c->k_rows | (uintptr_t)c->v_rows) % 16 == 0,
-               "rows must be 16-byte aligned");
+  PQ_CHECK_ARG(((uintptr_t)c->k_rows | (uintptr_t)c->v_rows | (uintptr_t)c->k_norms |
+                (uintptr_t)c->v_norms | (uintptr_t)c->positions | (uintptr_t)c->weights) % 16 == 0,
+               "the pool's arrays must be 16-byte aligned");
   return PQ_OK;
 }
 

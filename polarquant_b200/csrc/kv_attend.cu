@@ -29,9 +29,8 @@
 // is free as long as the queries have the same one.  A packed byte is decoded
 // by one shared-memory lookup that gives both of its centroids as an f16 pair
 // (4 bits; at 8 bits one centroid as f16 hi + lo), from a table with a copy for
-// each lane, 256 bytes per entry with keys in the lower and values in the
-// upper half: no bank conflicts, and the address is a single byte permute.  2
-// bits are decoded by byte permutes on a table of four in registers.
+// each lane: no bank conflicts, and the address is one dp4a.  2 bits are
+// decoded by byte permutes on a table of four in registers.
 //
 // What bounds it: at 4 bits and d = 128 a token and head is 136 bytes, 128
 // lookups of the 32 a cycle that an SM's shared memory gives, 160 byte
@@ -55,8 +54,8 @@ namespace pqb {
 namespace kv {
 
 constexpr int kHeadsPer = 8;    // query heads of one block: the width of an mma
-constexpr int kAttWarps = 8;
 constexpr int kMaxWorkers = 384;  // blocks of the attention kernel
+constexpr int kLeastUnit = 64;   // tokens of the smallest unit of any shape
 constexpr float kLog2e = 1.4426950408889634f;
 constexpr float kLn2 = 0.6931471805599453f;
 // Softmax weights relative to the running maximum reach 2^3 before that follows,
@@ -101,41 +100,46 @@ __device__ __forceinline__ float ex2(float x) {
   return y;
 }
 
-// B bytes (2, 4, 8 or 16) of a row; streamed, so not kept in L1.
+// B bytes (2, 4, 8 or 16) at a shared-memory address.
 template <int B>
-__device__ __forceinline__ void load_bytes(const uint8_t* p, uint32_t* w) {
+__device__ __forceinline__ void shared_bytes(uint32_t at, uint32_t* w) {
   if constexpr (B == 16)
-    asm volatile("ld.global.L1::no_allocate.v4.b32 {%0,%1,%2,%3}, [%4];"
+    asm volatile("ld.shared.v4.b32 {%0,%1,%2,%3}, [%4];"
                  : "=r"(w[0]), "=r"(w[1]), "=r"(w[2]), "=r"(w[3])
-                 : "l"(p));
+                 : "r"(at));
   else if constexpr (B == 8)
-    asm volatile("ld.global.L1::no_allocate.v2.b32 {%0,%1}, [%2];"
-                 : "=r"(w[0]), "=r"(w[1])
-                 : "l"(p));
+    asm volatile("ld.shared.v2.b32 {%0,%1}, [%2];" : "=r"(w[0]), "=r"(w[1]) : "r"(at));
   else if constexpr (B == 4)
-    asm volatile("ld.global.L1::no_allocate.b32 %0, [%1];" : "=r"(w[0]) : "l"(p));
+    asm volatile("ld.shared.b32 %0, [%1];" : "=r"(w[0]) : "r"(at));
   else
-    asm volatile("{\n\t.reg .b16 h;\n\tld.global.L1::no_allocate.b16 h, [%1];\n\tcvt.u32.u16 %0, h;\n\t}"
+    asm volatile("{\n\t.reg .b16 h;\n\tld.shared.b16 h, [%1];\n\tcvt.u32.u16 %0, h;\n\t}"
                  : "=r"(w[0])
-                 : "l"(p));
+                 : "r"(at));
 }
 
-__device__ __forceinline__ float load_norm(const float* p) {
+__device__ __forceinline__ float shared_float(uint32_t at) {
   float x;
-  asm volatile("ld.global.L1::no_allocate.f32 %0, [%1];" : "=f"(x) : "l"(p));
+  asm volatile("ld.shared.f32 %0, [%1];" : "=f"(x) : "r"(at));
   return x;
 }
 
-// Asks for `bytes` (a multiple of 16) at p to be brought into L2.
-__device__ __forceinline__ void prefetch_l2(const void* p, uint32_t bytes) {
-  asm volatile("cp.async.bulk.prefetch.L2.global [%0], %1;" ::"l"(p), "r"(bytes) : "memory");
+__device__ __forceinline__ void copy16(uint32_t to, const void* from) {
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(to), "l"(from) : "memory");
+}
+__device__ __forceinline__ void copy_commit() {
+  asm volatile("cp.async.commit_group;" ::: "memory");
+}
+template <int N>
+__device__ __forceinline__ void copy_wait() {
+  asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory");
 }
 
 // How a row of D coordinates is dealt to L lanes: lane i holds bytes
 // [u * L * UB + i * UB, + UB) of it for each unit u, CU codes a unit.
 template <int D, int BITS, int L>
 struct Deal {
-  static constexpr int bytes = D * BITS / 8 / L;
+  static constexpr int row = D * BITS / 8;  // bytes of a row of D coordinates
+  static constexpr int bytes = row / L;
   static constexpr int UB = bytes < 16 ? bytes : 16;
   static constexpr int units = bytes / UB;
   static constexpr int words = (bytes + 3) / 4;
@@ -144,53 +148,57 @@ struct Deal {
   static __device__ __forceinline__ int dim(int lane, int n) {
     return (n / CU) * L * CU + lane * CU + n % CU;
   }
-  // The lane's place in a row.  A row shorter than D coordinates ends before
-  // some lanes' places: these read its start, as codes of coordinates that meet
-  // zeros in the queries and are dropped from the values.
-  static __device__ __forceinline__ void places(int ldb, int lane, int (&off)[units]) {
-#pragma unroll
-    for (int u = 0; u < units; ++u) {
-      off[u] = u * L * UB + lane * UB;
-      if (off[u] >= ldb) off[u] = 0;
-    }
-  }
-  static __device__ __forceinline__ void load(const uint8_t* row, const int (&off)[units],
-                                              uint32_t (&w)[words]) {
-#pragma unroll
-    for (int u = 0; u < units; ++u) load_bytes<UB>(row + off[u], &w[u * UB / 4]);
-  }
 };
 
-// Decoding.  Tables in shared memory as described above; `lane_off` is the
-// lane's offset in an entry.  lo: offset of the 4-bit tables' lo parts.
-constexpr uint32_t kTableBytes = 65536;
+// Sixteen rows lie in shared memory as in the pool, except that in rows of full
+// size the 16-byte pieces are exchanged so that a warp's loads meet no bank
+// twice: keys are read by 8 rows x 4 pieces, values by 4 rows (2t and 2t + 1
+// alternating) x 8 lanes.  Where piece n of the sixteen rows lies:
+template <int ROW>
+__device__ __forceinline__ int key_piece(int n) {
+  return ROW >= 128 ? n ^ ((n / (ROW / 16) & 1) << 2) : n;
+}
+template <int ROW>
+__device__ __forceinline__ int value_piece(int n) {
+  return ROW >= 128 ? n ^ ((n / (ROW / 16) >> 1 & 3) << 1)
+         : ROW >= 32 ? n ^ ((n / (ROW / 16) >> 2 & 1) << 1)
+                     : n;
+}
 
-__device__ __forceinline__ uint32_t lookup(const uint8_t* table, uint32_t lane_off, uint32_t w,
-                                           int byte) {
-  return *reinterpret_cast<const uint32_t*>(table +
-                                            __byte_perm(w, lane_off, 0x5504u | (byte << 4)));
+// Decoding.  A side's table has 256 entries of 128 bytes, a copy of the entry's
+// word for every lane; keys' first, values' behind them, then (4 bits, hi + lo)
+// both lo tables.  `base` is the lane's place in entry 0 as a shared-memory
+// address; one dp4a adds 128 times a byte of the packed word to it.
+constexpr uint32_t kTableBytes = 32768;
+
+template <int LO>
+__device__ __forceinline__ uint32_t lookup(uint32_t base, uint32_t w, int byte) {
+  const uint32_t at = __dp4a(w, 128u << (8 * byte), base);
+  uint32_t x;
+  asm("ld.shared.b32 %0, [%1+%2];" : "=r"(x) : "r"(at), "n"(LO * 2 * (int)kTableBytes));
+  return x;
 }
 
 // The four codes that a lane gives to one K step: pairs a (first operand
 // register) and b (third), hi and lo.  2 bits: the pairs are codes (2, 0) and
 // (3, 1) of the byte, else (0, 1) and (2, 3).
 template <int BITS, bool LO, int W>
-__device__ __forceinline__ void decode_key(const uint32_t (&w)[W], int s, const uint8_t* table,
-                                           uint32_t lane_off, const uint32_t (&reg)[4],
+__device__ __forceinline__ void decode_key(const uint32_t (&w)[W], int s, uint32_t base,
+                                           const uint32_t (&reg)[4],
                                            uint32_t& ah, uint32_t& bh, uint32_t& al, uint32_t& bl) {
   if constexpr (BITS == 4) {
     const uint32_t x = w[s >> 1];
     const int b = (s & 1) * 2;
-    ah = lookup(table, lane_off, x, b);
-    bh = lookup(table, lane_off, x, b + 1);
+    ah = lookup<0>(base, x, b);
+    bh = lookup<0>(base, x, b + 1);
     if constexpr (LO) {
-      al = lookup(table + kTableBytes, lane_off, x, b);
-      bl = lookup(table + kTableBytes, lane_off, x, b + 1);
+      al = lookup<1>(base, x, b);
+      bl = lookup<1>(base, x, b + 1);
     }
   } else if constexpr (BITS == 8) {
     const uint32_t x = w[s];
-    const uint32_t e0 = lookup(table, lane_off, x, 0), e1 = lookup(table, lane_off, x, 1);
-    const uint32_t e2 = lookup(table, lane_off, x, 2), e3 = lookup(table, lane_off, x, 3);
+    const uint32_t e0 = lookup<0>(base, x, 0), e1 = lookup<0>(base, x, 1);
+    const uint32_t e2 = lookup<0>(base, x, 2), e3 = lookup<0>(base, x, 3);
     ah = __byte_perm(e0, e1, 0x5410);
     bh = __byte_perm(e2, e3, 0x5410);
     if constexpr (LO) {
@@ -216,26 +224,25 @@ __device__ __forceinline__ void decode_key(const uint32_t (&w)[W], int s, const 
 // Codes 2m and 2m + 1 of two tokens' rows: the pairs (x's, y's) of either code.
 template <int BITS, bool LO, int W>
 __device__ __forceinline__ void decode_value(const uint32_t (&x)[W], const uint32_t (&y)[W], int m,
-                                             const uint8_t* table, uint32_t lane_off,
-                                             const uint32_t (&reg)[4], uint32_t& eh, uint32_t& oh,
+                                             uint32_t base, const uint32_t (&reg)[4], uint32_t& eh, uint32_t& oh,
                                              uint32_t& el, uint32_t& ol) {
   if constexpr (BITS == 4) {
-    const uint32_t p = lookup(table, lane_off, x[m >> 2], m & 3);
-    const uint32_t q = lookup(table, lane_off, y[m >> 2], m & 3);
+    const uint32_t p = lookup<0>(base, x[m >> 2], m & 3);
+    const uint32_t q = lookup<0>(base, y[m >> 2], m & 3);
     eh = __byte_perm(p, q, 0x5410);
     oh = __byte_perm(p, q, 0x7632);
     if constexpr (LO) {
-      const uint32_t r = lookup(table + kTableBytes, lane_off, x[m >> 2], m & 3);
-      const uint32_t t = lookup(table + kTableBytes, lane_off, y[m >> 2], m & 3);
+      const uint32_t r = lookup<1>(base, x[m >> 2], m & 3);
+      const uint32_t t = lookup<1>(base, y[m >> 2], m & 3);
       el = __byte_perm(r, t, 0x5410);
       ol = __byte_perm(r, t, 0x7632);
     }
   } else if constexpr (BITS == 8) {
     const int b = 2 * (m & 1);
-    const uint32_t p0 = lookup(table, lane_off, x[m >> 1], b);
-    const uint32_t p1 = lookup(table, lane_off, x[m >> 1], b + 1);
-    const uint32_t q0 = lookup(table, lane_off, y[m >> 1], b);
-    const uint32_t q1 = lookup(table, lane_off, y[m >> 1], b + 1);
+    const uint32_t p0 = lookup<0>(base, x[m >> 1], b);
+    const uint32_t p1 = lookup<0>(base, x[m >> 1], b + 1);
+    const uint32_t q0 = lookup<0>(base, y[m >> 1], b);
+    const uint32_t q1 = lookup<0>(base, y[m >> 1], b + 1);
     eh = __byte_perm(p0, q0, 0x5410);
     oh = __byte_perm(p1, q1, 0x5410);
     if constexpr (LO) {
@@ -276,7 +283,11 @@ struct Work {
   int unit;                         // tokens of a unit
   const int* first;                 // [batch + 1] first unit of each sequence
 
-  __device__ int units_of(int len) const { return (len + unit - 1) / unit; }
+  // A segment's units: an empty one, then its tokens'.  The empty one stands for
+  // what taking up a segment costs a block, about as much as a unit of tokens:
+  // without it, the block that gets a batch's short sequences ends last (16
+  // sequences of 0 to 32768 tokens: 24 % of the time of the other SMs).
+  __device__ int units_of(int len) const { return len ? 1 + (len + unit - 1) / unit : 0; }
 };
 
 // Worker of a unit: worker w of n takes units [w * total / n, (w + 1) * total / n).
@@ -396,55 +407,67 @@ struct Parts {
 
 template <int D, int KB, int VB, int PREC>
 struct AttendShape {
-  // Steps of 32 tokens where the registers hold them, else of 16.
-  static constexpr int MT = D == 256 || (PREC >= 2 && (KB == 8 || VB == 8)) ? 1 : 2;
   static constexpr bool tables = KB != 2 || VB != 2;
   static constexpr bool lo_tables = (PREC >= 2 && KB == 4) || (PREC == 3 && VB == 4);
-  static constexpr int unit = kAttWarps * 16 * MT;
-  static constexpr size_t table_bytes =
-      tables ? (lo_tables ? 2 * (size_t)kTableBytes : (size_t)kTableBytes) : 0;
-  static constexpr int ostride = D + 8;
-  static constexpr size_t smem =
-      table_bytes + sizeof(float) * ((size_t)kAttWarps * kHeadsPer * ostride + 3 * 64);
-  static constexpr int ctas = D <= 128 && smem <= 110 * 1024 && PREC < 2 ? 2 : 1;
+  static constexpr int table_bytes = tables ? (lo_tables ? 4 : 2) * (int)kTableBytes : 0;
+  static constexpr int ostride = D + 8;  // of a partial result's head in shared memory
+  // A warp has two stages, a step's rows and norms each; a stage also holds the
+  // warp's partial result at a segment's end, while the next segment's first
+  // step comes into the other.
+  static constexpr int stage_of(int mt) {
+    const int step = 16 * mt * (D * KB / 8 + D * VB / 8 + 8);
+    const int part = kHeadsPer * ostride * 4;
+    return step > part ? step : part;
+  }
+  static constexpr int room = 227 * 1024 - 2048 - table_bytes;
+  static constexpr int fit(int mt) { return room / (2 * stage_of(mt)) / 2 * 2; }
+  // Registers allow 16 warps up to D = 128, fewer where operands come hi + lo
+  // or the output is wider.
+  static constexpr int most = D == 64 ? (PREC < 2 ? 16 : 12)
+                              : D == 128 ? (PREC < 2 ? 16 : 10) : (PREC == 0 ? 10 : 8);
+  // Steps of 32 tokens (two independent chains of products) where at least 10
+  // warps then fit, else of 16.
+  static constexpr int MT = D <= 128 && fit(2) >= 10 ? 2 : 1;
+  static constexpr int stage = stage_of(MT);
+  static constexpr int warps = fit(MT) < most ? fit(MT) : most;
+  static constexpr int threads = 32 * warps;
+  static constexpr int unit = warps * 16 * MT;
+  static constexpr int smem = table_bytes + 2 * warps * stage;
 };
 
 template <int D, int KB, int VB, int PREC>
-__global__ void __launch_bounds__(32 * kAttWarps, AttendShape<D, KB, VB, PREC>::ctas)
+__global__ void __launch_bounds__(AttendShape<D, KB, VB, PREC>::threads, 1)
 kv_attend_kernel(Side sk, Side sv, int pages, int page_shift, Work wk, QueryOut qo, Parts parts,
                  float* __restrict__ scores, int64_t score_width) {
   using Shape = AttendShape<D, KB, VB, PREC>;
-  constexpr int MT = Shape::MT;
+  constexpr int MT = Shape::MT, NW = Shape::warps;
   constexpr bool QLO = PREC >= 1, KLO = PREC >= 2, VLO = PREC >= 3;
   using KD = Deal<D, KB, 4>;
   using VD = Deal<D, VB, 8>;
   constexpr int KS = D / 16;  // K steps of a score, and pairs of coordinates of a value
-  extern __shared__ __align__(16) uint8_t smem[];
-  const uint8_t* table = smem;
-  float* so = reinterpret_cast<float*>(smem + Shape::table_bytes);
-  float* s_m = so + kAttWarps * kHeadsPer * Shape::ostride;  // [warp][head]
-  float* s_l = s_m + 64;
-  float* s_f = s_l + 64;
+  extern __shared__ __align__(128) uint8_t smem[];
+  __shared__ float s_m[NW][kHeadsPer], s_l[NW][kHeadsPer], s_v[NW];
   __shared__ int s_b;
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, g = lane >> 2, t = lane & 3;
   pdl_next();
 
   // Tables, from the codec's entries (set-up data: not written by the kernel
-  // before).  Thread i copies entry i to the 32 lanes' places.
+  // before).  A thread copies an entry to the 32 lanes' places.
   if constexpr (Shape::tables) {
 #pragma unroll
     for (int side = 0; side < 2; ++side) {
       const Codec& c = side ? sv.c : sk.c;
       if ((side ? VB : KB) == 2) continue;
 #pragma unroll
-      for (int part = 0; part < (Shape::lo_tables ? 2 : 1); ++part) {
-        const uint32_t e = c.pairs[part * 256 + tid];
-        const uint4 v = make_uint4(e, e, e, e);
+      for (int part = 0; part < (Shape::lo_tables ? 2 : 1); ++part)
+        for (int n = tid; n < 256; n += Shape::threads) {
+          const uint32_t e = c.pairs[part * 256 + n];
+          const uint4 v = make_uint4(e, e, e, e);
 #pragma unroll
-        for (int i = 0; i < 8; ++i)
-          *reinterpret_cast<uint4*>(smem + part * kTableBytes + tid * 256 + side * 128 +
-                                    ((i + tid) & 7) * 16) = v;
-      }
+          for (int i = 0; i < 8; ++i)
+            *reinterpret_cast<uint4*>(smem + (2 * part + side) * kTableBytes + n * 128 +
+                                      ((i + n) & 7) * 16) = v;
+        }
     }
   }
   uint32_t kreg[4], vreg[4];
@@ -453,11 +476,39 @@ kv_attend_kernel(Side sk, Side sv, int pages, int page_shift, Work wk, QueryOut 
     kreg[i] = KB == 2 ? sk.c.pairs[i] : 0u;
     vreg[i] = VB == 2 ? sv.c.pairs[i] : 0u;
   }
-  const uint32_t koff = lane * 4, voff = 128 + lane * 4;
-  const int kld = (int)sk.ldb, vld = (int)sv.ldb;
-  int kplace[KD::units], vplace[VD::units];
-  KD::places(kld, t, kplace);
-  VD::places(vld, g, vplace);
+  const uint32_t kbase = (uint32_t)__cvta_generic_to_shared(smem) + lane * 4;
+  const uint32_t vbase = kbase + kTableBytes;
+
+  // A stage: MT times sixteen rows of keys, of values, sixteen norms of either.
+  const uint32_t kld = (uint32_t)sk.ldb, vld = (uint32_t)sv.ldb;
+  const bool kfull = kld == KD::row, vfull = vld == VD::row;
+  const uint32_t group_bytes = 16 * (kld + vld + 8);
+  const uint32_t stage0 = (uint32_t)__cvta_generic_to_shared(smem) + Shape::table_bytes +
+                          warp * 2 * Shape::stage;
+  // Row r of the scores (lane: r = g and g + 8) is token r ^ (r >> 1 & 1), so that
+  // the tokens of lane (g, t)'s value operands, those of rows 2t, 2t + 1 (+ 8),
+  // alternate between even and odd rows of shared memory over t.
+  const int tok_k = g ^ (g >> 1 & 1), tok_v = 2 * t + (t & 1);
+  // The lane's places in a group's rows.  A row shorter than D coordinates ends
+  // before some lanes' places: these read its start, as codes of coordinates
+  // that meet zeros in the queries and are dropped from the values.
+  uint32_t kat[KD::units], vat[2][VD::units];
+#pragma unroll
+  for (int u = 0; u < KD::units; ++u) {
+    const int off = (u * 4 + t) * KD::UB;
+    kat[u] = tok_k * kld + (off < (int)kld ? off : 0);
+    if (kfull) kat[u] = key_piece<KD::row>(kat[u] / 16) * 16 + kat[u] % 16;
+  }
+#pragma unroll
+  for (int e = 0; e < 2; ++e)
+#pragma unroll
+    for (int u = 0; u < VD::units; ++u) {
+      const int off = (u * 8 + g) * VD::UB;
+      uint32_t at = (tok_v ^ e) * vld + (off < (int)vld ? off : 0);
+      if (vfull) at = value_piece<VD::row>(at / 16) * 16 + at % 16;
+      vat[e][u] = 16 * kld + at;
+    }
+  const uint32_t norm_at = 16 * (kld + vld) + 4 * tok_k;
   pdl_wait();
 
   const int per = wk.heads * wk.blocks;
@@ -466,28 +517,88 @@ kv_attend_kernel(Side sk, Side sv, int pages, int page_shift, Work wk, QueryOut 
   if ((int)blockIdx.x >= n) return;
   int64_t u = (int64_t)blockIdx.x * total / n;
   const int64_t uend = ((int64_t)blockIdx.x + 1) * total / n;
-  for (int i = tid; i < wk.batch; i += 32 * kAttWarps)
+  for (int i = tid; i < wk.batch; i += Shape::threads)
     if (wk.first[i] <= u && u < wk.first[i + 1]) s_b = i;
   __syncthreads();
-  int b = s_b;
 
-  while (u < uend) {
-    // The segment of unit u and this block's share of it.
-    while (u >= wk.first[b + 1]) ++b;
-    const int len = clamp_length(wk.lengths[b], wk.table_width, 1 << page_shift);
-    const int nu = wk.units_of(len);
-    const int r = (int)(u - wk.first[b]), seg_in = r / nu, u0 = r % nu;
-    const int u1 = (int)min((int64_t)nu, u0 + (uend - u));
-    const int h = seg_in / wk.blocks, hb = seg_in % wk.blocks;
-    const int seg = b * per + seg_in;
-    const int t0 = u0 * Shape::unit, t1 = min(len, u1 * Shape::unit);
-    const int32_t* trow = wk.table + b * wk.table_stride;
+  constexpr int stride = Shape::unit;
+  struct Segment {
+    int b, seg, hb, h, t0, t1, base;  // tokens [t0, t1), the warp's next step's first
+    int pid[MT];                      // and the pages of its groups; -1 for none
+  } cur, nxt;
+  auto page_of = [&](const Segment& x, int base, int i) {
+    const int tok = base + 16 * i;
+    int p = -1;
+    if (tok < x.t1) {
+      p = __ldg(wk.table + x.b * wk.table_stride + (tok >> page_shift));
+      if (p >= pages) p = -1;
+    }
+    return p;
+  };
+  // The segment of unit u and this block's share of it; u moves behind it.
+  auto take = [&](Segment& x, int b) {
+    x.t0 = x.t1 = x.base = 0;
+    x.b = b;
+    while (u < uend) {
+      while (u >= wk.first[x.b + 1]) ++x.b;
+      const int len = clamp_length(wk.lengths[x.b], wk.table_width, 1 << page_shift);
+      const int nu = wk.units_of(len);
+      const int r = (int)(u - wk.first[x.b]), in = r / nu, u0 = max(r % nu, 1);
+      const int u1 = (int)min((int64_t)nu, r % nu + (uend - u));
+      u += u1 - r % nu;
+      if (u1 <= u0) continue;  // the empty unit alone, at the end of the run
+      x.h = in / wk.blocks;
+      x.hb = in % wk.blocks;
+      x.seg = x.b * per + in;
+      x.t0 = (u0 - 1) * stride;
+      x.t1 = min(len, (u1 - 1) * stride);
+      x.base = x.t0 + warp * 16 * MT;
+#pragma unroll
+      for (int i = 0; i < MT; ++i) x.pid[i] = page_of(x, x.base, i);
+      return;
+    }
+  };
+  // Copies the step at x.base to a stage.  Groups without a page read page 0:
+  // what tokens that are not there decode to is finite, and meets a weight of 0.
+  // (A pool has fewer than 2^32 rows.)
+  auto fetch = [&](const Segment& x, uint32_t stage) {
+#pragma unroll
+    for (int i = 0; i < MT; ++i) {
+      const uint32_t row = ((uint32_t)(max(x.pid[i], 0) * wk.heads + x.h) << page_shift) +
+                           (uint32_t)((x.base + 16 * i) & ((1 << page_shift) - 1));
+      const uint8_t* kp = sk.rows + (uint64_t)row * kld + lane * 16;
+      const uint8_t* vp = sv.rows + (uint64_t)row * vld + lane * 16;
+      const uint32_t to = stage + i * group_bytes;
+#pragma unroll
+      for (int j = 0; j < (KD::row + 31) / 32; ++j) {
+        const int piece = lane + 32 * j;
+        if (piece < (int)kld)
+          copy16(to + 16 * (kfull ? key_piece<KD::row>(piece) : piece), kp + 512 * j);
+      }
+#pragma unroll
+      for (int j = 0; j < (VD::row + 31) / 32; ++j) {
+        const int piece = lane + 32 * j;
+        if (piece < (int)vld)
+          copy16(to + 16 * (kld + (vfull ? value_piece<VD::row>(piece) : piece)), vp + 512 * j);
+      }
+      if (lane < 8)
+        copy16(to + 16 * (kld + vld + lane), (lane & 4 ? sv.norms : sk.norms) + row + (lane & 3) * 4);
+    }
+    copy_commit();
+  };
+
+  take(cur, s_b);
+  int p = 0;  // stage of the step to come
+  if (cur.base < cur.t1) fetch(cur, stage0);
+  while (cur.t0 < cur.t1) {
+    take(nxt, cur.b);
+    const int t1 = cur.t1, hb = cur.hb;
 
     // The queries as B operands: lane (g, t) holds head g.
     uint32_t qh[KS][2], ql[QLO ? KS : 1][2];
     {
-      const __half* hi = qo.hi + ((int64_t)seg * kHeadsPer + g) * D;
-      const __half* lo = qo.lo + ((int64_t)seg * kHeadsPer + g) * D;
+      const __half* hi = qo.hi + ((int64_t)cur.seg * kHeadsPer + g) * D;
+      const __half* lo = qo.lo + ((int64_t)cur.seg * kHeadsPer + g) * D;
 #pragma unroll
       for (int s = 0; s < KS; ++s) {
         const int dim = KD::dim(t, 4 * s);
@@ -505,133 +616,94 @@ kv_attend_kernel(Side sk, Side sv, int pages, int page_shift, Work wk, QueryOut 
         }
       }
     }
-    const float f0 = qo.factor[(int64_t)seg * kHeadsPer + 2 * t];
-    const float f1 = qo.factor[(int64_t)seg * kHeadsPer + 2 * t + 1];
+    const float f0 = qo.factor[(int64_t)cur.seg * kHeadsPer + 2 * t];
+    const float f1 = qo.factor[(int64_t)cur.seg * kHeadsPer + 2 * t + 1];
 
     float o[KS][4];
 #pragma unroll
     for (int m = 0; m < KS; ++m) o[m][0] = o[m][1] = o[m][2] = o[m][3] = 0.f;
     float m0 = -FLT_MAX, m1 = -FLT_MAX, l0 = 0.f, l1 = 0.f;
     float vinv = 0.f, vlim = 0.f, vref = 0.f;  // value norms are taken times vinv = 2^10 / vref
+    int pid1[MT];  // pages of the step after the one to come
+#pragma unroll
+    for (int i = 0; i < MT; ++i) pid1[i] = page_of(cur, cur.base + stride, i);
 
-    uint32_t kw[MT][2][KD::words], vw[MT][4][VD::words];
-    float kn[MT][2], vn[MT][2];
-    int pid[MT], pid1[MT], pid2[MT];  // pages of this step's groups and of the next ones
-    // Page of 16-token group i of the step at token `base`; -1 for none.
-    auto page_of = [&](int base, int i) {
-      const int tok = base + 16 * i;
-      int p = -1;
-      if (tok < t1) {
-        p = __ldg(trow + (tok >> page_shift));
-        if (p >= pages) p = -1;
-      }
-      return p;
-    };
-    // First row of the group.  Groups without a page read page 0: what tokens
-    // that are not there decode to is finite, and meets a weight of 0.
-    auto row_of = [&](int p, int base, int i) {
-      return (((int64_t)max(p, 0) * wk.heads + h) << page_shift) +
-             ((base + 16 * i) & ((1 << page_shift) - 1));
-    };
-    auto load_keys = [&](int base) {
+    while (cur.base < t1) {
+      const int base = cur.base;
+      const uint32_t st = stage0 + p * Shape::stage;
+      bool there = base + 16 * MT <= t1;
+      uint32_t gone = 0;  // groups without a page
 #pragma unroll
       for (int i = 0; i < MT; ++i) {
-        const int64_t row = row_of(pid[i], base, i) + g;
-        const uint8_t* p = sk.rows + row * kld;
-        KD::load(p, kplace, kw[i][0]);
-        KD::load(p + 8 * kld, kplace, kw[i][1]);
-        kn[i][0] = load_norm(sk.norms + row);
-        kn[i][1] = load_norm(sk.norms + row + 8);
+        if (cur.pid[i] < 0) gone |= 1u << i;
+        cur.pid[i] = pid1[i];
       }
-    };
-    auto load_values = [&](int base) {
+      there = there && gone == 0;
+      cur.base += stride;
+      p ^= 1;
+      if (cur.base < t1) {
+        fetch(cur, stage0 + p * Shape::stage);
 #pragma unroll
-      for (int i = 0; i < MT; ++i) {
-        const int64_t row = row_of(pid[i], base, i);
-        const uint8_t* p = sv.rows + (row + 2 * t) * vld;
-        VD::load(p, vplace, vw[i][0]);
-        VD::load(p + vld, vplace, vw[i][1]);
-        VD::load(p + 8 * vld, vplace, vw[i][2]);
-        VD::load(p + 9 * vld, vplace, vw[i][3]);
-        vn[i][0] = load_norm(sv.norms + row + g);
-        vn[i][1] = load_norm(sv.norms + row + g + 8);
+        for (int i = 0; i < MT; ++i) pid1[i] = page_of(cur, cur.base + stride, i);
+        copy_wait<1>();
+      } else {
+        copy_wait<0>();
       }
-    };
-    auto prefetch = [&](const int (&p)[MT], int base) {
-      if (lane < 2 * MT) {
-        const int i = lane >> 1;
-        int pg = p[0];
-        if (MT > 1 && i) pg = p[MT - 1];
-        if (pg >= 0) {
-          const int64_t row = row_of(pg, base, i);
-          if (lane & 1)
-            prefetch_l2(sv.rows + row * vld, 16 * vld);
-          else
-            prefetch_l2(sk.rows + row * kld, 16 * kld);
-        }
-      }
-    };
+      __syncwarp();
 
-    constexpr int stride = Shape::unit;
-    int base = t0 + warp * 16 * MT;
-#pragma unroll
-    for (int i = 0; i < MT; ++i) {
-      pid[i] = page_of(base, i);
-      pid1[i] = page_of(base + stride, i);
-      pid2[i] = page_of(base + 2 * stride, i);
-    }
-    if (base < t1) {
-      load_keys(base);
-      load_values(base);
-      prefetch(pid1, base + stride);
-    }
-    for (; base < t1; base += stride) {
-      // Scores: S^T, tokens g and g + 8, heads 2t and 2t + 1.
+      // Scores: S^T, tokens of rows g and g + 8, heads 2t and 2t + 1.
       float s[MT][4];
 #pragma unroll
       for (int i = 0; i < MT; ++i) {
+        uint32_t kw[2][KD::words];
+#pragma unroll
+        for (int e = 0; e < 2; ++e)
+#pragma unroll
+          for (int un = 0; un < KD::units; ++un)
+            shared_bytes<KD::UB>(st + i * group_bytes + e * 8 * kld + kat[un],
+                                 &kw[e][un * KD::UB / 4]);
         s[i][0] = s[i][1] = s[i][2] = s[i][3] = 0.f;
 #pragma unroll
         for (int k = 0; k < KS; ++k) {
           uint32_t a0, a1, a2, a3, c0 = 0, c1 = 0, c2 = 0, c3 = 0;
-          decode_key<KB, KLO>(kw[i][0], k, table, koff, kreg, a0, a2, c0, c2);
-          decode_key<KB, KLO>(kw[i][1], k, table, koff, kreg, a1, a3, c1, c3);
+          decode_key<KB, KLO>(kw[0], k, kbase, kreg, a0, a2, c0, c2);
+          decode_key<KB, KLO>(kw[1], k, kbase, kreg, a1, a3, c1, c3);
           mma16816(s[i], a0, a1, a2, a3, qh[k][0], qh[k][1]);
           if constexpr (QLO) mma16816(s[i], a0, a1, a2, a3, ql[k][0], ql[k][1]);
           if constexpr (KLO) mma16816(s[i], c0, c1, c2, c3, qh[k][0], qh[k][1]);
         }
       }
-      bool there = base + 16 * MT <= t1;
-#pragma unroll
-      for (int i = 0; i < MT; ++i) there = there && pid[i] >= 0;
-      float mx0 = -FLT_MAX, mx1 = -FLT_MAX, vmx = 0.f;
+      float mx0 = -FLT_MAX, mx1 = -FLT_MAX, vmx = 0.f, vn[MT][2];
 #pragma unroll
       for (int i = 0; i < MT; ++i)
 #pragma unroll
         for (int e = 0; e < 2; ++e) {
-          s[i][2 * e] *= kn[i][e] * f0;
-          s[i][2 * e + 1] *= kn[i][e] * f1;
+          const uint32_t at = st + i * group_bytes + norm_at + 32 * e;
+          const float kn = shared_float(at);
+          vn[i][e] = shared_float(at + 64);
+          s[i][2 * e] *= kn * f0;
+          s[i][2 * e + 1] *= kn * f1;
         }
       if (!there) {
 #pragma unroll
         for (int i = 0; i < MT; ++i)
 #pragma unroll
           for (int e = 0; e < 2; ++e)
-            if (pid[i] < 0 || base + 16 * i + g + 8 * e >= t1) {
+            if ((gone >> i & 1) || base + 16 * i + tok_k + 8 * e >= t1) {
               s[i][2 * e] = s[i][2 * e + 1] = -INFINITY;
               vn[i][e] = 0.f;
             }
       }
-      float vnow[MT][2];
 #pragma unroll
       for (int i = 0; i < MT; ++i)
 #pragma unroll
         for (int e = 0; e < 2; ++e) {
           const float x = s[i][2 * e], y = s[i][2 * e + 1];
           if (PREC >= 2 && scores) {
-            const int tok = base + 16 * i + g + 8 * e;
+            const int tok = base + 16 * i + tok_k + 8 * e;
             if (tok < t1) {
-              float* to = scores + (((int64_t)b * wk.heads + h) * score_width + tok) * wk.group +
+              float* to = scores +
+                          (((int64_t)cur.b * wk.heads + cur.h) * score_width + tok) * wk.group +
                           hb * kHeadsPer + 2 * t;
               if (hb * kHeadsPer + 2 * t < wk.group) to[0] = x;
               if (hb * kHeadsPer + 2 * t + 1 < wk.group) to[1] = y;
@@ -640,21 +712,7 @@ kv_attend_kernel(Side sk, Side sv, int pages, int page_shift, Work wk, QueryOut 
           mx0 = fmaxf(mx0, x);
           mx1 = fmaxf(mx1, y);
           vmx = fmaxf(vmx, vn[i][e]);
-          vnow[i][e] = vn[i][e];
         }
-      // The next step's keys, and into L2 what the one after it reads.
-#pragma unroll
-      for (int i = 0; i < MT; ++i) {
-        pid[i] = pid1[i];
-        pid1[i] = pid2[i];
-      }
-      const bool more = base + stride < t1;
-      if (more) {
-        load_keys(base + stride);
-        prefetch(pid1, base + 2 * stride);
-      }
-#pragma unroll
-      for (int i = 0; i < MT; ++i) pid2[i] = page_of(base + 3 * stride, i);
 
       if (__any_sync(0xffffffffu, mx0 > m0 + kRescale || mx1 > m1 + kRescale || vmx > vlim)) {
 #pragma unroll
@@ -687,7 +745,7 @@ kv_attend_kernel(Side sk, Side sv, int pages, int page_shift, Work wk, QueryOut 
           o[m][3] *= e1;
         }
       }
-      // P^T as B operands: tokens 2t, 2t + 1 (and + 8), head g.
+      // P^T as B operands: tokens of rows 2t, 2t + 1 (and + 8), head g.
       uint32_t ph[MT][2], pl[MT][2];
 #pragma unroll
       for (int i = 0; i < MT; ++i)
@@ -696,7 +754,7 @@ kv_attend_kernel(Side sk, Side sv, int pages, int page_shift, Work wk, QueryOut 
           const float p0 = ex2(s[i][2 * e] - m0), p1 = ex2(s[i][2 * e + 1] - m1);
           l0 += p0;
           l1 += p1;
-          const float w = vnow[i][e] * vinv;
+          const float w = vn[i][e] * vinv;
           const float x = p0 * w, y = p1 * w;
           const uint32_t hi = pack_half2(x, y);
           ph[i][e] = transpose8(hi);
@@ -707,35 +765,47 @@ kv_attend_kernel(Side sk, Side sv, int pages, int page_shift, Work wk, QueryOut 
         }
 #pragma unroll
       for (int i = 0; i < MT; ++i) {
+        uint32_t vw[4][VD::words];
+#pragma unroll
+        for (int e = 0; e < 4; ++e)
+#pragma unroll
+          for (int un = 0; un < VD::units; ++un)
+            shared_bytes<VD::UB>(st + i * group_bytes + (e >> 1) * 8 * vld + vat[e & 1][un],
+                                 &vw[e][un * VD::UB / 4]);
 #pragma unroll
         for (int m = 0; m < KS; ++m) {
           uint32_t a0, a1, a2, a3, c0 = 0, c1 = 0, c2 = 0, c3 = 0;
-          decode_value<VB, VLO>(vw[i][0], vw[i][1], m, table, voff, vreg, a0, a1, c0, c1);
-          decode_value<VB, VLO>(vw[i][2], vw[i][3], m, table, voff, vreg, a2, a3, c2, c3);
+          decode_value<VB, VLO>(vw[0], vw[1], m, vbase, vreg, a0, a1, c0, c1);
+          decode_value<VB, VLO>(vw[2], vw[3], m, vbase, vreg, a2, a3, c2, c3);
           mma16816(o[m], a0, a1, a2, a3, ph[i][0], ph[i][1]);
           if constexpr (QLO) mma16816(o[m], a0, a1, a2, a3, pl[i][0], pl[i][1]);
           if constexpr (VLO) mma16816(o[m], c0, c1, c2, c3, ph[i][0], ph[i][1]);
         }
       }
-      if (more) load_values(base + stride);
+      __syncwarp();
     }
 
-    // The block's partial result: warps joined in order.
+    // The next segment's first step comes while this one's partial results are
+    // joined, warps in order, by way of each warp's other stage.
+    if (nxt.base < nxt.t1) fetch(nxt, stage0 + p * Shape::stage);
 #pragma unroll
     for (int w = 4; w < 32; w <<= 1) {
       l0 += __shfl_xor_sync(0xffffffffu, l0, w);
       l1 += __shfl_xor_sync(0xffffffffu, l1, w);
     }
     if (g == 0) {
-      s_m[warp * 8 + 2 * t] = m0;
-      s_m[warp * 8 + 2 * t + 1] = m1;
-      s_l[warp * 8 + 2 * t] = l0;
-      s_l[warp * 8 + 2 * t + 1] = l1;
+      s_m[warp][2 * t] = m0;
+      s_m[warp][2 * t + 1] = m1;
+      s_l[warp][2 * t] = l0;
+      s_l[warp][2 * t + 1] = l1;
     }
-    if (lane == 0) s_f[warp] = vref;
-    const int active = min(kAttWarps, (t1 - t0 + 16 * MT - 1) / (16 * MT));
+    const int active = min(NW, (t1 - cur.t0 + 16 * MT - 1) / (16 * MT));
+    uint8_t* own = smem + Shape::table_bytes + (warp * 2 + (p ^ 1)) * Shape::stage;
+    if (lane == 0) s_v[warp] = vref;
+    __shared__ const float* s_part[NW];
+    if (lane == 0) s_part[warp] = reinterpret_cast<const float*>(own);
     if (warp < active) {
-      float* dst = so + (warp * kHeadsPer + 2 * t) * Shape::ostride;
+      float* dst = reinterpret_cast<float*>(own) + 2 * t * Shape::ostride;
 #pragma unroll
       for (int m = 0; m < KS; ++m) {
         const int dim = VD::dim(g, 2 * m);
@@ -744,23 +814,23 @@ kv_attend_kernel(Side sk, Side sv, int pages, int page_shift, Work wk, QueryOut 
       }
     }
     __syncthreads();
-    const int64_t slot = (int64_t)blockIdx.x + seg;
+    const int64_t slot = (int64_t)blockIdx.x + cur.seg;
     const int ng = min(kHeadsPer, wk.group - hb * kHeadsPer);
-    for (int i = tid; i < ng * D; i += 32 * kAttWarps) {
+    for (int i = tid; i < ng * D; i += Shape::threads) {
       const int hd = i / D, j = i % D;
       float mm = -FLT_MAX;
-      for (int w = 0; w < active; ++w) mm = fmaxf(mm, s_m[w * 8 + hd]);
+      for (int w = 0; w < active; ++w) mm = fmaxf(mm, s_m[w][hd]);
       float sum = 0.f, l = 0.f;
       for (int w = 0; w < active; ++w) {
-        const float f = ex2(s_m[w * 8 + hd] - mm);
-        sum = fmaf(so[(w * kHeadsPer + hd) * Shape::ostride + j], f * s_f[w], sum);
-        l = fmaf(s_l[w * 8 + hd], f, l);
+        const float f = ex2(s_m[w][hd] - mm);
+        sum = fmaf(s_part[w][hd * Shape::ostride + j], f * s_v[w], sum);
+        l = fmaf(s_l[w][hd], f, l);
       }
       parts.o[slot * kHeadsPer * D + i] = sum;
       if (j == 0) parts.ml[slot * kHeadsPer + hd] = make_float2(mm, l);
     }
     __syncthreads();
-    u += u1 - u0;
+    cur = nxt;
   }
 }
 
@@ -790,7 +860,7 @@ kv_join_kernel(Parts parts, Work wk, int workers, int d, int page_size,
   if (nu) {
     const int n = min(workers, total);
     const int64_t u0 = wk.first[b] + (int64_t)seg_in * nu;
-    w0 = worker_of(u0, n, total);
+    w0 = worker_of(u0 + 1, n, total);
     nw = worker_of(u0 + nu - 1, n, total) - w0 + 1;
   }
   const int64_t slot0 = (int64_t)w0 + seg;
@@ -896,10 +966,10 @@ inline AttendPlan attend_plan(const pq_kv_cache& c, int batch, int q_heads, int 
   p.width = (int64_t)table_width * c.page_size;
   const int64_t segments = (int64_t)batch * c.heads * p.blocks;
   p.segments = (int)segments;
-  // Two blocks an SM where their shared memory allows it, never more than the
-  // units (of at least 128 tokens) that the table has room for.
-  const int64_t units = segments * ((p.width + 127) / 128);
-  p.workers = (int)max((int64_t)1, min(units, (int64_t)min(2 * num_sms(), kMaxWorkers)));
+  // A block per SM, never more than the units (of at least kLeastUnit tokens, and
+  // a segment's empty one) that the table has room for.
+  const int64_t units = segments * (1 + (p.width + kLeastUnit - 1) / kLeastUnit);
+  p.workers = (int)max((int64_t)1, min(units, (int64_t)min(num_sms(), kMaxWorkers)));
   Carve cv(ws, ws_bytes);
   p.q.hi = cv.take<__half>(segments * kHeadsPer * p.D);
   p.q.lo = cv.take<__half>(segments * kHeadsPer * p.D);
@@ -938,9 +1008,10 @@ int launch_attend(const pq_kv_cache& c, Work wk, const AttendPlan& p, int worker
   auto kern = kv_attend_kernel<D, KB, VB, PREC>;
   int page_shift = 4;
   while ((1 << page_shift) < c.page_size) ++page_shift;
+  static_assert(Shape::warps >= 4 && Shape::unit >= kLeastUnit, "too little shared memory");
   PQ_CUDA_TRY(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize,
                                    (int)Shape::smem));
-  return launch_pdl(kern, dim3(workers), 32 * kAttWarps, Shape::smem, st, true, side_k(c),
+  return launch_pdl(kern, dim3(workers), Shape::threads, Shape::smem, st, true, side_k(c),
                     side_v(c), c.pages, page_shift, wk, p.q, p.parts, p.scores, p.width);
 }
 
@@ -974,12 +1045,6 @@ struct UnitOf {
   template <int D, int KB, int VB, int PREC>
   int operator()() const {
     return AttendShape<D, KB, VB, PREC>::unit;
-  }
-};
-struct CtasOf {
-  template <int D, int KB, int VB, int PREC>
-  int operator()() const {
-    return AttendShape<D, KB, VB, PREC>::ctas;
   }
 };
 struct LaunchAttend {
@@ -1040,10 +1105,11 @@ int pq_kv_attend(const pq_kv_cache* cache, const void* q, int dtype, int64_t q_s
   PQ_CHECK_ARG(isfinite(scale), "scale must be finite");
   if (batch == 0) return PQ_OK;
   PQ_CHECK_ARG(q && out, "null pointer argument");
-  const int64_t widest = ((int64_t)table_width * c.page_size + 127) / 128;
+  const int64_t widest =
+      1 + ((int64_t)table_width * c.page_size + kv::kLeastUnit - 1) / kv::kLeastUnit;
   PQ_CHECK_ARG((int64_t)batch * q_heads < (1ll << 28) &&
-                   (int64_t)batch * q_heads * max(widest, (int64_t)1) < (1ll << 31),
-               "a call takes fewer than 2^28 query rows and 2^31 pieces of 128 tokens");
+                   (int64_t)batch * q_heads * widest < (1ll << 31),
+               "a call takes fewer than 2^28 query rows and 2^31 pieces of 64 tokens");
   const kv::AttendPlan p =
       kv::attend_plan(c, batch, q_heads, table_width, accumulate, ws, ws_bytes);
   if (!ws || ws_bytes < p.bytes)
@@ -1062,8 +1128,7 @@ int pq_kv_attend(const pq_kv_cache* cache, const void* q, int dtype, int64_t q_s
   wk.blocks = p.blocks;
   wk.first = p.first;
   wk.unit = kv::with_shape(p.D, c.k_bits, c.v_bits, prec, kv::UnitOf{});
-  const int workers =
-      min(p.workers, num_sms() * kv::with_shape(p.D, c.k_bits, c.v_bits, prec, kv::CtasOf{}));
+  const int workers = p.workers;
   PQ_KV_DISPATCH_T(dtype, {
     rc = p.D == 64 ? kv::launch_query<T_, 64>(c, q, q_stride_b, q_stride_h, scale, wk, p, st)
                    : p.D == 128

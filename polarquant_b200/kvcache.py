@@ -140,8 +140,9 @@ class KVCache:
             self.pages = int(buffers["k_rows"].shape[0])
             if pages is not None and int(pages) != self.pages:
                 raise ValueError(f"buffers hold {self.pages} pages, not {pages}")
-        if self.pages * self.page_size >= 1 << 31 or self.pages * self.heads >= 1 << 31:
-            raise ValueError("a pool has fewer than 2^31 slots")
+        if self.pages * self.page_size >= 1 << 31 or self.pages * self.heads >= 1 << 31 \
+                or self.pages * self.heads * self.page_size >= 1 << 32:
+            raise ValueError("a pool has fewer than 2^31 slots and 2^32 rows")
         pool = (self.pages, self.heads, self.page_size)
         kinds = {"k_rows": (pool + (row_stride(self.d, key.bits),), torch.uint8),
                  "v_rows": (pool + (row_stride(self.d, value.bits),), torch.uint8),

@@ -27,7 +27,7 @@ BAD_CACHES = [
     (dict(d=0), b"d must"), (dict(d=257), b"d must"), (dict(k_bits=3), b"bits"), (dict(v_bits=1), b"bits"),
     (dict(heads=0), b"heads"), (dict(pages=-1), b"pages"), (dict(page_size=24), b"page_size"), (dict(page_size=8), b"page_size"),
     (dict(page_size=2048), b"page_size"), (dict(pages=1 << 27), b"2^31"), (dict(pages=1 << 20, heads=1 << 12), b"2^31"),
-    (dict(k_ldb=24), b"ldb"), (dict(v_ldb=16), b"ldb"), (dict(k_codec=0), b"codec"), (dict(k_rows=0), b"pool"),
+    (dict(k_ldb=24), b"ldb"), (dict(v_ldb=16), b"ldb"), (dict(k_ldb=48), b"ldb"), (dict(pages=1 << 20, heads=1 << 8), b"2^32"), (dict(k_codec=0), b"codec"), (dict(k_rows=0), b"pool"),
     (dict(weights=0), b"pool"), (dict(v_rows=4100), b"aligned"),
 ]
 

@@ -12,28 +12,44 @@ namespace kv {
 struct Codec {
   const float* R;         // d x d
   const float* RT;        // its transpose
-  const float* bounds;    // 2^bits - 1
+  const float* bounds;    // 2^bits - 1, then infinity
   const float* cent;      // 2^bits
   const uint32_t* pairs;  // [2][256] centroids * 2^exponent for decoding in f16
                           // 4 bits: both of a byte's, hi parts; then lo parts
                           // 8 bits: hi and lo part of the byte's
                           // 2 bits: bytes 0 and 1 of the four hi parts, of the lo parts
   const int* exponent;    // the largest centroid * 2^exponent lies in [2^13, 2^14)
+  const float* range;     // cell of y = saturate(y * range[0] + range[1]) * (cells - 1), rounded
+  const uint2* cells;     // [2048]: the cell's boundary (f32) and the code below it
+  const uint2* planes;    // [2][D / 8][D / 16][32]: R * 2^14 as f16 hi and lo, in the order
+                          // of mma.m16n8k16's B operand (kv_rows.cu)
 };
 
+constexpr int kCells = 2048;      // of a codec of 8 bits
+constexpr int kFewCells = 64;     // of one of 2 or 4 bits
+inline int padded_d(int d) { return d <= 64 ? 64 : d <= 128 ? 128 : 256; }
+
 inline size_t codec_bytes(int d, int /*bits*/) {
-  return (size_t)2 * align_up((size_t)d * d * sizeof(float), 256) + 4 * 1024 + 256;
+  const size_t D = padded_d(d);
+  return (size_t)2 * align_up((size_t)d * d * sizeof(float), 256) + 4 * 1024 + 256 +
+         kCells * sizeof(uint2) + 2 * D * D * 2;
 }
 
 inline Codec codec_of(const void* tables, int d) {
   const char* b = (const char*)tables;
   const size_t m = align_up((size_t)d * d * sizeof(float), 256);
-  return Codec{(const float*)b,
-               (const float*)(b + m),
-               (const float*)(b + 2 * m),
-               (const float*)(b + 2 * m + 1024),
-               (const uint32_t*)(b + 2 * m + 2048),
-               (const int*)(b + 2 * m + 4096)};
+  Codec c;
+  c.R = (const float*)b;
+  c.RT = (const float*)(b + m);
+  b += 2 * m;
+  c.bounds = (const float*)b;
+  c.cent = (const float*)(b + 1024);
+  c.pairs = (const uint32_t*)(b + 2048);
+  c.exponent = (const int*)(b + 4096);
+  c.range = (const float*)(b + 4096 + 64);
+  c.cells = (const uint2*)(b + 4096 + 256);
+  c.planes = c.cells + kCells;
+  return c;
 }
 
 // One side of the pool.

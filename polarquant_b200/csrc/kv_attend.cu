@@ -959,7 +959,7 @@ struct AttendPlan {
 inline AttendPlan attend_plan(const pq_kv_cache& c, int batch, int q_heads, int table_width,
                               int accumulate, void* ws, size_t ws_bytes) {
   AttendPlan p;
-  p.D = c.d <= 64 ? 64 : c.d <= 128 ? 128 : 256;
+  p.D = padded_d(c.d);
   const int group = q_heads / c.heads;
   p.blocks = (group + kHeadsPer - 1) / kHeadsPer;
   p.rows = (int64_t)batch * q_heads;

@@ -6,27 +6,84 @@
 namespace pqb {
 namespace kv {
 
-__global__ void prepare_codec_kernel(const float* __restrict__ R, const float* __restrict__ bounds,
-                                     const float* __restrict__ cent, int d, int bits,
-                                     float* __restrict__ oR, float* __restrict__ oRT,
-                                     float* __restrict__ ob, float* __restrict__ oc,
-                                     uint32_t* __restrict__ pairs, int* __restrict__ exponent) {
-  const int t = blockIdx.x * blockDim.x + threadIdx.x;
-  for (int i = t; i < d * d; i += gridDim.x * blockDim.x) {
-    const float v = R[i];
-    oR[i] = v;
-    oRT[(i % d) * d + i / d] = v;
+// ---------------------------------------------------------------------------
+// The codec's tables
+// ---------------------------------------------------------------------------
+
+// Entry of a cell, for cells of [i - 1/2, i + 1/2) / scale + lo widened by `slack`:
+// the boundary in it and the number of boundaries below that.  A cell without a
+// boundary has one at 1e30, a cell with several NaN: their coordinates are
+// recomputed exactly.
+__device__ uint2 cell_entry(const float* bounds, int count, int i, int cells, float lo, float width,
+                            float slack) {
+  const float from = i == 0 ? -INFINITY : lo + (i - 0.5f) * width - slack;
+  const float to = i == cells - 1 ? INFINITY : lo + (i + 0.5f) * width + slack;
+  int below = 0, in = 0;
+  for (int k = 0; k < count; ++k) {
+    if (bounds[k] < from)
+      ++below;
+    else if (bounds[k] <= to)
+      ++in;
   }
-  if (t < 256) {
-    ob[t] = t < (1 << bits) - 1 ? bounds[t] : INFINITY;
-    oc[t] = t < (1 << bits) ? cent[t] : 0.f;
+  const float b = in == 0 ? 1e30f : in == 1 ? bounds[below] : __int_as_float(0x7fc00000);
+  return make_uint2(__float_as_uint(b), (uint32_t)below);
+}
+
+__global__ void prepare_codec_kernel(const float* __restrict__ R, const float* __restrict__ bounds,
+                                     const float* __restrict__ cent, int d, int bits, int D,
+                                     Codec out) {
+  const int t = blockIdx.x * blockDim.x + threadIdx.x, threads = gridDim.x * blockDim.x;
+  const int levels = 1 << bits;
+  for (int i = t; i < d * d; i += threads) {
+    const float v = R[i];
+    const_cast<float*>(out.R)[i] = v;
+    const_cast<float*>(out.RT)[(i % d) * d + i / d] = v;
+  }
+  // Planes: operand register r of lane (g, t) for columns of tile n and step s.
+  for (int i = t; i < D / 8 * (D / 16) * 32; i += threads) {
+    const int lane = i & 31, s = (i >> 5) % (D / 16), n = (i >> 5) / (D / 16);
+    const int g = lane >> 2, tt = lane & 3;
+    const int col = (g >> 1) * (D / 4) + (n >> 2) * 8 + 2 * (n & 3) + (g & 1);
+    __half hi[4], lo[4];
+    for (int k = 0; k < 4; ++k) {
+      const int row = tt * (D / 4) + 4 * s + k;
+      const float v = col < d && row < d ? R[col * d + row] * 16384.f : 0.f;
+      hi[k] = __float2half_rn(v);
+      lo[k] = __float2half_rn(v - __half2float(hi[k]));
+    }
+    uint2* p = const_cast<uint2*>(out.planes);
+    p[i] = make_uint2(__half_as_ushort(hi[0]) | (uint32_t)__half_as_ushort(hi[1]) << 16,
+                      __half_as_ushort(hi[2]) | (uint32_t)__half_as_ushort(hi[3]) << 16);
+    p[D / 8 * (D / 16) * 32 + i] =
+        make_uint2(__half_as_ushort(lo[0]) | (uint32_t)__half_as_ushort(lo[1]) << 16,
+                   __half_as_ushort(lo[2]) | (uint32_t)__half_as_ushort(lo[3]) << 16);
+  }
+  // Cells between the first and the last boundary.
+  {
+    const int cells = bits == 8 ? kCells : kFewCells;
+    const float lo = bounds[0], hi = bounds[levels - 2];
+    float width = (hi - lo) / (cells - 1);
+    if (!(width > 1e-30f && width < 1e30f)) width = 0.f;  // one cell for all
+    const float scale = width > 0.f ? 1.f / (hi - lo) : 0.f;
+    for (int i = t; i < cells; i += threads)
+      const_cast<uint2*>(out.cells)[i] =
+          width > 0.f ? cell_entry(bounds, levels - 1, i, cells, lo, width, 0.01f * width + 1e-5f)
+                      : make_uint2(0x7fc00000u, 0u);
+    if (t == 0) {
+      const_cast<float*>(out.range)[0] = scale;
+      const_cast<float*>(out.range)[1] = width > 0.f ? -lo * scale : 0.f;
+    }
   }
   if (blockIdx.x) return;
+  if (t < 256) {
+    const_cast<float*>(out.bounds)[t] = t < levels - 1 ? bounds[t] : INFINITY;
+    const_cast<float*>(out.cent)[t] = t < levels ? cent[t] : 0.f;
+  }
   __shared__ uint32_t s_half[256];  // hi | lo << 16
   __shared__ int s_mx;
   if (threadIdx.x == 0) s_mx = 0;
   __syncthreads();
-  const float c = threadIdx.x < (1 << bits) ? cent[threadIdx.x] : 0.f;
+  const float c = threadIdx.x < levels ? cent[threadIdx.x] : 0.f;
   atomicMax(&s_mx, __float_as_int(fabsf(c)));  // ordered as the floats are
   __syncthreads();
   const float mx = __int_as_float(s_mx);
@@ -49,77 +106,356 @@ __global__ void prepare_codec_kernel(const float* __restrict__ R, const float* _
     if (i < 4)  // byte i of the four 32-bit hi | lo words
       for (int k = 0; k < 4; ++k) p0 |= ((s_half[k] >> (8 * i)) & 255u) << (8 * k);
   }
-  pairs[i] = p0;
-  pairs[256 + i] = p1;
-  if (i == 0) *exponent = e;
+  const_cast<uint32_t*>(out.pairs)[i] = p0;
+  const_cast<uint32_t*>(out.pairs)[256 + i] = p1;
+  if (i == 0) *const_cast<int*>(out.exponent) = e;
 }
 
-// Append.  x -> norm = f32(sqrt(sum_f64 x^2)), u = x / max(norm, 1e-8) in f32,
-// code_j = #{boundaries < sum_i u_i R_ji}, the sum in f64.  One warp per row;
-// lane l holds columns l, l + 32, ...
-constexpr int kAppendWarps = 8;
+// ---------------------------------------------------------------------------
+// Append
+//
+// x -> norm = f32(sqrt(sum_f64 x^2)), u = x / max(norm, 1e-8) in f32, code_j =
+// #{boundaries < sum_i u_i R_ji}, exactly.
+//
+// The rotation runs on mma.m16n8k16 (f16 operands, f32 sums): a row's x times a
+// power of two is f16 hi (exact for 16-bit inputs but for elements below 2^-28
+// of the largest) or hi + lo (f32), R * 2^14 is hi + lo, and hi*hi + hi*lo (+
+// lo*hi) are summed; the scales and 1 / max(norm, 1e-8) come after.  That is
+// within (steps + 8) * 2^-23 of the exact product (each of the sum's `steps`
+// additions loses at most 2^-23 of a partial sum, which is at most |u||R_j| = 1;
+// operands lose 2^-22): coordinates that near a boundary are recomputed by the
+// warp in f64.  So codes do not depend on how the product was taken.
+//
+// Which column and which element stands where in the operands is free, so a
+// lane (g, t) loads a quarter of row g from its t-th run of d / 4 elements, and
+// gets the coordinates of the same run back: it packs whole words.  Counting
+// boundaries takes one table lookup: cells narrower than the gaps between
+// boundaries hold at most one (from a copy for each lane at 2 and 4 bits, with
+// the code in the low four bits of the boundary).
+//
+// A warp takes `ROWS` rows (32: the planes' operands, read from shared memory,
+// serve two of them) through all columns with the planes of a side resident in
+// shared memory; a call of few rows instead spreads the columns over the warps
+// and reads the planes from L2.
+// ---------------------------------------------------------------------------
 
-template <class T>
-__global__ void __launch_bounds__(32 * kAppendWarps)
-append_kernel(const T* __restrict__ k, const T* __restrict__ v, int64_t k_sn, int64_t k_sh,
-              int64_t v_sn, int64_t v_sh, int64_t n, int heads, int d, int64_t slots_end,
-              int page_size, Side sk, Side sv, const int64_t* __restrict__ slots,
-              const int32_t* __restrict__ positions, const float* __restrict__ weights,
-              int32_t* __restrict__ out_pos, float* __restrict__ out_w) {
-  __shared__ float su[kAppendWarps][PQ_KV_MAX_D];
-  __shared__ uint8_t sc[kAppendWarps][PQ_KV_MAX_D];
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  const bool is_v = blockIdx.y != 0;
-  const Side& s = is_v ? sv : sk;
-  const int64_t r = (int64_t)blockIdx.x * kAppendWarps + warp;
-  if (r >= n * heads) return;
-  const int64_t tok = r / heads;
-  const int h = (int)(r % heads);
-  const int64_t slot = slots[tok];
-  if (slot < 0 || slot >= slots_end) return;
-  const T* x = is_v ? v + tok * v_sn + h * v_sh : k + tok * k_sn + h * k_sh;
-  double ss = 0.0;
-  for (int i = lane; i < d; i += 32) {
-    const float f = to_f32<T>(x[i]);
-    su[warp][i] = f;
-    ss = fma((double)f, (double)f, ss);
+__device__ __forceinline__ void mma_rows(float (&c)[4], const uint32_t (&a)[4], uint2 b) {
+  asm volatile(
+      "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, "
+      "{%0,%1,%2,%3};"
+      : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
+      : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b.x), "r"(b.y));
+}
+
+struct AppendArgs {
+  const void *k, *v;
+  int64_t k_sn, k_sh, v_sn, v_sh;
+  int64_t rows, slots_end;
+  int heads, d, page_size;
+  bool k_vec, v_vec;  // rows can be read 16 bytes at a time
+  Side sk, sv;
+  const int64_t* slots;
+  const int32_t* positions;
+  const float* weights;
+  int32_t* out_pos;
+  float* out_w;
+};
+
+template <class T, int D, bool SMALL>
+struct AppendShape {
+  static constexpr bool wide = sizeof(T) == 4;  // x is hi + lo
+  static constexpr int MT = SMALL || wide || D == 256 ? 1 : 2;
+  static constexpr int rows = 16 * MT;
+  static constexpr int steps = D / 16;
+  static constexpr int chunks = D / 32;                      // of 8 columns a lane
+  static constexpr int per = SMALL ? 1 : (D == 256 ? 4 : chunks);  // chunks of a warp
+  static constexpr int parts = SMALL ? 1 : chunks / per;     // blocks that share a row's columns
+  static constexpr int warps = SMALL ? chunks : (D == 64 ? 16 : 12);
+  static constexpr int groups = SMALL ? 1 : warps;           // row groups of a block at a time
+  static constexpr int run = per * 8;                        // columns of a lane in a row
+  static constexpr int plane = D / 8 / parts * steps * 32;   // uint2 of a plane in the block
+};
+
+template <class T, int D, int BITS, bool SMALL>
+__global__ void __launch_bounds__(32 * AppendShape<T, D, SMALL>::warps, 1)
+kv_append_kernel(AppendArgs a) {
+  using S = AppendShape<T, D, SMALL>;
+  constexpr int MT = S::MT;
+  constexpr int run_bytes = S::run * BITS / 8, words = (run_bytes + 3) / 4;
+  constexpr int cells = BITS == 8 ? kCells : kFewCells;
+  extern __shared__ __align__(16) uint8_t smem[];
+  uint2* s_plane = reinterpret_cast<uint2*>(smem);
+  uint32_t* s_cell = reinterpret_cast<uint32_t*>(smem + (SMALL ? 0 : 2 * S::plane * sizeof(uint2)));
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
+  // blockIdx.y: the part of the columns and, lowest, the side.
+  const bool is_v = blockIdx.y & 1;
+  const int part = blockIdx.y >> 1;
+  const Side& sd = is_v ? a.sv : a.sk;
+  const Codec& cd = sd.c;
+  if (sd.bits != BITS) return;
+  const T* src = reinterpret_cast<const T*>(is_v ? a.v : a.k);
+  const int64_t sn = is_v ? a.v_sn : a.k_sn, sh = is_v ? a.v_sh : a.k_sh;
+  const bool vec = is_v ? a.v_vec : a.k_vec;
+  const int d = a.d;
+
+  if constexpr (!SMALL) {
+    const uint2* p = cd.planes + part * S::plane;
+    for (int i = threadIdx.x; i < S::plane; i += blockDim.x) {
+      s_plane[i] = p[i];
+      s_plane[S::plane + i] = p[D / 8 * S::steps * 32 + i];
+    }
   }
+  if constexpr (BITS == 8) {
+    for (int i = threadIdx.x; i < cells; i += blockDim.x)
+      reinterpret_cast<uint2*>(s_cell)[i] = cd.cells[i];
+  } else {
+    for (int i = threadIdx.x; i < cells * 32; i += blockDim.x) {
+      const uint2 c = cd.cells[i >> 5];
+      s_cell[i] = (c.x & ~15u) | c.y;
+    }
+  }
+  __syncthreads();
+  const float cs = cd.range[0], co = cd.range[1];
+  // (a boundary below 1 with its low four bits taken loses 15 * 2^-24 < 1e-6)
+  constexpr float band =
+      (S::steps * (S::wide ? 3 : 2) + 8) * 1.1920929e-7f + (BITS == 8 ? 0.f : 1e-6f);
+
+  const int64_t groups = (a.rows + S::rows - 1) / S::rows;
+  for (int64_t gr = (int64_t)blockIdx.x * S::groups + (SMALL ? 0 : warp); gr < groups;
+       gr += (int64_t)gridDim.x * S::groups) {
+    // x of rows g, g + 8 (, g + 16, g + 24) in f32, a quarter of each a lane.
+    const int64_t row0 = gr * S::rows;
+    uint32_t ah[MT][S::steps][4], al[S::wide ? MT : 1][S::wide ? S::steps : 1][4];
+    float inv[2 * MT], den[2 * MT], nrm[2 * MT];
 #pragma unroll
-  for (int o = 16; o > 0; o >>= 1) ss += __shfl_xor_sync(0xffffffffu, ss, o);
-  const float nrm = __double2float_rn(__dsqrt_rn(ss));
-  const float den = fmaxf(nrm, 1e-8f);
-  for (int i = lane; i < d; i += 32) su[warp][i] = __fdiv_rn(su[warp][i], den);
-  __syncwarp();
-  const int levels = 1 << s.bits;
-  for (int j = lane; j < PQ_KV_MAX_D; j += 32) {
-    uint32_t code = 0;
-    if (j < d) {
-      double y = 0.0;
-      for (int i = 0; i < d; ++i) y = fma((double)su[warp][i], (double)s.c.RT[i * d + j], y);
-      for (int step = levels >> 1; step > 0; step >>= 1)
-        if (y > (double)s.c.bounds[code + step - 1]) code += step;
+    for (int i = 0; i < 2 * MT; ++i) {
+      const int64_t r = min(row0 + g + 8 * i, a.rows - 1);
+      const T* x = src + (r / a.heads) * sn + (r % a.heads) * sh + t * (D / 4);
+      float f[D / 4];
+      if (vec) {
+        constexpr int E = 16 / sizeof(T);
+#pragma unroll
+        for (int j = 0; j < D / 4; j += E) {
+          uint4 w = make_uint4(0u, 0u, 0u, 0u);
+          if (t * (D / 4) + j < d) w = *reinterpret_cast<const uint4*>(x + j);
+          const T* e = reinterpret_cast<const T*>(&w);
+#pragma unroll
+          for (int k = 0; k < E; ++k) f[j + k] = to_f32<T>(e[k]);
+        }
+      } else {
+#pragma unroll
+        for (int j = 0; j < D / 4; ++j) f[j] = t * (D / 4) + j < d ? to_f32<T>(x[j]) : 0.f;
+      }
+      double ss = 0.0;
+      float mx = 0.f;
+#pragma unroll
+      for (int j = 0; j < D / 4; ++j) {
+        ss = fma((double)f[j], (double)f[j], ss);
+        mx = fmaxf(mx, fabsf(f[j]));
+      }
+#pragma unroll
+      for (int o = 1; o < 4; o <<= 1) {
+        ss += __shfl_xor_sync(0xffffffffu, ss, o);
+        mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, o));
+      }
+      nrm[i] = __double2float_rn(__dsqrt_rn(ss));
+      den[i] = fmaxf(nrm[i], 1e-8f);
+      // max |x| * 2^e in [2^14, 2^15): f16's range, and sums of at most 2^29 sqrt(d)
+      const int e = mx > 0.f && mx < INFINITY ? max(-126, min(126, 14 - ilogbf(mx))) : 0;
+      const float up = __int_as_float((127 + e) << 23);
+      inv[i] = __int_as_float((127 - e) << 23) / 16384.f / den[i];
+      // Registers 0 and 2 of the A operand hold row g, 1 and 3 row g + 8.
+#pragma unroll
+      for (int s = 0; s < S::steps; ++s)
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+          const float x0 = f[4 * s + 2 * h] * up, x1 = f[4 * s + 2 * h + 1] * up;
+          const __half2 hi = __floats2half2_rn(x0, x1);
+          ah[i >> 1][s][2 * h + (i & 1)] = *reinterpret_cast<const uint32_t*>(&hi);
+          if constexpr (S::wide) {
+            const float2 b = __half22float2(hi);
+            const __half2 lo = __floats2half2_rn(x0 - b.x, x1 - b.y);
+            al[i >> 1][s][2 * h + (i & 1)] = *reinterpret_cast<const uint32_t*>(&lo);
+          }
+        }
     }
-    sc[warp][j] = (uint8_t)code;
-  }
-  __syncwarp();
-  const int64_t at = ((slot / page_size) * heads + h) * page_size + slot % page_size;
-  uint8_t* row = s.rows + at * s.ldb;
-  const int per = 8 / s.bits;
-  for (int b = lane; b < s.ldb; b += 32) {
-    uint32_t w = 0;
-    for (int t = 0; t < per; ++t) {
-      const int j = b * per + t;
-      w = (w << s.bits) | (j < PQ_KV_MAX_D ? sc[warp][j] : 0u);
+
+    uint32_t packed[2 * MT][words];
+#pragma unroll
+    for (int i = 0; i < 2 * MT; ++i)
+#pragma unroll
+      for (int w = 0; w < words; ++w) packed[i][w] = 0u;
+#pragma unroll
+    for (int c = 0; c < S::per; ++c) {
+      const int chunk = SMALL ? warp : part * S::per + c;
+      float acc[MT][4][4];
+#pragma unroll
+      for (int m = 0; m < MT; ++m)
+#pragma unroll
+        for (int q = 0; q < 4; ++q) acc[m][q][0] = acc[m][q][1] = acc[m][q][2] = acc[m][q][3] = 0.f;
+#pragma unroll
+      for (int s = 0; s < S::steps; ++s)
+#pragma unroll
+        for (int q = 0; q < 4; ++q) {
+          uint2 bh, bl;
+          if constexpr (SMALL) {
+            const int at = ((chunk * 4 + q) * S::steps + s) * 32 + lane;
+            bh = __ldg(cd.planes + at);
+            bl = __ldg(cd.planes + D / 8 * S::steps * 32 + at);
+          } else {
+            const int at = ((c * 4 + q) * S::steps + s) * 32 + lane;
+            bh = s_plane[at];
+            bl = s_plane[S::plane + at];
+          }
+#pragma unroll
+          for (int m = 0; m < MT; ++m) {
+            mma_rows(acc[m][q], ah[m][s], bh);
+            mma_rows(acc[m][q], ah[m][s], bl);
+            if constexpr (S::wide) mma_rows(acc[m][q], al[m][s], bh);
+          }
+        }
+      // Codes of rows g + 8i, columns t * D / 4 + chunk * 8 + 2q + e.
+      const int col0 = t * (D / 4) + chunk * 8;
+#pragma unroll
+      for (int i = 0; i < 2 * MT; ++i) {
+        uint32_t near = 0, code[8];
+#pragma unroll
+        for (int k = 0; k < 8; ++k) {
+          const float y = acc[i >> 1][k >> 1][2 * (i & 1) + (k & 1)] * inv[i];
+          const float cell = fmaf(__saturatef(fmaf(y, cs, co)), (float)(cells - 1), 8388608.f);
+          float b;
+          uint32_t below;
+          if constexpr (BITS == 8) {
+            const uint2 e = reinterpret_cast<const uint2*>(s_cell)[__float_as_uint(cell) & (cells - 1)];
+            b = __uint_as_float(e.x);
+            below = e.y;
+          } else {
+            const uint32_t e = s_cell[(__float_as_uint(cell) & (cells - 1)) * 32 + lane];
+            b = __uint_as_float(e);
+            below = e & 15u;
+          }
+          const float off = y - b;
+          code[k] = below + (off > 0.f ? 1u : 0u);
+          if (!(fabsf(off) >= band)) near |= 1u << k;
+        }
+        if (col0 + 8 > d) {
+#pragma unroll
+          for (int k = 0; k < 8; ++k)
+            if (col0 + k >= d) {
+              code[k] = 0u;
+              near &= ~(1u << k);
+            }
+        }
+        if (row0 + g + 8 * i >= a.rows) near = 0u;
+        // Coordinates next to a boundary, by the whole warp.
+        uint32_t pend = __ballot_sync(0xffffffffu, near != 0u);
+        while (pend) {
+          const int from = __ffs(pend) - 1;
+          pend &= pend - 1;
+          uint32_t mask = __shfl_sync(0xffffffffu, near, from);
+          const int64_t r = row0 + (from >> 2) + 8 * i;
+          const float dn = __shfl_sync(0xffffffffu, den[i], from);
+          const T* x = src + (r / a.heads) * sn + (r % a.heads) * sh;
+          while (mask) {
+            const int k = __ffs(mask) - 1;
+            mask &= mask - 1;
+            const float* rr = cd.R + ((from & 3) * (D / 4) + chunk * 8 + k) * d;
+            double y = 0.0;
+            for (int j = lane; j < d; j += 32)
+              y = fma((double)__fdiv_rn(to_f32<T>(x[j]), dn), (double)__ldg(rr + j), y);
+#pragma unroll
+            for (int o = 16; o > 0; o >>= 1) y += __shfl_xor_sync(0xffffffffu, y, o);
+            uint32_t exact = 0;
+#pragma unroll
+            for (int step = 1 << (BITS - 1); step > 0; step >>= 1)
+              if (y > (double)__ldg(cd.bounds + exact + step - 1)) exact += step;
+            if (lane == from) {
+#pragma unroll
+              for (int z = 0; z < 8; ++z)
+                if (z == k) code[z] = exact;
+            }
+          }
+        }
+        // Eight codes: BITS bytes, the first code highest in its byte.
+#pragma unroll
+        for (int k = 0; k < 8; ++k) {
+          const int bit = (c * 8 + k) * BITS;  // of the run
+          packed[i][bit >> 5] |= code[k] << ((bit & 24) + 8 - BITS - (bit & 7));
+        }
+      }
     }
-    row[b] = (uint8_t)w;
-  }
-  if (lane == 0) {
-    s.norms[at] = nrm;
-    if (!is_v) {
-      out_pos[at] = positions[tok];
-      out_w[at] = weights ? weights[r] : 0.f;
+
+#pragma unroll
+    for (int i = 0; i < 2 * MT; ++i) {
+      const int64_t r = row0 + g + 8 * i;
+      if (r >= a.rows) continue;
+      const int64_t tok = r / a.heads;
+      const int64_t slot = a.slots[tok];
+      if (slot < 0 || slot >= a.slots_end) continue;
+      const int64_t at =
+          ((slot / a.page_size) * a.heads + r % a.heads) * a.page_size + slot % a.page_size;
+      const int off = (t * (D / 4) + (SMALL ? warp : part * S::per) * 8) * BITS / 8;
+      uint8_t* to = sd.rows + at * sd.ldb + off;
+      if constexpr (run_bytes >= 16) {
+#pragma unroll
+        for (int w = 0; w < words; w += 4)
+          if (off + 4 * w < sd.ldb)
+            *reinterpret_cast<uint4*>(to + 4 * w) =
+                make_uint4(packed[i][w], packed[i][w + 1], packed[i][w + 2], packed[i][w + 3]);
+      } else if (off < sd.ldb) {
+        if constexpr (run_bytes == 8)
+          *reinterpret_cast<uint2*>(to) = make_uint2(packed[i][0], packed[i][1]);
+        else if constexpr (run_bytes == 4)
+          *reinterpret_cast<uint32_t*>(to) = packed[i][0];
+        else
+          *reinterpret_cast<uint16_t*>(to) = (uint16_t)packed[i][0];
+      }
+      if (t == 0 && part == 0 && (!SMALL || warp == 0)) {
+        sd.norms[at] = nrm[i];
+        if (!is_v) {
+          a.out_pos[at] = a.positions[tok];
+          a.out_w[at] = a.weights ? a.weights[r] : 0.f;
+        }
+      }
     }
   }
+}
+
+template <class T, int D, int BITS, bool SMALL>
+int launch_append(const AppendArgs& a, cudaStream_t st) {
+  using S = AppendShape<T, D, SMALL>;
+  constexpr int smem = (SMALL ? 0 : 2 * S::plane * (int)sizeof(uint2)) +
+                       (BITS == 8 ? kCells * 8 : kFewCells * 128);
+  auto kern = kv_append_kernel<T, D, BITS, SMALL>;
+  PQ_CUDA_TRY(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, smem));
+  const int64_t groups = (a.rows + S::rows - 1) / S::rows;
+  const int64_t blocks = (groups + S::groups - 1) / S::groups;
+  // A launch for both sides where their bits are the same; a side of other bits
+  // leaves at once.
+  const int64_t most = SMALL ? 1 << 20 : max(1, num_sms() / (2 * S::parts));
+  kern<<<dim3((unsigned)min(blocks, most), 2 * S::parts), 32 * S::warps, smem, st>>>(a);
+  PQ_LAUNCH_CHECK("kv_append_kernel");
+  return PQ_OK;
+}
+
+template <class T, int D, int BITS>
+int launch_append_rows(const AppendArgs& a, cudaStream_t st) {
+  // Few rows: as many blocks of 16 rows as there are, each reading the planes
+  // from L2; more than two waves of them: resident planes.
+  if (a.rows <= 16 * num_sms()) return launch_append<T, D, BITS, true>(a, st);
+  return launch_append<T, D, BITS, false>(a, st);
+}
+
+template <class T, int D>
+int launch_append_bits(const AppendArgs& a, cudaStream_t st) {
+  for (int side = 0; side < (a.sk.bits == a.sv.bits ? 1 : 2); ++side) {
+    const int bits = side ? a.sv.bits : a.sk.bits;
+    const int rc = bits == 2 ? launch_append_rows<T, D, 2>(a, st)
+                   : bits == 4 ? launch_append_rows<T, D, 4>(a, st)
+                               : launch_append_rows<T, D, 8>(a, st);
+    if (rc) return rc;
+  }
+  return PQ_OK;
 }
 
 // Read: one warp per row, norm * centroid[code].
@@ -165,10 +501,8 @@ int pq_kv_prepare_codec(const float* R, const float* boundaries, const float* ce
   if (codec_bytes < kv::codec_bytes(d, bits))
     return fail(PQ_ERR_WORKSPACE, "pq_kv_prepare_codec needs %zu bytes, got %zu",
                 kv::codec_bytes(d, bits), codec_bytes);
-  const kv::Codec c = kv::codec_of(codec, d);
   kv::prepare_codec_kernel<<<64, 256, 0, (cudaStream_t)stream>>>(
-      R, boundaries, centroids, d, bits, (float*)c.R, (float*)c.RT, (float*)c.bounds,
-      (float*)c.cent, (uint32_t*)c.pairs, (int*)c.exponent);
+      R, boundaries, centroids, d, bits, kv::padded_d(d), kv::codec_of(codec, d));
   PQ_LAUNCH_CHECK("prepare_codec_kernel");
   return PQ_OK;
 }
@@ -184,17 +518,40 @@ int pq_kv_append(const pq_kv_cache* cache, const void* k, const void* v, int dty
   PQ_CHECK_ARG(n >= 0 && n * cache->heads < (1ll << 31), "a call takes fewer than 2^31 rows");
   if (n == 0) return PQ_OK;
   PQ_CHECK_ARG(k && v && slots && positions, "null pointer argument");
-  const int64_t rows = n * cache->heads;
-  const dim3 grid((unsigned)((rows + kv::kAppendWarps - 1) / kv::kAppendWarps), 2);
+  kv::AppendArgs a;
+  a.k = k;
+  a.v = v;
+  a.k_sn = k_stride_n;
+  a.k_sh = k_stride_h;
+  a.v_sn = v_stride_n;
+  a.v_sh = v_stride_h;
+  a.rows = n * cache->heads;
+  a.slots_end = (int64_t)cache->pages * cache->page_size;
+  a.heads = cache->heads;
+  a.d = cache->d;
+  a.page_size = cache->page_size;
+  const int size = dtype == PQ_KV_F32 ? 4 : 2;
+  auto vec = [&](const void* p, int64_t sn, int64_t sh) {
+    return (uintptr_t)p % 16 == 0 && sn * size % 16 == 0 && sh * size % 16 == 0 &&
+           cache->d * size % 16 == 0;
+  };
+  a.k_vec = vec(k, k_stride_n, k_stride_h);
+  a.v_vec = vec(v, v_stride_n, v_stride_h);
+  a.sk = kv::side_k(*cache);
+  a.sv = kv::side_v(*cache);
+  a.slots = slots;
+  a.positions = positions;
+  a.weights = weights;
+  a.out_pos = cache->positions;
+  a.out_w = cache->weights;
+  const int D = kv::padded_d(cache->d);
+  const cudaStream_t st = (cudaStream_t)stream;
   PQ_KV_DISPATCH_T(dtype, {
-    kv::append_kernel<T_><<<grid, 32 * kv::kAppendWarps, 0, (cudaStream_t)stream>>>(
-        (const T_*)k, (const T_*)v, k_stride_n, k_stride_h, v_stride_n, v_stride_h, n,
-        cache->heads, cache->d, (int64_t)cache->pages * cache->page_size, cache->page_size,
-        kv::side_k(*cache), kv::side_v(*cache), slots, positions, weights, cache->positions,
-        cache->weights);
+    rc = D == 64 ? kv::launch_append_bits<T_, 64>(a, st)
+                 : D == 128 ? kv::launch_append_bits<T_, 128>(a, st)
+                            : kv::launch_append_bits<T_, 256>(a, st);
   });
-  PQ_LAUNCH_CHECK("kv::append_kernel");
-  return PQ_OK;
+  return rc;
 }
 
 int pq_kv_read(const pq_kv_cache* cache, const int64_t* slots, int64_t n, void* k, void* v,

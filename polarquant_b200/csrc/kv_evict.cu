@@ -2,21 +2,36 @@
 //
 // For every sequence and head: the `budget` first tokens by (protected, weight
 // descending, slot ascending) stay.  A radix selection on a monotone 32-bit key
-// of the weight finds the key of the last one that stays and how many of its
-// equals do; then the evicted tokens before the budget (holes) and the kept
-// ones behind it (movers), equally many, are listed in slot order and
-// move_kernel copies the j-th mover to the j-th hole.  Sources lie behind the
-// budget and destinations before it, so the copies do not depend on each other.
+// of the weight (11, 11 and 10 bits) finds the key of the last one that stays
+// and how many of its equals do; then the evicted tokens before the budget
+// (holes) and the kept ones behind it (movers), equally many, are listed in slot
+// order and kv_move_kernel copies the j-th mover to the j-th hole.  Sources lie
+// behind the budget and destinations before it, so the copies do not depend on
+// each other, and what does not have to move stays: at a constant budget a step
+// moves as many rows as it evicts.
+//
+// A sequence and head is one block, or a cluster of eight when tables have room
+// for more than 4096 tokens: each block keeps the keys of an eighth of the
+// tokens in shared memory (up to kKeep; beyond that they are read again), counts
+// go to the first block's histogram through distributed shared memory.  One
+// pass over weights and positions; bound by the latency of some eight cluster
+// barriers (65536 tokens, 48 heads: DRAM time is 2 us).
+#include <cooperative_groups.h>
+
 #include "kv.cuh"
 
 namespace pqb {
 namespace kv {
 
-constexpr int kEvictThreads = 1024;
+namespace cg = cooperative_groups;
+
+constexpr int kEvictThreads = 512;
+constexpr int kKeep = 16384;  // keys of a block in shared memory
+constexpr int kBins = 2048;
 
 struct EvictArgs {
   Side sk, sv;
-  int heads, pages, page_size, table_width, budget, recent, sinks;
+  int heads, pages, page_shift, table_width, budget, recent, sinks;
   const int32_t* table;
   int64_t table_stride;
   const int32_t* lengths;
@@ -31,19 +46,15 @@ struct EvictArgs {
   int64_t list_width;
 
   __device__ int length(int b) const {
-    const int len = clamp_length(lengths[b], table_width, page_size);
+    const int len = clamp_length(lengths[b], table_width, 1 << page_shift);
     return prompt ? min(len, prompt_width) : len;
   }
   // Index of token t in the pools of one value a token; -1 without a page.
   __device__ int64_t at(int b, int h, int t) const {
-    const int pg = table[b * table_stride + t / page_size];
-    return pg >= 0 && pg < pages ? ((int64_t)pg * heads + h) * page_size + t % page_size : -1;
-  }
-  __device__ int position(int64_t at, int t) const {
-    return prompt ? t : (at < 0 ? INT32_MIN : positions[at]);
-  }
-  __device__ float weight(int b, int h, int64_t at, int t) const {
-    return prompt ? prompt[b * prompt_sb + h * prompt_sh + t] : (at < 0 ? -INFINITY : weights[at]);
+    const int pg = __ldg(table + b * table_stride + (t >> page_shift));
+    return pg >= 0 && pg < pages
+               ? (((int64_t)pg * heads + h) << page_shift) + (t & ((1 << page_shift) - 1))
+               : -1;
   }
 };
 
@@ -55,8 +66,9 @@ __device__ __forceinline__ uint32_t weight_key(float w, bool safe) {
   return (u >> 31) ? ~u : (u | 0x80000000u);
 }
 
-// Exclusive prefix sum over the block; `total` gets the sum.
+// Exclusive prefix sum over the block's kEvictThreads; `total` gets the sum.
 __device__ __forceinline__ int block_scan(int x, int* s_warp, int& total) {
+  constexpr int warps = kEvictThreads / 32;
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   int v = x;
 #pragma unroll
@@ -67,135 +79,250 @@ __device__ __forceinline__ int block_scan(int x, int* s_warp, int& total) {
   __syncthreads();
   if (lane == 31) s_warp[warp] = v;
   __syncthreads();
-  if (warp == 0) {
-    int w = s_warp[lane];
+  int before = 0;
+  total = 0;
 #pragma unroll
-    for (int o = 1; o < 32; o <<= 1) {
-      const int y = __shfl_up_sync(0xffffffffu, w, o);
-      if (lane >= o) w += y;
-    }
-    s_warp[lane] = w;
+  for (int i = 0; i < warps; ++i) {
+    const int y = s_warp[i];
+    if (i < warp) before += y;
+    total += y;
   }
-  __syncthreads();
-  total = s_warp[31];
-  return v - x + (warp ? s_warp[warp - 1] : 0);
+  return v - x + before;
 }
 
-__global__ void __launch_bounds__(kEvictThreads) select_kernel(EvictArgs a) {
-  __shared__ int s_hist[256], s_warp[32], s_max, s_digit, s_need;
-  const int b = blockIdx.x / a.heads, h = blockIdx.x % a.heads, tid = threadIdx.x;
+template <int CL>
+__global__ void __launch_bounds__(kEvictThreads) kv_select_kernel(EvictArgs a) {
+  extern __shared__ uint32_t s_key[];
+  __shared__ int s_hist[kBins], s_warp[32], s_rank[3][CL], s_max, s_digit, s_left;
+  auto cluster = cg::this_cluster();
+  const int rank = CL > 1 ? (int)cluster.block_rank() : 0;
+  const int row = blockIdx.x / CL, b = row / a.heads, h = row % a.heads, tid = threadIdx.x;
+  auto sync = [&] {
+    if constexpr (CL > 1)
+      cluster.sync();
+    else
+      __syncthreads();
+  };
+  // A shared variable of block r of the cluster.
+  auto of = [&](int* p, int r) {
+    if constexpr (CL > 1)
+      return cluster.map_shared_rank(p, r);
+    else
+      return p;
+  };
   const int len = a.length(b);
-  if (h == 0 && tid == 0) a.new_lengths[b] = min(len, a.budget);
-  int32_t* holes = a.lists + (int64_t)blockIdx.x * 2 * a.list_width;
-  int32_t* movers = holes + a.list_width;
-  if (len <= a.budget) {
-    if (tid == 0) a.counts[blockIdx.x] = 0;
-    if (a.prompt)
-      for (int t = tid; t < len; t += kEvictThreads) {
+  const int chunk = (len + CL - 1) / CL, begin = min(rank * chunk, len),
+            end = min(begin + chunk, len);
+  if (h == 0 && rank == 0 && tid == 0) a.new_lengths[b] = min(len, a.budget);
+  const float* given = a.prompt ? a.prompt + b * a.prompt_sb + h * a.prompt_sh : nullptr;
+  if (len <= a.budget) {  // the same for the whole cluster
+    if (rank == 0 && tid == 0) a.counts[row] = 0;
+    if (given)
+      for (int t = begin + tid; t < end; t += kEvictThreads) {
         const int64_t at = a.at(b, h, t);
         if (at >= 0) {
-          a.weights[at] = a.weight(b, h, at, t);
+          a.weights[at] = given[t];
           a.positions[at] = t;
         }
       }
     return;
   }
+
   // The largest position.
-  if (tid == 0) s_max = INT32_MIN;
-  __syncthreads();
-  int mx = INT32_MIN;
-  if (a.prompt)
-    mx = len - 1;
-  else
-    for (int t = tid; t < len; t += kEvictThreads) mx = max(mx, a.position(a.at(b, h, t), t));
-  atomicMax(&s_max, mx);
-  __syncthreads();
-  const int64_t recent_from = (int64_t)s_max - a.recent;
-  auto key = [&](int t) {
+  int64_t recent_from = (int64_t)(len - 1) - a.recent;
+  if (!given) {
+    int mx = INT32_MIN;
+    if (a.recent > 0)
+      for (int t = begin + tid; t < end; t += kEvictThreads) {
+        const int64_t at = a.at(b, h, t);
+        if (at >= 0) mx = max(mx, a.positions[at]);
+      }
+    if (tid == 0) s_max = INT32_MIN;
+    sync();
+    mx = __reduce_max_sync(0xffffffffu, mx);
+    if ((tid & 31) == 0 && mx != INT32_MIN)
+      for (int r = 0; r < CL; ++r) atomicMax(of(&s_max, r), mx);
+    sync();
+    recent_from = a.recent > 0 ? (int64_t)s_max - a.recent : INT64_MAX;
+  } else if (a.recent == 0) {
+    recent_from = INT64_MAX;
+  }
+  auto read_key = [&](int t) {
     const int64_t at = a.at(b, h, t);
     if (at < 0) return 0u;
-    const int pos = a.position(at, t);
-    return weight_key(a.weight(b, h, at, t),
-                      pos < a.sinks || (int64_t)pos > recent_from);
+    const int pos = given ? t : (a.sinks > 0 || a.recent > 0 ? a.positions[at] : INT32_MAX);
+    const bool safe = pos < a.sinks || (int64_t)pos > recent_from;
+    return weight_key(given ? __ldg(given + t) : a.weights[at], safe);
   };
-  // The key of the last token that stays, eight bits at a time.
+  for (int t = begin + tid; t < min(end, begin + kKeep); t += kEvictThreads)
+    s_key[t - begin] = read_key(t);
+  auto key = [&](int t) { return t - begin < kKeep ? s_key[t - begin] : read_key(t); };
+
+  // The key of the last token that stays, and how many of its equals do.
   uint32_t prefix = 0, mask = 0;
   int need = a.budget;
-  for (int shift = 24; shift >= 0 && need > 0; shift -= 8) {
-    if (tid < 256) s_hist[tid] = 0;
-    __syncthreads();
-    for (int t = tid; t < len; t += kEvictThreads) {
+#pragma unroll 1
+  for (int pass = 0; pass < 3 && a.budget > 0; ++pass) {
+    const int shift = pass == 0 ? 21 : pass == 1 ? 10 : 0, bits = pass == 2 ? 10 : 11;
+    for (int i = tid; i < kBins; i += kEvictThreads) s_hist[i] = 0;
+    sync();
+    for (int t = begin + tid; t < end; t += kEvictThreads) {
       const uint32_t k = key(t);
-      if ((k & mask) == prefix) atomicAdd(&s_hist[(k >> shift) & 255u], 1);
+      if ((k & mask) == prefix) atomicAdd(&s_hist[(k >> shift) & ((1u << bits) - 1u)], 1);
     }
-    __syncthreads();
-    if (tid == 0) {
-      int dgt = 255, left = need;
-      while (dgt > 0 && s_hist[dgt] < left) left -= s_hist[dgt--];
-      s_digit = dgt;
-      s_need = left;
-    }
-    __syncthreads();
-    prefix |= (uint32_t)s_digit << shift;
-    mask |= 255u << shift;
-    need = s_need;
-    __syncthreads();
-  }
-  // Tokens above `prefix` and the first `need` of its equals stay.  In slot
-  // order: ties taken, holes and movers so far.
-  int ties = 0, nh = 0, nm = 0;
-  for (int t0 = 0; t0 < len; t0 += kEvictThreads) {
-    const int t = t0 + tid;
-    const uint32_t k = t < len ? key(t) : 0u;
-    const bool tie = t < len && k == prefix;
-    int total;
-    const int rank = block_scan(tie, s_warp, total) + ties;
-    ties += total;
-    const bool kept = t < len && a.budget > 0 && (k > prefix || (tie && rank < need));
-    const bool hole = t < min(len, a.budget) && !kept, mover = kept && t >= a.budget;
-    const int both = block_scan((hole ? 1 : 0) | (mover ? 1 << 16 : 0), s_warp, total);
-    if (hole) holes[nh + (both & 0xffff)] = t;
-    if (mover) movers[nm + (both >> 16)] = t;
-    nh += total & 0xffff;
-    nm += total >> 16;
-    if (a.prompt && kept && !mover) {
-      const int64_t at = a.at(b, h, t);
-      if (at >= 0) {
-        a.weights[at] = a.weight(b, h, at, t);
-        a.positions[at] = t;
+    if constexpr (CL > 1) {
+      __syncthreads();
+      if (rank) {
+        int* first = of(s_hist, 0);
+        for (int i = tid; i < kBins; i += kEvictThreads)
+          if (s_hist[i]) atomicAdd(first + i, s_hist[i]);
       }
     }
+    sync();
+    if (rank == 0) {
+      // Four bins a thread from the highest down: where the count reaches `need`.
+      constexpr int each = kBins / kEvictThreads;
+      int c[each], sum = 0, total;
+#pragma unroll
+      for (int i = 0; i < each; ++i) {
+        c[i] = s_hist[kBins - 1 - (tid * each + i)];
+        sum += c[i];
+      }
+      int before = block_scan(sum, s_warp, total);
+#pragma unroll
+      for (int i = 0; i < each; ++i) {
+        if (before < need && before + c[i] >= need)
+          for (int r = 0; r < CL; ++r) {
+            *of(&s_digit, r) = kBins - 1 - (tid * each + i);
+            *of(&s_left, r) = need - before;
+          }
+        before += c[i];
+      }
+    }
+    sync();
+    prefix |= (uint32_t)s_digit << shift;
+    mask |= ((1u << bits) - 1u) << shift;
+    need = s_left;
   }
-  if (tid == 0) a.counts[blockIdx.x] = min(nh, nm);
+
+  // Tokens above `prefix` and the first `need` of its equals stay: count the
+  // equals before this block, then its holes and movers, then list them.
+  const int budget = a.budget;
+  int ties = 0;
+  if (budget > 0) {
+    for (int t = begin + tid; t < end; t += kEvictThreads) ties += key(t) == prefix;
+    ties = __reduce_add_sync(0xffffffffu, ties);
+  }
+  if (tid < CL) s_rank[0][tid] = 0;
+  sync();
+  if ((tid & 31) == 0 && ties)
+    for (int r = 0; r < CL; ++r) atomicAdd(of(&s_rank[0][rank], r), ties);
+  sync();
+  int tie0 = 0;
+  for (int r = 0; r < rank; ++r) tie0 += s_rank[0][r];
+  int32_t* holes = a.lists + (int64_t)row * 2 * a.list_width;
+  int32_t* movers = holes + a.list_width;
+  // Twice the same walk: to count, and with what the blocks before have to write.
+  int nh = 0, nm = 0;
+#pragma unroll 1
+  for (int pass = CL > 1 ? 0 : 1; pass < 2; ++pass) {
+    int tie = tie0, hs = nh, ms = nm;
+#pragma unroll 1
+    for (int t0 = begin; t0 < end; t0 += kEvictThreads) {
+      const int t = t0 + tid;
+      const uint32_t k = t < end ? key(t) : 0u;
+      const bool eq = t < end && budget > 0 && k == prefix;
+      bool kept = t < end && budget > 0 && k > prefix;
+      int total;
+      if (tie < need && __syncthreads_or(eq)) {
+        const int x = block_scan(eq, s_warp, total);
+        kept = kept || (eq && tie + x < need);
+        tie += total;
+      }
+      const bool hole = t < min(end, budget) && !kept, mover = kept && t >= budget;
+      const int both = block_scan((hole ? 1 : 0) | (mover ? 1 << 16 : 0), s_warp, total);
+      if (pass) {
+        if (hole) holes[hs + (both & 0xffff)] = t;
+        if (mover) movers[ms + (both >> 16)] = t;
+        if (given && kept && !mover) {
+          const int64_t at = a.at(b, h, t);
+          if (at >= 0) {
+            a.weights[at] = given[t];
+            a.positions[at] = t;
+          }
+        }
+      }
+      hs += total & 0xffff;
+      ms += total >> 16;
+    }
+    if (pass == 0) {
+      if (tid == 0)
+        for (int r = 0; r < CL; ++r) {
+          *of(&s_rank[1][rank], r) = hs;
+          *of(&s_rank[2][rank], r) = ms;
+        }
+      sync();
+      for (int r = 0; r < rank; ++r) {
+        nh += s_rank[1][r];
+        nm += s_rank[2][r];
+      }
+    } else if (rank == CL - 1 && tid == 0) {
+      a.counts[row] = min(hs, ms);
+    }
+  }
+  if constexpr (CL > 1) cluster.sync();  // no block leaves while others write to it
 }
 
-// One warp per moved token.
-__global__ void __launch_bounds__(256) move_kernel(EvictArgs a) {
-  const int b = blockIdx.y / a.heads, h = blockIdx.y % a.heads, lane = threadIdx.x & 31;
-  const int n = a.counts[blockIdx.y];
-  const int32_t* holes = a.lists + (int64_t)blockIdx.y * 2 * a.list_width;
+// A warp takes 32 pairs: a lane each for the addresses, then the rows' 16-byte
+// pieces one after another.
+__global__ void __launch_bounds__(256) kv_move_kernel(EvictArgs a) {
+  const int lane = threadIdx.x & 31;
+  const int row = blockIdx.y, b = row / a.heads, h = row % a.heads;
+  const int n = a.counts[row];
+  const int32_t* holes = a.lists + (int64_t)row * 2 * a.list_width;
   const int32_t* movers = holes + a.list_width;
   const int warps = gridDim.x * (blockDim.x >> 5);
-  for (int i = blockIdx.x * (blockDim.x >> 5) + (threadIdx.x >> 5); i < n; i += warps) {
-    const int ts = movers[i];
-    const int64_t to = a.at(b, h, holes[i]), from = a.at(b, h, ts);
-    if (to < 0 || from < 0) continue;
-    const int nk = (int)(a.sk.ldb / 16), nv = (int)(a.sv.ldb / 16);
-    const uint4* ks = reinterpret_cast<const uint4*>(a.sk.rows + from * a.sk.ldb);
-    const uint4* vs = reinterpret_cast<const uint4*>(a.sv.rows + from * a.sv.ldb);
-    uint4* kd = reinterpret_cast<uint4*>(a.sk.rows + to * a.sk.ldb);
-    uint4* vd = reinterpret_cast<uint4*>(a.sv.rows + to * a.sv.ldb);
-    for (int j = lane; j < nk + nv; j += 32) {
-      if (j < nk)
-        kd[j] = ks[j];
-      else
-        vd[j - nk] = vs[j - nk];
+  const int nk = (int)(a.sk.ldb / 16), pieces = nk + (int)(a.sv.ldb / 16);
+  for (int i0 = (blockIdx.x * (blockDim.x >> 5) + (threadIdx.x >> 5)) * 32; i0 < n;
+       i0 += warps * 32) {
+    const int i = i0 + lane;
+    int64_t to = -1, from = -1;
+    if (i < n) {
+      const int ts = movers[i];
+      to = a.at(b, h, holes[i]);
+      from = a.at(b, h, ts);
+      if (to < 0 || from < 0) {
+        to = from = -1;
+      } else {
+        a.sk.norms[to] = a.sk.norms[from];
+        a.sv.norms[to] = a.sv.norms[from];
+        a.positions[to] = a.prompt ? ts : a.positions[from];
+        a.weights[to] =
+            a.prompt ? a.prompt[b * a.prompt_sb + h * a.prompt_sh + ts] : a.weights[from];
+      }
     }
-    if (lane == 0) {
-      a.sk.norms[to] = a.sk.norms[from];
-      a.sv.norms[to] = a.sv.norms[from];
-      a.positions[to] = a.position(from, ts);
-      a.weights[to] = a.weight(b, h, from, ts);
+    // Four loads before their stores.
+    for (int j0 = 0; j0 < pieces; j0 += 4) {
+      uint4 w[4];
+      uint4* dst[4];
+#pragma unroll
+      for (int u = 0; u < 4; ++u) {
+        const int j = lane + 32 * (j0 + u), pair = min(j / pieces, 31), piece = j % pieces;
+        const int64_t x = __shfl_sync(0xffffffffu, from, pair);
+        const int64_t y = __shfl_sync(0xffffffffu, to, pair);
+        dst[u] = nullptr;
+        if (j0 + u < pieces && x >= 0) {
+          const uint8_t* src = piece < nk ? a.sk.rows + x * a.sk.ldb + piece * 16
+                                          : a.sv.rows + x * a.sv.ldb + (piece - nk) * 16;
+          dst[u] = reinterpret_cast<uint4*>(piece < nk
+                                                ? a.sk.rows + y * a.sk.ldb + piece * 16
+                                                : a.sv.rows + y * a.sv.ldb + (piece - nk) * 16);
+          w[u] = *reinterpret_cast<const uint4*>(src);
+        }
+      }
+#pragma unroll
+      for (int u = 0; u < 4; ++u)
+        if (dst[u]) *dst[u] = w[u];
     }
   }
 }
@@ -217,6 +344,27 @@ inline size_t evict_bytes(const pq_kv_cache& c, int batch, int table_width, int 
     a->list_width = w;
   }
   return cv.off;
+}
+
+template <int CL>
+int launch_select(const EvictArgs& a, int rows, int64_t width, cudaStream_t st) {
+  const int keep = (int)min((int64_t)kKeep, (width + CL - 1) / CL);
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3((unsigned)rows * CL);
+  cfg.blockDim = dim3(kEvictThreads);
+  cfg.dynamicSmemBytes = (size_t)keep * 4;
+  cfg.stream = st;
+  cudaLaunchAttribute at;
+  at.id = cudaLaunchAttributeClusterDimension;
+  at.val.clusterDim.x = CL;
+  at.val.clusterDim.y = at.val.clusterDim.z = 1;
+  cfg.attrs = &at;
+  cfg.numAttrs = 1;
+  PQ_CUDA_TRY(cudaFuncSetAttribute(kv_select_kernel<CL>, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                                   kKeep * 4));
+  PQ_CUDA_TRY(cudaLaunchKernelEx(&cfg, kv_select_kernel<CL>, a));
+  PQ_LAUNCH_CHECK("kv_select_kernel");
+  return PQ_OK;
 }
 
 }  // namespace kv
@@ -257,7 +405,8 @@ int pq_kv_evict(const pq_kv_cache* cache, const int32_t* table, int64_t table_st
   a.sv = kv::side_v(c);
   a.heads = c.heads;
   a.pages = c.pages;
-  a.page_size = c.page_size;
+  a.page_shift = 4;
+  while ((1 << a.page_shift) < c.page_size) ++a.page_shift;
   a.table_width = table_width;
   a.budget = budget;
   a.recent = recent;
@@ -274,13 +423,15 @@ int pq_kv_evict(const pq_kv_cache* cache, const int32_t* table, int64_t table_st
   a.new_lengths = new_lengths;
   const cudaStream_t st = (cudaStream_t)stream;
   const int rows = batch * c.heads;
-  kv::select_kernel<<<rows, kv::kEvictThreads, 0, st>>>(a);
-  PQ_LAUNCH_CHECK("kv::select_kernel");
+  const int64_t width = (int64_t)table_width * c.page_size;
+  rc = width <= 4096 ? kv::launch_select<1>(a, rows, width, st)
+                     : kv::launch_select<8>(a, rows, width, st);
+  if (rc) return rc;
   if (a.list_width) {
-    const int64_t per = (a.list_width + 7) / 8;
+    const int64_t per = (a.list_width + 255) / 256;
     const dim3 grid((unsigned)min(per, (int64_t)max(1, 8 * num_sms() / rows)), rows);
-    kv::move_kernel<<<grid, 256, 0, st>>>(a);
-    PQ_LAUNCH_CHECK("kv::move_kernel");
+    kv::kv_move_kernel<<<grid, 256, 0, st>>>(a);
+    PQ_LAUNCH_CHECK("kv_move_kernel");
   }
   return PQ_OK;
 }

@@ -177,13 +177,11 @@ struct AppendShape {
 };
 
 template <class T, int D, int BITS, bool SMALL>
-__global__ void __launch_bounds__(32 * AppendShape<T, D, SMALL>::warps, 1)
-kv_append_kernel(AppendArgs a) {
+__device__ __forceinline__ void append_rows(const AppendArgs& a, uint8_t* smem) {
   using S = AppendShape<T, D, SMALL>;
   constexpr int MT = S::MT;
   constexpr int run_bytes = S::run * BITS / 8, words = (run_bytes + 3) / 4;
   constexpr int cells = BITS == 8 ? kCells : kFewCells;
-  extern __shared__ __align__(16) uint8_t smem[];
   uint2* s_plane = reinterpret_cast<uint2*>(smem);
   uint32_t* s_cell = reinterpret_cast<uint32_t*>(smem + (SMALL ? 0 : 2 * S::plane * sizeof(uint2)));
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
@@ -192,7 +190,6 @@ kv_append_kernel(AppendArgs a) {
   const int part = blockIdx.y >> 1;
   const Side& sd = is_v ? a.sv : a.sk;
   const Codec& cd = sd.c;
-  if (sd.bits != BITS) return;
   const T* src = reinterpret_cast<const T*>(is_v ? a.v : a.k);
   const int64_t sn = is_v ? a.v_sn : a.k_sn, sh = is_v ? a.v_sh : a.k_sh;
   const bool vec = is_v ? a.v_vec : a.k_vec;
@@ -421,64 +418,153 @@ kv_append_kernel(AppendArgs a) {
   }
 }
 
-template <class T, int D, int BITS, bool SMALL>
+template <class T, int D, bool SMALL>
+__global__ void __launch_bounds__(32 * AppendShape<T, D, SMALL>::warps, 1)
+kv_append_kernel(AppendArgs a) {
+  extern __shared__ __align__(16) uint8_t smem[];
+  const int bits = blockIdx.y & 1 ? a.sv.bits : a.sk.bits;
+  if (bits == 2)
+    append_rows<T, D, 2, SMALL>(a, smem);
+  else if (bits == 4)
+    append_rows<T, D, 4, SMALL>(a, smem);
+  else
+    append_rows<T, D, 8, SMALL>(a, smem);
+}
+
+template <class T, int D, bool SMALL>
 int launch_append(const AppendArgs& a, cudaStream_t st) {
   using S = AppendShape<T, D, SMALL>;
-  constexpr int smem = (SMALL ? 0 : 2 * S::plane * (int)sizeof(uint2)) +
-                       (BITS == 8 ? kCells * 8 : kFewCells * 128);
-  auto kern = kv_append_kernel<T, D, BITS, SMALL>;
+  constexpr int smem =
+      (SMALL ? 0 : 2 * S::plane * (int)sizeof(uint2)) + (kCells * 8 > kFewCells * 128 ? kCells * 8 : kFewCells * 128);
+  auto kern = kv_append_kernel<T, D, SMALL>;
   PQ_CUDA_TRY(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, smem));
   const int64_t groups = (a.rows + S::rows - 1) / S::rows;
   const int64_t blocks = (groups + S::groups - 1) / S::groups;
-  // A launch for both sides where their bits are the same; a side of other bits
-  // leaves at once.
   const int64_t most = SMALL ? 1 << 20 : max(1, num_sms() / (2 * S::parts));
   kern<<<dim3((unsigned)min(blocks, most), 2 * S::parts), 32 * S::warps, smem, st>>>(a);
   PQ_LAUNCH_CHECK("kv_append_kernel");
   return PQ_OK;
 }
 
-template <class T, int D, int BITS>
+template <class T, int D>
 int launch_append_rows(const AppendArgs& a, cudaStream_t st) {
   // Few rows: as many blocks of 16 rows as there are, each reading the planes
   // from L2; more than two waves of them: resident planes.
-  if (a.rows <= 16 * num_sms()) return launch_append<T, D, BITS, true>(a, st);
-  return launch_append<T, D, BITS, false>(a, st);
+  if (a.rows <= 16 * num_sms()) return launch_append<T, D, true>(a, st);
+  return launch_append<T, D, false>(a, st);
 }
 
-template <class T, int D>
-int launch_append_bits(const AppendArgs& a, cudaStream_t st) {
-  for (int side = 0; side < (a.sk.bits == a.sv.bits ? 1 : 2); ++side) {
-    const int bits = side ? a.sv.bits : a.sk.bits;
-    const int rc = bits == 2 ? launch_append_rows<T, D, 2>(a, st)
-                   : bits == 4 ? launch_append_rows<T, D, 4>(a, st)
-                               : launch_append_rows<T, D, 8>(a, st);
-    if (rc) return rc;
-  }
-  return PQ_OK;
-}
+// ---------------------------------------------------------------------------
+// Read: norm * centroid[code], rounded once.
+//
+// A lane takes 16 codes of a row; a warp 32 such pieces of one token.  Bound by
+// the bytes written; the lookups are from tables with a copy for each lane (or
+// each pair of lanes half a warp apart, for 64-bit entries): an f32 centroid at
+// 8 bits, both of a byte's at 4, both of a nibble's at 2.
+// ---------------------------------------------------------------------------
 
-// Read: one warp per row, norm * centroid[code].
-template <class T>
-__global__ void __launch_bounds__(256)
-read_kernel(Side sk, Side sv, const int64_t* __restrict__ slots, int64_t n, int heads, int d,
-            int64_t slots_end, int page_size, T* __restrict__ ok, T* __restrict__ ov) {
-  __shared__ float cent[256];
-  const Side& s = blockIdx.y ? sv : sk;
-  T* out = blockIdx.y ? ov : ok;
-  if (threadIdx.x < 256) cent[threadIdx.x] = s.c.cent[threadIdx.x];
-  __syncthreads();
+struct ReadArgs {
+  Side sk, sv;
+  const int64_t* slots;
+  int64_t n, slots_end;
+  int heads, d, page_size, pieces, per_token;  // 16-code pieces of a row, warps of a token
+  bool vec;                                    // rows of the output are 16-byte aligned
+  void *k, *v;
+};
+
+constexpr int kReadThreads = 512;
+
+template <class T, int BITS>
+__device__ __forceinline__ void read_rows(const ReadArgs& a, uint32_t* table) {
+  const bool is_v = blockIdx.y != 0;
+  const Side& s = is_v ? a.sv : a.sk;
+  T* out = reinterpret_cast<T*>(is_v ? a.v : a.k);
   const int lane = threadIdx.x & 31;
-  const int64_t r = (int64_t)blockIdx.x * (blockDim.x >> 5) + (threadIdx.x >> 5);
-  if (r >= n * heads) return;
-  const int64_t slot = slots[r / heads];
-  const bool in = slot >= 0 && slot < slots_end;
-  const int64_t at =
-      in ? ((slot / page_size) * heads + r % heads) * page_size + slot % page_size : 0;
-  const float nrm = in ? s.norms[at] : 0.f;
-  for (int j = lane; j < d; j += 32)
-    out[r * d + j] =
-        from_f32<T>(in ? __fmul_rn(nrm, cent[code_at(s.rows + at * s.ldb, j, s.bits)]) : 0.f);
+  constexpr int entries = BITS == 2 ? 16 : 256;  // of 128 bytes
+  for (int i = threadIdx.x; i < entries * 32; i += kReadThreads) {
+    const int e = i >> 5;
+    float c;
+    if (BITS == 8)
+      c = s.c.cent[e];
+    else
+      c = s.c.cent[i & 1 ? e & ((1 << BITS) - 1) : e >> BITS];
+    table[i] = __float_as_uint(c);
+  }
+  __syncthreads();
+  const uint32_t base = (uint32_t)__cvta_generic_to_shared(table) +
+                        (BITS == 8 ? lane * 4 : (lane & 15) * 8);
+  const int64_t tasks = a.n * a.per_token;
+  const int64_t step = (int64_t)gridDim.x * (kReadThreads / 32);
+  for (int64_t w = (int64_t)blockIdx.x * (kReadThreads / 32) + (threadIdx.x >> 5); w < tasks;
+       w += step) {
+    const int64_t tok = a.per_token == 1 ? w : w / a.per_token;
+    const int unit = (int)(w - tok * a.per_token) * 32 + lane;
+    const int h = unit / a.pieces, piece = unit - h * a.pieces;
+    if (h >= a.heads) continue;
+    const int64_t slot = a.slots[tok];
+    const bool in = slot >= 0 && slot < a.slots_end;
+    uint32_t x[4] = {0u, 0u, 0u, 0u};
+    float nrm = 0.f;
+    if (in) {
+      const int64_t at =
+          (((int64_t)((uint32_t)slot / (uint32_t)a.page_size)) * a.heads + h) * a.page_size +
+          (uint32_t)slot % (uint32_t)a.page_size;
+      const uint8_t* row = s.rows + at * s.ldb + piece * (2 * BITS);
+      if (BITS == 8)
+        *reinterpret_cast<uint4*>(x) = *reinterpret_cast<const uint4*>(row);
+      else if (BITS == 4)
+        *reinterpret_cast<uint2*>(x) = *reinterpret_cast<const uint2*>(row);
+      else
+        x[0] = *reinterpret_cast<const uint32_t*>(row);
+      nrm = s.norms[at];
+    }
+    float f[16];
+#pragma unroll
+    for (int i = 0; i < (BITS == 8 ? 16 : 8); ++i) {
+      if constexpr (BITS == 8) {
+        asm("ld.shared.f32 %0, [%1];"
+            : "=f"(f[i])
+            : "r"(__dp4a(x[i >> 2], 128u << (8 * (i & 3)), base)));
+      } else {
+        uint32_t at;
+        if constexpr (BITS == 4) {
+          at = __dp4a(x[i >> 2], 128u << (8 * (i & 3)), base);
+        } else {
+          // nibble i, the high one of a byte first
+          const int low = (i >> 1) * 8 + (i & 1 ? 0 : 4);
+          at = base + ((x[0] >> low) & 15u) * 128u;
+        }
+        asm("ld.shared.v2.f32 {%0,%1}, [%2];" : "=f"(f[2 * i]), "=f"(f[2 * i + 1]) : "r"(at));
+      }
+    }
+    __align__(16) T y[16];
+#pragma unroll
+    for (int i = 0; i < 16; ++i) y[i] = from_f32<T>(in ? __fmul_rn(nrm, f[i]) : 0.f);
+    T* to = out + ((tok * a.heads + h) * a.d + piece * 16);
+    const int left = a.d - piece * 16;
+    if (a.vec) {
+      constexpr int E = 16 / sizeof(T);
+#pragma unroll
+      for (int i = 0; i < 16; i += E)
+        if (i < left) *reinterpret_cast<uint4*>(to + i) = *reinterpret_cast<const uint4*>(y + i);
+    } else {
+#pragma unroll
+      for (int i = 0; i < 16; ++i)
+        if (i < left) to[i] = y[i];
+    }
+  }
+}
+
+template <class T>
+__global__ void __launch_bounds__(kReadThreads) kv_read_kernel(ReadArgs a) {
+  __shared__ uint32_t table[256 * 32];
+  const int bits = blockIdx.y ? a.sv.bits : a.sk.bits;
+  if (bits == 2)
+    read_rows<T, 2>(a, table);
+  else if (bits == 4)
+    read_rows<T, 4>(a, table);
+  else
+    read_rows<T, 8>(a, table);
 }
 
 }  // namespace kv
@@ -547,9 +633,9 @@ int pq_kv_append(const pq_kv_cache* cache, const void* k, const void* v, int dty
   const int D = kv::padded_d(cache->d);
   const cudaStream_t st = (cudaStream_t)stream;
   PQ_KV_DISPATCH_T(dtype, {
-    rc = D == 64 ? kv::launch_append_bits<T_, 64>(a, st)
-                 : D == 128 ? kv::launch_append_bits<T_, 128>(a, st)
-                            : kv::launch_append_bits<T_, 256>(a, st);
+    rc = D == 64 ? kv::launch_append_rows<T_, 64>(a, st)
+                 : D == 128 ? kv::launch_append_rows<T_, 128>(a, st)
+                            : kv::launch_append_rows<T_, 256>(a, st);
   });
   return rc;
 }
@@ -563,13 +649,27 @@ int pq_kv_read(const pq_kv_cache* cache, const int64_t* slots, int64_t n, void* 
   PQ_CHECK_ARG(n >= 0 && n * cache->heads < (1ll << 31), "a call takes fewer than 2^31 rows");
   if (n == 0) return PQ_OK;
   PQ_CHECK_ARG(slots && k && v, "null pointer argument");
-  const dim3 grid((unsigned)((n * cache->heads + 7) / 8), 2);
+  kv::ReadArgs a;
+  a.sk = kv::side_k(*cache);
+  a.sv = kv::side_v(*cache);
+  a.slots = slots;
+  a.n = n;
+  a.slots_end = (int64_t)cache->pages * cache->page_size;
+  a.heads = cache->heads;
+  a.d = cache->d;
+  a.page_size = cache->page_size;
+  a.pieces = (cache->d + 15) / 16;
+  a.per_token = (int)(((int64_t)cache->heads * a.pieces + 31) / 32);
+  a.k = k;
+  a.v = v;
+  a.vec = cache->d * (dtype == PQ_KV_F32 ? 4 : 2) % 16 == 0 && (uintptr_t)k % 16 == 0 &&
+          (uintptr_t)v % 16 == 0;
+  const int64_t blocks = (n * a.per_token + kv::kReadThreads / 32 - 1) / (kv::kReadThreads / 32);
+  const dim3 grid((unsigned)min(blocks, (int64_t)2 * num_sms()), 2);
   PQ_KV_DISPATCH_T(dtype, {
-    kv::read_kernel<T_><<<grid, 256, 0, (cudaStream_t)stream>>>(
-        kv::side_k(*cache), kv::side_v(*cache), slots, n, cache->heads, cache->d,
-        (int64_t)cache->pages * cache->page_size, cache->page_size, (T_*)k, (T_*)v);
+    kv::kv_read_kernel<T_><<<grid, kv::kReadThreads, 0, (cudaStream_t)stream>>>(a);
   });
-  PQ_LAUNCH_CHECK("kv::read_kernel");
+  PQ_LAUNCH_CHECK("kv_read_kernel");
   return PQ_OK;
 }
 

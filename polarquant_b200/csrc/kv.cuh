@@ -68,6 +68,12 @@ inline Side side_v(const pq_kv_cache& c) {
   return Side{c.v_rows, c.v_norms, c.v_ldb, c.v_bits, codec_of(c.v_codec, c.d)};
 }
 
+inline int page_shift_of(const pq_kv_cache& c) {
+  int s = 4;
+  while ((1 << s) < c.page_size) ++s;
+  return s;
+}
+
 inline bool bits_ok(int b) { return b == 2 || b == 4 || b == 8; }
 
 inline int check_cache(const pq_kv_cache* c) {

@@ -1006,8 +1006,7 @@ int launch_attend(const pq_kv_cache& c, Work wk, const AttendPlan& p, int worker
                   cudaStream_t st) {
   using Shape = AttendShape<D, KB, VB, PREC>;
   auto kern = kv_attend_kernel<D, KB, VB, PREC>;
-  int page_shift = 4;
-  while ((1 << page_shift) < c.page_size) ++page_shift;
+  const int page_shift = page_shift_of(c);
   static_assert(Shape::warps >= 4 && Shape::unit >= kLeastUnit, "too little shared memory");
   PQ_CUDA_TRY(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize,
                                    (int)Shape::smem));

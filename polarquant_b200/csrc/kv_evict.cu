@@ -405,8 +405,7 @@ int pq_kv_evict(const pq_kv_cache* cache, const int32_t* table, int64_t table_st
   a.sv = kv::side_v(c);
   a.heads = c.heads;
   a.pages = c.pages;
-  a.page_shift = 4;
-  while ((1 << a.page_shift) < c.page_size) ++a.page_shift;
+  a.page_shift = kv::page_shift_of(c);
   a.table_width = table_width;
   a.budget = budget;
   a.recent = recent;

@@ -150,8 +150,9 @@ __device__ __forceinline__ void mma_rows(float (&c)[4], const uint32_t (&a)[4], 
 struct AppendArgs {
   const void *k, *v;
   int64_t k_sn, k_sh, v_sn, v_sh;
-  int64_t rows, slots_end;
-  int heads, d, page_size;
+  uint32_t rows, heads;
+  int64_t slots_end;
+  int d, page_shift;
   bool k_vec, v_vec;  // rows can be read 16 bytes at a time
   Side sk, sv;
   const int64_t* slots;
@@ -159,7 +160,18 @@ struct AppendArgs {
   const float* weights;
   int32_t* out_pos;
   float* out_w;
+
+  // Index of row r (token r / heads, head r % heads) in the pool; -1 for none.
+  __device__ int64_t place(uint32_t r) const {
+    const int64_t slot = slots[r / heads];
+    if (slot < 0 || slot >= slots_end) return -1;
+    const uint32_t s = (uint32_t)slot;
+    return ((int64_t)(s >> page_shift) * heads + r % heads << page_shift) +
+           (s & ((1u << page_shift) - 1u));
+  }
 };
+
+constexpr int kCellWords = 2 * kCells > 32 * kFewCells ? 2 * kCells : 32 * kFewCells;
 
 template <class T, int D, bool SMALL>
 struct AppendShape {
@@ -174,7 +186,24 @@ struct AppendShape {
   static constexpr int groups = SMALL ? 1 : warps;           // row groups of a block at a time
   static constexpr int run = per * 8;                        // columns of a lane in a row
   static constexpr int plane = D / 8 / parts * steps * 32;   // uint2 of a plane in the block
+  static constexpr int plane_bytes = SMALL ? 0 : 2 * plane * 8;
+  static constexpr int smem = plane_bytes + 4 * kCellWords + warps * 2 * MT * 8 * 128;
 };
+
+// 16 bytes of x as f32.
+template <class T>
+__device__ __forceinline__ void widen16(const uint4& w, float* f) {
+  if constexpr (sizeof(T) == 4) {
+    f[0] = __uint_as_float(w.x);
+    f[1] = __uint_as_float(w.y);
+    f[2] = __uint_as_float(w.z);
+    f[3] = __uint_as_float(w.w);
+  } else {
+    const T* e = reinterpret_cast<const T*>(&w);
+#pragma unroll
+    for (int k = 0; k < 8; ++k) f[k] = to_f32<T>(e[k]);
+  }
+}
 
 template <class T, int D, int BITS, bool SMALL>
 __device__ __forceinline__ void append_rows(const AppendArgs& a, uint8_t* smem) {
@@ -183,8 +212,10 @@ __device__ __forceinline__ void append_rows(const AppendArgs& a, uint8_t* smem) 
   constexpr int run_bytes = S::run * BITS / 8, words = (run_bytes + 3) / 4;
   constexpr int cells = BITS == 8 ? kCells : kFewCells;
   uint2* s_plane = reinterpret_cast<uint2*>(smem);
-  uint32_t* s_cell = reinterpret_cast<uint32_t*>(smem + (SMALL ? 0 : 2 * S::plane * sizeof(uint2)));
+  uint32_t* s_cell = reinterpret_cast<uint32_t*>(smem + S::plane_bytes);
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
+  // The lane's packed runs, one of each of its rows: word w of row i.
+  uint32_t* s_run = s_cell + kCellWords + warp * (2 * MT * 8 * 32) + lane;
   // blockIdx.y: the part of the columns and, lowest, the side.
   const bool is_v = blockIdx.y & 1;
   const int part = blockIdx.y >> 1;
@@ -194,6 +225,7 @@ __device__ __forceinline__ void append_rows(const AppendArgs& a, uint8_t* smem) 
   const int64_t sn = is_v ? a.v_sn : a.k_sn, sh = is_v ? a.v_sh : a.k_sh;
   const bool vec = is_v ? a.v_vec : a.k_vec;
   const int d = a.d;
+  const uint32_t rows = a.rows, heads = a.heads;
 
   if constexpr (!SMALL) {
     const uint2* p = cd.planes + part * S::plane;
@@ -217,28 +249,28 @@ __device__ __forceinline__ void append_rows(const AppendArgs& a, uint8_t* smem) 
   constexpr float band =
       (S::steps * (S::wide ? 3 : 2) + 8) * 1.1920929e-7f + (BITS == 8 ? 0.f : 1e-6f);
 
-  const int64_t groups = (a.rows + S::rows - 1) / S::rows;
-  for (int64_t gr = (int64_t)blockIdx.x * S::groups + (SMALL ? 0 : warp); gr < groups;
-       gr += (int64_t)gridDim.x * S::groups) {
+  const uint32_t groups = (rows + S::rows - 1) / S::rows;
+#pragma unroll 1
+  for (uint32_t gr = blockIdx.x * S::groups + (SMALL ? 0 : warp); gr < groups;
+       gr += gridDim.x * S::groups) {
     // x of rows g, g + 8 (, g + 16, g + 24) in f32, a quarter of each a lane.
-    const int64_t row0 = gr * S::rows;
+    const uint32_t row0 = gr * S::rows;
     uint32_t ah[MT][S::steps][4], al[S::wide ? MT : 1][S::wide ? S::steps : 1][4];
-    float inv[2 * MT], den[2 * MT], nrm[2 * MT];
+    float inv[2 * MT], den[2 * MT];
 #pragma unroll
     for (int i = 0; i < 2 * MT; ++i) {
-      const int64_t r = min(row0 + g + 8 * i, a.rows - 1);
-      const T* x = src + (r / a.heads) * sn + (r % a.heads) * sh + t * (D / 4);
+      const uint32_t r = min(row0 + g + 8 * i, rows - 1);
+      const T* x = src + (int64_t)(r / heads) * sn + (r % heads) * sh + t * (D / 4);
       float f[D / 4];
+      constexpr int E = 16 / sizeof(T);
       if (vec) {
-        constexpr int E = 16 / sizeof(T);
+        uint4 w[D / 4 / E];
 #pragma unroll
-        for (int j = 0; j < D / 4; j += E) {
-          uint4 w = make_uint4(0u, 0u, 0u, 0u);
-          if (t * (D / 4) + j < d) w = *reinterpret_cast<const uint4*>(x + j);
-          const T* e = reinterpret_cast<const T*>(&w);
+        for (int j = 0; j < D / 4 / E; ++j)
+          w[j] = t * (D / 4) + j * E < d ? *reinterpret_cast<const uint4*>(x + j * E)
+                                         : make_uint4(0u, 0u, 0u, 0u);
 #pragma unroll
-          for (int k = 0; k < E; ++k) f[j + k] = to_f32<T>(e[k]);
-        }
+        for (int j = 0; j < D / 4 / E; ++j) widen16<T>(w[j], f + j * E);
       } else {
 #pragma unroll
         for (int j = 0; j < D / 4; ++j) f[j] = t * (D / 4) + j < d ? to_f32<T>(x[j]) : 0.f;
@@ -255,10 +287,21 @@ __device__ __forceinline__ void append_rows(const AppendArgs& a, uint8_t* smem) 
         ss += __shfl_xor_sync(0xffffffffu, ss, o);
         mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, o));
       }
-      nrm[i] = __double2float_rn(__dsqrt_rn(ss));
-      den[i] = fmaxf(nrm[i], 1e-8f);
+      const float nrm = __double2float_rn(__dsqrt_rn(ss));
+      den[i] = fmaxf(nrm, 1e-8f);
+      if (t == 0 && part == 0 && (!SMALL || warp == 0) && row0 + g + 8 * i < rows) {
+        const int64_t at = a.place(r);
+        if (at >= 0) {
+          sd.norms[at] = nrm;
+          if (!is_v) {
+            a.out_pos[at] = a.positions[r / heads];
+            a.out_w[at] = a.weights ? a.weights[r] : 0.f;
+          }
+        }
+      }
       // max |x| * 2^e in [2^14, 2^15): f16's range, and sums of at most 2^29 sqrt(d)
-      const int e = mx > 0.f && mx < INFINITY ? max(-126, min(126, 14 - ilogbf(mx))) : 0;
+      const int e =
+          mx > 0.f && mx < INFINITY ? max(-126, min(126, 14 - ilogbf(mx))) : 0;
       const float up = __int_as_float((127 + e) << 23);
       inv[i] = __int_as_float((127 - e) << 23) / 16384.f / den[i];
       // Registers 0 and 2 of the A operand hold row g, 1 and 3 row g + 8.
@@ -277,12 +320,9 @@ __device__ __forceinline__ void append_rows(const AppendArgs& a, uint8_t* smem) 
         }
     }
 
-    uint32_t packed[2 * MT][words];
-#pragma unroll
-    for (int i = 0; i < 2 * MT; ++i)
-#pragma unroll
-      for (int w = 0; w < words; ++w) packed[i][w] = 0u;
-#pragma unroll
+    // Eight columns a lane at a time.  (One body for all: unrolled over the
+    // chunks the code does not fit the instruction cache.)
+#pragma unroll 1
     for (int c = 0; c < S::per; ++c) {
       const int chunk = SMALL ? warp : part * S::per + c;
       float acc[MT][4][4];
@@ -290,20 +330,14 @@ __device__ __forceinline__ void append_rows(const AppendArgs& a, uint8_t* smem) 
       for (int m = 0; m < MT; ++m)
 #pragma unroll
         for (int q = 0; q < 4; ++q) acc[m][q][0] = acc[m][q][1] = acc[m][q][2] = acc[m][q][3] = 0.f;
+      const uint2* bp = SMALL ? cd.planes + chunk * 4 * S::steps * 32 + lane
+                              : s_plane + c * 4 * S::steps * 32 + lane;
+      constexpr int lo_at = SMALL ? D / 8 * S::steps * 32 : S::plane;
 #pragma unroll
       for (int s = 0; s < S::steps; ++s)
 #pragma unroll
         for (int q = 0; q < 4; ++q) {
-          uint2 bh, bl;
-          if constexpr (SMALL) {
-            const int at = ((chunk * 4 + q) * S::steps + s) * 32 + lane;
-            bh = __ldg(cd.planes + at);
-            bl = __ldg(cd.planes + D / 8 * S::steps * 32 + at);
-          } else {
-            const int at = ((c * 4 + q) * S::steps + s) * 32 + lane;
-            bh = s_plane[at];
-            bl = s_plane[S::plane + at];
-          }
+          const uint2 bh = bp[(q * S::steps + s) * 32], bl = bp[lo_at + (q * S::steps + s) * 32];
 #pragma unroll
           for (int m = 0; m < MT; ++m) {
             mma_rows(acc[m][q], ah[m][s], bh);
@@ -311,108 +345,127 @@ __device__ __forceinline__ void append_rows(const AppendArgs& a, uint8_t* smem) 
             if constexpr (S::wide) mma_rows(acc[m][q], al[m][s], bh);
           }
         }
-      // Codes of rows g + 8i, columns t * D / 4 + chunk * 8 + 2q + e.
-      const int col0 = t * (D / 4) + chunk * 8;
+      // Codes of rows g + 8i, columns t * D / 4 + chunk * 8 + k: packed, the first
+      // code highest in its byte, and which of them are next to a boundary.
+      constexpr int cw = BITS == 8 ? 2 : 1;
+      uint32_t packed[2 * MT][cw], near = 0;
+      const int left = min(8, d - (t * (D / 4) + chunk * 8));  // columns that there are
 #pragma unroll
       for (int i = 0; i < 2 * MT; ++i) {
-        uint32_t near = 0, code[8];
+#pragma unroll
+        for (int w = 0; w < cw; ++w) packed[i][w] = 0u;
 #pragma unroll
         for (int k = 0; k < 8; ++k) {
           const float y = acc[i >> 1][k >> 1][2 * (i & 1) + (k & 1)] * inv[i];
           const float cell = fmaf(__saturatef(fmaf(y, cs, co)), (float)(cells - 1), 8388608.f);
           float b;
-          uint32_t below;
+          uint32_t code;
           if constexpr (BITS == 8) {
-            const uint2 e = reinterpret_cast<const uint2*>(s_cell)[__float_as_uint(cell) & (cells - 1)];
+            const uint2 e =
+                reinterpret_cast<const uint2*>(s_cell)[__float_as_uint(cell) & (cells - 1)];
             b = __uint_as_float(e.x);
-            below = e.y;
+            code = e.y;
           } else {
             const uint32_t e = s_cell[(__float_as_uint(cell) & (cells - 1)) * 32 + lane];
             b = __uint_as_float(e);
-            below = e & 15u;
+            code = e & 15u;
           }
           const float off = y - b;
-          code[k] = below + (off > 0.f ? 1u : 0u);
-          if (!(fabsf(off) >= band)) near |= 1u << k;
+          if (off > 0.f) ++code;
+          if (!(fabsf(off) >= band)) near |= 1u << (8 * i + k);
+          const int bit = k * BITS;
+          packed[i][bit >> 5] |= code << ((bit & 24) + 8 - BITS - (bit & 7));
         }
-        if (col0 + 8 > d) {
+      }
+      if (left < 8) {
+        // Bits of the columns behind the row's end are 0.
+#pragma unroll
+        for (int i = 0; i < 2 * MT; ++i)
 #pragma unroll
           for (int k = 0; k < 8; ++k)
-            if (col0 + k >= d) {
-              code[k] = 0u;
-              near &= ~(1u << k);
+            if (k >= left) {
+              const int bit = k * BITS;
+              packed[i][bit >> 5] &=
+                  ~(((1u << BITS) - 1u) << ((bit & 24) + 8 - BITS - (bit & 7)));
+              near &= ~(1u << (8 * i + k));
             }
-        }
-        if (row0 + g + 8 * i >= a.rows) near = 0u;
-        // Coordinates next to a boundary, by the whole warp.
-        uint32_t pend = __ballot_sync(0xffffffffu, near != 0u);
-        while (pend) {
-          const int from = __ffs(pend) - 1;
-          pend &= pend - 1;
-          uint32_t mask = __shfl_sync(0xffffffffu, near, from);
-          const int64_t r = row0 + (from >> 2) + 8 * i;
-          const float dn = __shfl_sync(0xffffffffu, den[i], from);
-          const T* x = src + (r / a.heads) * sn + (r % a.heads) * sh;
-          while (mask) {
-            const int k = __ffs(mask) - 1;
-            mask &= mask - 1;
-            const float* rr = cd.R + ((from & 3) * (D / 4) + chunk * 8 + k) * d;
-            double y = 0.0;
-            for (int j = lane; j < d; j += 32)
-              y = fma((double)__fdiv_rn(to_f32<T>(x[j]), dn), (double)__ldg(rr + j), y);
+      }
 #pragma unroll
-            for (int o = 16; o > 0; o >>= 1) y += __shfl_xor_sync(0xffffffffu, y, o);
-            uint32_t exact = 0;
+      for (int i = 0; i < 2 * MT; ++i)
+        if (row0 + g + 8 * i >= rows) near &= ~(255u << (8 * i));
+      // Coordinates next to a boundary, by the whole warp.
+      uint32_t pend = __ballot_sync(0xffffffffu, near != 0u);
+#pragma unroll 1
+      while (pend) {
+        const int from = __ffs(pend) - 1;
+        pend &= pend - 1;
+        uint32_t mask = __shfl_sync(0xffffffffu, near, from);
+#pragma unroll 1
+        while (mask) {
+          const int n = __ffs(mask) - 1, i = n >> 3, k = n & 7;
+          mask &= mask - 1;
+          float dn = den[0];
 #pragma unroll
-            for (int step = 1 << (BITS - 1); step > 0; step >>= 1)
-              if (y > (double)__ldg(cd.bounds + exact + step - 1)) exact += step;
-            if (lane == from) {
+          for (int z = 1; z < 2 * MT; ++z)
+            if (z == i) dn = den[z];
+          dn = __shfl_sync(0xffffffffu, dn, from);
+          const uint32_t r = row0 + (from >> 2) + 8 * i;
+          const T* x = src + (int64_t)(r / heads) * sn + (r % heads) * sh;
+          const float* rr = cd.R + ((from & 3) * (D / 4) + chunk * 8 + k) * d;
+          double y = 0.0;
+          for (int j = lane; j < d; j += 32)
+            y = fma((double)__fdiv_rn(to_f32<T>(x[j]), dn), (double)__ldg(rr + j), y);
 #pragma unroll
-              for (int z = 0; z < 8; ++z)
-                if (z == k) code[z] = exact;
-            }
+          for (int o = 16; o > 0; o >>= 1) y += __shfl_xor_sync(0xffffffffu, y, o);
+          uint32_t code = 0;
+#pragma unroll
+          for (int step = 1 << (BITS - 1); step > 0; step >>= 1)
+            if (y > (double)__ldg(cd.bounds + code + step - 1)) code += step;
+          const int bit = k * BITS, shift = (bit & 24) + 8 - BITS - (bit & 7);
+          if (lane == from) {
+#pragma unroll
+            for (int z = 0; z < 2 * MT; ++z)
+#pragma unroll
+              for (int w = 0; w < cw; ++w)
+                if (z == i && w == bit >> 5)
+                  packed[z][w] = (packed[z][w] & ~(((1u << BITS) - 1u) << shift)) | code << shift;
           }
         }
-        // Eight codes: BITS bytes, the first code highest in its byte.
+      }
 #pragma unroll
-        for (int k = 0; k < 8; ++k) {
-          const int bit = (c * 8 + k) * BITS;  // of the run
-          packed[i][bit >> 5] |= code[k] << ((bit & 24) + 8 - BITS - (bit & 7));
+      for (int i = 0; i < 2 * MT; ++i) {
+        if constexpr (BITS == 2) {
+          uint16_t* to = reinterpret_cast<uint16_t*>(s_run + (i * 8 + (c >> 1)) * 32) + (c & 1);
+          *to = (uint16_t)packed[i][0];
+        } else {
+#pragma unroll
+          for (int w = 0; w < cw; ++w) s_run[(i * 8 + c * cw + w) * 32] = packed[i][w];
         }
       }
     }
 
-#pragma unroll
+#pragma unroll 1
     for (int i = 0; i < 2 * MT; ++i) {
-      const int64_t r = row0 + g + 8 * i;
-      if (r >= a.rows) continue;
-      const int64_t tok = r / a.heads;
-      const int64_t slot = a.slots[tok];
-      if (slot < 0 || slot >= a.slots_end) continue;
-      const int64_t at =
-          ((slot / a.page_size) * a.heads + r % a.heads) * a.page_size + slot % a.page_size;
+      const uint32_t r = row0 + g + 8 * i;
+      if (r >= rows) break;
+      const int64_t at = a.place(r);
+      if (at < 0) continue;
       const int off = (t * (D / 4) + (SMALL ? warp : part * S::per) * 8) * BITS / 8;
       uint8_t* to = sd.rows + at * sd.ldb + off;
+      const uint32_t* w = s_run + i * 8 * 32;
       if constexpr (run_bytes >= 16) {
 #pragma unroll
-        for (int w = 0; w < words; w += 4)
-          if (off + 4 * w < sd.ldb)
-            *reinterpret_cast<uint4*>(to + 4 * w) =
-                make_uint4(packed[i][w], packed[i][w + 1], packed[i][w + 2], packed[i][w + 3]);
+        for (int j = 0; j < words; j += 4)
+          if (off + 4 * j < sd.ldb)
+            *reinterpret_cast<uint4*>(to + 4 * j) =
+                make_uint4(w[j * 32], w[(j + 1) * 32], w[(j + 2) * 32], w[(j + 3) * 32]);
       } else if (off < sd.ldb) {
         if constexpr (run_bytes == 8)
-          *reinterpret_cast<uint2*>(to) = make_uint2(packed[i][0], packed[i][1]);
+          *reinterpret_cast<uint2*>(to) = make_uint2(w[0], w[32]);
         else if constexpr (run_bytes == 4)
-          *reinterpret_cast<uint32_t*>(to) = packed[i][0];
+          *reinterpret_cast<uint32_t*>(to) = w[0];
         else
-          *reinterpret_cast<uint16_t*>(to) = (uint16_t)packed[i][0];
-      }
-      if (t == 0 && part == 0 && (!SMALL || warp == 0)) {
-        sd.norms[at] = nrm[i];
-        if (!is_v) {
-          a.out_pos[at] = a.positions[tok];
-          a.out_w[at] = a.weights ? a.weights[r] : 0.f;
-        }
+          *reinterpret_cast<uint16_t*>(to) = (uint16_t)w[0];
       }
     }
   }
@@ -434,11 +487,10 @@ kv_append_kernel(AppendArgs a) {
 template <class T, int D, bool SMALL>
 int launch_append(const AppendArgs& a, cudaStream_t st) {
   using S = AppendShape<T, D, SMALL>;
-  constexpr int smem =
-      (SMALL ? 0 : 2 * S::plane * (int)sizeof(uint2)) + (kCells * 8 > kFewCells * 128 ? kCells * 8 : kFewCells * 128);
+  constexpr int smem = S::smem;
   auto kern = kv_append_kernel<T, D, SMALL>;
   PQ_CUDA_TRY(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, smem));
-  const int64_t groups = (a.rows + S::rows - 1) / S::rows;
+  const int64_t groups = ((int64_t)a.rows + S::rows - 1) / S::rows;
   const int64_t blocks = (groups + S::groups - 1) / S::groups;
   const int64_t most = SMALL ? 1 << 20 : max(1, num_sms() / (2 * S::parts));
   kern<<<dim3((unsigned)min(blocks, most), 2 * S::parts), 32 * S::warps, smem, st>>>(a);
@@ -450,7 +502,7 @@ template <class T, int D>
 int launch_append_rows(const AppendArgs& a, cudaStream_t st) {
   // Few rows: as many blocks of 16 rows as there are, each reading the planes
   // from L2; more than two waves of them: resident planes.
-  if (a.rows <= 16 * num_sms()) return launch_append<T, D, true>(a, st);
+  if (a.rows <= 16u * num_sms()) return launch_append<T, D, true>(a, st);
   return launch_append<T, D, false>(a, st);
 }
 
@@ -611,11 +663,11 @@ int pq_kv_append(const pq_kv_cache* cache, const void* k, const void* v, int dty
   a.k_sh = k_stride_h;
   a.v_sn = v_stride_n;
   a.v_sh = v_stride_h;
-  a.rows = n * cache->heads;
+  a.rows = (uint32_t)(n * cache->heads);
   a.slots_end = (int64_t)cache->pages * cache->page_size;
   a.heads = cache->heads;
   a.d = cache->d;
-  a.page_size = cache->page_size;
+  a.page_shift = kv::page_shift_of(*cache);
   const int size = dtype == PQ_KV_F32 ? 4 : 2;
   auto vec = [&](const void* p, int64_t sn, int64_t sh) {
     return (uintptr_t)p % 16 == 0 && sn * size % 16 == 0 && sh * size % 16 == 0 &&

@@ -23,6 +23,7 @@ struct Codec {
   const uint2* cells;     // [2048]: the cell's boundary (f32) and the code below it
   const uint2* planes;    // [2][D / 8][D / 16][32]: R * 2^14 as f16 hi and lo, in the order
                           // of mma.m16n8k16's B operand (kv_rows.cu)
+  const __half* rows;     // [2][D][D]: the same planes row by row
 };
 
 constexpr int kCells = 2048;      // of a codec of 8 bits
@@ -32,7 +33,7 @@ inline int padded_d(int d) { return d <= 64 ? 64 : d <= 128 ? 128 : 256; }
 inline size_t codec_bytes(int d, int /*bits*/) {
   const size_t D = padded_d(d);
   return (size_t)2 * align_up((size_t)d * d * sizeof(float), 256) + 4 * 1024 + 256 +
-         kCells * sizeof(uint2) + 2 * D * D * 2;
+         kCells * sizeof(uint2) + 2 * 2 * D * D * sizeof(__half);
 }
 
 inline Codec codec_of(const void* tables, int d) {
@@ -49,6 +50,8 @@ inline Codec codec_of(const void* tables, int d) {
   c.range = (const float*)(b + 4096 + 64);
   c.cells = (const uint2*)(b + 4096 + 256);
   c.planes = c.cells + kCells;
+  const int D = padded_d(d);
+  c.rows = (const __half*)(c.planes + D * D / 2);
   return c;
 }
 

@@ -2,6 +2,7 @@
 // (norm, rotation, Lloyd-Max codes, packing, scatter into the pages) and
 // reading slots back as vectors.
 #include "kv.cuh"
+#include "tc.cuh"
 
 namespace pqb {
 namespace kv {
@@ -57,6 +58,15 @@ __global__ void prepare_codec_kernel(const float* __restrict__ R, const float* _
     p[D / 8 * (D / 16) * 32 + i] =
         make_uint2(__half_as_ushort(lo[0]) | (uint32_t)__half_as_ushort(lo[1]) << 16,
                    __half_as_ushort(lo[2]) | (uint32_t)__half_as_ushort(lo[3]) << 16);
+  }
+  // The same, row by row.
+  for (int i = t; i < D * D; i += threads) {
+    const int col = i / D, row = i % D;
+    const float v = col < d && row < d ? R[col * d + row] * 16384.f : 0.f;
+    const __half hi = __float2half_rn(v);
+    __half* p = const_cast<__half*>(out.rows);
+    p[i] = hi;
+    p[D * D + i] = __float2half_rn(v - __half2float(hi));
   }
   // Cells between the first and the last boundary.
   {
@@ -117,26 +127,24 @@ __global__ void prepare_codec_kernel(const float* __restrict__ R, const float* _
 // x -> norm = f32(sqrt(sum_f64 x^2)), u = x / max(norm, 1e-8) in f32, code_j =
 // #{boundaries < sum_i u_i R_ji}, exactly.
 //
-// The rotation runs on mma.m16n8k16 (f16 operands, f32 sums): a row's x times a
-// power of two is f16 hi (exact for 16-bit inputs but for elements below 2^-28
-// of the largest) or hi + lo (f32), R * 2^14 is hi + lo, and hi*hi + hi*lo (+
-// lo*hi) are summed; the scales and 1 / max(norm, 1e-8) come after.  That is
+// The rotation runs on the tensor cores in f16 operands and f32 sums: a row's x
+// times a power of two is f16 hi (exact for 16-bit inputs but for elements below
+// 2^-28 of the largest) or hi + lo (f32), R * 2^14 is hi + lo, and hi*hi + hi*lo
+// (+ lo*hi) are summed; the scales and 1 / max(norm, 1e-8) come after.  That is
 // within (steps + 8) * 2^-23 of the exact product (each of the sum's `steps`
 // additions loses at most 2^-23 of a partial sum, which is at most |u||R_j| = 1;
-// operands lose 2^-22): coordinates that near a boundary are recomputed by the
+// operands lose 2^-22): coordinates that near a boundary are recomputed by a
 // warp in f64.  So codes do not depend on how the product was taken.
 //
-// Which column and which element stands where in the operands is free, so a
-// lane (g, t) loads a quarter of row g from its t-th run of d / 4 elements, and
-// gets the coordinates of the same run back: it packs whole words.  Counting
-// boundaries takes one table lookup: cells narrower than the gaps between
-// boundaries hold at most one (from a copy for each lane at 2 and 4 bits, with
-// the code in the low four bits of the boundary).
+// Counting boundaries takes one table lookup: cells narrower than the gaps
+// between boundaries hold at most one (from a copy for each lane at 2 and 4
+// bits, with the code in the low four bits of the boundary).
 //
-// A warp takes `ROWS` rows (32: the planes' operands, read from shared memory,
-// serve two of them) through all columns with the planes of a side resident in
-// shared memory; a call of few rows instead spreads the columns over the warps
-// and reads the planes from L2.
+// Two kernels.  Calls of few rows (kv_append_few_kernel, mma.m16n8k16): a block
+// takes 16 rows, its warps 32 columns each, planes of R from L2.  Which column
+// and which element stands where in the operands is free, so a lane (g, t) loads
+// a quarter of row g from its t-th run of d / 4 elements and gets coordinates of
+// the same run back.  Others (kv_append_kernel, tcgen05): below.
 // ---------------------------------------------------------------------------
 
 __device__ __forceinline__ void mma_rows(float (&c)[4], const uint32_t (&a)[4], uint2 b) {
@@ -169,25 +177,25 @@ struct AppendArgs {
     return ((int64_t)(s >> page_shift) * heads + r % heads << page_shift) +
            (s & ((1u << page_shift) - 1u));
   }
+  // What a token holds besides codes, by one thread of a row.
+  __device__ void write_token(const Side& sd, bool is_v, uint32_t r, int64_t at,
+                              float norm) const {
+    sd.norms[at] = norm;
+    if (!is_v) {
+      out_pos[at] = positions[r / heads];
+      out_w[at] = weights ? weights[r] : 0.f;
+    }
+  }
 };
 
 constexpr int kCellWords = 2 * kCells > 32 * kFewCells ? 2 * kCells : 32 * kFewCells;
 
-template <class T, int D, bool SMALL>
-struct AppendShape {
+template <class T, int D>
+struct FewShape {
   static constexpr bool wide = sizeof(T) == 4;  // x is hi + lo
-  static constexpr int MT = SMALL || wide || D == 256 ? 1 : 2;
-  static constexpr int rows = 16 * MT;
+  static constexpr int rows = 16;
   static constexpr int steps = D / 16;
-  static constexpr int chunks = D / 32;                      // of 8 columns a lane
-  static constexpr int per = SMALL ? 1 : (D == 256 ? 4 : chunks);  // chunks of a warp
-  static constexpr int parts = SMALL ? 1 : chunks / per;     // blocks that share a row's columns
-  static constexpr int warps = SMALL ? chunks : (D == 64 ? 16 : 12);
-  static constexpr int groups = SMALL ? 1 : warps;           // row groups of a block at a time
-  static constexpr int run = per * 8;                        // columns of a lane in a row
-  static constexpr int plane = D / 8 / parts * steps * 32;   // uint2 of a plane in the block
-  static constexpr int plane_bytes = SMALL ? 0 : 2 * plane * 8;
-  static constexpr int smem = plane_bytes + 4 * kCellWords + warps * 2 * MT * 8 * 128;
+  static constexpr int warps = D / 32;          // 32 columns each, 8 a lane
 };
 
 // 16 bytes of x as f32.
@@ -205,305 +213,606 @@ __device__ __forceinline__ void widen16(const uint4& w, float* f) {
   }
 }
 
-template <class T, int D, int BITS, bool SMALL>
-__device__ __forceinline__ void append_rows(const AppendArgs& a, uint8_t* smem) {
-  using S = AppendShape<T, D, SMALL>;
-  constexpr int MT = S::MT;
-  constexpr int run_bytes = S::run * BITS / 8, words = (run_bytes + 3) / 4;
-  constexpr int cells = BITS == 8 ? kCells : kFewCells;
-  uint2* s_plane = reinterpret_cast<uint2*>(smem);
-  uint32_t* s_cell = reinterpret_cast<uint32_t*>(smem + S::plane_bytes);
+// The table of cells in shared memory (kCellWords), by all threads of the block.
+template <int BITS>
+__device__ __forceinline__ void fill_cells(const Codec& cd, uint32_t* s_cell) {
+  if constexpr (BITS == 8) {
+    for (int i = threadIdx.x; i < kCells; i += blockDim.x)
+      reinterpret_cast<uint2*>(s_cell)[i] = cd.cells[i];
+  } else {
+    for (int i = threadIdx.x; i < kFewCells * 32; i += blockDim.x) {
+      const uint2 c = cd.cells[i >> 5];
+      s_cell[i] = (c.x & ~15u) | c.y;
+    }
+  }
+}
+
+// Coding of a product x (a sum of the operands as they are scaled): y = x * inv.
+template <int BITS>
+struct Coder {
+  uint32_t base;  // the lane's place in the table, less what the bits of 2^23 come to in it
+  float scale, offset;
+  static constexpr int cells = BITS == 8 ? kCells : kFewCells;
+
+  __device__ __forceinline__ Coder(const Codec& cd, const uint32_t* s_cell)
+      : base((uint32_t)__cvta_generic_to_shared(s_cell) +
+             (BITS == 8 ? 0u : (threadIdx.x & 31) * 4u) - 0x4b000000u * (BITS == 8 ? 8u : 128u)),
+        scale(cd.range[0]),
+        offset(cd.range[1]) {}
+
+  // Number of boundaries below y, right unless `off`, the distance to the cell's
+  // boundary, is within the band or NaN.
+  __device__ __forceinline__ uint32_t code(float x, float inv, float& off) const {
+    const float cell =
+        fmaf(__saturatef(fmaf(x, inv * scale, offset)), (float)(cells - 1), 8388608.f);
+    uint32_t e, c;
+    if constexpr (BITS == 8) {
+      asm("ld.shared.v2.b32 {%0,%1}, [%2];"
+          : "=r"(e), "=r"(c)
+          : "r"(__float_as_uint(cell) * 8u + base));
+    } else {
+      asm("ld.shared.b32 %0, [%1];" : "=r"(e) : "r"(__float_as_uint(cell) * 128u + base));
+      c = e & 15u;
+    }
+    off = fmaf(x, inv, -__uint_as_float(e));
+    return c + (off > 0.f ? 1u : 0u);
+  }
+};
+
+// A boundary below 1 with its low four bits taken loses 15 * 2^-24 < 1e-6.
+__host__ __device__ constexpr float band_of(int products, int bits) {
+  return (products + 8) * 1.1920929e-7f + (bits == 8 ? 0.f : 1e-6f);
+}
+
+// The code of column `col` of the row at x, by the warp, in f64.
+template <class T, int BITS>
+__device__ __forceinline__ uint32_t exact_code(const T* x, float den, const Codec& cd, int col,
+                                               int d) {
+  const int lane = threadIdx.x & 31;
+  const float* rr = cd.R + col * d;
+  double y = 0.0;
+#pragma unroll 4
+  for (int j = lane; j < d; j += 32)
+    y = fma((double)__fdiv_rn(to_f32<T>(x[j]), den), (double)__ldg(rr + j), y);
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) y += __shfl_xor_sync(0xffffffffu, y, o);
+  uint32_t code = 0;
+#pragma unroll
+  for (int step = 1 << (BITS - 1); step > 0; step >>= 1)
+    if (y > (double)__ldg(cd.bounds + code + step - 1)) code += step;
+  return code;
+}
+
+// A quarter of a row, from x on (the row's coordinate k0): D / 4 elements.
+template <class T, int D>
+__device__ __forceinline__ void load_quarter(const T* x, int k0, int d, bool vec,
+                                             uint4 (&w)[D / 4 * sizeof(T) / 16]) {
+  constexpr int E = 16 / sizeof(T), N = D / 4 / E;
+  if (vec) {
+#pragma unroll
+    for (int j = 0; j < N; ++j)
+      w[j] = k0 + j * E < d ? *reinterpret_cast<const uint4*>(x + j * E) : make_uint4(0u, 0u, 0u, 0u);
+  } else {
+#pragma unroll
+    for (int j = 0; j < N; ++j) {
+      uint32_t v[4];
+#pragma unroll
+      for (int k = 0; k < 4; ++k) {
+        if constexpr (sizeof(T) == 4) {
+          v[k] = k0 + j * E + k < d ? __float_as_uint(to_f32<T>(x[j * E + k])) : 0u;
+        } else {
+          const uint16_t* p = reinterpret_cast<const uint16_t*>(x) + j * E + 2 * k;
+          const int at = k0 + j * E + 2 * k;
+          v[k] = (at < d ? p[0] : 0u) | (uint32_t)(at + 1 < d ? p[1] : 0u) << 16;
+        }
+      }
+      w[j] = make_uint4(v[0], v[1], v[2], v[3]);
+    }
+  }
+}
+
+// A row's norm, and the power of two for its f16 planes.  The row is in four
+// neighbouring lanes, a quarter each.
+struct RowScale {
+  float norm, den, up, inv;  // inv: of a sum of scaled operands, to the unit vector's coordinate
+};
+
+template <class T, int N>
+__device__ __forceinline__ RowScale scale_row(const uint4 (&w)[N]) {
+  double ss = 0.0;
+  float mx = 0.f;
+#pragma unroll
+  for (int j = 0; j < N; ++j) {
+    float f[16 / sizeof(T)];
+    widen16<T>(w[j], f);
+#pragma unroll
+    for (int k = 0; k < 16 / (int)sizeof(T); ++k) {
+      ss = fma((double)f[k], (double)f[k], ss);
+      mx = fmaxf(mx, fabsf(f[k]));
+    }
+  }
+#pragma unroll
+  for (int o = 1; o < 4; o <<= 1) {
+    ss += __shfl_xor_sync(0xffffffffu, ss, o);
+    mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, o));
+  }
+  RowScale r;
+  r.norm = __double2float_rn(__dsqrt_rn(ss));
+  r.den = fmaxf(r.norm, 1e-8f);
+  // max |x| * 2^e in [2^14, 2^15): f16's range, and sums of at most 2^29 sqrt(d)
+  const int e = mx > 0.f && mx < INFINITY ? max(-126, min(126, 14 - ilogbf(mx))) : 0;
+  r.up = __int_as_float((127 + e) << 23);
+  r.inv = __int_as_float((127 - e) << 23) / 16384.f / r.den;
+  return r;
+}
+
+template <class T, int D, int BITS>
+__device__ __forceinline__ void append_few(const AppendArgs& a, uint32_t* s_cell) {
+  using S = FewShape<T, D>;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
-  // The lane's packed runs, one of each of its rows: word w of row i.
-  uint32_t* s_run = s_cell + kCellWords + warp * (2 * MT * 8 * 32) + lane;
-  // blockIdx.y: the part of the columns and, lowest, the side.
+  const bool is_v = blockIdx.y != 0;
+  const Side& sd = is_v ? a.sv : a.sk;
+  const Codec& cd = sd.c;
+  const T* src = reinterpret_cast<const T*>(is_v ? a.v : a.k);
+  const int64_t sn = is_v ? a.v_sn : a.k_sn, sh = is_v ? a.v_sh : a.k_sh;
+  const int d = a.d;
+  const uint32_t rows = a.rows, heads = a.heads, row0 = blockIdx.x * S::rows;
+  fill_cells<BITS>(cd, s_cell);
+  __syncthreads();
+  const Coder<BITS> coder(cd, s_cell);
+  constexpr float band = band_of(S::steps * (S::wide ? 3 : 2), BITS);
+
+  // Rows g and g + 8: registers 0 and 2 of the A operand hold the first, 1 and 3
+  // the second.
+  uint32_t ah[S::steps][4], al[S::wide ? S::steps : 1][4];
+  float inv[2], den[2];
+#pragma unroll
+  for (int i = 0; i < 2; ++i) {
+    const uint32_t r = min(row0 + g + 8 * i, rows - 1);
+    const T* x = src + (int64_t)(r / heads) * sn + (r % heads) * sh + t * (D / 4);
+    constexpr int E = 16 / sizeof(T), N = D / 4 / E;
+    uint4 w[N];
+    load_quarter<T, D>(x, t * (D / 4), d, is_v ? a.v_vec : a.k_vec, w);
+    const RowScale rs = scale_row<T>(w);
+    inv[i] = rs.inv;
+    den[i] = rs.den;
+    if (t == 0 && warp == 0 && row0 + g + 8 * i < rows) {
+      const int64_t at = a.place(r);
+      if (at >= 0) a.write_token(sd, is_v, r, at, rs.norm);
+    }
+#pragma unroll
+    for (int j = 0; j < N; ++j) {
+      float f[E];
+      widen16<T>(w[j], f);
+#pragma unroll
+      for (int k = 0; k < E; k += 2) {
+        const int n = j * E + k, s = n >> 2, h = (n >> 1) & 1;
+        const __half2 hi = __floats2half2_rn(f[k] * rs.up, f[k + 1] * rs.up);
+        ah[s][2 * h + i] = *reinterpret_cast<const uint32_t*>(&hi);
+        if constexpr (S::wide) {
+          const float2 b = __half22float2(hi);
+          const __half2 lo = __floats2half2_rn(f[k] * rs.up - b.x, f[k + 1] * rs.up - b.y);
+          al[s][2 * h + i] = *reinterpret_cast<const uint32_t*>(&lo);
+        }
+      }
+    }
+  }
+  float acc[4][4];
+#pragma unroll
+  for (int q = 0; q < 4; ++q) acc[q][0] = acc[q][1] = acc[q][2] = acc[q][3] = 0.f;
+  const uint2* bp = cd.planes + warp * 4 * S::steps * 32 + lane;
+#pragma unroll
+  for (int s = 0; s < S::steps; ++s)
+#pragma unroll
+    for (int q = 0; q < 4; ++q) {
+      const uint2 bh = __ldg(bp + (q * S::steps + s) * 32);
+      const uint2 bl = __ldg(bp + (D / 8 + q) * S::steps * 32 + s * 32);
+      mma_rows(acc[q], ah[s], bh);
+      mma_rows(acc[q], ah[s], bl);
+      if constexpr (S::wide) mma_rows(acc[q], al[s], bh);
+    }
+  // Codes of columns t * D / 4 + warp * 8 + k: packed, the first code highest in
+  // its byte, and which of them are next to a boundary.
+  constexpr int cw = BITS == 8 ? 2 : 1;
+  const int col0 = t * (D / 4) + warp * 8;
+  uint32_t packed[2][cw], near = 0;
+#pragma unroll
+  for (int i = 0; i < 2; ++i) {
+#pragma unroll
+    for (int w = 0; w < cw; ++w) packed[i][w] = 0u;
+#pragma unroll
+    for (int k = 0; k < 8; ++k) {
+      float off;
+      uint32_t code = coder.code(acc[k >> 1][2 * i + (k & 1)], inv[i], off);
+      if (col0 + k >= d) code = 0u;
+      if (!(fabsf(off) >= band) && col0 + k < d && row0 + g + 8 * i < rows)
+        near |= 1u << (8 * i + k);
+      const int bit = k * BITS;
+      packed[i][bit >> 5] |= code << ((bit & 24) + 8 - BITS - (bit & 7));
+    }
+  }
+  uint32_t pend = __ballot_sync(0xffffffffu, near != 0u);
+#pragma unroll 1
+  while (pend) {
+    const int from = __ffs(pend) - 1;
+    pend &= pend - 1;
+    uint32_t mask = __shfl_sync(0xffffffffu, near, from);
+#pragma unroll 1
+    while (mask) {
+      const int n = __ffs(mask) - 1, i = n >> 3, k = n & 7;
+      mask &= mask - 1;
+      const float dn = __shfl_sync(0xffffffffu, i ? den[1] : den[0], from);
+      const uint32_t r = row0 + (from >> 2) + 8 * i;
+      const T* x = src + (int64_t)(r / heads) * sn + (r % heads) * sh;
+      const uint32_t code =
+          exact_code<T, BITS>(x, dn, cd, (from & 3) * (D / 4) + warp * 8 + k, d);
+      const int bit = k * BITS, shift = (bit & 24) + 8 - BITS - (bit & 7);
+      if (lane == from) {
+#pragma unroll
+        for (int z = 0; z < 2; ++z)
+#pragma unroll
+          for (int w = 0; w < cw; ++w)
+            if (z == i && w == bit >> 5)
+              packed[z][w] = (packed[z][w] & ~(((1u << BITS) - 1u) << shift)) | code << shift;
+      }
+    }
+  }
+#pragma unroll
+  for (int i = 0; i < 2; ++i) {
+    const uint32_t r = row0 + g + 8 * i;
+    if (r >= rows) break;
+    const int64_t at = a.place(r);
+    const int off = col0 * BITS / 8;
+    if (at < 0 || off >= sd.ldb) continue;
+    uint8_t* to = sd.rows + at * sd.ldb + off;
+    if constexpr (BITS == 8)
+      *reinterpret_cast<uint2*>(to) = make_uint2(packed[i][0], packed[i][1]);
+    else if constexpr (BITS == 4)
+      *reinterpret_cast<uint32_t*>(to) = packed[i][0];
+    else
+      *reinterpret_cast<uint16_t*>(to) = (uint16_t)packed[i][0];
+  }
+}
+
+template <class T, int D>
+__global__ void __launch_bounds__(32 * FewShape<T, D>::warps, 1)
+kv_append_few_kernel(AppendArgs a) {
+  __shared__ __align__(16) uint32_t s_cell[kCellWords];
+  const int bits = blockIdx.y ? a.sv.bits : a.sk.bits;
+  if (bits == 2)
+    append_few<T, D, 2>(a, s_cell);
+  else if (bits == 4)
+    append_few<T, D, 4>(a, s_cell);
+  else
+    append_few<T, D, 8>(a, s_cell);
+}
+
+// ---------------------------------------------------------------------------
+// Append of many rows.  A persistent block per SM takes one side (at D = 256 a
+// part of its columns too), with R's planes resident in shared memory, and tiles
+// of 128 rows: warps 8-15 load rows (four lanes a row), scale and split them into
+// 128-byte-swizzled K-major f16 tiles; one thread of warp 16 issues the
+// tcgen05.mma (M = 128, N = the block's columns) into one of two TMEM
+// accumulators; warps 0-7 read an accumulator, a lane per row, code, pack and
+// store it.  The three run on different tiles.
+//
+// Bound by the instructions of the two ends, some 75 a row and 32 lanes: 25 to
+// widen, square and split 128 coordinates, 12 a coordinate to code it.
+// ---------------------------------------------------------------------------
+
+template <class T, int D>
+struct ManyShape {
+  static constexpr bool wide = sizeof(T) == 4;
+  static constexpr int planes = wide ? 2 : 1;
+  static constexpr int cols = D <= 128 ? D : wide ? 64 : 128;  // of a block
+  static constexpr int parts = D / cols;
+  static constexpr int kblocks = D / 64;                      // of 64 elements, 128 bytes a row
+  static constexpr int a_bytes = planes * kblocks * 128 * 128;
+  static constexpr int b_bytes = 2 * kblocks * cols * 128;
+  static constexpr int buffers = D <= 128 ? 2 : 1;
+  static constexpr int tmem = cols < 16 ? 32 : 2 * cols;
+  static constexpr int smem = 1024 + b_bytes + buffers * a_bytes + 4 * kCellWords;
+};
+constexpr int kManyThreads = 17 * 32;
+
+template <class T, int D, int BITS>
+__device__ __forceinline__ void append_many(const AppendArgs& a, uint8_t* smem, float (*s_inv)[128],
+                                            float (*s_norm)[128], uint32_t bars, uint32_t tmem,
+                                            volatile int* abort) {
+  using S = ManyShape<T, D>;
+  constexpr int NB = S::buffers;
+  uint8_t* s_b = smem;
+  uint8_t* s_a = smem + S::b_bytes;
+  uint32_t* s_cell = reinterpret_cast<uint32_t*>(smem + S::b_bytes + NB * S::a_bytes);
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const bool is_v = blockIdx.y & 1;
   const int part = blockIdx.y >> 1;
   const Side& sd = is_v ? a.sv : a.sk;
   const Codec& cd = sd.c;
   const T* src = reinterpret_cast<const T*>(is_v ? a.v : a.k);
   const int64_t sn = is_v ? a.v_sn : a.k_sn, sh = is_v ? a.v_sh : a.k_sh;
-  const bool vec = is_v ? a.v_vec : a.k_vec;
   const int d = a.d;
   const uint32_t rows = a.rows, heads = a.heads;
 
-  if constexpr (!SMALL) {
-    const uint2* p = cd.planes + part * S::plane;
-    for (int i = threadIdx.x; i < S::plane; i += blockDim.x) {
-      s_plane[i] = p[i];
-      s_plane[S::plane + i] = p[D / 8 * S::steps * 32 + i];
-    }
+  // R's planes: [plane][kblock][column][64], 16-byte pieces exchanged by row & 7.
+  for (int i = threadIdx.x; i < 2 * S::cols * (D / 8); i += kManyThreads) {
+    const int piece = i % (D / 8), col = i / (D / 8) % S::cols, plane = i / (D / 8) / S::cols;
+    const uint4 v = *reinterpret_cast<const uint4*>(cd.rows + (size_t)plane * D * D +
+                                                    (size_t)(part * S::cols + col) * D + piece * 8);
+    const int kb = piece >> 3, c = piece & 7;
+    *reinterpret_cast<uint4*>(s_b + ((plane * S::kblocks + kb) * S::cols + col) * 128 +
+                              ((c ^ (col & 7)) << 4)) = v;
   }
-  if constexpr (BITS == 8) {
-    for (int i = threadIdx.x; i < cells; i += blockDim.x)
-      reinterpret_cast<uint2*>(s_cell)[i] = cd.cells[i];
-  } else {
-    for (int i = threadIdx.x; i < cells * 32; i += blockDim.x) {
-      const uint2 c = cd.cells[i >> 5];
-      s_cell[i] = (c.x & ~15u) | c.y;
-    }
-  }
+  fill_cells<BITS>(cd, s_cell);
+  asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
   __syncthreads();
-  const float cs = cd.range[0], co = cd.range[1];
-  // (a boundary below 1 with its low four bits taken loses 15 * 2^-24 < 1e-6)
-  constexpr float band =
-      (S::steps * (S::wide ? 3 : 2) + 8) * 1.1920929e-7f + (BITS == 8 ? 0.f : 1e-6f);
 
-  const uint32_t groups = (rows + S::rows - 1) / S::rows;
-#pragma unroll 1
-  for (uint32_t gr = blockIdx.x * S::groups + (SMALL ? 0 : warp); gr < groups;
-       gr += gridDim.x * S::groups) {
-    // x of rows g, g + 8 (, g + 16, g + 24) in f32, a quarter of each a lane.
-    const uint32_t row0 = gr * S::rows;
-    uint32_t ah[MT][S::steps][4], al[S::wide ? MT : 1][S::wide ? S::steps : 1][4];
-    float inv[2 * MT], den[2 * MT];
-#pragma unroll
-    for (int i = 0; i < 2 * MT; ++i) {
-      const uint32_t r = min(row0 + g + 8 * i, rows - 1);
+  const uint32_t AFULL = bars, AEMPTY = bars + 16, TFULL = bars + 32, TEMPTY = bars + 48,
+                 DRAIN = bars + 64;
+  const uint32_t tiles = (rows + 127) / 128;
+  if (warp >= 8 && warp < 16) {
+    // ---- rows into A tiles: 16 rows a warp, four lanes a row, in two turns ----
+    const int g = lane >> 2, t = lane & 3;
+    const bool vec = is_v ? a.v_vec : a.k_vec;
+    constexpr int E = 16 / sizeof(T), N = D / 4 / E;
+    constexpr int AHEAD = D <= 128 ? 2 : 1;  // turns whose loads are in registers
+    uint4 w[AHEAD][N];
+    auto load = [&](uint32_t tile, int turn) {
+      const uint32_t r = min(tile * 128 + (warp - 8) * 16 + turn * 8 + g, rows - 1);
       const T* x = src + (int64_t)(r / heads) * sn + (r % heads) * sh + t * (D / 4);
-      float f[D / 4];
-      constexpr int E = 16 / sizeof(T);
-      if (vec) {
-        uint4 w[D / 4 / E];
+      load_quarter<T, D>(x, t * (D / 4), d, vec, w[turn % AHEAD]);
+    };
+    uint32_t n = 0;
+    if (blockIdx.x < tiles) {
 #pragma unroll
-        for (int j = 0; j < D / 4 / E; ++j)
-          w[j] = t * (D / 4) + j * E < d ? *reinterpret_cast<const uint4*>(x + j * E)
-                                         : make_uint4(0u, 0u, 0u, 0u);
-#pragma unroll
-        for (int j = 0; j < D / 4 / E; ++j) widen16<T>(w[j], f + j * E);
-      } else {
-#pragma unroll
-        for (int j = 0; j < D / 4; ++j) f[j] = t * (D / 4) + j < d ? to_f32<T>(x[j]) : 0.f;
-      }
-      double ss = 0.0;
-      float mx = 0.f;
-#pragma unroll
-      for (int j = 0; j < D / 4; ++j) {
-        ss = fma((double)f[j], (double)f[j], ss);
-        mx = fmaxf(mx, fabsf(f[j]));
-      }
-#pragma unroll
-      for (int o = 1; o < 4; o <<= 1) {
-        ss += __shfl_xor_sync(0xffffffffu, ss, o);
-        mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, o));
-      }
-      const float nrm = __double2float_rn(__dsqrt_rn(ss));
-      den[i] = fmaxf(nrm, 1e-8f);
-      if (t == 0 && part == 0 && (!SMALL || warp == 0) && row0 + g + 8 * i < rows) {
-        const int64_t at = a.place(r);
-        if (at >= 0) {
-          sd.norms[at] = nrm;
-          if (!is_v) {
-            a.out_pos[at] = a.positions[r / heads];
-            a.out_w[at] = a.weights ? a.weights[r] : 0.f;
-          }
-        }
-      }
-      // max |x| * 2^e in [2^14, 2^15): f16's range, and sums of at most 2^29 sqrt(d)
-      const int e =
-          mx > 0.f && mx < INFINITY ? max(-126, min(126, 14 - ilogbf(mx))) : 0;
-      const float up = __int_as_float((127 + e) << 23);
-      inv[i] = __int_as_float((127 - e) << 23) / 16384.f / den[i];
-      // Registers 0 and 2 of the A operand hold row g, 1 and 3 row g + 8.
-#pragma unroll
-      for (int s = 0; s < S::steps; ++s)
-#pragma unroll
-        for (int h = 0; h < 2; ++h) {
-          const float x0 = f[4 * s + 2 * h] * up, x1 = f[4 * s + 2 * h + 1] * up;
-          const __half2 hi = __floats2half2_rn(x0, x1);
-          ah[i >> 1][s][2 * h + (i & 1)] = *reinterpret_cast<const uint32_t*>(&hi);
-          if constexpr (S::wide) {
-            const float2 b = __half22float2(hi);
-            const __half2 lo = __floats2half2_rn(x0 - b.x, x1 - b.y);
-            al[i >> 1][s][2 * h + (i & 1)] = *reinterpret_cast<const uint32_t*>(&lo);
-          }
-        }
+      for (int turn = 0; turn < AHEAD; ++turn) load(blockIdx.x, turn);
     }
-
-    // Eight columns a lane at a time.  (One body for all: unrolled over the
-    // chunks the code does not fit the instruction cache.)
-#pragma unroll 1
-    for (int c = 0; c < S::per; ++c) {
-      const int chunk = SMALL ? warp : part * S::per + c;
-      float acc[MT][4][4];
+    for (uint32_t tile = blockIdx.x; tile < tiles; tile += gridDim.x, ++n) {
+      const int buf = n % NB;
+      if (!tc::mbar_wait(AEMPTY + 8 * buf, ((n / NB) & 1) ^ 1, abort, tc::kErrWaitStageEmpty)) break;
+      uint8_t* dst = s_a + buf * S::a_bytes;
 #pragma unroll
-      for (int m = 0; m < MT; ++m)
-#pragma unroll
-        for (int q = 0; q < 4; ++q) acc[m][q][0] = acc[m][q][1] = acc[m][q][2] = acc[m][q][3] = 0.f;
-      const uint2* bp = SMALL ? cd.planes + chunk * 4 * S::steps * 32 + lane
-                              : s_plane + c * 4 * S::steps * 32 + lane;
-      constexpr int lo_at = SMALL ? D / 8 * S::steps * 32 : S::plane;
-#pragma unroll
-      for (int s = 0; s < S::steps; ++s)
-#pragma unroll
-        for (int q = 0; q < 4; ++q) {
-          const uint2 bh = bp[(q * S::steps + s) * 32], bl = bp[lo_at + (q * S::steps + s) * 32];
-#pragma unroll
-          for (int m = 0; m < MT; ++m) {
-            mma_rows(acc[m][q], ah[m][s], bh);
-            mma_rows(acc[m][q], ah[m][s], bl);
-            if constexpr (S::wide) mma_rows(acc[m][q], al[m][s], bh);
-          }
+      for (int turn = 0; turn < 2; ++turn) {
+        const int lr = (warp - 8) * 16 + turn * 8 + g;  // row of the tile
+        const RowScale rs = scale_row<T>(w[turn % AHEAD]);
+        if (t == 0) {
+          s_inv[n & 3][lr] = rs.inv;
+          s_norm[n & 3][lr] = rs.norm;
         }
-      // Codes of rows g + 8i, columns t * D / 4 + chunk * 8 + k: packed, the first
-      // code highest in its byte, and which of them are next to a boundary.
-      constexpr int cw = BITS == 8 ? 2 : 1;
-      uint32_t packed[2 * MT][cw], near = 0;
-      const int left = min(8, d - (t * (D / 4) + chunk * 8));  // columns that there are
+        // Pieces of eight f16.
 #pragma unroll
-      for (int i = 0; i < 2 * MT; ++i) {
+        for (int p = 0; p < D / 32; ++p) {
+          uint32_t hi[4], lo[4];
 #pragma unroll
-        for (int w = 0; w < cw; ++w) packed[i][w] = 0u;
-#pragma unroll
-        for (int k = 0; k < 8; ++k) {
-          const float y = acc[i >> 1][k >> 1][2 * (i & 1) + (k & 1)] * inv[i];
-          const float cell = fmaf(__saturatef(fmaf(y, cs, co)), (float)(cells - 1), 8388608.f);
-          float b;
-          uint32_t code;
-          if constexpr (BITS == 8) {
-            const uint2 e =
-                reinterpret_cast<const uint2*>(s_cell)[__float_as_uint(cell) & (cells - 1)];
-            b = __uint_as_float(e.x);
-            code = e.y;
-          } else {
-            const uint32_t e = s_cell[(__float_as_uint(cell) & (cells - 1)) * 32 + lane];
-            b = __uint_as_float(e);
-            code = e & 15u;
-          }
-          const float off = y - b;
-          if (off > 0.f) ++code;
-          if (!(fabsf(off) >= band)) near |= 1u << (8 * i + k);
-          const int bit = k * BITS;
-          packed[i][bit >> 5] |= code << ((bit & 24) + 8 - BITS - (bit & 7));
-        }
-      }
-      if (left < 8) {
-        // Bits of the columns behind the row's end are 0.
-#pragma unroll
-        for (int i = 0; i < 2 * MT; ++i)
-#pragma unroll
-          for (int k = 0; k < 8; ++k)
-            if (k >= left) {
-              const int bit = k * BITS;
-              packed[i][bit >> 5] &=
-                  ~(((1u << BITS) - 1u) << ((bit & 24) + 8 - BITS - (bit & 7)));
-              near &= ~(1u << (8 * i + k));
+          for (int k = 0; k < 4; ++k) {
+            float f[E];
+            widen16<T>(w[turn % AHEAD][(8 * p + 2 * k) / E], f);
+            const float x0 = f[(8 * p + 2 * k) % E] * rs.up, x1 = f[(8 * p + 2 * k) % E + 1] * rs.up;
+            const __half2 h = __floats2half2_rn(x0, x1);
+            hi[k] = *reinterpret_cast<const uint32_t*>(&h);
+            if constexpr (S::wide) {
+              const float2 b = __half22float2(h);
+              const __half2 l = __floats2half2_rn(x0 - b.x, x1 - b.y);
+              lo[k] = *reinterpret_cast<const uint32_t*>(&l);
             }
+          }
+          const int piece = t * (D / 32) + p, kb = piece >> 3, c = piece & 7;
+          uint8_t* to = dst + (kb * 128 + lr) * 128 + ((c ^ (lr & 7)) << 4);
+          *reinterpret_cast<uint4*>(to) = make_uint4(hi[0], hi[1], hi[2], hi[3]);
+          if constexpr (S::wide)
+            *reinterpret_cast<uint4*>(to + S::kblocks * 128 * 128) =
+                make_uint4(lo[0], lo[1], lo[2], lo[3]);
+        }
+        if (AHEAD == 1 && turn == 0)
+          load(tile, 1);
+        else if (tile + gridDim.x < tiles)
+          load(tile + gridDim.x, AHEAD == 1 ? 0 : turn);
       }
+      asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+      __syncwarp();
+      if (lane == 0) tc::mbar_arrive(AFULL + 8 * buf);
+    }
+  } else if (warp == 16) {
+    if (lane == 0) {
+      // ---- products ----
+      const uint32_t b0 = tc::smem_u32(s_b), idesc = tc::idesc_f16_f32(128, S::cols);
+      uint32_t n = 0;
+      for (uint32_t tile = blockIdx.x; tile < tiles; tile += gridDim.x, ++n) {
+        const int buf = n % NB, acc = n & 1;
+        if (!tc::mbar_wait(TEMPTY + 8 * acc, ((n >> 1) & 1) ^ 1, abort, tc::kErrWaitAccEmpty)) break;
+        if (!tc::mbar_wait(AFULL + 8 * buf, (n / NB) & 1, abort, tc::kErrWaitTmaFull)) break;
+        tc::tc_fence_after();
+        const uint32_t a0 = tc::smem_u32(s_a) + buf * S::a_bytes, dt = tmem + acc * S::cols;
+        for (int kb = 0; kb < S::kblocks; ++kb) {
+          const uint32_t ah = a0 + kb * 128 * 128, bh = b0 + kb * S::cols * 128;
+          const uint32_t al = ah + S::kblocks * 128 * 128, bl = bh + S::kblocks * S::cols * 128;
 #pragma unroll
-      for (int i = 0; i < 2 * MT; ++i)
-        if (row0 + g + 8 * i >= rows) near &= ~(255u << (8 * i));
-      // Coordinates next to a boundary, by the whole warp.
-      uint32_t pend = __ballot_sync(0xffffffffu, near != 0u);
+          for (int kk = 0; kk < 4; ++kk) {
+            const uint32_t off = kk * 32;
+            tc::mma_f16(dt, tc::sw128_desc(ah + off), tc::sw128_desc(bh + off), idesc,
+                        (kb | kk) != 0);
+            tc::mma_f16(dt, tc::sw128_desc(ah + off), tc::sw128_desc(bl + off), idesc, 1);
+            if constexpr (S::wide)
+              tc::mma_f16(dt, tc::sw128_desc(al + off), tc::sw128_desc(bh + off), idesc, 1);
+          }
+        }
+        tc::mma_commit(AEMPTY + 8 * buf);
+        tc::mma_commit(TFULL + 8 * acc);
+        tc::mbar_arrive(TFULL + 8 * acc);  // hands on what the loading warps wrote besides
+      }
+      // Before the block ends, every product that was issued has completed.
+      tc::mma_commit(DRAIN);
+      volatile int never = 0;
+      tc::mbar_wait(DRAIN, 0, &never, tc::kErrWaitAccFull);
+    }
+  } else if (warp < 8) {
+    // ---- accumulators into codes: warps w and w + 4 the halves of the columns ----
+    const int q = warp & 3, half = warp >> 2;
+    const Coder<BITS> coder(cd, s_cell);
+    constexpr float band = band_of(S::kblocks * 4 * (S::wide ? 3 : 2), BITS);
+    uint32_t n = 0;
+    auto place = [&](uint32_t tile) {
+      const uint32_t r = tile * 128 + q * 32 + lane;
+      return tile < tiles && r < rows ? a.place(r) : (int64_t)-1;
+    };
+    int64_t next = place(blockIdx.x);
+    for (uint32_t tile = blockIdx.x; tile < tiles; tile += gridDim.x, ++n) {
+      const int acc = n & 1;
+      if (!tc::mbar_wait(TFULL + 8 * acc, (n >> 1) & 1, abort, tc::kErrWaitAccFull)) break;
+      tc::tc_fence_after();
+      const uint32_t row = tile * 128 + q * 32 + lane;
+      const float inv = s_inv[n & 3][q * 32 + lane], norm = s_norm[n & 3][q * 32 + lane];
+      const float den = fmaxf(norm, 1e-8f);
+      const int64_t at = next;
+      next = place(tile + gridDim.x);
+      if (half == 0 && part == 0 && at >= 0) a.write_token(sd, is_v, row, at, norm);
+      uint8_t* to = sd.rows + at * sd.ldb;
 #pragma unroll 1
-      while (pend) {
-        const int from = __ffs(pend) - 1;
-        pend &= pend - 1;
-        uint32_t mask = __shfl_sync(0xffffffffu, near, from);
-#pragma unroll 1
-        while (mask) {
-          const int n = __ffs(mask) - 1, i = n >> 3, k = n & 7;
-          mask &= mask - 1;
-          float dn = den[0];
+      for (int c = half * (S::cols / 2); c < (half + 1) * (S::cols / 2); c += 32) {
+        uint32_t v[32];
+        __syncwarp();
+        tc::tmem_ld32(tmem + ((uint32_t)(32 * q) << 16) + acc * S::cols + c, v);
+        tc::tmem_ld_wait(v);
+        const int col0 = part * S::cols + c, left = d - col0;
+        if (left <= 0) {
+          // Columns behind the row's end: zeros up to its padded length.
+          const int off = col0 * BITS / 8;
+          if (at >= 0)
+            for (int j = off; j < min(off + 4 * BITS, (int)sd.ldb); j += 4)
+              *reinterpret_cast<uint32_t*>(to + j) = 0u;
+          continue;
+        }
+        uint32_t packed[BITS], near = 0;
 #pragma unroll
-          for (int z = 1; z < 2 * MT; ++z)
-            if (z == i) dn = den[z];
-          dn = __shfl_sync(0xffffffffu, dn, from);
-          const uint32_t r = row0 + (from >> 2) + 8 * i;
+        for (int w = 0; w < BITS; ++w) {
+          constexpr int per = 32 / BITS;
+          uint32_t x = 0;
+#pragma unroll
+          for (int k = 0; k < per; ++k) {
+            float off;
+            const uint32_t code = coder.code(__uint_as_float(v[w * per + k]), inv, off);
+            if (!(fabsf(off) >= band)) near |= 1u << (w * per + k);
+            if constexpr (BITS == 8)
+              x |= code << (8 * k);
+            else
+              x = (x << BITS) + code;
+          }
+          packed[w] = BITS == 8 ? x : __byte_perm(x, 0u, 0x0123);
+        }
+        if (left < 32) {
+          near &= (1u << left) - 1u;
+#pragma unroll
+          for (int w = 0; w < BITS; ++w) {
+            const int keep = min(max(left * BITS - 32 * w, 0), 32);  // bits, from the first code on
+            const uint32_t m = keep >= 32 ? 0xffffffffu : ~(0xffffffffu >> keep);
+            packed[w] &= __byte_perm(m, 0u, 0x0123);
+          }
+        }
+        if (at < 0) near = 0u;
+        uint32_t pend = __ballot_sync(0xffffffffu, near != 0u);
+#pragma unroll 1
+        while (pend) {
+          const int from = __ffs(pend) - 1;
+          pend &= pend - 1;
+          uint32_t mask = __shfl_sync(0xffffffffu, near, from);
+          const uint32_t r = tile * 128 + q * 32 + from;
+          const float dn = __shfl_sync(0xffffffffu, den, from);
           const T* x = src + (int64_t)(r / heads) * sn + (r % heads) * sh;
-          const float* rr = cd.R + ((from & 3) * (D / 4) + chunk * 8 + k) * d;
-          double y = 0.0;
-          for (int j = lane; j < d; j += 32)
-            y = fma((double)__fdiv_rn(to_f32<T>(x[j]), dn), (double)__ldg(rr + j), y);
+#pragma unroll 1
+          while (mask) {
+            const int k = __ffs(mask) - 1;
+            mask &= mask - 1;
+            const uint32_t code = exact_code<T, BITS>(x, dn, cd, col0 + k, d);
+            const int bit = k * BITS, shift = (bit & 24) + 8 - BITS - (bit & 7);
+            if (lane == from) {
 #pragma unroll
-          for (int o = 16; o > 0; o >>= 1) y += __shfl_xor_sync(0xffffffffu, y, o);
-          uint32_t code = 0;
+              for (int w = 0; w < BITS; ++w)
+                if (w == bit >> 5)
+                  packed[w] = (packed[w] & ~(((1u << BITS) - 1u) << shift)) | code << shift;
+            }
+          }
+        }
+        if (at >= 0) {
+          const int off = col0 * BITS / 8;
+          if constexpr (BITS == 2) {
+            if (off < sd.ldb) *reinterpret_cast<uint2*>(to + off) = make_uint2(packed[0], packed[1]);
+          } else {
 #pragma unroll
-          for (int step = 1 << (BITS - 1); step > 0; step >>= 1)
-            if (y > (double)__ldg(cd.bounds + code + step - 1)) code += step;
-          const int bit = k * BITS, shift = (bit & 24) + 8 - BITS - (bit & 7);
-          if (lane == from) {
-#pragma unroll
-            for (int z = 0; z < 2 * MT; ++z)
-#pragma unroll
-              for (int w = 0; w < cw; ++w)
-                if (z == i && w == bit >> 5)
-                  packed[z][w] = (packed[z][w] & ~(((1u << BITS) - 1u) << shift)) | code << shift;
+            for (int w = 0; w < BITS; w += 4)
+              if (off + 4 * w < sd.ldb)
+                *reinterpret_cast<uint4*>(to + off + 4 * w) =
+                    make_uint4(packed[w], packed[w + 1], packed[w + 2], packed[w + 3]);
           }
         }
       }
-#pragma unroll
-      for (int i = 0; i < 2 * MT; ++i) {
-        if constexpr (BITS == 2) {
-          uint16_t* to = reinterpret_cast<uint16_t*>(s_run + (i * 8 + (c >> 1)) * 32) + (c & 1);
-          *to = (uint16_t)packed[i][0];
-        } else {
-#pragma unroll
-          for (int w = 0; w < cw; ++w) s_run[(i * 8 + c * cw + w) * 32] = packed[i][w];
-        }
-      }
-    }
-
-#pragma unroll 1
-    for (int i = 0; i < 2 * MT; ++i) {
-      const uint32_t r = row0 + g + 8 * i;
-      if (r >= rows) break;
-      const int64_t at = a.place(r);
-      if (at < 0) continue;
-      const int off = (t * (D / 4) + (SMALL ? warp : part * S::per) * 8) * BITS / 8;
-      uint8_t* to = sd.rows + at * sd.ldb + off;
-      const uint32_t* w = s_run + i * 8 * 32;
-      if constexpr (run_bytes >= 16) {
-#pragma unroll
-        for (int j = 0; j < words; j += 4)
-          if (off + 4 * j < sd.ldb)
-            *reinterpret_cast<uint4*>(to + 4 * j) =
-                make_uint4(w[j * 32], w[(j + 1) * 32], w[(j + 2) * 32], w[(j + 3) * 32]);
-      } else if (off < sd.ldb) {
-        if constexpr (run_bytes == 8)
-          *reinterpret_cast<uint2*>(to) = make_uint2(w[0], w[32]);
-        else if constexpr (run_bytes == 4)
-          *reinterpret_cast<uint32_t*>(to) = w[0];
-        else
-          *reinterpret_cast<uint16_t*>(to) = (uint16_t)w[0];
-      }
+      tc::tc_fence_before();
+      __syncwarp();
+      if (lane == 0) tc::mbar_arrive(TEMPTY + 8 * acc);
     }
   }
-}
-
-template <class T, int D, bool SMALL>
-__global__ void __launch_bounds__(32 * AppendShape<T, D, SMALL>::warps, 1)
-kv_append_kernel(AppendArgs a) {
-  extern __shared__ __align__(16) uint8_t smem[];
-  const int bits = blockIdx.y & 1 ? a.sv.bits : a.sk.bits;
-  if (bits == 2)
-    append_rows<T, D, 2, SMALL>(a, smem);
-  else if (bits == 4)
-    append_rows<T, D, 4, SMALL>(a, smem);
-  else
-    append_rows<T, D, 8, SMALL>(a, smem);
-}
-
-template <class T, int D, bool SMALL>
-int launch_append(const AppendArgs& a, cudaStream_t st) {
-  using S = AppendShape<T, D, SMALL>;
-  constexpr int smem = S::smem;
-  auto kern = kv_append_kernel<T, D, SMALL>;
-  PQ_CUDA_TRY(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, smem));
-  const int64_t groups = ((int64_t)a.rows + S::rows - 1) / S::rows;
-  const int64_t blocks = (groups + S::groups - 1) / S::groups;
-  const int64_t most = SMALL ? 1 << 20 : max(1, num_sms() / (2 * S::parts));
-  kern<<<dim3((unsigned)min(blocks, most), 2 * S::parts), 32 * S::warps, smem, st>>>(a);
-  PQ_LAUNCH_CHECK("kv_append_kernel");
-  return PQ_OK;
 }
 
 template <class T, int D>
-int launch_append_rows(const AppendArgs& a, cudaStream_t st) {
-  // Few rows: as many blocks of 16 rows as there are, each reading the planes
-  // from L2; more than two waves of them: resident planes.
-  if (a.rows <= 16u * num_sms()) return launch_append<T, D, true>(a, st);
-  return launch_append<T, D, false>(a, st);
+__global__ void __launch_bounds__(kManyThreads, 1) kv_append_kernel(AppendArgs a) {
+  using S = ManyShape<T, D>;
+  extern __shared__ __align__(16) uint8_t smem_raw[];
+  __shared__ float s_inv[4][128], s_norm[4][128];
+  __shared__ __align__(8) uint64_t s_bar[9];
+  __shared__ uint32_t s_tmem;
+  __shared__ int s_abort;
+  const uint32_t raw = tc::smem_u32(smem_raw);
+  uint8_t* smem = smem_raw + (((raw + 1023u) & ~1023u) - raw);
+  const uint32_t bars = tc::smem_u32(s_bar);
+  if (threadIdx.x == 0) {
+    for (int i = 0; i < 2; ++i) {
+      tc::mbar_init(bars + 8 * i, 8);        // AFULL: the loading warps
+      tc::mbar_init(bars + 16 + 8 * i, 1);   // AEMPTY: a commit
+      tc::mbar_init(bars + 32 + 8 * i, 2);   // TFULL: a commit and the thread itself
+      tc::mbar_init(bars + 48 + 8 * i, 8);   // TEMPTY: the coding warps
+    }
+    tc::mbar_init(bars + 64, 1);
+    s_abort = 0;
+    tc::fence_barrier_init();
+  }
+  if (threadIdx.x >> 5 == 16) tc::tmem_alloc(tc::smem_u32(&s_tmem), S::tmem);
+  tc::tc_fence_before();
+  __syncthreads();
+  tc::tc_fence_after();
+  const uint32_t tmem = s_tmem;
+  const int bits = blockIdx.y & 1 ? a.sv.bits : a.sk.bits;
+  if (bits == 2)
+    append_many<T, D, 2>(a, smem, s_inv, s_norm, bars, tmem, &s_abort);
+  else if (bits == 4)
+    append_many<T, D, 4>(a, smem, s_inv, s_norm, bars, tmem, &s_abort);
+  else
+    append_many<T, D, 8>(a, smem, s_inv, s_norm, bars, tmem, &s_abort);
+  tc::tc_fence_before();
+  __syncthreads();
+  if (threadIdx.x >> 5 == 16) {
+    tc::tc_fence_after();
+    tc::tmem_dealloc(tmem, S::tmem);
+  }
+}
+
+template <class T, int D>
+int launch_append(const AppendArgs& a, cudaStream_t st) {
+  // Few rows (two waves of blocks of 16, 12 us at D = 128 next to 20 us of one
+  // tile's way through the other kernel): the planes from L2.
+  if (a.rows <= 16u * num_sms()) {
+    using S = FewShape<T, D>;
+    kv_append_few_kernel<T, D>
+        <<<dim3((a.rows + S::rows - 1) / S::rows, 2), 32 * S::warps, 0, st>>>(a);
+    PQ_LAUNCH_CHECK("kv_append_few_kernel");
+    return PQ_OK;
+  }
+  using S = ManyShape<T, D>;
+  auto kern = kv_append_kernel<T, D>;
+  PQ_CUDA_TRY(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, S::smem));
+  const uint32_t tiles = (a.rows + 127) / 128;
+  const dim3 grid(min(tiles, (uint32_t)max(1, num_sms() / (2 * S::parts))), 2 * S::parts);
+  kern<<<grid, kManyThreads, S::smem, st>>>(a);
+  PQ_LAUNCH_CHECK("kv_append_kernel");
+  return PQ_OK;
 }
 
 // ---------------------------------------------------------------------------
@@ -685,9 +994,9 @@ int pq_kv_append(const pq_kv_cache* cache, const void* k, const void* v, int dty
   const int D = kv::padded_d(cache->d);
   const cudaStream_t st = (cudaStream_t)stream;
   PQ_KV_DISPATCH_T(dtype, {
-    rc = D == 64 ? kv::launch_append_rows<T_, 64>(a, st)
-                 : D == 128 ? kv::launch_append_rows<T_, 128>(a, st)
-                            : kv::launch_append_rows<T_, 256>(a, st);
+    rc = D == 64 ? kv::launch_append<T_, 64>(a, st)
+                 : D == 128 ? kv::launch_append<T_, 128>(a, st)
+                            : kv::launch_append<T_, 256>(a, st);
   });
   return rc;
 }

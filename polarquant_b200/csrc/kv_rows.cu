@@ -158,7 +158,7 @@ __device__ __forceinline__ void mma_rows(float (&c)[4], const uint32_t (&a)[4], 
 struct AppendArgs {
   const void *k, *v;
   int64_t k_sn, k_sh, v_sn, v_sh;
-  uint32_t rows, heads;
+  uint32_t rows, heads, first_tile;
   int64_t slots_end;
   int d, page_shift;
   bool k_vec, v_vec;  // rows can be read 16 bytes at a time
@@ -213,9 +213,11 @@ __device__ __forceinline__ void widen16(const uint4& w, float* f) {
   }
 }
 
-// The table of cells in shared memory (kCellWords), by all threads of the block.
+// The table of cells (kCellWords) and the boundaries in shared memory, by all
+// threads of the block.
 template <int BITS>
-__device__ __forceinline__ void fill_cells(const Codec& cd, uint32_t* s_cell) {
+__device__ __forceinline__ void fill_cells(const Codec& cd, uint32_t* s_cell, float* s_bounds) {
+  for (int i = threadIdx.x; i < 256; i += blockDim.x) s_bounds[i] = cd.bounds[i];
   if constexpr (BITS == 8) {
     for (int i = threadIdx.x; i < kCells; i += blockDim.x)
       reinterpret_cast<uint2*>(s_cell)[i] = cd.cells[i];
@@ -264,23 +266,119 @@ __host__ __device__ constexpr float band_of(int products, int bits) {
   return (products + 8) * 1.1920929e-7f + (bits == 8 ? 0.f : 1e-6f);
 }
 
-// The code of column `col` of the row at x, by the warp, in f64.
+// The code of column `col` of the row at x by the exact product, by eight
+// neighbouring lanes (all lanes of the warp call it; `valid` ones have a row).
+//
+// First sum_i x_i R_ji / den in f64: rounding x_i / den to f32 first moves that by
+// at most 2^-24 sum |u_i R_ji| <= 2^-24, so only within 1e-7 of a boundary the
+// divisions are taken one by one.  All of a lane's loads of 128 coordinates come
+// before their use (a loop of one after another made 13 us of an event).
 template <class T, int BITS>
-__device__ __forceinline__ uint32_t exact_code(const T* x, float den, const Codec& cd, int col,
-                                               int d) {
+__device__ __noinline__ uint32_t exact_code(const T* x, float den, const float* rr,
+                                            const float* s_bounds, int d, bool vec, bool valid) {
   const int lane = threadIdx.x & 31;
-  const float* rr = cd.R + col * d;
+  constexpr int E = 16 / sizeof(T);
   double y = 0.0;
-#pragma unroll 4
-  for (int j = lane; j < d; j += 32)
-    y = fma((double)__fdiv_rn(to_f32<T>(x[j]), den), (double)__ldg(rr + j), y);
+  if (valid) {
+#pragma unroll 1
+    for (int j0 = (lane & 7) * 8; j0 < d; j0 += 128) {
+      uint4 w[2][8 / E];
+      float4 m[2][2];
 #pragma unroll
-  for (int o = 16; o > 0; o >>= 1) y += __shfl_xor_sync(0xffffffffu, y, o);
-  uint32_t code = 0;
+      for (int h = 0; h < 2; ++h) {
+        const int j = j0 + 64 * h;
+        if (vec && d % 8 == 0 && j < d) {
 #pragma unroll
-  for (int step = 1 << (BITS - 1); step > 0; step >>= 1)
-    if (y > (double)__ldg(cd.bounds + code + step - 1)) code += step;
+          for (int k = 0; k < 8 / E; ++k) w[h][k] = *reinterpret_cast<const uint4*>(x + j + k * E);
+          m[h][0] = __ldg(reinterpret_cast<const float4*>(rr + j));
+          m[h][1] = __ldg(reinterpret_cast<const float4*>(rr + j + 4));
+        } else {
+#pragma unroll
+          for (int k = 0; k < 8 / E; ++k) {
+            __align__(16) T e[E];
+#pragma unroll
+            for (int z = 0; z < E; ++z)
+              e[z] = j + k * E + z < d ? x[j + k * E + z] : from_f32<T>(0.f);
+            w[h][k] = *reinterpret_cast<const uint4*>(e);
+          }
+          float r[8];
+#pragma unroll
+          for (int k = 0; k < 8; ++k) r[k] = j + k < d ? __ldg(rr + j + k) : 0.f;
+          m[h][0] = make_float4(r[0], r[1], r[2], r[3]);
+          m[h][1] = make_float4(r[4], r[5], r[6], r[7]);
+        }
+      }
+#pragma unroll
+      for (int h = 0; h < 2; ++h) {
+        float f[8];
+#pragma unroll
+        for (int k = 0; k < 8 / E; ++k) widen16<T>(w[h][k], f + k * E);
+        const float r[8] = {m[h][0].x, m[h][0].y, m[h][0].z, m[h][0].w,
+                            m[h][1].x, m[h][1].y, m[h][1].z, m[h][1].w};
+#pragma unroll
+        for (int k = 0; k < 8; ++k) y = fma((double)f[k], (double)r[k], y);
+      }
+    }
+  }
+#pragma unroll
+  for (int o = 4; o > 0; o >>= 1) y += __shfl_xor_sync(0xffffffffu, y, o);
+  y /= (double)den;
+  auto count = [&](double v) {
+    uint32_t code = 0;
+#pragma unroll
+    for (int step = 1 << (BITS - 1); step > 0; step >>= 1)
+      if (v > (double)s_bounds[code + step - 1]) code += step;
+    return code;
+  };
+  uint32_t code = count(y);
+  // (or the sum is not finite, of a row whose norm overflows)
+  if (__any_sync(0xffffffffu, valid && !(count(y - 1e-7) == count(y + 1e-7) && isfinite(y)))) {
+    y = 0.0;
+    if (valid)
+      for (int j = lane & 7; j < d; j += 8)
+        y = fma((double)__fdiv_rn(to_f32<T>(x[j]), den), (double)__ldg(rr + j), y);
+#pragma unroll
+    for (int o = 4; o > 0; o >>= 1) y += __shfl_xor_sync(0xffffffffu, y, o);
+    code = count(y);
+  }
   return code;
+}
+
+// Replaces the codes of flagged coordinates, four at a time.  `near`: the lane's
+// flags; where(from, n, ...) gives the row, column and divisor of lane `from`'s
+// flag n; patch(n, code) is called on the lane that had the flag.
+template <class T, int BITS, class Where, class Patch>
+__device__ __forceinline__ void recompute(uint32_t near, const Codec& cd, const float* s_bounds,
+                                          int d, bool vec, Where where, Patch patch) {
+  const int lane = threadIdx.x & 31;
+  uint32_t pend = __ballot_sync(0xffffffffu, near != 0u);
+#pragma unroll 1
+  while (pend) {
+    int from[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      from[i] = pend ? __ffs(pend) - 1 : -1;
+      pend &= pend - 1;
+    }
+    const int mine = lane < 8 ? from[0] : lane < 16 ? from[1] : lane < 24 ? from[2] : from[3];
+    const uint32_t flags = __shfl_sync(0xffffffffu, near, max(mine, 0));
+    const int n = max(__ffs(flags) - 1, 0);
+    const T* x;
+    int col;
+    float den;
+    where(max(mine, 0), n, x, col, den);
+    const uint32_t code =
+        exact_code<T, BITS>(x, den, cd.R + (int64_t)col * d, s_bounds, d, vec, mine >= 0);
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const uint32_t c = __shfl_sync(0xffffffffu, code, 8 * i);
+      if (lane == from[i]) {
+        patch(__ffs(near) - 1, c);
+        near &= near - 1;
+      }
+    }
+    if (!pend) pend = __ballot_sync(0xffffffffu, near != 0u);
+  }
 }
 
 // A quarter of a row, from x on (the row's coordinate k0): D / 4 elements.
@@ -319,7 +417,7 @@ struct RowScale {
 
 template <class T, int N>
 __device__ __forceinline__ RowScale scale_row(const uint4 (&w)[N]) {
-  double ss = 0.0;
+  double s4[4] = {0.0, 0.0, 0.0, 0.0};  // four chains
   float mx = 0.f;
 #pragma unroll
   for (int j = 0; j < N; ++j) {
@@ -327,10 +425,11 @@ __device__ __forceinline__ RowScale scale_row(const uint4 (&w)[N]) {
     widen16<T>(w[j], f);
 #pragma unroll
     for (int k = 0; k < 16 / (int)sizeof(T); ++k) {
-      ss = fma((double)f[k], (double)f[k], ss);
+      s4[k & 3] = fma((double)f[k], (double)f[k], s4[k & 3]);
       mx = fmaxf(mx, fabsf(f[k]));
     }
   }
+  double ss = (s4[0] + s4[1]) + (s4[2] + s4[3]);
 #pragma unroll
   for (int o = 1; o < 4; o <<= 1) {
     ss += __shfl_xor_sync(0xffffffffu, ss, o);
@@ -347,7 +446,7 @@ __device__ __forceinline__ RowScale scale_row(const uint4 (&w)[N]) {
 }
 
 template <class T, int D, int BITS>
-__device__ __forceinline__ void append_few(const AppendArgs& a, uint32_t* s_cell) {
+__device__ __forceinline__ void append_few(const AppendArgs& a, uint32_t* s_cell, float* s_bounds) {
   using S = FewShape<T, D>;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
   const bool is_v = blockIdx.y != 0;
@@ -357,7 +456,7 @@ __device__ __forceinline__ void append_few(const AppendArgs& a, uint32_t* s_cell
   const int64_t sn = is_v ? a.v_sn : a.k_sn, sh = is_v ? a.v_sh : a.k_sh;
   const int d = a.d;
   const uint32_t rows = a.rows, heads = a.heads, row0 = blockIdx.x * S::rows;
-  fill_cells<BITS>(cd, s_cell);
+  fill_cells<BITS>(cd, s_cell, s_bounds);
   __syncthreads();
   const Coder<BITS> coder(cd, s_cell);
   constexpr float band = band_of(S::steps * (S::wide ? 3 : 2), BITS);
@@ -431,32 +530,25 @@ __device__ __forceinline__ void append_few(const AppendArgs& a, uint32_t* s_cell
       packed[i][bit >> 5] |= code << ((bit & 24) + 8 - BITS - (bit & 7));
     }
   }
-  uint32_t pend = __ballot_sync(0xffffffffu, near != 0u);
-#pragma unroll 1
-  while (pend) {
-    const int from = __ffs(pend) - 1;
-    pend &= pend - 1;
-    uint32_t mask = __shfl_sync(0xffffffffu, near, from);
-#pragma unroll 1
-    while (mask) {
-      const int n = __ffs(mask) - 1, i = n >> 3, k = n & 7;
-      mask &= mask - 1;
-      const float dn = __shfl_sync(0xffffffffu, i ? den[1] : den[0], from);
-      const uint32_t r = row0 + (from >> 2) + 8 * i;
-      const T* x = src + (int64_t)(r / heads) * sn + (r % heads) * sh;
-      const uint32_t code =
-          exact_code<T, BITS>(x, dn, cd, (from & 3) * (D / 4) + warp * 8 + k, d);
-      const int bit = k * BITS, shift = (bit & 24) + 8 - BITS - (bit & 7);
-      if (lane == from) {
+  recompute<T, BITS>(
+      near, cd, s_bounds, d, is_v ? a.v_vec : a.k_vec,
+      [&](int from, int n, const T*& x, int& col, float& dn) {
+        const uint32_t r = min(row0 + (from >> 2) + 8 * (n >> 3), rows - 1);
+        x = src + (int64_t)(r / heads) * sn + (r % heads) * sh;
+        col = min((from & 3) * (D / 4) + warp * 8 + (n & 7), d - 1);
+        const float d0 = __shfl_sync(0xffffffffu, den[0], from);
+        const float d1 = __shfl_sync(0xffffffffu, den[1], from);
+        dn = n >> 3 ? d1 : d0;
+      },
+      [&](int n, uint32_t code) {
+        const int bit = (n & 7) * BITS, shift = (bit & 24) + 8 - BITS - (bit & 7);
 #pragma unroll
         for (int z = 0; z < 2; ++z)
 #pragma unroll
           for (int w = 0; w < cw; ++w)
-            if (z == i && w == bit >> 5)
+            if (z == n >> 3 && w == bit >> 5)
               packed[z][w] = (packed[z][w] & ~(((1u << BITS) - 1u) << shift)) | code << shift;
-      }
-    }
-  }
+      });
 #pragma unroll
   for (int i = 0; i < 2; ++i) {
     const uint32_t r = row0 + g + 8 * i;
@@ -478,27 +570,45 @@ template <class T, int D>
 __global__ void __launch_bounds__(32 * FewShape<T, D>::warps, 1)
 kv_append_few_kernel(AppendArgs a) {
   __shared__ __align__(16) uint32_t s_cell[kCellWords];
+  __shared__ float s_bounds[256];
   const int bits = blockIdx.y ? a.sv.bits : a.sk.bits;
   if (bits == 2)
-    append_few<T, D, 2>(a, s_cell);
+    append_few<T, D, 2>(a, s_cell, s_bounds);
   else if (bits == 4)
-    append_few<T, D, 4>(a, s_cell);
+    append_few<T, D, 4>(a, s_cell, s_bounds);
   else
-    append_few<T, D, 8>(a, s_cell);
+    append_few<T, D, 8>(a, s_cell, s_bounds);
 }
 
 // ---------------------------------------------------------------------------
 // Append of many rows.  A persistent block per SM takes one side (at D = 256 a
 // part of its columns too), with R's planes resident in shared memory, and tiles
-// of 128 rows: warps 8-15 load rows (four lanes a row), scale and split them into
-// 128-byte-swizzled K-major f16 tiles; one thread of warp 16 issues the
-// tcgen05.mma (M = 128, N = the block's columns) into one of two TMEM
-// accumulators; warps 0-7 read an accumulator, a lane per row, code, pack and
-// store it.  The three run on different tiles.
+// of 128 rows: sixteen warps load rows (four lanes a row; the next tile's are on
+// their way while this one's are scaled) and split them into 128-byte-swizzled
+// K-major f16 tiles; one thread issues the tcgen05.mma (M = 128, N = the block's
+// columns) into one of two TMEM accumulators; eight other warps read an accumulator, a
+// lane per row, code, pack and store it.  The three run on different tiles.
 //
 // Bound by the instructions of the two ends, some 75 a row and 32 lanes: 25 to
 // widen, square and split 128 coordinates, 12 a coordinate to code it.
 // ---------------------------------------------------------------------------
+
+// tc::mbar_wait that sleeps: the waiting warps would otherwise issue as many
+// instructions as the working ones (measured: 10 us of 75).
+__device__ __forceinline__ bool wait(uint32_t bar, uint32_t parity, volatile int* abort, int err) {
+  if (tc::mbar_try_wait(bar, parity)) return true;
+  const long long t0 = clock64();
+  while (true) {
+    __nanosleep(20);
+    if (tc::mbar_try_wait(bar, parity)) return true;
+    if (*abort) return false;
+    if (clock64() - t0 > tc::kWaitCycles) {
+      *abort = err;
+      device_fail(err);
+      return false;
+    }
+  }
+}
 
 template <class T, int D>
 struct ManyShape {
@@ -509,16 +619,21 @@ struct ManyShape {
   static constexpr int kblocks = D / 64;                      // of 64 elements, 128 bytes a row
   static constexpr int a_bytes = planes * kblocks * 128 * 128;
   static constexpr int b_bytes = 2 * kblocks * cols * 128;
-  static constexpr int buffers = D <= 128 ? 2 : 1;
+  static constexpr int buffers = D <= 64 || (D == 128 && !wide) ? 2 : 1;
+  // Coordinates to recompute that a block lists, and the tiles it takes in a
+  // launch: about half to three quarters of the list at 8 bits and normal data.
+  static constexpr int listed = D <= 128 ? 2048 : 1024;
+  static constexpr int most_tiles = D <= 128 ? 24 : 8;
   static constexpr int tmem = cols < 16 ? 32 : 2 * cols;
-  static constexpr int smem = 1024 + b_bytes + buffers * a_bytes + 4 * kCellWords;
+  static constexpr int smem = 1024 + b_bytes + buffers * a_bytes + 4 * kCellWords + 1024 + 9 * listed;
 };
-constexpr int kManyThreads = 17 * 32;
+constexpr int kCodeWarps = 8, kLoadWarps = 16;
+constexpr int kManyThreads = 32 * (kCodeWarps + kLoadWarps);
 
 template <class T, int D, int BITS>
 __device__ __forceinline__ void append_many(const AppendArgs& a, uint8_t* smem, float (*s_inv)[128],
                                             float (*s_norm)[128], uint32_t bars, uint32_t tmem,
-                                            volatile int* abort) {
+                                            volatile int* abort, int* s_listed) {
   using S = ManyShape<T, D>;
   constexpr int NB = S::buffers;
   uint8_t* s_b = smem;
@@ -533,6 +648,7 @@ __device__ __forceinline__ void append_many(const AppendArgs& a, uint8_t* smem, 
   const int64_t sn = is_v ? a.v_sn : a.k_sn, sh = is_v ? a.v_sh : a.k_sh;
   const int d = a.d;
   const uint32_t rows = a.rows, heads = a.heads;
+  const uint32_t first = blockIdx.x + a.first_tile;
 
   // R's planes: [plane][kblock][column][64], 16-byte pieces exchanged by row & 7.
   for (int i = threadIdx.x; i < 2 * S::cols * (D / 8); i += kManyThreads) {
@@ -543,109 +659,120 @@ __device__ __forceinline__ void append_many(const AppendArgs& a, uint8_t* smem, 
     *reinterpret_cast<uint4*>(s_b + ((plane * S::kblocks + kb) * S::cols + col) * 128 +
                               ((c ^ (col & 7)) << 4)) = v;
   }
-  fill_cells<BITS>(cd, s_cell);
+  float* s_bounds = reinterpret_cast<float*>(s_cell + kCellWords);
+  float* l_den = s_bounds + 256;  // the list: divisor, row, column
+  uint32_t* l_row = reinterpret_cast<uint32_t*>(l_den + S::listed);
+  uint8_t* l_col = reinterpret_cast<uint8_t*>(l_row + S::listed);
+  fill_cells<BITS>(cd, s_cell, s_bounds);
   asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
   __syncthreads();
 
   const uint32_t AFULL = bars, AEMPTY = bars + 16, TFULL = bars + 32, TEMPTY = bars + 48,
                  DRAIN = bars + 64;
-  const uint32_t tiles = (rows + 127) / 128;
-  if (warp >= 8 && warp < 16) {
-    // ---- rows into A tiles: 16 rows a warp, four lanes a row, in two turns ----
-    const int g = lane >> 2, t = lane & 3;
+  const uint32_t tiles = min((rows + 127) / 128, a.first_tile + gridDim.x * S::most_tiles);
+  if (warp >= kCodeWarps) {
+    // ---- rows into A tiles: 8 rows a warp, four lanes a row ----
+    const int t = lane & 3, lr = (warp - kCodeWarps) * 8 + (lane >> 2);  // row of the tile
     const bool vec = is_v ? a.v_vec : a.k_vec;
     constexpr int E = 16 / sizeof(T), N = D / 4 / E;
-    constexpr int AHEAD = D <= 128 ? 2 : 1;  // turns whose loads are in registers
-    uint4 w[AHEAD][N];
-    auto load = [&](uint32_t tile, int turn) {
-      const uint32_t r = min(tile * 128 + (warp - 8) * 16 + turn * 8 + g, rows - 1);
+    constexpr bool AHEAD = N <= 4;  // registers for two tiles' rows
+    uint4 w[N], w1[AHEAD ? N : 1];
+    auto load = [&](uint32_t tile, uint4 (&to)[N]) {
+      const uint32_t r = min(tile * 128 + lr, rows - 1);
       const T* x = src + (int64_t)(r / heads) * sn + (r % heads) * sh + t * (D / 4);
-      load_quarter<T, D>(x, t * (D / 4), d, vec, w[turn % AHEAD]);
+      load_quarter<T, D>(x, t * (D / 4), d, vec, to);
     };
-    uint32_t n = 0;
-    if (blockIdx.x < tiles) {
+    // The products of the block's n-th tile, by one thread of the first of these
+    // warps, once all of them have brought their rows.
+    auto multiply = [&](uint32_t n) {
+      bool ok = true;
+      if (lane == 0) {
+        const int buf = n % NB, acc = n & 1;
+        ok = wait(TEMPTY + 8 * acc, ((n >> 1) & 1) ^ 1, abort, tc::kErrWaitAccEmpty) &&
+             wait(AFULL + 8 * buf, (n / NB) & 1, abort, tc::kErrWaitTmaFull);
+        if (ok) {
+          tc::tc_fence_after();
+          const uint32_t idesc = tc::idesc_f16_f32(128, S::cols);
+          const uint32_t a0 = tc::smem_u32(s_a) + buf * S::a_bytes, b0 = tc::smem_u32(s_b);
+          const uint32_t dt = tmem + acc * S::cols;
+#pragma unroll 1
+          for (int kb = 0; kb < S::kblocks; ++kb) {
+            const uint32_t ah = a0 + kb * 128 * 128, bh = b0 + kb * S::cols * 128;
+            const uint32_t al = ah + S::kblocks * 128 * 128, bl = bh + S::kblocks * S::cols * 128;
 #pragma unroll
-      for (int turn = 0; turn < AHEAD; ++turn) load(blockIdx.x, turn);
-    }
-    for (uint32_t tile = blockIdx.x; tile < tiles; tile += gridDim.x, ++n) {
-      const int buf = n % NB;
-      if (!tc::mbar_wait(AEMPTY + 8 * buf, ((n / NB) & 1) ^ 1, abort, tc::kErrWaitStageEmpty)) break;
-      uint8_t* dst = s_a + buf * S::a_bytes;
-#pragma unroll
-      for (int turn = 0; turn < 2; ++turn) {
-        const int lr = (warp - 8) * 16 + turn * 8 + g;  // row of the tile
-        const RowScale rs = scale_row<T>(w[turn % AHEAD]);
-        if (t == 0) {
-          s_inv[n & 3][lr] = rs.inv;
-          s_norm[n & 3][lr] = rs.norm;
-        }
-        // Pieces of eight f16.
-#pragma unroll
-        for (int p = 0; p < D / 32; ++p) {
-          uint32_t hi[4], lo[4];
-#pragma unroll
-          for (int k = 0; k < 4; ++k) {
-            float f[E];
-            widen16<T>(w[turn % AHEAD][(8 * p + 2 * k) / E], f);
-            const float x0 = f[(8 * p + 2 * k) % E] * rs.up, x1 = f[(8 * p + 2 * k) % E + 1] * rs.up;
-            const __half2 h = __floats2half2_rn(x0, x1);
-            hi[k] = *reinterpret_cast<const uint32_t*>(&h);
-            if constexpr (S::wide) {
-              const float2 b = __half22float2(h);
-              const __half2 l = __floats2half2_rn(x0 - b.x, x1 - b.y);
-              lo[k] = *reinterpret_cast<const uint32_t*>(&l);
+            for (int kk = 0; kk < 4; ++kk) {
+              const uint32_t off = kk * 32;
+              tc::mma_f16(dt, tc::sw128_desc(ah + off), tc::sw128_desc(bh + off), idesc,
+                          (kb | kk) != 0);
+              tc::mma_f16(dt, tc::sw128_desc(ah + off), tc::sw128_desc(bl + off), idesc, 1);
+              if constexpr (S::wide)
+                tc::mma_f16(dt, tc::sw128_desc(al + off), tc::sw128_desc(bh + off), idesc, 1);
             }
           }
-          const int piece = t * (D / 32) + p, kb = piece >> 3, c = piece & 7;
-          uint8_t* to = dst + (kb * 128 + lr) * 128 + ((c ^ (lr & 7)) << 4);
-          *reinterpret_cast<uint4*>(to) = make_uint4(hi[0], hi[1], hi[2], hi[3]);
-          if constexpr (S::wide)
-            *reinterpret_cast<uint4*>(to + S::kblocks * 128 * 128) =
-                make_uint4(lo[0], lo[1], lo[2], lo[3]);
+          tc::mma_commit(AEMPTY + 8 * buf);
+          tc::mma_commit(TFULL + 8 * acc);
+          tc::mbar_arrive(TFULL + 8 * acc);  // hands on what the loading warps wrote besides
         }
-        if (AHEAD == 1 && turn == 0)
-          load(tile, 1);
-        else if (tile + gridDim.x < tiles)
-          load(tile + gridDim.x, AHEAD == 1 ? 0 : turn);
+      }
+      return __shfl_sync(0xffffffffu, (int)ok, 0) != 0;
+    };
+    uint32_t n = 0;
+    if (first < tiles) load(first, w);
+    for (uint32_t tile = first; tile < tiles; tile += gridDim.x, ++n) {
+      const int buf = n % NB;
+      const bool more = tile + gridDim.x < tiles;
+      if constexpr (AHEAD)
+        if (more) load(tile + gridDim.x, w1);
+      const RowScale rs = scale_row<T>(w);
+      if (!wait(AEMPTY + 8 * buf, ((n / NB) & 1) ^ 1, abort, tc::kErrWaitStageEmpty)) break;
+      uint8_t* dst = s_a + buf * S::a_bytes;
+      if (t == 0) {
+        s_inv[n & 3][lr] = rs.inv;
+        s_norm[n & 3][lr] = rs.norm;
+      }
+      // Pieces of eight f16.
+#pragma unroll
+      for (int p = 0; p < D / 32; ++p) {
+        uint32_t hi[4], lo[4];
+#pragma unroll
+        for (int k = 0; k < 4; ++k) {
+          float f[E];
+          widen16<T>(w[(8 * p + 2 * k) / E], f);
+          const float x0 = f[(8 * p + 2 * k) % E] * rs.up, x1 = f[(8 * p + 2 * k) % E + 1] * rs.up;
+          const __half2 h = __floats2half2_rn(x0, x1);
+          hi[k] = *reinterpret_cast<const uint32_t*>(&h);
+          if constexpr (S::wide) {
+            const float2 b = __half22float2(h);
+            const __half2 l = __floats2half2_rn(x0 - b.x, x1 - b.y);
+            lo[k] = *reinterpret_cast<const uint32_t*>(&l);
+          }
+        }
+        const int piece = t * (D / 32) + p, kb = piece >> 3, c = piece & 7;
+        uint8_t* to = dst + (kb * 128 + lr) * 128 + ((c ^ (lr & 7)) << 4);
+        *reinterpret_cast<uint4*>(to) = make_uint4(hi[0], hi[1], hi[2], hi[3]);
+        if constexpr (S::wide)
+          *reinterpret_cast<uint4*>(to + S::kblocks * 128 * 128) =
+              make_uint4(lo[0], lo[1], lo[2], lo[3]);
       }
       asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
       __syncwarp();
       if (lane == 0) tc::mbar_arrive(AFULL + 8 * buf);
-    }
-  } else if (warp == 16) {
-    if (lane == 0) {
-      // ---- products ----
-      const uint32_t b0 = tc::smem_u32(s_b), idesc = tc::idesc_f16_f32(128, S::cols);
-      uint32_t n = 0;
-      for (uint32_t tile = blockIdx.x; tile < tiles; tile += gridDim.x, ++n) {
-        const int buf = n % NB, acc = n & 1;
-        if (!tc::mbar_wait(TEMPTY + 8 * acc, ((n >> 1) & 1) ^ 1, abort, tc::kErrWaitAccEmpty)) break;
-        if (!tc::mbar_wait(AFULL + 8 * buf, (n / NB) & 1, abort, tc::kErrWaitTmaFull)) break;
-        tc::tc_fence_after();
-        const uint32_t a0 = tc::smem_u32(s_a) + buf * S::a_bytes, dt = tmem + acc * S::cols;
-        for (int kb = 0; kb < S::kblocks; ++kb) {
-          const uint32_t ah = a0 + kb * 128 * 128, bh = b0 + kb * S::cols * 128;
-          const uint32_t al = ah + S::kblocks * 128 * 128, bl = bh + S::kblocks * S::cols * 128;
+      if (warp == kCodeWarps && !multiply(n)) break;
+      if constexpr (AHEAD) {
 #pragma unroll
-          for (int kk = 0; kk < 4; ++kk) {
-            const uint32_t off = kk * 32;
-            tc::mma_f16(dt, tc::sw128_desc(ah + off), tc::sw128_desc(bh + off), idesc,
-                        (kb | kk) != 0);
-            tc::mma_f16(dt, tc::sw128_desc(ah + off), tc::sw128_desc(bl + off), idesc, 1);
-            if constexpr (S::wide)
-              tc::mma_f16(dt, tc::sw128_desc(al + off), tc::sw128_desc(bh + off), idesc, 1);
-          }
-        }
-        tc::mma_commit(AEMPTY + 8 * buf);
-        tc::mma_commit(TFULL + 8 * acc);
-        tc::mbar_arrive(TFULL + 8 * acc);  // hands on what the loading warps wrote besides
+        for (int j = 0; j < N; ++j) w[j] = w1[j];
+      } else {
+        if (more) load(tile + gridDim.x, w);
       }
+    }
+    if (warp == kCodeWarps && lane == 0) {
       // Before the block ends, every product that was issued has completed.
       tc::mma_commit(DRAIN);
       volatile int never = 0;
-      tc::mbar_wait(DRAIN, 0, &never, tc::kErrWaitAccFull);
+      wait(DRAIN, 0, &never, tc::kErrWaitAccFull);
     }
-  } else if (warp < 8) {
+    __syncwarp();
+  } else {
     // ---- accumulators into codes: warps w and w + 4 the halves of the columns ----
     const int q = warp & 3, half = warp >> 2;
     const Coder<BITS> coder(cd, s_cell);
@@ -655,10 +782,10 @@ __device__ __forceinline__ void append_many(const AppendArgs& a, uint8_t* smem, 
       const uint32_t r = tile * 128 + q * 32 + lane;
       return tile < tiles && r < rows ? a.place(r) : (int64_t)-1;
     };
-    int64_t next = place(blockIdx.x);
-    for (uint32_t tile = blockIdx.x; tile < tiles; tile += gridDim.x, ++n) {
+    int64_t next = place(first);
+    for (uint32_t tile = first; tile < tiles; tile += gridDim.x, ++n) {
       const int acc = n & 1;
-      if (!tc::mbar_wait(TFULL + 8 * acc, (n >> 1) & 1, abort, tc::kErrWaitAccFull)) break;
+      if (!wait(TFULL + 8 * acc, (n >> 1) & 1, abort, tc::kErrWaitAccFull)) break;
       tc::tc_fence_after();
       const uint32_t row = tile * 128 + q * 32 + lane;
       const float inv = s_inv[n & 3][q * 32 + lane], norm = s_norm[n & 3][q * 32 + lane];
@@ -709,29 +836,36 @@ __device__ __forceinline__ void append_many(const AppendArgs& a, uint8_t* smem, 
           }
         }
         if (at < 0) near = 0u;
-        uint32_t pend = __ballot_sync(0xffffffffu, near != 0u);
+        // Coordinates next to a boundary go to the list; behind its end (a batch of
+        // zero vectors, say) they are recomputed at once.
+        if (near) {
+          const int cnt = __popc(near);
+          int i = atomicAdd(s_listed, cnt);
 #pragma unroll 1
-        while (pend) {
-          const int from = __ffs(pend) - 1;
-          pend &= pend - 1;
-          uint32_t mask = __shfl_sync(0xffffffffu, near, from);
-          const uint32_t r = tile * 128 + q * 32 + from;
-          const float dn = __shfl_sync(0xffffffffu, den, from);
-          const T* x = src + (int64_t)(r / heads) * sn + (r % heads) * sh;
-#pragma unroll 1
-          while (mask) {
-            const int k = __ffs(mask) - 1;
-            mask &= mask - 1;
-            const uint32_t code = exact_code<T, BITS>(x, dn, cd, col0 + k, d);
-            const int bit = k * BITS, shift = (bit & 24) + 8 - BITS - (bit & 7);
-            if (lane == from) {
-#pragma unroll
-              for (int w = 0; w < BITS; ++w)
-                if (w == bit >> 5)
-                  packed[w] = (packed[w] & ~(((1u << BITS) - 1u) << shift)) | code << shift;
-            }
+          while (near && i < S::listed) {
+            l_den[i] = den;
+            l_row[i] = row;
+            l_col[i] = (uint8_t)(col0 + __ffs(near) - 1);
+            near &= near - 1;
+            ++i;
           }
         }
+        if (__any_sync(0xffffffffu, near != 0u))
+          recompute<T, BITS>(
+              near, cd, s_bounds, d, is_v ? a.v_vec : a.k_vec,
+              [&](int from, int k, const T*& x, int& col, float& dn) {
+                const uint32_t r = min(tile * 128 + q * 32 + from, rows - 1);
+                x = src + (int64_t)(r / heads) * sn + (r % heads) * sh;
+                col = min(col0 + k, d - 1);
+                dn = __shfl_sync(0xffffffffu, den, from);
+              },
+              [&](int k, uint32_t code) {
+                const int bit = k * BITS, shift = (bit & 24) + 8 - BITS - (bit & 7);
+#pragma unroll
+                for (int w = 0; w < BITS; ++w)
+                  if (w == bit >> 5)
+                    packed[w] = (packed[w] & ~(((1u << BITS) - 1u) << shift)) | code << shift;
+              });
         if (at >= 0) {
           const int off = col0 * BITS / 8;
           if constexpr (BITS == 2) {
@@ -750,6 +884,27 @@ __device__ __forceinline__ void append_many(const AppendArgs& a, uint8_t* smem, 
       if (lane == 0) tc::mbar_arrive(TEMPTY + 8 * acc);
     }
   }
+
+  // The listed coordinates, by all warps, into the rows as they are stored (codes
+  // of one word may be replaced at the same time: by atomics on their own bits).
+  __syncthreads();
+  const int listed = min(*s_listed, S::listed);
+#pragma unroll 1
+  for (int e0 = warp * 4; e0 < listed; e0 += kManyThreads / 32 * 4) {
+    const int e = min(e0 + (lane >> 3), listed - 1);
+    const bool valid = e0 + (lane >> 3) < listed;
+    const uint32_t r = l_row[e];
+    const int col = l_col[e];
+    const uint32_t code = exact_code<T, BITS>(
+        src + (int64_t)(r / heads) * sn + (r % heads) * sh, l_den[e], cd.R + (int64_t)col * d,
+        s_bounds, d, is_v ? a.v_vec : a.k_vec, valid);
+    if (valid && (lane & 7) == 0) {
+      const int bit = col * BITS, shift = (bit & 24) + 8 - BITS - (bit & 7);
+      uint32_t* word = reinterpret_cast<uint32_t*>(sd.rows + a.place(r) * sd.ldb) + (bit >> 5);
+      atomicAnd(word, ~(((1u << BITS) - 1u) << shift));
+      atomicOr(word, code << shift);
+    }
+  }
 }
 
 template <class T, int D>
@@ -759,36 +914,36 @@ __global__ void __launch_bounds__(kManyThreads, 1) kv_append_kernel(AppendArgs a
   __shared__ float s_inv[4][128], s_norm[4][128];
   __shared__ __align__(8) uint64_t s_bar[9];
   __shared__ uint32_t s_tmem;
-  __shared__ int s_abort;
+  __shared__ int s_abort, s_listed;
   const uint32_t raw = tc::smem_u32(smem_raw);
   uint8_t* smem = smem_raw + (((raw + 1023u) & ~1023u) - raw);
   const uint32_t bars = tc::smem_u32(s_bar);
   if (threadIdx.x == 0) {
     for (int i = 0; i < 2; ++i) {
-      tc::mbar_init(bars + 8 * i, 8);        // AFULL: the loading warps
-      tc::mbar_init(bars + 16 + 8 * i, 1);   // AEMPTY: a commit
-      tc::mbar_init(bars + 32 + 8 * i, 2);   // TFULL: a commit and the thread itself
-      tc::mbar_init(bars + 48 + 8 * i, 8);   // TEMPTY: the coding warps
+      tc::mbar_init(bars + 8 * i, kLoadWarps);       // AFULL: the loading warps
+      tc::mbar_init(bars + 16 + 8 * i, 1);           // AEMPTY: a commit
+      tc::mbar_init(bars + 32 + 8 * i, 2);           // TFULL: a commit and the thread itself
+      tc::mbar_init(bars + 48 + 8 * i, kCodeWarps);  // TEMPTY: the coding warps
     }
     tc::mbar_init(bars + 64, 1);
-    s_abort = 0;
+    s_abort = s_listed = 0;
     tc::fence_barrier_init();
   }
-  if (threadIdx.x >> 5 == 16) tc::tmem_alloc(tc::smem_u32(&s_tmem), S::tmem);
+  if (threadIdx.x >> 5 == kCodeWarps) tc::tmem_alloc(tc::smem_u32(&s_tmem), S::tmem);
   tc::tc_fence_before();
   __syncthreads();
   tc::tc_fence_after();
   const uint32_t tmem = s_tmem;
   const int bits = blockIdx.y & 1 ? a.sv.bits : a.sk.bits;
   if (bits == 2)
-    append_many<T, D, 2>(a, smem, s_inv, s_norm, bars, tmem, &s_abort);
+    append_many<T, D, 2>(a, smem, s_inv, s_norm, bars, tmem, &s_abort, &s_listed);
   else if (bits == 4)
-    append_many<T, D, 4>(a, smem, s_inv, s_norm, bars, tmem, &s_abort);
+    append_many<T, D, 4>(a, smem, s_inv, s_norm, bars, tmem, &s_abort, &s_listed);
   else
-    append_many<T, D, 8>(a, smem, s_inv, s_norm, bars, tmem, &s_abort);
+    append_many<T, D, 8>(a, smem, s_inv, s_norm, bars, tmem, &s_abort, &s_listed);
   tc::tc_fence_before();
   __syncthreads();
-  if (threadIdx.x >> 5 == 16) {
+  if (threadIdx.x >> 5 == kCodeWarps) {
     tc::tc_fence_after();
     tc::tmem_dealloc(tmem, S::tmem);
   }
@@ -810,8 +965,11 @@ int launch_append(const AppendArgs& a, cudaStream_t st) {
   PQ_CUDA_TRY(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, S::smem));
   const uint32_t tiles = (a.rows + 127) / 128;
   const dim3 grid(min(tiles, (uint32_t)max(1, num_sms() / (2 * S::parts))), 2 * S::parts);
-  kern<<<grid, kManyThreads, S::smem, st>>>(a);
-  PQ_LAUNCH_CHECK("kv_append_kernel");
+  AppendArgs part = a;
+  for (part.first_tile = 0; part.first_tile < tiles; part.first_tile += grid.x * S::most_tiles) {
+    kern<<<grid, kManyThreads, S::smem, st>>>(part);
+    PQ_LAUNCH_CHECK("kv_append_kernel");
+  }
   return PQ_OK;
 }
 
@@ -973,6 +1131,7 @@ int pq_kv_append(const pq_kv_cache* cache, const void* k, const void* v, int dty
   a.v_sn = v_stride_n;
   a.v_sh = v_stride_h;
   a.rows = (uint32_t)(n * cache->heads);
+  a.first_tile = 0;
   a.slots_end = (int64_t)cache->pages * cache->page_size;
   a.heads = cache->heads;
   a.d = cache->d;

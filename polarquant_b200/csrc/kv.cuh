@@ -3,6 +3,8 @@
 #pragma once
 #include <cuda_bf16.h>
 
+#include <atomic>
+
 #include "common.cuh"
 
 namespace pqb {
@@ -120,6 +122,21 @@ inline int check_sequences(const int32_t* table, int table_width, const int32_t*
                "a sequence has at most 2^30 tokens");
   PQ_CHECK_ARG((table || table_width == 0) && lengths, "null table or lengths");
   PQ_CHECK_ARG(batch >= 0, "batch must be at least 0");
+  return PQ_OK;
+}
+
+// Lets a kernel take more than 48 KB of dynamic shared memory, once on each
+// device (the runtime's call costs 1 us; a device's number above 63 asks anew).
+// K is the kernel itself, so that each has a mask of its own.
+template <auto K>
+inline int allow_smem(int bytes) {
+  static std::atomic<uint64_t> done{0};
+  int dev = 0;
+  PQ_CUDA_TRY(cudaGetDevice(&dev));
+  const uint64_t bit = dev < 64 ? 1ull << dev : 0ull;
+  if (done.load(std::memory_order_relaxed) & bit) return PQ_OK;
+  PQ_CUDA_TRY(cudaFuncSetAttribute(K, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes));
+  done.fetch_or(bit, std::memory_order_relaxed);
   return PQ_OK;
 }
 

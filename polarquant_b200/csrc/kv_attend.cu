@@ -1008,8 +1008,8 @@ int launch_attend(const pq_kv_cache& c, Work wk, const AttendPlan& p, int worker
   auto kern = kv_attend_kernel<D, KB, VB, PREC>;
   const int page_shift = page_shift_of(c);
   static_assert(Shape::warps >= 4 && Shape::unit >= kLeastUnit, "too little shared memory");
-  PQ_CUDA_TRY(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize,
-                                   (int)Shape::smem));
+  const int rc = allow_smem<kv_attend_kernel<D, KB, VB, PREC>>(Shape::smem);
+  if (rc) return rc;
   return launch_pdl(kern, dim3(workers), Shape::threads, Shape::smem, st, true, side_k(c),
                     side_v(c), c.pages, page_shift, wk, p.q, p.parts, p.scores, p.width);
 }

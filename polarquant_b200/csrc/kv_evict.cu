@@ -360,8 +360,8 @@ int launch_select(const EvictArgs& a, int rows, int64_t width, cudaStream_t st) 
   at.val.clusterDim.y = at.val.clusterDim.z = 1;
   cfg.attrs = &at;
   cfg.numAttrs = 1;
-  PQ_CUDA_TRY(cudaFuncSetAttribute(kv_select_kernel<CL>, cudaFuncAttributeMaxDynamicSharedMemorySize,
-                                   kKeep * 4));
+  const int rc = allow_smem<kv_select_kernel<CL>>(kKeep * 4);
+  if (rc) return rc;
   PQ_CUDA_TRY(cudaLaunchKernelEx(&cfg, kv_select_kernel<CL>, a));
   PQ_LAUNCH_CHECK("kv_select_kernel");
   return PQ_OK;

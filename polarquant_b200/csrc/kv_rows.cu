@@ -962,7 +962,8 @@ int launch_append(const AppendArgs& a, cudaStream_t st) {
   }
   using S = ManyShape<T, D>;
   auto kern = kv_append_kernel<T, D>;
-  PQ_CUDA_TRY(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, S::smem));
+  const int rc = allow_smem<kv_append_kernel<T, D>>(S::smem);
+  if (rc) return rc;
   const uint32_t tiles = (a.rows + 127) / 128;
   const dim3 grid(min(tiles, (uint32_t)max(1, num_sms() / (2 * S::parts))), 2 * S::parts);
   AppendArgs part = a;

@@ -169,6 +169,8 @@ class KVCache:
             heads=self.heads, page_size=self.page_size, d=self.d, k_bits=key.bits,
             v_bits=value.bits)
         self._ref = ctypes.byref(self._desc)
+        self._scale = 1.0 / math.sqrt(self.d)
+        self._sizes: Dict[tuple, int] = {}
 
     @property
     def nbytes(self) -> int:
@@ -178,23 +180,37 @@ class KVCache:
                     self.weights))
 
     # -- checks ----------------------------------------------------------------
+    # (A generation step calls attend and append once a layer, on work of a few
+    # microseconds: sizes of workspaces are kept, and what is right is found right
+    # in one comparison.)
     def _call(self, name: str, *args) -> None:
         """The entry point on the cache's device and its current stream."""
-        if torch.cuda.current_device() != self.device.index:
-            with torch.cuda.device(self.device):
+        index = self.device.index
+        if torch.cuda.current_device() != index:
+            with torch.cuda.device(index):
                 _lib.call(name, self._ref, *args, stream_ptr(self.device))
         else:
-            _lib.call(name, self._ref, *args, stream_ptr(self.device))
+            _lib.call(name, self._ref, *args, torch._C._cuda_getCurrentRawStream(index))
+
+    def _workspace(self, name: str, *sizes: int) -> torch.Tensor:
+        nbytes = self._sizes.get((name, sizes))
+        if nbytes is None:
+            nbytes = max(256, _lib.query(name, self._ref, *sizes))
+            if len(self._sizes) >= 4096:
+                self._sizes.clear()
+            self._sizes[name, sizes] = nbytes
+        return self.k_rows.new_empty(nbytes)
 
     def _tensor(self, name: str, t, dtype: torch.dtype, shape: Tuple[int, ...]) -> None:
         if not isinstance(t, torch.Tensor):
             raise TypeError(f"{name} must be a tensor, got {type(t).__name__}")
+        if t.dtype is dtype and t.shape == shape and t.device == self.device:
+            return
         if t.device != self.device:
             raise ValueError(f"{name} is on {t.device}, the cache on {self.device}")
         if t.dtype != dtype:
             raise TypeError(f"{name} must be {dtype}, got {t.dtype}")
-        if tuple(t.shape) != shape:
-            raise ValueError(f"{name} must have shape {shape}, got {tuple(t.shape)}")
+        raise ValueError(f"{name} must have shape {shape}, got {tuple(t.shape)}")
 
     def _vectors(self, name: str, t, shape: Tuple[int, ...]) -> int:
         if not isinstance(t, torch.Tensor):
@@ -213,29 +229,31 @@ class KVCache:
                              f"under torch.no_grad() or detach it")
         return code
 
-    def _sequences(self, table, lengths) -> int:
+    def _vector(self, name: str, t, dtype: torch.dtype, n: int) -> None:
+        self._tensor(name, t, dtype, (n,))
+        if n > 1 and t.stride(0) != 1:
+            raise ValueError(f"{name} must be contiguous")
+
+    def _sequences(self, table, lengths) -> Tuple[int, int]:
         if not isinstance(table, torch.Tensor) or table.dim() != 2:
             raise ValueError("table must be a (sequences, pages) tensor")
-        batch = table.shape[0]
-        self._tensor("table", table, torch.int32, (batch, table.shape[1]))
-        self._tensor("lengths", lengths, torch.int32, (batch,))
-        if table.shape[1] > 1 and table.stride(1) != 1:
+        batch, width = shape = tuple(table.shape)
+        self._tensor("table", table, torch.int32, shape)
+        self._vector("lengths", lengths, torch.int32, batch)
+        if width > 1 and table.stride(1) != 1:
             raise ValueError("table's last dimension must be contiguous")
-        if batch > 1 and lengths.stride(0) != 1:
-            raise ValueError("lengths must be contiguous")
-        if table.shape[1] * self.page_size > 1 << 30:
+        if width * self.page_size > 1 << 30:
             raise ValueError("a sequence has at most 2^30 tokens")
-        return batch
+        return batch, width
 
     def _slots(self, slots) -> int:
         if not isinstance(slots, torch.Tensor) or slots.dim() != 1:
             raise ValueError("slots must be a 1-d tensor")
-        self._tensor("slots", slots, torch.int64, (slots.shape[0],))
-        if slots.shape[0] > 1 and slots.stride(0) != 1:
-            raise ValueError("slots must be contiguous")
-        if slots.shape[0] * self.heads >= 1 << 31:
+        n = slots.shape[0]
+        self._vector("slots", slots, torch.int64, n)
+        if n * self.heads >= 1 << 31:
             raise ValueError("a call takes fewer than 2^31 rows")
-        return slots.shape[0]
+        return n
 
     # -- operators ---------------------------------------------------------------
     def append(self, k: torch.Tensor, v: torch.Tensor, slots: torch.Tensor,
@@ -257,9 +275,7 @@ class KVCache:
         self._vectors("v", v, shape)
         if k.dtype != v.dtype:
             raise TypeError(f"k and v must have one type, got {k.dtype} and {v.dtype}")
-        self._tensor("positions", positions, torch.int32, (n,))
-        if n > 1 and positions.stride(0) != 1:
-            raise ValueError("positions must be contiguous")
+        self._vector("positions", positions, torch.int32, n)
         if weights is not None:
             self._tensor("weights", weights, torch.float32, shape[:2])
             if not weights.is_contiguous():
@@ -282,8 +298,7 @@ class KVCache:
         if dtype not in DTYPES:
             raise TypeError(f"dtype must be float32, float16 or bfloat16, got {dtype}")
         kind = dtype if rotated else torch.float32
-        k, v = (torch.empty((n, self.heads, self.d), dtype=kind, device=self.device)
-                for _ in range(2))
+        k, v = (self.weights.new_empty((n, self.heads, self.d), dtype=kind) for _ in range(2))
         if n:
             self._call("pq_kv_read", slots.data_ptr(), n, k.data_ptr(), v.data_ptr(), DTYPES[kind])
         if not rotated:
@@ -324,26 +339,26 @@ class KVCache:
         heads of its key-value head, to ``weights``, which ``evict`` goes by.
         (The sum of several sequences that share a page is taken in no fixed
         order.)"""
-        batch = self._sequences(table, lengths)
+        batch, width = self._sequences(table, lengths)
         if not isinstance(q, torch.Tensor) or q.dim() != 3:
             raise ValueError("q must be a (sequences, query heads, d) tensor")
         hq = q.shape[1]
         if hq == 0 or hq % self.heads:
             raise ValueError(f"query heads must be a multiple of the cache's {self.heads}, got {hq}")
         code = self._vectors("q", q, (batch, hq, self.d))
-        scale = 1.0 / math.sqrt(self.d) if scale is None else float(scale)
-        if not math.isfinite(scale):
+        if scale is None:
+            scale = self._scale
+        elif not math.isfinite(scale):
             raise ValueError(f"scale must be finite, got {scale}")
-        out = torch.empty((batch, hq, self.d), dtype=q.dtype, device=self.device)
-        lse = torch.empty((batch, hq), dtype=torch.float32, device=self.device) if return_lse \
-            else None
+        out = q.new_empty((batch, hq, self.d))
+        lse = self.weights.new_empty((batch, hq)) if return_lse else None
         if batch:
-            ws = workspace(_lib.query("pq_kv_attend_workspace_bytes", self._ref, batch, hq,
-                                      table.shape[1], int(accumulate)), self.device)
-            self._call("pq_kv_attend", q.data_ptr(), code, q.stride(0), q.stride(1),
-                       table.data_ptr(), table.stride(0), table.shape[1], lengths.data_ptr(),
-                       batch, hq, scale, out.data_ptr(), 0 if lse is None else lse.data_ptr(),
-                       int(accumulate), ws.data_ptr(), ws.numel())
+            accumulate = int(bool(accumulate))
+            ws = self._workspace("pq_kv_attend_workspace_bytes", batch, hq, width, accumulate)
+            self._call("pq_kv_attend", q.data_ptr(), code, *q.stride()[:2], table.data_ptr(),
+                       table.stride(0), width, lengths.data_ptr(), batch, hq, scale,
+                       out.data_ptr(), lse.data_ptr() if return_lse else 0, accumulate,
+                       ws.data_ptr(), ws.numel())
         return (out, lse) if return_lse else out
 
     def evict(self, table: torch.Tensor, lengths: torch.Tensor, budget: int, *, recent: int = 0,
@@ -364,7 +379,7 @@ class KVCache:
 
         A page must belong to one sequence only: a shared prefix is copied, or
         left out of the table, before."""
-        batch = self._sequences(table, lengths)
+        batch, table_width = self._sequences(table, lengths)
         for name, x in (("budget", budget), ("recent", recent), ("sinks", sinks)):
             if int(x) != x or not 0 <= x < 1 << 31:
                 raise ValueError(f"{name} must be an integer in [0, 2^31), got {x}")
@@ -378,11 +393,10 @@ class KVCache:
                 raise ValueError("weights' last dimension must be contiguous")
             given = (weights.data_ptr() or self.weights.data_ptr(), weights.stride(0),
                      weights.stride(1))
-        new = torch.empty(batch, dtype=torch.int32, device=self.device)
+        new = self.positions.new_empty(batch)
         if batch:
-            ws = workspace(_lib.query("pq_kv_evict_workspace_bytes", self._ref, batch,
-                                      table.shape[1], int(budget)), self.device)
-            self._call("pq_kv_evict", table.data_ptr(), table.stride(0), table.shape[1],
+            ws = self._workspace("pq_kv_evict_workspace_bytes", batch, table_width, int(budget))
+            self._call("pq_kv_evict", table.data_ptr(), table.stride(0), table_width,
                        lengths.data_ptr(), batch, int(budget), int(recent), int(sinks), *given,
                        width, new.data_ptr(), ws.data_ptr(), ws.numel())
         return new

@@ -300,7 +300,7 @@ struct QueryOut {
   float* factor;    // [segment][8]: score = factor * key norm * product, in log2
 };
 
-// Blocks that turn rows by a D x D matrix: kRotParts threads a column share its
+// Turning rows by a D x D matrix: kRotParts threads a column share its
 // products, so that few blocks have many loads of the matrix in flight (64 KB
 // from L2 at D = 128; one row of loads after another took 16 us).
 constexpr int kRotParts = 4;

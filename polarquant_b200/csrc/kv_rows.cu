@@ -261,6 +261,16 @@ struct Coder {
   }
 };
 
+// A word of codes of 0.
+template <int BITS>
+__device__ __forceinline__ uint32_t zero_codes(const float* s_bounds) {
+  uint32_t code = 0;
+#pragma unroll
+  for (int step = 1 << (BITS - 1); step > 0; step >>= 1)
+    if (0.f > s_bounds[code + step - 1]) code += step;
+  return code * (BITS == 8 ? 0x01010101u : BITS == 4 ? 0x11111111u : 0x55555555u);
+}
+
 // A boundary below 1 with its low four bits taken loses 15 * 2^-24 < 1e-6.
 __host__ __device__ constexpr float band_of(int products, int bits) {
   return (products + 8) * 1.1920929e-7f + (bits == 8 ? 0.f : 1e-6f);
@@ -465,6 +475,7 @@ __device__ __forceinline__ void append_few(const AppendArgs& a, uint32_t* s_cell
   // the second.
   uint32_t ah[S::steps][4], al[S::wide ? S::steps : 1][4];
   float inv[2], den[2];
+  bool zero[2];
 #pragma unroll
   for (int i = 0; i < 2; ++i) {
     const uint32_t r = min(row0 + g + 8 * i, rows - 1);
@@ -475,6 +486,7 @@ __device__ __forceinline__ void append_few(const AppendArgs& a, uint32_t* s_cell
     const RowScale rs = scale_row<T>(w);
     inv[i] = rs.inv;
     den[i] = rs.den;
+    zero[i] = rs.norm == 0.f;
     if (t == 0 && warp == 0 && row0 + g + 8 * i < rows) {
       const int64_t at = a.place(r);
       if (at >= 0) a.write_token(sd, is_v, r, at, rs.norm);
@@ -528,6 +540,19 @@ __device__ __forceinline__ void append_few(const AppendArgs& a, uint32_t* s_cell
         near |= 1u << (8 * i + k);
       const int bit = k * BITS;
       packed[i][bit >> 5] |= code << ((bit & 24) + 8 - BITS - (bit & 7));
+    }
+    if (zero[i]) {  // all coordinates 0, which may be next to a boundary
+      near &= ~(255u << (8 * i));
+      const uint32_t word = zero_codes<BITS>(s_bounds);
+#pragma unroll
+      for (int w = 0; w < cw; ++w) packed[i][w] = 0u;
+#pragma unroll
+      for (int k = 0; k < 8; ++k) {
+        const int bit = k * BITS;
+        if (col0 + k < d)
+          packed[i][bit >> 5] |=
+              word & ((1u << BITS) - 1u) << ((bit & 24) + 8 - BITS - (bit & 7));
+      }
     }
   }
   recompute<T, BITS>(
@@ -825,6 +850,11 @@ __device__ __forceinline__ void append_many(const AppendArgs& a, uint8_t* smem, 
               x = (x << BITS) + code;
           }
           packed[w] = BITS == 8 ? x : __byte_perm(x, 0u, 0x0123);
+        }
+        if (norm == 0.f) {  // all coordinates 0, which may be next to a boundary
+          near = 0u;
+#pragma unroll
+          for (int w = 0; w < BITS; ++w) packed[w] = zero_codes<BITS>(s_bounds);
         }
         if (left < 32) {
           near &= (1u << left) - 1u;

@@ -202,6 +202,115 @@ def test_large_append(gpu):
     c.check_pool()
 
 
+def encoded(x, R, boundaries):
+    """Codes and norms of vectors on the GPU, the product in 64 bits."""
+    x = x.float()
+    norms = x.double().square().sum(-1).sqrt().float()
+    unit = x / norms.clamp_min(1e-8)[..., None]
+    R, edges = (torch.tensor(t, device="cuda").double() for t in (R, boundaries))
+    turned = torch.cat([u.double() @ R.T for u in unit.flatten(0, 1).split(100000)])
+    return torch.bucketize(turned, edges, out_int32=True).view(x.shape), norms
+
+
+def check_rows(cache, codecs, k, v, slots):
+    """Codes (as values) and norms of tokens that were appended in order."""
+    page = cache.page_size
+    got = cache.read(slots, rotated=True)
+    for x, y, codec, norms in ((k, got[0], codecs[0], cache.k_norms), (v, got[1], codecs[1], cache.v_norms)):
+        code, norm = encoded(x, codec[0], codec[1])
+        assert torch.equal(norms[slots // page, :, slots % page], norm)
+        assert torch.equal(y, torch.tensor(codec[2], device="cuda")[code] * norm[..., None])
+
+
+@pytest.mark.parametrize("dtype", ["f32", "f16", "bf16"])
+@pytest.mark.parametrize("d,k_bits,v_bits", [(64, 4, 8), (128, 4, 4), (128, 8, 2), (256, 4, 8), (256, 2, 2), (96, 8, 4),
+                                             (40, 4, 4), (200, 8, 8), (131, 4, 2), (7, 8, 8), (1, 2, 4)])
+def test_append_many_rows(gpu, d, k_bits, v_bits, dtype):
+    """Calls of many rows (more than 16 a multiprocessor) take another kernel than those of few."""
+    (kq, kc), (vq, vc) = codec(d, k_bits), codec(d, v_bits, 43)
+    n, heads = 1201, 5
+    cache = KVCache(kq, vq, heads=heads, pages=1500 // 16, page_size=16)
+    gen = torch.Generator(device="cuda").manual_seed(d)
+    k, v = (torch.randn(2, n, heads, d, generator=gen, device="cuda") * 3).to(TYPES[dtype])
+    k[5], v[17, 2] = 0, 0
+    slots = torch.randperm(1500 // 16 * 16, generator=gen, device="cuda")[:n]
+    before = [t.clone() for t in (cache.k_rows, cache.v_rows)]
+    cache.append(k, v, slots, torch.arange(n, dtype=torch.int32, device="cuda"))
+    check_rows(cache, (kc, vc), k, v, slots)
+    assert torch.equal(cache.positions[slots // 16, :, slots % 16], torch.arange(n, dtype=torch.int32, device="cuda")[:, None].expand(n, heads))
+    # rows of no token are as they were, and what is behind a row's codes is 0
+    rest = torch.ones(cache.pages * 16, dtype=torch.bool, device="cuda")
+    rest[slots] = False
+    for t, b, bits in ((cache.k_rows, before[0], k_bits), (cache.v_rows, before[1], v_bits)):
+        t, b = (x.transpose(1, 2).reshape(cache.pages * 16, heads, -1) for x in (t, b))
+        assert torch.equal(t[rest], b[rest])
+        used, odd = d * bits // 8, d * bits % 8
+        assert not t[..., used + (odd > 0):].any()
+        assert not odd or not (t[..., used] & (255 >> odd)).any()
+
+
+def test_append_many_rows_strided_and_padded(gpu):
+    (kq, kc), (vq, vc) = codec(64, 4), codec(64, 4, 43)
+    cache = KVCache(kq, vq, heads=4, pages=100, page_size=16)
+    wide = torch.randn(1000, 9, 150, device="cuda").bfloat16()
+    for k, v in ((wide[:, 1:5, 3:67], wide[:, 5:9, 80:144]), (wide[:, :4, 64:128], wide[:, ::2, :64][:, :4])):
+        slots = torch.randperm(1600, device="cuda")[:1000]
+        slots[::7] = -1
+        slots[3::7] = 1600
+        cache.append(k, v, slots, torch.zeros(1000, dtype=torch.int32, device="cuda"))
+        ok = (slots >= 0) & (slots < 1600)
+        check_rows(cache, (kc, vc), k[ok], v[ok], slots[ok])
+
+
+def test_append_of_zero_vectors_and_boundary_values(gpu):
+    """Vectors all of whose coordinates are next to boundaries: more than a block lists."""
+    d = 64
+    q, c = codec(d, 4)
+    R = c[0].astype(np.float64)
+    heads, n = 8, 2000
+    cache = KVCache(q, heads=heads, pages=n // 16 + 1, page_size=16)
+    rng = np.random.default_rng(0)
+    # unit vectors whose rotated coordinates are boundaries, up to the last, which makes the length 1
+    edges = np.sort(np.abs(c[1][c[1] != 0]))
+    y = rng.choice(edges[: len(edges) // 2], (n * heads, d)) * rng.choice([-1, 1], (n * heads, d))
+    y[:, -1] = 0
+    scale = 0.999 / np.maximum(np.linalg.norm(y, axis=1, keepdims=True), 0.999)
+    y *= scale
+    y[:, -1] = np.sqrt(np.maximum(0, 1 - (y ** 2).sum(1)))
+    k = torch.tensor((y @ R).reshape(n, heads, d)).float().cuda()
+    v = torch.zeros_like(k)
+    slots = torch.arange(n, device="cuda")
+    cache.append(k, v, slots, torch.zeros(n, dtype=torch.int32, device="cuda"))
+    check_rows(cache, (c, c), k, v, slots)
+
+
+def test_append_in_several_launches(gpu):
+    """More rows than one launch of the append of many rows takes."""
+    q, c = codec(64, 8)
+    n, heads = 60000, 8
+    cache = KVCache(q, heads=heads, pages=n // 64 + 1, page_size=64)
+    k, v = torch.randn(2, n, heads, 64, device="cuda").half()
+    slots = torch.arange(n, device="cuda")
+    cache.append(k, v, slots, torch.zeros(n, dtype=torch.int32, device="cuda"))
+    check_rows(cache, (c, c), k, v, slots)
+
+
+def test_codec_of_odd_tables(gpu):
+    """Boundaries that coincide, or lie closer than the kernels' tables resolve."""
+    d = 64
+    R = codec(d, 4)[1][0]
+    for edges in (np.zeros(15), np.repeat([-0.1, 0.0, 0.1], 5), np.linspace(-1e-4, 1e-4, 15),
+                  np.r_[-1e30, np.linspace(-0.2, 0.2, 13), 1e30], np.r_[np.full(14, -0.0), 0.05]):
+        c = (R, edges.astype(np.float32), np.linspace(-1, 1, 16).astype(np.float32))
+        cache = KVCache(KVCodec(*c), heads=4, pages=100, page_size=16)
+        for n in (3, 1500):
+            k, v = torch.randn(2, n, 4, d, device="cuda")
+            k[0] = 0
+            slots = torch.arange(n, device="cuda")
+            cache.append(k, v, slots, torch.zeros(n, dtype=torch.int32, device="cuda"))
+            check_rows(cache, (c, c), k, v, slots)
+
+
 @pytest.mark.parametrize("dtype", ["f32", "f16", "bf16"])
 def test_read_types(gpu, dtype):
     c = Case(80, 4, 8, lengths=(20,))

@@ -150,8 +150,8 @@ struct Deal {
   }
 };
 
-// Sixteen rows lie in shared memory as in the pool, except that in rows of full
-// size the 16-byte pieces are exchanged so that a warp's loads meet no bank
+// Sixteen rows lie in shared memory one after another, each with the room of D
+// coordinates, their 16-byte pieces exchanged so that a warp's loads meet no bank
 // twice: keys are read by 8 rows x 4 pieces, values by 4 rows (2t and 2t + 1
 // alternating) x 8 lanes.  Where piece n of the sixteen rows lies:
 template <int ROW>
@@ -480,35 +480,49 @@ kv_attend_kernel(Side sk, Side sv, int pages, int page_shift, Work wk, QueryOut 
   const uint32_t vbase = kbase + kTableBytes;
 
   // A stage: MT times sixteen rows of keys, of values, sixteen norms of either.
+  constexpr int values_at = 16 * KD::row, norms_at = 16 * (KD::row + VD::row);
+  constexpr int group = norms_at + 128;
   const uint32_t kld = (uint32_t)sk.ldb, vld = (uint32_t)sv.ldb;
-  const bool kfull = kld == KD::row, vfull = vld == VD::row;
-  const uint32_t group_bytes = 16 * (kld + vld + 8);
   const uint32_t stage0 = (uint32_t)__cvta_generic_to_shared(smem) + Shape::table_bytes +
                           warp * 2 * Shape::stage;
   // Row r of the scores (lane: r = g and g + 8) is token r ^ (r >> 1 & 1), so that
   // the tokens of lane (g, t)'s value operands, those of rows 2t, 2t + 1 (+ 8),
   // alternate between even and odd rows of shared memory over t.
   const int tok_k = g ^ (g >> 1 & 1), tok_v = 2 * t + (t & 1);
-  // The lane's places in a group's rows.  A row shorter than D coordinates ends
-  // before some lanes' places: these read its start, as codes of coordinates
-  // that meet zeros in the queries and are dropped from the values.
+  // The lane's places in a group.  (Where a row is shorter than D coordinates,
+  // what lies behind it meets zeros in the queries and is dropped from the
+  // values; any bytes decode to finite centroids.)
   uint32_t kat[KD::units], vat[2][VD::units];
 #pragma unroll
   for (int u = 0; u < KD::units; ++u) {
-    const int off = (u * 4 + t) * KD::UB;
-    kat[u] = tok_k * kld + (off < (int)kld ? off : 0);
-    if (kfull) kat[u] = key_piece<KD::row>(kat[u] / 16) * 16 + kat[u] % 16;
+    const int at = tok_k * KD::row + (u * 4 + t) * KD::UB;
+    kat[u] = key_piece<KD::row>(at / 16) * 16 + at % 16;
   }
 #pragma unroll
   for (int e = 0; e < 2; ++e)
 #pragma unroll
     for (int u = 0; u < VD::units; ++u) {
-      const int off = (u * 8 + g) * VD::UB;
-      uint32_t at = (tok_v ^ e) * vld + (off < (int)vld ? off : 0);
-      if (vfull) at = value_piece<VD::row>(at / 16) * 16 + at % 16;
-      vat[e][u] = 16 * kld + at;
+      const int at = (tok_v ^ e) * VD::row + (u * 8 + g) * VD::UB;
+      vat[e][u] = values_at + value_piece<VD::row>(at / 16) * 16 + at % 16;
     }
-  const uint32_t norm_at = 16 * (kld + vld) + 4 * tok_k;
+  const uint32_t norm_at = norms_at + 4 * tok_k;
+  // Copies: the lane's pieces of a group (piece n of the pool's sixteen rows is
+  // piece n % (ld / 16) of row n / (ld / 16)), and where they come from.
+  constexpr int KJ = (KD::row + 31) / 32, VJ = (VD::row + 31) / 32;
+  uint32_t kto[KJ], vto[VJ];
+#pragma unroll
+  for (int j = 0; j < KJ; ++j) {
+    const int n = lane + 32 * j, per_row = kld / 16;
+    kto[j] = 16 * key_piece<KD::row>(n / per_row * (KD::row / 16) + n % per_row);
+  }
+#pragma unroll
+  for (int j = 0; j < VJ; ++j) {
+    const int n = lane + 32 * j, per_row = vld / 16;
+    vto[j] = values_at + 16 * value_piece<VD::row>(n / per_row * (VD::row / 16) + n % per_row);
+  }
+  const uint8_t *kfrom = sk.rows + lane * 16, *vfrom = sv.rows + lane * 16;
+  const float* nfrom = (lane & 4 ? sv.norms : sk.norms) + (lane & 3) * 4;
+  const uint32_t nto = norms_at + 16 * lane;
   pdl_wait();
 
   const int per = wk.heads * wk.blocks;
@@ -524,13 +538,14 @@ kv_attend_kernel(Side sk, Side sv, int pages, int page_shift, Work wk, QueryOut 
   constexpr int stride = Shape::unit;
   struct Segment {
     int b, seg, hb, h, t0, t1, base;  // tokens [t0, t1), the warp's next step's first
+    const int32_t* pages;             // its row of the table
     int pid[MT];                      // and the pages of its groups; -1 for none
   } cur, nxt;
   auto page_of = [&](const Segment& x, int base, int i) {
     const int tok = base + 16 * i;
     int p = -1;
     if (tok < x.t1) {
-      p = __ldg(wk.table + x.b * wk.table_stride + (tok >> page_shift));
+      p = __ldg(x.pages + (tok >> page_shift));
       if (p >= pages) p = -1;
     }
     return p;
@@ -550,6 +565,7 @@ kv_attend_kernel(Side sk, Side sv, int pages, int page_shift, Work wk, QueryOut 
       x.h = in / wk.blocks;
       x.hb = in % wk.blocks;
       x.seg = x.b * per + in;
+      x.pages = wk.table + x.b * wk.table_stride;
       x.t0 = (u0 - 1) * stride;
       x.t1 = min(len, (u1 - 1) * stride);
       x.base = x.t0 + warp * 16 * MT;
@@ -566,23 +582,15 @@ kv_attend_kernel(Side sk, Side sv, int pages, int page_shift, Work wk, QueryOut 
     for (int i = 0; i < MT; ++i) {
       const uint32_t row = ((uint32_t)(max(x.pid[i], 0) * wk.heads + x.h) << page_shift) +
                            (uint32_t)((x.base + 16 * i) & ((1 << page_shift) - 1));
-      const uint8_t* kp = sk.rows + (uint64_t)row * kld + lane * 16;
-      const uint8_t* vp = sv.rows + (uint64_t)row * vld + lane * 16;
-      const uint32_t to = stage + i * group_bytes;
+      const uint8_t* kp = kfrom + (uint64_t)row * kld;
+      const uint8_t* vp = vfrom + (uint64_t)row * vld;
 #pragma unroll
-      for (int j = 0; j < (KD::row + 31) / 32; ++j) {
-        const int piece = lane + 32 * j;
-        if (piece < (int)kld)
-          copy16(to + 16 * (kfull ? key_piece<KD::row>(piece) : piece), kp + 512 * j);
-      }
+      for (int j = 0; j < KJ; ++j)
+        if (lane + 32 * j < (int)kld) copy16(stage + i * group + kto[j], kp + 512 * j);
 #pragma unroll
-      for (int j = 0; j < (VD::row + 31) / 32; ++j) {
-        const int piece = lane + 32 * j;
-        if (piece < (int)vld)
-          copy16(to + 16 * (kld + (vfull ? value_piece<VD::row>(piece) : piece)), vp + 512 * j);
-      }
-      if (lane < 8)
-        copy16(to + 16 * (kld + vld + lane), (lane & 4 ? sv.norms : sk.norms) + row + (lane & 3) * 4);
+      for (int j = 0; j < VJ; ++j)
+        if (lane + 32 * j < (int)vld) copy16(stage + i * group + vto[j], vp + 512 * j);
+      if (lane < 8) copy16(stage + i * group + nto, nfrom + row);
     }
     copy_commit();
   };
@@ -660,7 +668,7 @@ kv_attend_kernel(Side sk, Side sv, int pages, int page_shift, Work wk, QueryOut 
         for (int e = 0; e < 2; ++e)
 #pragma unroll
           for (int un = 0; un < KD::units; ++un)
-            shared_bytes<KD::UB>(st + i * group_bytes + e * 8 * kld + kat[un],
+            shared_bytes<KD::UB>(st + kat[un] + (i * group + e * 8 * KD::row),
                                  &kw[e][un * KD::UB / 4]);
         s[i][0] = s[i][1] = s[i][2] = s[i][3] = 0.f;
 #pragma unroll
@@ -678,7 +686,7 @@ kv_attend_kernel(Side sk, Side sv, int pages, int page_shift, Work wk, QueryOut 
       for (int i = 0; i < MT; ++i)
 #pragma unroll
         for (int e = 0; e < 2; ++e) {
-          const uint32_t at = st + i * group_bytes + norm_at + 32 * e;
+          const uint32_t at = st + norm_at + (i * group + 32 * e);
           const float kn = shared_float(at);
           vn[i][e] = shared_float(at + 64);
           s[i][2 * e] *= kn * f0;
@@ -770,7 +778,7 @@ kv_attend_kernel(Side sk, Side sv, int pages, int page_shift, Work wk, QueryOut 
         for (int e = 0; e < 4; ++e)
 #pragma unroll
           for (int un = 0; un < VD::units; ++un)
-            shared_bytes<VD::UB>(st + i * group_bytes + (e >> 1) * 8 * vld + vat[e & 1][un],
+            shared_bytes<VD::UB>(st + vat[e & 1][un] + (i * group + (e >> 1) * 8 * VD::row),
                                  &vw[e][un * VD::UB / 4]);
 #pragma unroll
         for (int m = 0; m < KS; ++m) {

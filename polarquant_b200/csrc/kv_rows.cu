@@ -263,7 +263,7 @@ struct Coder {
 
 // A word of codes of 0.
 template <int BITS>
-__device__ __forceinline__ uint32_t zero_codes(const float* s_bounds) {
+__device__ __noinline__ uint32_t zero_codes(const float* s_bounds) {
   uint32_t code = 0;
 #pragma unroll
   for (int step = 1 << (BITS - 1); step > 0; step >>= 1)
@@ -853,8 +853,9 @@ __device__ __forceinline__ void append_many(const AppendArgs& a, uint8_t* smem, 
         }
         if (norm == 0.f) {  // all coordinates 0, which may be next to a boundary
           near = 0u;
+          const uint32_t word = zero_codes<BITS>(s_bounds);
 #pragma unroll
-          for (int w = 0; w < BITS; ++w) packed[w] = zero_codes<BITS>(s_bounds);
+          for (int w = 0; w < BITS; ++w) packed[w] = word;
         }
         if (left < 32) {
           near &= (1u << left) - 1u;

@@ -419,7 +419,7 @@ struct AttendShape {
     const int part = kHeadsPer * ostride * 4;
     return step > part ? step : part;
   }
-  static constexpr int room = 227 * 1024 - 2048 - table_bytes;
+  static constexpr int room = 227 * 1024 - 3072 - table_bytes;
   static constexpr int fit(int mt) { return room / (2 * stage_of(mt)) / 2 * 2; }
   // Registers allow 16 warps up to D = 128, fewer where operands come hi + lo
   // or the output is wider.
@@ -529,59 +529,67 @@ kv_attend_kernel(Side sk, Side sv, int pages, int page_shift, Work wk, QueryOut 
   const int total = wk.first[wk.batch];
   const int n = min((int)gridDim.x, total);
   if ((int)blockIdx.x >= n) return;
-  int64_t u = (int64_t)blockIdx.x * total / n;
-  const int64_t uend = ((int64_t)blockIdx.x + 1) * total / n;
+  int u = (int)((int64_t)blockIdx.x * total / n);
+  const int uend = (int)(((int64_t)blockIdx.x + 1) * total / n);
   for (int i = tid; i < wk.batch; i += Shape::threads)
     if (wk.first[i] <= u && u < wk.first[i + 1]) s_b = i;
   __syncthreads();
 
   constexpr int stride = Shape::unit;
+  // A segment and the block's share of it, tokens [t0, t1).  Those of a warp's
+  // segment and its next one wait in shared memory: the loop has no registers to
+  // spare for them.
   struct Segment {
-    int b, seg, hb, h, t0, t1, base;  // tokens [t0, t1), the warp's next step's first
-    const int32_t* pages;             // its row of the table
-    int pid[MT];                      // and the pages of its groups; -1 for none
-  } cur, nxt;
-  auto page_of = [&](const Segment& x, int base, int i) {
+    int b, seg, hb, h, t0, t1;
+    int pid[MT];  // pages of the warp's first step's groups; -1 for none
+  };
+  __shared__ Segment s_segment[2][NW];
+  auto page_of = [&](const int32_t* row, int t1, int base, int i) {
     const int tok = base + 16 * i;
     int p = -1;
-    if (tok < x.t1) {
-      p = __ldg(x.pages + (tok >> page_shift));
+    if (tok < t1) {
+      p = __ldg(row + (tok >> page_shift));
       if (p >= pages) p = -1;
     }
     return p;
   };
-  // The segment of unit u and this block's share of it; u moves behind it.
-  auto take = [&](Segment& x, int b) {
-    x.t0 = x.t1 = x.base = 0;
+  // The segment of unit u, from sequence b on; u moves behind it.
+  auto take = [&](int which, int b) {
+    Segment x;
+    x.t0 = x.t1 = 0;
     x.b = b;
+    x.seg = x.hb = x.h = 0;
+#pragma unroll
+    for (int i = 0; i < MT; ++i) x.pid[i] = -1;
     while (u < uend) {
       while (u >= wk.first[x.b + 1]) ++x.b;
       const int len = clamp_length(wk.lengths[x.b], wk.table_width, 1 << page_shift);
       const int nu = wk.units_of(len);
-      const int r = (int)(u - wk.first[x.b]), in = r / nu, u0 = max(r % nu, 1);
-      const int u1 = (int)min((int64_t)nu, r % nu + (uend - u));
-      u += u1 - r % nu;
+      const int r = u - wk.first[x.b], in = r / nu, from = r % nu, u0 = max(from, 1);
+      const int u1 = min(nu, from + (uend - u));
+      u += u1 - from;
       if (u1 <= u0) continue;  // the empty unit alone, at the end of the run
       x.h = in / wk.blocks;
       x.hb = in % wk.blocks;
       x.seg = x.b * per + in;
-      x.pages = wk.table + x.b * wk.table_stride;
       x.t0 = (u0 - 1) * stride;
       x.t1 = min(len, (u1 - 1) * stride);
-      x.base = x.t0 + warp * 16 * MT;
 #pragma unroll
-      for (int i = 0; i < MT; ++i) x.pid[i] = page_of(x, x.base, i);
-      return;
+      for (int i = 0; i < MT; ++i)
+        x.pid[i] = page_of(wk.table + x.b * wk.table_stride, x.t1, x.t0 + warp * 16 * MT, i);
+      break;
     }
+    if (lane == 0) s_segment[which][warp] = x;
+    __syncwarp();
   };
-  // Copies the step at x.base to a stage.  Groups without a page read page 0:
+  // Copies the step at `base`, its groups on pages pid, to a stage.  Groups without a page read page 0:
   // what tokens that are not there decode to is finite, and meets a weight of 0.
   // (A pool has fewer than 2^32 rows.)
-  auto fetch = [&](const Segment& x, uint32_t stage) {
+  auto fetch = [&](const int (&pid)[MT], int h, int base, uint32_t stage) {
 #pragma unroll
     for (int i = 0; i < MT; ++i) {
-      const uint32_t row = ((uint32_t)(max(x.pid[i], 0) * wk.heads + x.h) << page_shift) +
-                           (uint32_t)((x.base + 16 * i) & ((1 << page_shift) - 1));
+      const uint32_t row = ((uint32_t)(max(pid[i], 0) * wk.heads + h) << page_shift) +
+                           (uint32_t)((base + 16 * i) & ((1 << page_shift) - 1));
       const uint8_t* kp = kfrom + (uint64_t)row * kld;
       const uint8_t* vp = vfrom + (uint64_t)row * vld;
 #pragma unroll
@@ -595,18 +603,32 @@ kv_attend_kernel(Side sk, Side sv, int pages, int page_shift, Work wk, QueryOut 
     copy_commit();
   };
 
-  take(cur, s_b);
+  take(0, s_b);
   int p = 0;  // stage of the step to come
-  if (cur.base < cur.t1) fetch(cur, stage0);
-  while (cur.t0 < cur.t1) {
-    take(nxt, cur.b);
-    const int t1 = cur.t1, hb = cur.hb;
+  {
+    const Segment& x = s_segment[0][warp];
+    if (x.t0 + warp * 16 * MT < x.t1) fetch(x.pid, x.h, x.t0 + warp * 16 * MT, stage0);
+  }
+#pragma unroll 1
+  for (int which = 0;; which ^= 1) {
+    const Segment& seg = s_segment[which][warp];
+    const int t1 = seg.t1, h = seg.h;
+    if (seg.t0 >= t1) break;
+    take(which ^ 1, seg.b);
+    const int32_t* prow = wk.table + seg.b * wk.table_stride;
+    int base = seg.t0 + warp * 16 * MT;
+    int pid[MT], pid1[MT];  // pages of the step to come and of the one after it
+#pragma unroll
+    for (int i = 0; i < MT; ++i) {
+      pid[i] = seg.pid[i];
+      pid1[i] = page_of(prow, t1, base + stride, i);
+    }
 
     // The queries as B operands: lane (g, t) holds head g.
     uint32_t qh[KS][2], ql[QLO ? KS : 1][2];
     {
-      const __half* hi = qo.hi + ((int64_t)cur.seg * kHeadsPer + g) * D;
-      const __half* lo = qo.lo + ((int64_t)cur.seg * kHeadsPer + g) * D;
+      const __half* hi = qo.hi + ((int64_t)seg.seg * kHeadsPer + g) * D;
+      const __half* lo = qo.lo + ((int64_t)seg.seg * kHeadsPer + g) * D;
 #pragma unroll
       for (int s = 0; s < KS; ++s) {
         const int dim = KD::dim(t, 4 * s);
@@ -624,35 +646,31 @@ kv_attend_kernel(Side sk, Side sv, int pages, int page_shift, Work wk, QueryOut 
         }
       }
     }
-    const float f0 = qo.factor[(int64_t)cur.seg * kHeadsPer + 2 * t];
-    const float f1 = qo.factor[(int64_t)cur.seg * kHeadsPer + 2 * t + 1];
+    const float f0 = qo.factor[(int64_t)seg.seg * kHeadsPer + 2 * t];
+    const float f1 = qo.factor[(int64_t)seg.seg * kHeadsPer + 2 * t + 1];
 
     float o[KS][4];
 #pragma unroll
     for (int m = 0; m < KS; ++m) o[m][0] = o[m][1] = o[m][2] = o[m][3] = 0.f;
     float m0 = -FLT_MAX, m1 = -FLT_MAX, l0 = 0.f, l1 = 0.f;
     float vinv = 0.f, vlim = 0.f, vref = 0.f;  // value norms are taken times vinv = 2^10 / vref
-    int pid1[MT];  // pages of the step after the one to come
-#pragma unroll
-    for (int i = 0; i < MT; ++i) pid1[i] = page_of(cur, cur.base + stride, i);
 
-    while (cur.base < t1) {
-      const int base = cur.base;
+#pragma unroll 1
+    for (; base < t1; base += stride) {
       const uint32_t st = stage0 + p * Shape::stage;
       bool there = base + 16 * MT <= t1;
       uint32_t gone = 0;  // groups without a page
 #pragma unroll
       for (int i = 0; i < MT; ++i) {
-        if (cur.pid[i] < 0) gone |= 1u << i;
-        cur.pid[i] = pid1[i];
+        if (pid[i] < 0) gone |= 1u << i;
+        pid[i] = pid1[i];
       }
       there = there && gone == 0;
-      cur.base += stride;
       p ^= 1;
-      if (cur.base < t1) {
-        fetch(cur, stage0 + p * Shape::stage);
+      if (base + stride < t1) {
+        fetch(pid, h, base + stride, stage0 + p * Shape::stage);
 #pragma unroll
-        for (int i = 0; i < MT; ++i) pid1[i] = page_of(cur, cur.base + stride, i);
+        for (int i = 0; i < MT; ++i) pid1[i] = page_of(prow, t1, base + 2 * stride, i);
         copy_wait<1>();
       } else {
         copy_wait<0>();
@@ -711,10 +729,10 @@ kv_attend_kernel(Side sk, Side sv, int pages, int page_shift, Work wk, QueryOut 
             const int tok = base + 16 * i + tok_k + 8 * e;
             if (tok < t1) {
               float* to = scores +
-                          (((int64_t)cur.b * wk.heads + cur.h) * score_width + tok) * wk.group +
-                          hb * kHeadsPer + 2 * t;
-              if (hb * kHeadsPer + 2 * t < wk.group) to[0] = x;
-              if (hb * kHeadsPer + 2 * t + 1 < wk.group) to[1] = y;
+                          (((int64_t)seg.b * wk.heads + h) * score_width + tok) * wk.group +
+                          seg.hb * kHeadsPer + 2 * t;
+              if (seg.hb * kHeadsPer + 2 * t < wk.group) to[0] = x;
+              if (seg.hb * kHeadsPer + 2 * t + 1 < wk.group) to[1] = y;
             }
           }
           mx0 = fmaxf(mx0, x);
@@ -795,7 +813,11 @@ kv_attend_kernel(Side sk, Side sv, int pages, int page_shift, Work wk, QueryOut 
 
     // The next segment's first step comes while this one's partial results are
     // joined, warps in order, by way of each warp's other stage.
-    if (nxt.base < nxt.t1) fetch(nxt, stage0 + p * Shape::stage);
+    {
+      const Segment& x = s_segment[which ^ 1][warp];
+      if (x.t0 + warp * 16 * MT < x.t1)
+        fetch(x.pid, x.h, x.t0 + warp * 16 * MT, stage0 + p * Shape::stage);
+    }
 #pragma unroll
     for (int w = 4; w < 32; w <<= 1) {
       l0 += __shfl_xor_sync(0xffffffffu, l0, w);
@@ -807,7 +829,7 @@ kv_attend_kernel(Side sk, Side sv, int pages, int page_shift, Work wk, QueryOut 
       s_l[warp][2 * t] = l0;
       s_l[warp][2 * t + 1] = l1;
     }
-    const int active = min(NW, (t1 - cur.t0 + 16 * MT - 1) / (16 * MT));
+    const int active = min(NW, (t1 - seg.t0 + 16 * MT - 1) / (16 * MT));
     uint8_t* own = smem + Shape::table_bytes + (warp * 2 + (p ^ 1)) * Shape::stage;
     if (lane == 0) s_v[warp] = vref;
     __shared__ const float* s_part[NW];
@@ -822,8 +844,8 @@ kv_attend_kernel(Side sk, Side sv, int pages, int page_shift, Work wk, QueryOut 
       }
     }
     __syncthreads();
-    const int64_t slot = (int64_t)blockIdx.x + cur.seg;
-    const int ng = min(kHeadsPer, wk.group - hb * kHeadsPer);
+    const int64_t slot = (int64_t)blockIdx.x + seg.seg;
+    const int ng = min(kHeadsPer, wk.group - seg.hb * kHeadsPer);
     for (int i = tid; i < ng * D; i += Shape::threads) {
       const int hd = i / D, j = i % D;
       float mm = -FLT_MAX;
@@ -838,7 +860,6 @@ kv_attend_kernel(Side sk, Side sv, int pages, int page_shift, Work wk, QueryOut 
       if (j == 0) parts.ml[slot * kHeadsPer + hd] = make_float2(mm, l);
     }
     __syncthreads();
-    cur = nxt;
   }
 }
 

@@ -16,10 +16,10 @@ struct Codec {
   const float* RT;        // its transpose
   const float* bounds;    // 2^bits - 1, then infinity
   const float* cent;      // 2^bits
-  const uint32_t* pairs;  // [2][256] centroids * 2^exponent for decoding in f16
-                          // 4 bits: both of a byte's, hi parts; then lo parts
-                          // 8 bits: hi and lo part of the byte's
-                          // 2 bits: bytes 0 and 1 of the four hi parts, of the lo parts
+  const uint2* pairs;     // [2][256] centroids * 2^exponent as f16, what a byte decodes to
+                          // 4 bits: its two, twice; hi parts, then lo parts
+                          // 2 bits: its first two and last two; hi, then lo
+                          // 8 bits: hi and lo part, twice; then nothing
   const int* exponent;    // the largest centroid * 2^exponent lies in [2^13, 2^14)
   const float* range;     // cell of y = saturate(y * range[0] + range[1]) * (cells - 1), rounded
   const uint2* cells;     // [2048]: the cell's boundary (f32) and the code below it
@@ -34,7 +34,7 @@ inline int padded_d(int d) { return d <= 64 ? 64 : d <= 128 ? 128 : 256; }
 
 inline size_t codec_bytes(int d, int /*bits*/) {
   const size_t D = padded_d(d);
-  return (size_t)2 * align_up((size_t)d * d * sizeof(float), 256) + 4 * 1024 + 256 +
+  return (size_t)2 * align_up((size_t)d * d * sizeof(float), 256) + 6 * 1024 + 256 +
          kCells * sizeof(uint2) + 2 * 2 * D * D * sizeof(__half);
 }
 
@@ -47,10 +47,10 @@ inline Codec codec_of(const void* tables, int d) {
   b += 2 * m;
   c.bounds = (const float*)b;
   c.cent = (const float*)(b + 1024);
-  c.pairs = (const uint32_t*)(b + 2048);
-  c.exponent = (const int*)(b + 4096);
-  c.range = (const float*)(b + 4096 + 64);
-  c.cells = (const uint2*)(b + 4096 + 256);
+  c.pairs = (const uint2*)(b + 2048);
+  c.exponent = (const int*)(b + 6144);
+  c.range = (const float*)(b + 6144 + 64);
+  c.cells = (const uint2*)(b + 6144 + 256);
   c.planes = c.cells + kCells;
   const int D = padded_d(d);
   c.rows = (const __half*)(c.planes + D * D / 2);

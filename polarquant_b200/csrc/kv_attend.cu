@@ -28,9 +28,9 @@
 // coordinates of its own operand registers, because the order of coordinates
 // is free as long as the queries have the same one.  A packed byte is decoded
 // by one shared-memory lookup that gives both of its centroids as an f16 pair
-// (4 bits; at 8 bits one centroid as f16 hi + lo), from a table with a copy for
-// each lane: no bank conflicts, and the address is one dp4a.  2 bits are
-// decoded by byte permutes on a table of four in registers.
+// (4 bits; at 8 bits one centroid as f16 hi + lo, at 2 bits four centroids as two
+// pairs), from a table with a copy for each lane (at 2 bits each lane of half a
+// warp): no bank conflicts, and the address is one dp4a.
 //
 // What bounds it: at 4 bits and d = 128 a token and head is 136 bytes, 128
 // lookups of the 32 a cycle that an SM's shared memory gives, 160 byte
@@ -166,10 +166,16 @@ __device__ __forceinline__ int value_piece(int n) {
 }
 
 // Decoding.  A side's table has 256 entries of 128 bytes, a copy of the entry's
-// word for every lane; keys' first, values' behind them, then (4 bits, hi + lo)
-// both lo tables.  `base` is the lane's place in entry 0 as a shared-memory
-// address; one dp4a adds 128 times a byte of the packed word to it.
+// word for every lane (2 bits: of its two words for every lane of half a warp);
+// keys' first, values' behind them, then (2 and 4 bits, hi + lo) both lo tables.
+// `base` is the lane's place in entry 0 as a shared-memory address; one dp4a adds
+// 128 times a byte of the packed word to it.
 constexpr uint32_t kTableBytes = 32768;
+
+template <int BITS>
+__device__ __forceinline__ uint32_t lane_place(int lane) {
+  return BITS == 2 ? (lane & 15) * 8 : lane * 4;
+}
 
 template <int LO>
 __device__ __forceinline__ uint32_t lookup(uint32_t base, uint32_t w, int byte) {
@@ -179,12 +185,20 @@ __device__ __forceinline__ uint32_t lookup(uint32_t base, uint32_t w, int byte) 
   return x;
 }
 
+template <int LO>
+__device__ __forceinline__ uint2 lookup2(uint32_t base, uint32_t w, int byte) {
+  const uint32_t at = __dp4a(w, 128u << (8 * byte), base);
+  uint2 x;
+  asm("ld.shared.v2.b32 {%0,%1}, [%2+%3];"
+      : "=r"(x.x), "=r"(x.y)
+      : "r"(at), "n"(LO * 2 * (int)kTableBytes));
+  return x;
+}
+
 // The four codes that a lane gives to one K step: pairs a (first operand
-// register) and b (third), hi and lo.  2 bits: the pairs are codes (2, 0) and
-// (3, 1) of the byte, else (0, 1) and (2, 3).
+// register) and b (third), hi and lo.
 template <int BITS, bool LO, int W>
 __device__ __forceinline__ void decode_key(const uint32_t (&w)[W], int s, uint32_t base,
-                                           const uint32_t (&reg)[4],
                                            uint32_t& ah, uint32_t& bh, uint32_t& al, uint32_t& bl) {
   if constexpr (BITS == 4) {
     const uint32_t x = w[s >> 1];
@@ -206,65 +220,62 @@ __device__ __forceinline__ void decode_key(const uint32_t (&w)[W], int s, uint32
       bl = __byte_perm(e2, e3, 0x7632);
     }
   } else {
-    const uint32_t x = w[s >> 2] >> (8 * (s & 3));
-    const uint32_t sel = (x & 0x33u) << 8 | ((x >> 2) & 0x33u);  // codes 2, 0, 3, 1
-    const uint32_t l = __byte_perm(reg[0], reg[1], sel);
-    const uint32_t h = __byte_perm(reg[0], reg[1], sel | 0x4444u);
-    ah = __byte_perm(l, h, 0x5140);
-    bh = __byte_perm(l, h, 0x7362);
+    const uint2 e = lookup2<0>(base, w[s >> 2], s & 3);
+    ah = e.x;
+    bh = e.y;
     if constexpr (LO) {
-      const uint32_t l2 = __byte_perm(reg[2], reg[3], sel);
-      const uint32_t h2 = __byte_perm(reg[2], reg[3], sel | 0x4444u);
-      al = __byte_perm(l2, h2, 0x5140);
-      bl = __byte_perm(l2, h2, 0x7362);
+      const uint2 f = lookup2<1>(base, w[s >> 2], s & 3);
+      al = f.x;
+      bl = f.y;
     }
   }
 }
 
-// Codes 2m and 2m + 1 of two tokens' rows: the pairs (x's, y's) of either code.
+// Codes 2m, 2m + 1 (and 2m + 2, 2m + 3) of two tokens' rows: of each code the pair
+// (x's, y's), even ones in `e`, odd ones in `o`.
 template <int BITS, bool LO, int W>
 __device__ __forceinline__ void decode_value(const uint32_t (&x)[W], const uint32_t (&y)[W], int m,
-                                             uint32_t base, const uint32_t (&reg)[4], uint32_t& eh, uint32_t& oh,
-                                             uint32_t& el, uint32_t& ol) {
+                                             uint32_t base, uint32_t (&eh)[2], uint32_t (&oh)[2],
+                                             uint32_t (&el)[2], uint32_t (&ol)[2]) {
   if constexpr (BITS == 4) {
-    const uint32_t p = lookup<0>(base, x[m >> 2], m & 3);
-    const uint32_t q = lookup<0>(base, y[m >> 2], m & 3);
-    eh = __byte_perm(p, q, 0x5410);
-    oh = __byte_perm(p, q, 0x7632);
-    if constexpr (LO) {
-      const uint32_t r = lookup<1>(base, x[m >> 2], m & 3);
-      const uint32_t t = lookup<1>(base, y[m >> 2], m & 3);
-      el = __byte_perm(r, t, 0x5410);
-      ol = __byte_perm(r, t, 0x7632);
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+      const int n = m + i;
+      const uint32_t p = lookup<0>(base, x[n >> 2], n & 3), q = lookup<0>(base, y[n >> 2], n & 3);
+      eh[i] = __byte_perm(p, q, 0x5410);
+      oh[i] = __byte_perm(p, q, 0x7632);
+      if constexpr (LO) {
+        const uint32_t r = lookup<1>(base, x[n >> 2], n & 3), t = lookup<1>(base, y[n >> 2], n & 3);
+        el[i] = __byte_perm(r, t, 0x5410);
+        ol[i] = __byte_perm(r, t, 0x7632);
+      }
     }
   } else if constexpr (BITS == 8) {
-    const int b = 2 * (m & 1);
-    const uint32_t p0 = lookup<0>(base, x[m >> 1], b);
-    const uint32_t p1 = lookup<0>(base, x[m >> 1], b + 1);
-    const uint32_t q0 = lookup<0>(base, y[m >> 1], b);
-    const uint32_t q1 = lookup<0>(base, y[m >> 1], b + 1);
-    eh = __byte_perm(p0, q0, 0x5410);
-    oh = __byte_perm(p1, q1, 0x5410);
-    if constexpr (LO) {
-      el = __byte_perm(p0, q0, 0x7632);
-      ol = __byte_perm(p1, q1, 0x7632);
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+      const int n = m + i, b = 2 * (n & 1);
+      const uint32_t p0 = lookup<0>(base, x[n >> 1], b), p1 = lookup<0>(base, x[n >> 1], b + 1);
+      const uint32_t q0 = lookup<0>(base, y[n >> 1], b), q1 = lookup<0>(base, y[n >> 1], b + 1);
+      eh[i] = __byte_perm(p0, q0, 0x5410);
+      oh[i] = __byte_perm(p1, q1, 0x5410);
+      if constexpr (LO) {
+        el[i] = __byte_perm(p0, q0, 0x7632);
+        ol[i] = __byte_perm(p1, q1, 0x7632);
+      }
     }
   } else {
-    // The byte of both tokens: codes 0, 1 (m even) or 2, 3 of it.
-    const uint32_t z = __byte_perm(x[m >> 3], y[m >> 3],
-                                   ((m >> 1) & 3) | (((m >> 1) & 3) + 4) << 4) & 0xffffu;
-    const uint32_t n = (m & 1) ? z : z >> 4;
-    // nibbles: odd code of x, even of x, odd of y, even of y
-    const uint32_t sel = (n & 0x0303u) | ((n & 0x0c0cu) << 2);
-    const uint32_t l = __byte_perm(reg[0], reg[1], sel);
-    const uint32_t h = __byte_perm(reg[0], reg[1], sel | 0x4444u);
-    oh = __byte_perm(l, h, 0x6240);
-    eh = __byte_perm(l, h, 0x7351);
+    const int n = m >> 1;  // byte of the row
+    const uint2 p = lookup2<0>(base, x[n >> 2], n & 3), q = lookup2<0>(base, y[n >> 2], n & 3);
+    eh[0] = __byte_perm(p.x, q.x, 0x5410);
+    oh[0] = __byte_perm(p.x, q.x, 0x7632);
+    eh[1] = __byte_perm(p.y, q.y, 0x5410);
+    oh[1] = __byte_perm(p.y, q.y, 0x7632);
     if constexpr (LO) {
-      const uint32_t l2 = __byte_perm(reg[2], reg[3], sel);
-      const uint32_t h2 = __byte_perm(reg[2], reg[3], sel | 0x4444u);
-      ol = __byte_perm(l2, h2, 0x6240);
-      el = __byte_perm(l2, h2, 0x7351);
+      const uint2 r = lookup2<1>(base, x[n >> 2], n & 3), t = lookup2<1>(base, y[n >> 2], n & 3);
+      el[0] = __byte_perm(r.x, t.x, 0x5410);
+      ol[0] = __byte_perm(r.x, t.x, 0x7632);
+      el[1] = __byte_perm(r.y, t.y, 0x5410);
+      ol[1] = __byte_perm(r.y, t.y, 0x7632);
     }
   }
 }
@@ -407,9 +418,9 @@ struct Parts {
 
 template <int D, int KB, int VB, int PREC>
 struct AttendShape {
-  static constexpr bool tables = KB != 2 || VB != 2;
-  static constexpr bool lo_tables = (PREC >= 2 && KB == 4) || (PREC == 3 && VB == 4);
-  static constexpr int table_bytes = tables ? (lo_tables ? 4 : 2) * (int)kTableBytes : 0;
+  // (8-bit entries hold both parts)
+  static constexpr bool lo_tables = (PREC >= 2 && KB != 8) || (PREC == 3 && VB != 8);
+  static constexpr int table_bytes = (lo_tables ? 4 : 2) * (int)kTableBytes;
   static constexpr int ostride = D + 8;  // of a partial result's head in shared memory
   // A warp has two stages, a step's rows and norms each; a stage also holds the
   // warp's partial result at a segment's end, while the next segment's first
@@ -453,31 +464,23 @@ kv_attend_kernel(Side sk, Side sv, int pages, int page_shift, Work wk, QueryOut 
 
   // Tables, from the codec's entries (set-up data: not written by the kernel
   // before).  A thread copies an entry to the 32 lanes' places.
-  if constexpr (Shape::tables) {
 #pragma unroll
-    for (int side = 0; side < 2; ++side) {
-      const Codec& c = side ? sv.c : sk.c;
-      if ((side ? VB : KB) == 2) continue;
+  for (int side = 0; side < 2; ++side) {
+    const Codec& c = side ? sv.c : sk.c;
 #pragma unroll
-      for (int part = 0; part < (Shape::lo_tables ? 2 : 1); ++part)
-        for (int n = tid; n < 256; n += Shape::threads) {
-          const uint32_t e = c.pairs[part * 256 + n];
-          const uint4 v = make_uint4(e, e, e, e);
+    for (int part = 0; part < (Shape::lo_tables ? 2 : 1); ++part)
+      for (int n = tid; n < 256; n += Shape::threads) {
+        const uint2 e = c.pairs[part * 256 + n];
+        const uint4 v = make_uint4(e.x, e.y, e.x, e.y);
 #pragma unroll
-          for (int i = 0; i < 8; ++i)
-            *reinterpret_cast<uint4*>(smem + (2 * part + side) * kTableBytes + n * 128 +
-                                      ((i + n) & 7) * 16) = v;
-        }
-    }
+        for (int i = 0; i < 8; ++i)
+          *reinterpret_cast<uint4*>(smem + (2 * part + side) * kTableBytes + n * 128 +
+                                    ((i + n) & 7) * 16) = v;
+      }
   }
-  uint32_t kreg[4], vreg[4];
-#pragma unroll
-  for (int i = 0; i < 4; ++i) {
-    kreg[i] = KB == 2 ? sk.c.pairs[i] : 0u;
-    vreg[i] = VB == 2 ? sv.c.pairs[i] : 0u;
-  }
-  const uint32_t kbase = (uint32_t)__cvta_generic_to_shared(smem) + lane * 4;
-  const uint32_t vbase = kbase + kTableBytes;
+  const uint32_t table0 = (uint32_t)__cvta_generic_to_shared(smem);
+  const uint32_t kbase = table0 + lane_place<KB>(lane);
+  const uint32_t vbase = table0 + kTableBytes + lane_place<VB>(lane);
 
   // A stage: MT times sixteen rows of keys, of values, sixteen norms of either.
   constexpr int values_at = 16 * KD::row, norms_at = 16 * (KD::row + VD::row);
@@ -633,14 +636,10 @@ kv_attend_kernel(Side sk, Side sv, int pages, int page_shift, Work wk, QueryOut 
       for (int s = 0; s < KS; ++s) {
         const int dim = KD::dim(t, 4 * s);
         uint2 x = *reinterpret_cast<const uint2*>(hi + dim);
-        if (KB == 2)
-          x = make_uint2(__byte_perm(x.x, x.y, 0x1054), __byte_perm(x.x, x.y, 0x3276));
         qh[s][0] = x.x;
         qh[s][1] = x.y;
         if constexpr (QLO) {
           x = *reinterpret_cast<const uint2*>(lo + dim);
-          if (KB == 2)
-            x = make_uint2(__byte_perm(x.x, x.y, 0x1054), __byte_perm(x.x, x.y, 0x3276));
           ql[s][0] = x.x;
           ql[s][1] = x.y;
         }
@@ -692,8 +691,8 @@ kv_attend_kernel(Side sk, Side sv, int pages, int page_shift, Work wk, QueryOut 
 #pragma unroll
         for (int k = 0; k < KS; ++k) {
           uint32_t a0, a1, a2, a3, c0 = 0, c1 = 0, c2 = 0, c3 = 0;
-          decode_key<KB, KLO>(kw[0], k, kbase, kreg, a0, a2, c0, c2);
-          decode_key<KB, KLO>(kw[1], k, kbase, kreg, a1, a3, c1, c3);
+          decode_key<KB, KLO>(kw[0], k, kbase, a0, a2, c0, c2);
+          decode_key<KB, KLO>(kw[1], k, kbase, a1, a3, c1, c3);
           mma16816(s[i], a0, a1, a2, a3, qh[k][0], qh[k][1]);
           if constexpr (QLO) mma16816(s[i], a0, a1, a2, a3, ql[k][0], ql[k][1]);
           if constexpr (KLO) mma16816(s[i], c0, c1, c2, c3, qh[k][0], qh[k][1]);
@@ -799,13 +798,16 @@ kv_attend_kernel(Side sk, Side sv, int pages, int page_shift, Work wk, QueryOut 
             shared_bytes<VD::UB>(st + vat[e & 1][un] + (i * group + (e >> 1) * 8 * VD::row),
                                  &vw[e][un * VD::UB / 4]);
 #pragma unroll
-        for (int m = 0; m < KS; ++m) {
-          uint32_t a0, a1, a2, a3, c0 = 0, c1 = 0, c2 = 0, c3 = 0;
-          decode_value<VB, VLO>(vw[0], vw[1], m, vbase, vreg, a0, a1, c0, c1);
-          decode_value<VB, VLO>(vw[2], vw[3], m, vbase, vreg, a2, a3, c2, c3);
-          mma16816(o[m], a0, a1, a2, a3, ph[i][0], ph[i][1]);
-          if constexpr (QLO) mma16816(o[m], a0, a1, a2, a3, pl[i][0], pl[i][1]);
-          if constexpr (VLO) mma16816(o[m], c0, c1, c2, c3, ph[i][0], ph[i][1]);
+        for (int m = 0; m < KS; m += 2) {
+          uint32_t a0[2], a1[2], a2[2], a3[2], c0[2], c1[2], c2[2], c3[2];
+          decode_value<VB, VLO>(vw[0], vw[1], m, vbase, a0, a1, c0, c1);
+          decode_value<VB, VLO>(vw[2], vw[3], m, vbase, a2, a3, c2, c3);
+#pragma unroll
+          for (int z = 0; z < 2; ++z) {
+            mma16816(o[m + z], a0[z], a1[z], a2[z], a3[z], ph[i][0], ph[i][1]);
+            if constexpr (QLO) mma16816(o[m + z], a0[z], a1[z], a2[z], a3[z], pl[i][0], pl[i][1]);
+            if constexpr (VLO) mma16816(o[m + z], c0[z], c1[z], c2[z], c3[z], ph[i][0], ph[i][1]);
+          }
         }
       }
       __syncwarp();

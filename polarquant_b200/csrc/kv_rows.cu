@@ -103,21 +103,20 @@ __global__ void prepare_codec_kernel(const float* __restrict__ R, const float* _
   s_half[threadIdx.x] = __half_as_ushort(hi) | (uint32_t)__half_as_ushort(lo) << 16;
   __syncthreads();
   const int i = threadIdx.x;
-  uint32_t p0, p1;
-  if (bits == 4) {
-    const uint32_t a = s_half[i >> 4], b = s_half[i & 15];
-    p0 = __byte_perm(a, b, 0x5410);
-    p1 = __byte_perm(a, b, 0x7632);
-  } else if (bits == 8) {
-    p0 = s_half[i];
-    p1 = 0u;
+  uint2 p0, p1;
+  if (bits == 8) {
+    p0 = make_uint2(s_half[i], s_half[i]);
+    p1 = make_uint2(0u, 0u);
   } else {
-    p0 = p1 = 0u;
-    if (i < 4)  // byte i of the four 32-bit hi | lo words
-      for (int k = 0; k < 4; ++k) p0 |= ((s_half[k] >> (8 * i)) & 255u) << (8 * k);
+    // The byte's codes: two at 4 bits, four at 2.
+    uint32_t c[4];
+    for (int k = 0; k < 4; ++k)
+      c[k] = s_half[bits == 4 ? (k & 1 ? i & 15 : i >> 4) : i >> (6 - 2 * k) & 3];
+    p0 = make_uint2(__byte_perm(c[0], c[1], 0x5410), __byte_perm(c[2], c[3], 0x5410));
+    p1 = make_uint2(__byte_perm(c[0], c[1], 0x7632), __byte_perm(c[2], c[3], 0x7632));
   }
-  const_cast<uint32_t*>(out.pairs)[i] = p0;
-  const_cast<uint32_t*>(out.pairs)[256 + i] = p1;
+  const_cast<uint2*>(out.pairs)[i] = p0;
+  const_cast<uint2*>(out.pairs)[256 + i] = p1;
   if (i == 0) *const_cast<int*>(out.exponent) = e;
 }
 

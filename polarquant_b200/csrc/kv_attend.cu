@@ -311,28 +311,56 @@ struct QueryOut {
   float* factor;    // [segment][8]: score = factor * key norm * product, in log2
 };
 
-// Turning rows by a D x D matrix: kRotParts threads a column share its
-// products, so that few blocks have many loads of the matrix in flight (64 KB
-// from L2 at D = 128; one row of loads after another took 16 us).
+// Turning rows by a D x D matrix: kRotParts threads a column share its products.
+// A thread's first elements of the matrix (64 KB from L2 at D = 128) are loaded
+// ahead, where the kernel still waits for the rows; x comes in 16-byte loads, as
+// one load for each product bounds the block by shared memory (D = 256: 11 us).
 constexpr int kRotParts = 4;
+constexpr int kRotAhead = 16;
 
-// acc[g] = sum over this thread's rows i of x[g][i] * M[i][j].
 template <int D>
-__device__ __forceinline__ void turn(const float (&x)[kHeadsPer][D], const float* __restrict__ M,
-                                     int d, int j, int part, float (&acc)[kHeadsPer]) {
+struct Turn {
+  float r[kRotAhead];
+  const float* m;
+  int d, j, i0;
+
+  __device__ __forceinline__ void ahead(const float* M, int d_, int j_, int part) {
+    m = M;
+    d = d_;
+    j = j_;
+    i0 = part * (D / kRotParts);
 #pragma unroll
-  for (int g = 0; g < kHeadsPer; ++g) acc[g] = 0.f;
-  constexpr int rows = D / kRotParts, chunk = rows < 32 ? rows : 32;
-  for (int i0 = part * rows; i0 < (part + 1) * rows; i0 += chunk) {
-    float r[chunk];
-#pragma unroll
-    for (int i = 0; i < chunk; ++i) r[i] = i0 + i < d && j < d ? __ldg(M + (i0 + i) * d + j) : 0.f;
-#pragma unroll
-    for (int i = 0; i < chunk; ++i)
-#pragma unroll
-      for (int g = 0; g < kHeadsPer; ++g) acc[g] = fmaf(x[g][i0 + i], r[i], acc[g]);
+    for (int i = 0; i < kRotAhead; ++i) r[i] = at(i0 + i);
   }
-}
+  __device__ __forceinline__ float at(int i) const {
+    return i < d && j < d ? __ldg(m + i * d + j) : 0.f;
+  }
+  // acc[g] = sum over this thread's rows i of x[g][i] * M[i][j].
+  __device__ __forceinline__ void run(const float (&x)[kHeadsPer][D], float (&acc)[kHeadsPer]) {
+#pragma unroll
+    for (int g = 0; g < kHeadsPer; ++g) acc[g] = 0.f;
+#pragma unroll 1
+    for (int i = i0; i < i0 + D / kRotParts; i += kRotAhead) {
+      float w[kRotAhead];
+#pragma unroll
+      for (int k = 0; k < kRotAhead; ++k) w[k] = r[k];
+      if (i + kRotAhead < i0 + D / kRotParts) {
+#pragma unroll
+        for (int k = 0; k < kRotAhead; ++k) r[k] = at(i + kRotAhead + k);
+      }
+#pragma unroll
+      for (int k = 0; k < kRotAhead; k += 4)
+#pragma unroll
+        for (int g = 0; g < kHeadsPer; ++g) {
+          const float4 v = *reinterpret_cast<const float4*>(&x[g][i + k]);
+          acc[g] = fmaf(v.x, w[k], acc[g]);
+          acc[g] = fmaf(v.y, w[k + 1], acc[g]);
+          acc[g] = fmaf(v.z, w[k + 2], acc[g]);
+          acc[g] = fmaf(v.w, w[k + 3], acc[g]);
+        }
+    }
+  }
+};
 
 template <class T, int D>
 __global__ void __launch_bounds__(kRotParts * D)
@@ -340,7 +368,8 @@ kv_query_kernel(const T* __restrict__ q, int64_t sb, int64_t sh, int d, int page
                 const float* __restrict__ RT, const int* __restrict__ exponent, float scale,
                 Work wk, QueryOut out, int* __restrict__ first) {
   constexpr int threads = kRotParts * D, warps = threads / 32;
-  __shared__ float sq[kHeadsPer][D], red[kRotParts][kHeadsPer][D];
+  __shared__ __align__(16) float sq[kHeadsPer][D];
+  __shared__ float red[kRotParts][kHeadsPer][D];
   __shared__ int s_part[warps];
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   pdl_next();
@@ -377,12 +406,14 @@ kv_query_kernel(const T* __restrict__ q, int64_t sb, int64_t sh, int d, int page
   const int ng = min(kHeadsPer, wk.group - hb * kHeadsPer);
   const T* src = q + b * sb + ((int64_t)h * wk.group + hb * kHeadsPer) * sh;
   const int j = tid % D, part = tid / D;
+  Turn<D> turn;
+  turn.ahead(RT, d, j, part);
 #pragma unroll
   for (int g = part; g < kHeadsPer; g += kRotParts)
     sq[g][j] = g < ng && j < d ? to_f32<T>(src[g * sh + j]) : 0.f;
   __syncthreads();
   float acc[kHeadsPer];
-  turn<D>(sq, RT, d, j, part, acc);
+  turn.run(sq, acc);
 #pragma unroll
   for (int g = 0; g < kHeadsPer; ++g) red[part][g][j] = acc[g];
   __syncthreads();
@@ -460,7 +491,6 @@ kv_attend_kernel(Side sk, Side sv, int pages, int page_shift, Work wk, QueryOut 
   __shared__ float s_m[NW][kHeadsPer], s_l[NW][kHeadsPer], s_v[NW];
   __shared__ int s_b;
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, g = lane >> 2, t = lane & 3;
-  pdl_next();
 
   // Tables, from the codec's entries (set-up data: not written by the kernel
   // before).  A thread copies an entry to the 32 lanes' places.
@@ -527,6 +557,7 @@ kv_attend_kernel(Side sk, Side sv, int pages, int page_shift, Work wk, QueryOut 
   const float* nfrom = (lane & 4 ? sv.norms : sk.norms) + (lane & 3) * 4;
   const uint32_t nto = norms_at + 16 * lane;
   pdl_wait();
+  pdl_next();
 
   const int per = wk.heads * wk.blocks;
   const int total = wk.first[wk.batch];
@@ -872,7 +903,8 @@ __global__ void __launch_bounds__(kRotParts * D)
 kv_join_kernel(Parts parts, Work wk, int workers, int d, int page_size,
                const float* __restrict__ R, const int* __restrict__ exponent, T* __restrict__ out,
                float* __restrict__ lse, float* __restrict__ lse2) {
-  __shared__ float so[kHeadsPer][D], s_l[kHeadsPer];
+  __shared__ __align__(16) float so[kHeadsPer][D];
+  __shared__ float s_l[kHeadsPer];
   // The partials' factors [worker][head], then the parts' sums [part][head][D].
   constexpr int room = kRotParts > kMaxWorkers / D ? kRotParts : kMaxWorkers / D;
   __shared__ float red[room][kHeadsPer][D];
@@ -884,7 +916,10 @@ kv_join_kernel(Parts parts, Work wk, int workers, int d, int page_size,
   const int64_t row0 = ((int64_t)b * wk.heads + h) * wk.group + hb * kHeadsPer;
   const float vscale = ldexpf(1.f / kWeightScale, -*exponent);
   pdl_next();
-  pdl_wait();
+  // (The kernel before lets this one in after the queries' kernel has ended: what
+  // that one left can be read before the wait for the partial results.)
+  Turn<D> turn;
+  turn.ahead(R, d, j, part);
   const int len = clamp_length(wk.lengths[b], wk.table_width, page_size);
   const int nu = wk.units_of(len), total = wk.first[wk.batch];
   int w0 = 0, nw = 0;
@@ -895,6 +930,7 @@ kv_join_kernel(Parts parts, Work wk, int workers, int d, int page_size,
     nw = worker_of(u0 + nu - 1, n, total) - w0 + 1;
   }
   const int64_t slot0 = (int64_t)w0 + seg;
+  pdl_wait();
   if (warp < kHeadsPer) {
     float m = -FLT_MAX, l = 0.f;
     for (int w = lane; w < nw; w += 32)
@@ -940,7 +976,7 @@ kv_join_kernel(Parts parts, Work wk, int workers, int d, int page_size,
     so[g][j] = g >= ng || s_l[g] == 0.f ? 0.f : x / s_l[g] * vscale;
   }
   __syncthreads();
-  turn<D>(so, R, d, j, part, acc);
+  turn.run(so, acc);
 #pragma unroll
   for (int g = 0; g < kHeadsPer; ++g) red[part][g][j] = acc[g];
   __syncthreads();

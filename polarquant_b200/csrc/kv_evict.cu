@@ -154,9 +154,28 @@ __global__ void __launch_bounds__(kEvictThreads) kv_select_kernel(EvictArgs a) {
     const bool safe = pos < a.sinks || (int64_t)pos > recent_from;
     return weight_key(given ? __ldg(given + t) : a.weights[at], safe);
   };
-  for (int t = begin + tid; t < min(end, begin + kKeep); t += kEvictThreads)
-    s_key[t - begin] = read_key(t);
-  auto key = [&](int t) { return t - begin < kKeep ? s_key[t - begin] : read_key(t); };
+  // Key i lies at i + i / 32, so that threads that walk runs of them meet
+  // different banks.
+  {
+    const int kept = min(end - begin, kKeep);
+    for (int i0 = tid; i0 < kept; i0 += 4 * kEvictThreads) {
+      uint32_t k[4];
+#pragma unroll
+      for (int u = 0; u < 4; ++u) {
+        const int i = i0 + u * kEvictThreads;
+        k[u] = read_key(begin + min(i, kept - 1));
+      }
+#pragma unroll
+      for (int u = 0; u < 4; ++u) {
+        const int i = i0 + u * kEvictThreads;
+        if (i < kept) s_key[i + (i >> 5)] = k[u];
+      }
+    }
+  }
+  auto key = [&](int t) {
+    const int i = t - begin;
+    return i < kKeep ? s_key[i + (i >> 5)] : read_key(t);
+  };
 
   // The key of the last token that stays, and how many of its equals do.
   uint32_t prefix = 0, mask = 0;
@@ -205,72 +224,74 @@ __global__ void __launch_bounds__(kEvictThreads) kv_select_kernel(EvictArgs a) {
     need = s_left;
   }
 
-  // Tokens above `prefix` and the first `need` of its equals stay: count the
-  // equals before this block, then its holes and movers, then list them.
+  // Tokens above `prefix` and the first `need` of its equals stay.  A thread takes
+  // a run of the block's tokens: it counts its equals, then its holes and movers,
+  // and lists them behind those of the threads and blocks before it.
   const int budget = a.budget;
+  __syncthreads();
+  const int run = (end - begin + kEvictThreads - 1) / kEvictThreads;
+  const int from = min(begin + tid * run, end), to = min(from + run, end);
   int ties = 0;
-  if (budget > 0) {
-    for (int t = begin + tid; t < end; t += kEvictThreads) ties += key(t) == prefix;
-    ties = __reduce_add_sync(0xffffffffu, ties);
+  if (budget > 0)
+    for (int t = from; t < to; ++t) ties += key(t) == prefix;
+  int total;
+  int tie = block_scan(ties, s_warp, total);
+  if constexpr (CL > 1) {
+    if (tid == 0)
+      for (int r = 0; r < CL; ++r) *of(&s_rank[0][rank], r) = total;
+    cluster.sync();
+    for (int r = 0; r < rank; ++r) tie += s_rank[0][r];
   }
-  if (tid < CL) s_rank[0][tid] = 0;
-  sync();
-  if ((tid & 31) == 0 && ties)
-    for (int r = 0; r < CL; ++r) atomicAdd(of(&s_rank[0][rank], r), ties);
-  sync();
-  int tie0 = 0;
-  for (int r = 0; r < rank; ++r) tie0 += s_rank[0][r];
+  auto stays = [&](uint32_t k, int& tie) {
+    if (budget == 0 || k < prefix) return false;
+    return k > prefix || tie++ < need;
+  };
+  int holes_n = 0, movers_n = 0, tie1 = tie;
+  for (int t = from; t < to; ++t) {
+    const bool kept = stays(key(t), tie1);
+    holes_n += t < budget && !kept;
+    movers_n += t >= budget && kept;
+  }
+  // (counts of a block are below 2^30: two scans, as one word holds only one)
+  int block_holes, block_movers;
+  int at_hole = block_scan(holes_n, s_warp, block_holes);
+  int at_mover = block_scan(movers_n, s_warp, block_movers);
+  if constexpr (CL > 1) {
+    if (tid == 0)
+      for (int r = 0; r < CL; ++r) {
+        *of(&s_rank[1][rank], r) = block_holes;
+        *of(&s_rank[2][rank], r) = block_movers;
+      }
+    cluster.sync();
+    for (int r = 0; r < rank; ++r) {
+      at_hole += s_rank[1][r];
+      at_mover += s_rank[2][r];
+    }
+    block_holes = block_movers = 0;
+    for (int r = 0; r < CL; ++r) {
+      block_holes += s_rank[1][r];
+      block_movers += s_rank[2][r];
+    }
+  }
+  if (rank == 0 && tid == 0) a.counts[row] = min(block_holes, block_movers);
   int32_t* holes = a.lists + (int64_t)row * 2 * a.list_width;
   int32_t* movers = holes + a.list_width;
-  // Twice the same walk: to count, and with what the blocks before have to write.
-  int nh = 0, nm = 0;
-#pragma unroll 1
-  for (int pass = CL > 1 ? 0 : 1; pass < 2; ++pass) {
-    int tie = tie0, hs = nh, ms = nm;
-#pragma unroll 1
-    for (int t0 = begin; t0 < end; t0 += kEvictThreads) {
-      const int t = t0 + tid;
-      const uint32_t k = t < end ? key(t) : 0u;
-      const bool eq = t < end && budget > 0 && k == prefix;
-      bool kept = t < end && budget > 0 && k > prefix;
-      int total;
-      if (tie < need && __syncthreads_or(eq)) {
-        const int x = block_scan(eq, s_warp, total);
-        kept = kept || (eq && tie + x < need);
-        tie += total;
+  for (int t = from; t < to; ++t) {
+    const bool kept = stays(key(t), tie);
+    if (t < budget && !kept) holes[at_hole++] = t;
+    if (t >= budget && kept) movers[at_mover++] = t;
+  }
+  if (given && begin < budget) {
+    // A kept token of a prompt that stays in its place gets its weight and position:
+    // every token before the budget does, and a hole's are overwritten by its mover's.
+    for (int t = begin + tid; t < min(end, budget); t += kEvictThreads) {
+      const int64_t at = a.at(b, h, t);
+      if (at >= 0) {
+        a.weights[at] = given[t];
+        a.positions[at] = t;
       }
-      const bool hole = t < min(end, budget) && !kept, mover = kept && t >= budget;
-      const int both = block_scan((hole ? 1 : 0) | (mover ? 1 << 16 : 0), s_warp, total);
-      if (pass) {
-        if (hole) holes[hs + (both & 0xffff)] = t;
-        if (mover) movers[ms + (both >> 16)] = t;
-        if (given && kept && !mover) {
-          const int64_t at = a.at(b, h, t);
-          if (at >= 0) {
-            a.weights[at] = given[t];
-            a.positions[at] = t;
-          }
-        }
-      }
-      hs += total & 0xffff;
-      ms += total >> 16;
-    }
-    if (pass == 0) {
-      if (tid == 0)
-        for (int r = 0; r < CL; ++r) {
-          *of(&s_rank[1][rank], r) = hs;
-          *of(&s_rank[2][rank], r) = ms;
-        }
-      sync();
-      for (int r = 0; r < rank; ++r) {
-        nh += s_rank[1][r];
-        nm += s_rank[2][r];
-      }
-    } else if (rank == CL - 1 && tid == 0) {
-      a.counts[row] = min(hs, ms);
     }
   }
-  if constexpr (CL > 1) cluster.sync();  // no block leaves while others write to it
 }
 
 // A warp takes 32 pairs: a lane each for the addresses, then the rows' 16-byte
@@ -349,10 +370,11 @@ inline size_t evict_bytes(const pq_kv_cache& c, int batch, int table_width, int 
 template <int CL>
 int launch_select(const EvictArgs& a, int rows, int64_t width, cudaStream_t st) {
   const int keep = (int)min((int64_t)kKeep, (width + CL - 1) / CL);
+  // (and the gaps between every 32 of them)
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3((unsigned)rows * CL);
   cfg.blockDim = dim3(kEvictThreads);
-  cfg.dynamicSmemBytes = (size_t)keep * 4;
+  cfg.dynamicSmemBytes = (size_t)(keep + keep / 32 + 1) * 4;
   cfg.stream = st;
   cudaLaunchAttribute at;
   at.id = cudaLaunchAttributeClusterDimension;
@@ -360,7 +382,7 @@ int launch_select(const EvictArgs& a, int rows, int64_t width, cudaStream_t st) 
   at.val.clusterDim.y = at.val.clusterDim.z = 1;
   cfg.attrs = &at;
   cfg.numAttrs = 1;
-  const int rc = allow_smem<kv_select_kernel<CL>>(kKeep * 4);
+  const int rc = allow_smem<kv_select_kernel<CL>>((kKeep + kKeep / 32 + 1) * 4);
   if (rc) return rc;
   PQ_CUDA_TRY(cudaLaunchKernelEx(&cfg, kv_select_kernel<CL>, a));
   PQ_LAUNCH_CHECK("kv_select_kernel");

@@ -4,6 +4,8 @@
 #include "kv.cuh"
 #include "tc.cuh"
 
+#include <type_traits>
+
 namespace pqb {
 namespace kv {
 
@@ -1016,8 +1018,9 @@ int launch_append(const AppendArgs& a, cudaStream_t st) {
 struct ReadArgs {
   Side sk, sv;
   const int64_t* slots;
-  int64_t n, slots_end;
-  int heads, d, page_size, pieces, per_token;  // 16-code pieces of a row, warps of a token
+  int64_t slots_end;
+  uint32_t tasks;
+  int heads, d, page_shift, pieces, per_token;  // 16-code pieces of a row, warps of a token
   bool vec;                                    // rows of the output are 16-byte aligned
   void *k, *v;
 };
@@ -1043,64 +1046,104 @@ __device__ __forceinline__ void read_rows(const ReadArgs& a, uint32_t* table) {
   __syncthreads();
   const uint32_t base = (uint32_t)__cvta_generic_to_shared(table) +
                         (BITS == 8 ? lane * 4 : (lane & 15) * 8);
-  const int64_t tasks = a.n * a.per_token;
-  const int64_t step = (int64_t)gridDim.x * (kReadThreads / 32);
-  for (int64_t w = (int64_t)blockIdx.x * (kReadThreads / 32) + (threadIdx.x >> 5); w < tasks;
-       w += step) {
-    const int64_t tok = a.per_token == 1 ? w : w / a.per_token;
-    const int unit = (int)(w - tok * a.per_token) * 32 + lane;
-    const int h = unit / a.pieces, piece = unit - h * a.pieces;
-    if (h >= a.heads) continue;
+  // A task is a warp's 32 pieces of a token; the next task's codes are on their way
+  // while this one's are decoded.
+  struct Piece {
+    uint32_t x[BITS == 8 ? 4 : BITS == 4 ? 2 : 1];
+    float norm;
+    bool there;    // a slot of the pool
+    int left;      // codes of the row from here on; 0 for no piece
+    int64_t to;
+  };
+  const uint32_t step = gridDim.x * (kReadThreads / 32);
+  auto fetch = [&](uint32_t w) {
+    Piece p;
+    p.there = false;
+    p.left = 0;
+    p.norm = 0.f;
+    p.to = 0;
+    if (w >= a.tasks) return p;
+    const uint32_t tok = a.per_token == 1 ? w : w / (uint32_t)a.per_token;
+    const uint32_t unit = (w - tok * a.per_token) * 32 + lane, h = unit / (uint32_t)a.pieces,
+                   piece = unit - h * a.pieces;
+    if (h >= (uint32_t)a.heads) return p;
     const int64_t slot = a.slots[tok];
-    const bool in = slot >= 0 && slot < a.slots_end;
-    uint32_t x[4] = {0u, 0u, 0u, 0u};
-    float nrm = 0.f;
-    if (in) {
-      const int64_t at =
-          (((int64_t)((uint32_t)slot / (uint32_t)a.page_size)) * a.heads + h) * a.page_size +
-          (uint32_t)slot % (uint32_t)a.page_size;
-      const uint8_t* row = s.rows + at * s.ldb + piece * (2 * BITS);
-      if (BITS == 8)
-        *reinterpret_cast<uint4*>(x) = *reinterpret_cast<const uint4*>(row);
-      else if (BITS == 4)
-        *reinterpret_cast<uint2*>(x) = *reinterpret_cast<const uint2*>(row);
+    p.left = a.d - (int)piece * 16;
+    p.to = ((int64_t)tok * a.heads + h) * a.d + piece * 16;
+    p.there = slot >= 0 && slot < a.slots_end;
+    if (p.there) {
+      const uint32_t sl = (uint32_t)slot;
+      const uint32_t at = (((sl >> a.page_shift) * a.heads + h) << a.page_shift) +
+                          (sl & ((1u << a.page_shift) - 1u));
+      const uint8_t* row = s.rows + (uint64_t)at * (uint32_t)s.ldb + piece * (2 * BITS);
+      if constexpr (BITS == 8)
+        *reinterpret_cast<uint4*>(p.x) = *reinterpret_cast<const uint4*>(row);
+      else if constexpr (BITS == 4)
+        *reinterpret_cast<uint2*>(p.x) = *reinterpret_cast<const uint2*>(row);
       else
-        x[0] = *reinterpret_cast<const uint32_t*>(row);
-      nrm = s.norms[at];
+        p.x[0] = *reinterpret_cast<const uint32_t*>(row);
+      p.norm = s.norms[at];
     }
-    float f[16];
+    return p;
+  };
+  uint32_t w = blockIdx.x * (kReadThreads / 32) + (threadIdx.x >> 5);
+  Piece next = fetch(w);
+#pragma unroll 1
+  for (; w < a.tasks; w += step) {
+    const Piece p = next;
+    next = fetch(w + step);
+    if (p.left <= 0) continue;
+    constexpr int E = 16 / sizeof(T);
+    uint4 y[16 / E];
+    if (p.there) {
+      float f[16];
 #pragma unroll
-    for (int i = 0; i < (BITS == 8 ? 16 : 8); ++i) {
-      if constexpr (BITS == 8) {
-        asm("ld.shared.f32 %0, [%1];"
-            : "=f"(f[i])
-            : "r"(__dp4a(x[i >> 2], 128u << (8 * (i & 3)), base)));
-      } else {
-        uint32_t at;
-        if constexpr (BITS == 4) {
-          at = __dp4a(x[i >> 2], 128u << (8 * (i & 3)), base);
+      for (int i = 0; i < (BITS == 8 ? 16 : 8); ++i) {
+        if constexpr (BITS == 8) {
+          asm("ld.shared.f32 %0, [%1];"
+              : "=f"(f[i])
+              : "r"(__dp4a(p.x[i >> 2], 128u << (8 * (i & 3)), base)));
         } else {
-          // nibble i, the high one of a byte first
-          const int low = (i >> 1) * 8 + (i & 1 ? 0 : 4);
-          at = base + ((x[0] >> low) & 15u) * 128u;
+          uint32_t at;
+          if constexpr (BITS == 4) {
+            at = __dp4a(p.x[i >> 2], 128u << (8 * (i & 3)), base);
+          } else {
+            // nibble i, the high one of a byte first
+            const int low = (i >> 1) * 8 + (i & 1 ? 0 : 4);
+            at = base + ((p.x[0] >> low) & 15u) * 128u;
+          }
+          asm("ld.shared.v2.f32 {%0,%1}, [%2];" : "=f"(f[2 * i]), "=f"(f[2 * i + 1]) : "r"(at));
         }
-        asm("ld.shared.v2.f32 {%0,%1}, [%2];" : "=f"(f[2 * i]), "=f"(f[2 * i + 1]) : "r"(at));
       }
-    }
-    __align__(16) T y[16];
+      uint32_t* o = reinterpret_cast<uint32_t*>(y);
 #pragma unroll
-    for (int i = 0; i < 16; ++i) y[i] = from_f32<T>(in ? __fmul_rn(nrm, f[i]) : 0.f);
-    T* to = out + ((tok * a.heads + h) * a.d + piece * 16);
-    const int left = a.d - piece * 16;
-    if (a.vec) {
-      constexpr int E = 16 / sizeof(T);
-#pragma unroll
-      for (int i = 0; i < 16; i += E)
-        if (i < left) *reinterpret_cast<uint4*>(to + i) = *reinterpret_cast<const uint4*>(y + i);
+      for (int i = 0; i < 16; i += 2) {
+        const float v0 = __fmul_rn(p.norm, f[i]), v1 = __fmul_rn(p.norm, f[i + 1]);
+        if constexpr (sizeof(T) == 4) {
+          o[i] = __float_as_uint(v0);
+          o[i + 1] = __float_as_uint(v1);
+        } else if constexpr (std::is_same<T, __half>::value) {
+          const __half2 v = __floats2half2_rn(v0, v1);
+          o[i >> 1] = *reinterpret_cast<const uint32_t*>(&v);
+        } else {
+          const __nv_bfloat162 v = __floats2bfloat162_rn(v0, v1);
+          o[i >> 1] = *reinterpret_cast<const uint32_t*>(&v);
+        }
+      }
     } else {
 #pragma unroll
+      for (int i = 0; i < 16 / E; ++i) y[i] = make_uint4(0u, 0u, 0u, 0u);
+    }
+    T* to = out + p.to;
+    if (a.vec) {
+#pragma unroll
+      for (int i = 0; i < 16 / E; ++i)
+        if (i * E < p.left) *reinterpret_cast<uint4*>(to + i * E) = y[i];
+    } else {
+      const T* e = reinterpret_cast<const T*>(y);
+#pragma unroll
       for (int i = 0; i < 16; ++i)
-        if (i < left) to[i] = y[i];
+        if (i < p.left) to[i] = e[i];
     }
   }
 }
@@ -1204,19 +1247,20 @@ int pq_kv_read(const pq_kv_cache* cache, const int64_t* slots, int64_t n, void* 
   a.sk = kv::side_k(*cache);
   a.sv = kv::side_v(*cache);
   a.slots = slots;
-  a.n = n;
   a.slots_end = (int64_t)cache->pages * cache->page_size;
   a.heads = cache->heads;
   a.d = cache->d;
-  a.page_size = cache->page_size;
+  a.page_shift = kv::page_shift_of(*cache);
   a.pieces = (cache->d + 15) / 16;
   a.per_token = (int)(((int64_t)cache->heads * a.pieces + 31) / 32);
+  a.tasks = (uint32_t)(n * a.per_token);
   a.k = k;
   a.v = v;
   a.vec = cache->d * (dtype == PQ_KV_F32 ? 4 : 2) % 16 == 0 && (uintptr_t)k % 16 == 0 &&
           (uintptr_t)v % 16 == 0;
-  const int64_t blocks = (n * a.per_token + kv::kReadThreads / 32 - 1) / (kv::kReadThreads / 32);
-  const dim3 grid((unsigned)min(blocks, (int64_t)2 * num_sms()), 2);
+  const int64_t blocks = ((int64_t)a.tasks + kv::kReadThreads / 32 - 1) / (kv::kReadThreads / 32);
+  // Three blocks an SM, those that fit, over both sides.
+  const dim3 grid((unsigned)min(blocks, (int64_t)3 * num_sms() / 2), 2);
   PQ_KV_DISPATCH_T(dtype, {
     kv::kv_read_kernel<T_><<<grid, kv::kReadThreads, 0, (cudaStream_t)stream>>>(a);
   });

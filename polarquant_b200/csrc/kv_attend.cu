@@ -55,7 +55,8 @@ namespace kv {
 
 constexpr int kHeadsPer = 8;    // query heads of one block: the width of an mma
 constexpr int kMaxWorkers = 384;  // blocks of the attention kernel
-constexpr int kLeastUnit = 64;   // tokens of the smallest unit of any shape
+constexpr int kLeastUnit = 64;     // tokens of the smallest unit of any shape
+constexpr int kSegmentCost = 768;  // what taking up a segment costs, in tokens
 constexpr float kLog2e = 1.4426950408889634f;
 constexpr float kLn2 = 0.6931471805599453f;
 // Softmax weights relative to the running maximum reach 2^3 before that follows,
@@ -294,11 +295,13 @@ struct Work {
   int unit;                         // tokens of a unit
   const int* first;                 // [batch + 1] first unit of each sequence
 
-  // A segment's units: an empty one, then its tokens'.  The empty one stands for
-  // what taking up a segment costs a block, about as much as a unit of tokens:
-  // without it, the block that gets a batch's short sequences ends last (16
-  // sequences of 0 to 32768 tokens: 24 % of the time of the other SMs).
-  __device__ int units_of(int len) const { return len ? 1 + (len + unit - 1) / unit : 0; }
+  int empty;                        // units without tokens, a segment's first
+
+  // A segment's units: first as many without tokens as taking it up costs a block
+  // (4 us at D = 128, 7 us at D = 256, as much as some 768 tokens).  Without
+  // them, the block that gets a batch's short sequences ends last (16 sequences
+  // of 0 to 32768 tokens: 24 % of the time of the other SMs).
+  __device__ int units_of(int len) const { return len ? empty + (len + unit - 1) / unit : 0; }
 };
 
 // Worker of a unit: worker w of n takes units [w * total / n, (w + 1) * total / n).
@@ -488,7 +491,7 @@ kv_attend_kernel(Side sk, Side sv, int pages, int page_shift, Work wk, QueryOut 
   using VD = Deal<D, VB, 8>;
   constexpr int KS = D / 16;  // K steps of a score, and pairs of coordinates of a value
   extern __shared__ __align__(128) uint8_t smem[];
-  __shared__ float s_m[NW][kHeadsPer], s_l[NW][kHeadsPer], s_v[NW];
+  __shared__ float s_m[NW][kHeadsPer], s_l[NW][kHeadsPer], s_f[NW][kHeadsPer], s_v[NW];
   __shared__ int s_b;
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, g = lane >> 2, t = lane & 3;
 
@@ -599,15 +602,15 @@ kv_attend_kernel(Side sk, Side sv, int pages, int page_shift, Work wk, QueryOut 
       while (u >= wk.first[x.b + 1]) ++x.b;
       const int len = clamp_length(wk.lengths[x.b], wk.table_width, 1 << page_shift);
       const int nu = wk.units_of(len);
-      const int r = u - wk.first[x.b], in = r / nu, from = r % nu, u0 = max(from, 1);
+      const int r = u - wk.first[x.b], in = r / nu, from = r % nu, u0 = max(from, wk.empty);
       const int u1 = min(nu, from + (uend - u));
       u += u1 - from;
-      if (u1 <= u0) continue;  // the empty unit alone, at the end of the run
+      if (u1 <= u0) continue;  // empty units alone, at the end of the run
       x.h = in / wk.blocks;
       x.hb = in % wk.blocks;
       x.seg = x.b * per + in;
-      x.t0 = (u0 - 1) * stride;
-      x.t1 = min(len, (u1 - 1) * stride);
+      x.t0 = (u0 - wk.empty) * stride;
+      x.t1 = min(len, (u1 - wk.empty) * stride);
 #pragma unroll
       for (int i = 0; i < MT; ++i)
         x.pid[i] = page_of(wk.table + x.b * wk.table_stride, x.t1, x.t0 + warp * 16 * MT, i);
@@ -648,7 +651,6 @@ kv_attend_kernel(Side sk, Side sv, int pages, int page_shift, Work wk, QueryOut 
     const Segment& seg = s_segment[which][warp];
     const int t1 = seg.t1, h = seg.h;
     if (seg.t0 >= t1) break;
-    take(which ^ 1, seg.b);
     const int32_t* prow = wk.table + seg.b * wk.table_stride;
     int base = seg.t0 + warp * 16 * MT;
     int pid[MT], pid1[MT];  // pages of the step to come and of the one after it
@@ -678,6 +680,7 @@ kv_attend_kernel(Side sk, Side sv, int pages, int page_shift, Work wk, QueryOut 
     }
     const float f0 = qo.factor[(int64_t)seg.seg * kHeadsPer + 2 * t];
     const float f1 = qo.factor[(int64_t)seg.seg * kHeadsPer + 2 * t + 1];
+    take(which ^ 1, seg.b);  // (while the queries come)
 
     float o[KS][4];
 #pragma unroll
@@ -879,18 +882,27 @@ kv_attend_kernel(Side sk, Side sv, int pages, int page_shift, Work wk, QueryOut 
     __syncthreads();
     const int64_t slot = (int64_t)blockIdx.x + seg.seg;
     const int ng = min(kHeadsPer, wk.group - seg.hb * kHeadsPer);
+    for (int hd = warp; hd < kHeadsPer; hd += NW) {
+      const bool in = lane < active;
+      const float m = in ? s_m[lane][hd] : -FLT_MAX;
+      float mm = m;
+#pragma unroll
+      for (int w = 16; w > 0; w >>= 1) mm = fmaxf(mm, __shfl_xor_sync(0xffffffffu, mm, w));
+      const float f = ex2(m - mm);
+      float l = in ? s_l[lane][hd] * f : 0.f;
+#pragma unroll
+      for (int w = 16; w > 0; w >>= 1) l += __shfl_xor_sync(0xffffffffu, l, w);
+      if (in) s_f[lane][hd] = f * s_v[lane];
+      if (lane == 0) parts.ml[slot * kHeadsPer + hd] = make_float2(mm, l);
+    }
+    __syncthreads();
     for (int i = tid; i < ng * D; i += Shape::threads) {
       const int hd = i / D, j = i % D;
-      float mm = -FLT_MAX;
-      for (int w = 0; w < active; ++w) mm = fmaxf(mm, s_m[w][hd]);
-      float sum = 0.f, l = 0.f;
-      for (int w = 0; w < active; ++w) {
-        const float f = ex2(s_m[w][hd] - mm);
-        sum = fmaf(s_part[w][hd * Shape::ostride + j], f * s_v[w], sum);
-        l = fmaf(s_l[w][hd], f, l);
-      }
+      float sum = 0.f;
+#pragma unroll 4
+      for (int w = 0; w < active; ++w)
+        sum = fmaf(s_part[w][hd * Shape::ostride + j], s_f[w][hd], sum);
       parts.o[slot * kHeadsPer * D + i] = sum;
-      if (j == 0) parts.ml[slot * kHeadsPer + hd] = make_float2(mm, l);
     }
     __syncthreads();
   }
@@ -926,7 +938,7 @@ kv_join_kernel(Parts parts, Work wk, int workers, int d, int page_size,
   if (nu) {
     const int n = min(workers, total);
     const int64_t u0 = wk.first[b] + (int64_t)seg_in * nu;
-    w0 = worker_of(u0 + 1, n, total);
+    w0 = worker_of(u0 + wk.empty, n, total);
     nw = worker_of(u0 + nu - 1, n, total) - w0 + 1;
   }
   const int64_t slot0 = (int64_t)w0 + seg;
@@ -1034,8 +1046,8 @@ inline AttendPlan attend_plan(const pq_kv_cache& c, int batch, int q_heads, int 
   const int64_t segments = (int64_t)batch * c.heads * p.blocks;
   p.segments = (int)segments;
   // A block per SM, never more than the units (of at least kLeastUnit tokens, and
-  // a segment's empty one) that the table has room for.
-  const int64_t units = segments * (1 + (p.width + kLeastUnit - 1) / kLeastUnit);
+  // a segment's empty ones) that the table has room for.
+  const int64_t units = segments * ((kSegmentCost + p.width) / kLeastUnit + 2);
   p.workers = (int)max((int64_t)1, min(units, (int64_t)min(num_sms(), kMaxWorkers)));
   Carve cv(ws, ws_bytes);
   p.q.hi = cv.take<__half>(segments * kHeadsPer * p.D);
@@ -1172,7 +1184,7 @@ int pq_kv_attend(const pq_kv_cache* cache, const void* q, int dtype, int64_t q_s
   if (batch == 0) return PQ_OK;
   PQ_CHECK_ARG(q && out, "null pointer argument");
   const int64_t widest =
-      1 + ((int64_t)table_width * c.page_size + kv::kLeastUnit - 1) / kv::kLeastUnit;
+      (kv::kSegmentCost + (int64_t)table_width * c.page_size) / kv::kLeastUnit + 2;
   PQ_CHECK_ARG((int64_t)batch * q_heads < (1ll << 28) &&
                    (int64_t)batch * q_heads * widest < (1ll << 31),
                "a call takes fewer than 2^28 query rows and 2^31 pieces of 64 tokens");
@@ -1194,6 +1206,7 @@ int pq_kv_attend(const pq_kv_cache* cache, const void* q, int dtype, int64_t q_s
   wk.blocks = p.blocks;
   wk.first = p.first;
   wk.unit = kv::with_shape(p.D, c.k_bits, c.v_bits, prec, kv::UnitOf{});
+  wk.empty = (kv::kSegmentCost + wk.unit - 1) / wk.unit;
   const int workers = p.workers;
   PQ_KV_DISPATCH_T(dtype, {
     rc = p.D == 64 ? kv::launch_query<T_, 64>(c, q, q_stride_b, q_stride_h, scale, wk, p, st)

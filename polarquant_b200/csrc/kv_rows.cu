@@ -701,7 +701,7 @@ __device__ __forceinline__ void append_many(const AppendArgs& a, uint8_t* smem, 
     const int t = lane & 3, lr = (warp - kCodeWarps) * 8 + (lane >> 2);  // row of the tile
     const bool vec = is_v ? a.v_vec : a.k_vec;
     constexpr int E = 16 / sizeof(T), N = D / 4 / E;
-    constexpr bool AHEAD = N <= 4;  // registers for two tiles' rows
+    constexpr bool AHEAD = N <= 2;  // registers for two tiles' rows (D = 64; above, spills cost more)
     uint4 w[N], w1[AHEAD ? N : 1];
     auto load = [&](uint32_t tile, uint4 (&to)[N]) {
       const uint32_t r = min(tile * 128 + lr, rows - 1);
@@ -852,14 +852,15 @@ __device__ __forceinline__ void append_many(const AppendArgs& a, uint8_t* smem, 
           }
           packed[w] = BITS == 8 ? x : __byte_perm(x, 0u, 0x0123);
         }
-        if (norm == 0.f) {  // all coordinates 0, which may be next to a boundary
+        if (left < 32) near &= (1u << left) - 1u;
+        if (at < 0) near = 0u;
+        if (near && norm == 0.f) {  // all coordinates 0, next to a boundary
           near = 0u;
           const uint32_t word = zero_codes<BITS>(s_bounds);
 #pragma unroll
           for (int w = 0; w < BITS; ++w) packed[w] = word;
         }
         if (left < 32) {
-          near &= (1u << left) - 1u;
 #pragma unroll
           for (int w = 0; w < BITS; ++w) {
             const int keep = min(max(left * BITS - 32 * w, 0), 32);  // bits, from the first code on
@@ -867,7 +868,6 @@ __device__ __forceinline__ void append_many(const AppendArgs& a, uint8_t* smem, 
             packed[w] &= __byte_perm(m, 0u, 0x0123);
           }
         }
-        if (at < 0) near = 0u;
         // Coordinates next to a boundary go to the list; behind its end (a batch of
         // zero vectors, say) they are recomputed at once.
         if (near) {

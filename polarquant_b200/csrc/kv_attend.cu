@@ -40,12 +40,15 @@
 // Roundings.  Centroids and queries are taken times powers of two that put the
 // largest at 2^13; f16 hi has 11 bits, hi + lo 22.  Softmax weights times value
 // norms (relative to a power of two near the largest so far) are rounded to
-// f16 for the product.  Precision levels (kPrec):
+// f16 for the product.  Precision levels (PREC):
 //   0 (bf16 out): hi alone everywhere: errors of 2^-12 next to the output's 2^-9
-//   1 (f16 out): queries and weights hi + lo, centroids hi
-//   2 (lse or accumulated weights are asked for, in f32): keys hi + lo too
-//   3 (f32): values hi + lo too
-// Maxima, sums and accumulators are f32.
+//   1 (bf16 out; lse or accumulated weights, in f32, too): scores hi + lo
+//   2 (f16 or f32 out): values and their weights hi + lo as well.  (f16 with
+//     the centroids' hi alone had up to 3.4 times the error of the output's own
+//     rounding: all tokens share the few centroids' errors, nothing averages.)
+// Maxima, sums and accumulators are f32.  The tensor cores' sums are cut off, not
+// rounded, and a chain of them drifts: at levels 1 and 2 scores are four sums put
+// together in f32, at 2 every group's values are added to the output in f32.
 #include <float.h>
 
 #include "kv.cuh"
@@ -453,7 +456,7 @@ struct Parts {
 template <int D, int KB, int VB, int PREC>
 struct AttendShape {
   // (8-bit entries hold both parts)
-  static constexpr bool lo_tables = (PREC >= 2 && KB != 8) || (PREC == 3 && VB != 8);
+  static constexpr bool lo_tables = (PREC >= 1 && KB != 8) || (PREC == 2 && VB != 8);
   static constexpr int table_bytes = (lo_tables ? 4 : 2) * (int)kTableBytes;
   static constexpr int ostride = D + 8;  // of a partial result's head in shared memory
   // A warp has two stages, a step's rows and norms each; a stage also holds the
@@ -464,12 +467,12 @@ struct AttendShape {
     const int part = kHeadsPer * ostride * 4;
     return step > part ? step : part;
   }
-  static constexpr int room = 227 * 1024 - 3072 - table_bytes;
+  static constexpr int room = 224 * 1024 - table_bytes;
   static constexpr int fit(int mt) { return room / (2 * stage_of(mt)) / 2 * 2; }
   // Registers allow 16 warps up to D = 128, fewer where operands come hi + lo
   // or the output is wider.
-  static constexpr int most = D == 64 ? (PREC < 2 ? 16 : 12)
-                              : D == 128 ? (PREC < 2 ? 16 : 10) : (PREC == 0 ? 10 : 8);
+  static constexpr int most = D == 64 ? (PREC == 0 ? 16 : 12)
+                              : D == 128 ? (PREC == 0 ? 16 : 10) : (PREC == 0 ? 10 : 8);
   // Steps of 32 tokens (two independent chains of products) where at least 10
   // warps then fit, else of 16.
   static constexpr int MT = D <= 128 && fit(2) >= 10 ? 2 : 1;
@@ -486,7 +489,7 @@ kv_attend_kernel(Side sk, Side sv, int pages, int page_shift, Work wk, QueryOut 
                  float* __restrict__ scores, int64_t score_width) {
   using Shape = AttendShape<D, KB, VB, PREC>;
   constexpr int MT = Shape::MT, NW = Shape::warps;
-  constexpr bool QLO = PREC >= 1, KLO = PREC >= 2, VLO = PREC >= 3;
+  constexpr bool KLO = PREC >= 1, VLO = PREC >= 2;
   using KD = Deal<D, KB, 4>;
   using VD = Deal<D, VB, 8>;
   constexpr int KS = D / 16;  // K steps of a score, and pairs of coordinates of a value
@@ -661,7 +664,7 @@ kv_attend_kernel(Side sk, Side sv, int pages, int page_shift, Work wk, QueryOut 
     }
 
     // The queries as B operands: lane (g, t) holds head g.
-    uint32_t qh[KS][2], ql[QLO ? KS : 1][2];
+    uint32_t qh[KS][2], ql[KLO ? KS : 1][2];
     {
       const __half* hi = qo.hi + ((int64_t)seg.seg * kHeadsPer + g) * D;
       const __half* lo = qo.lo + ((int64_t)seg.seg * kHeadsPer + g) * D;
@@ -671,7 +674,7 @@ kv_attend_kernel(Side sk, Side sv, int pages, int page_shift, Work wk, QueryOut 
         uint2 x = *reinterpret_cast<const uint2*>(hi + dim);
         qh[s][0] = x.x;
         qh[s][1] = x.y;
-        if constexpr (QLO) {
+        if constexpr (KLO) {
           x = *reinterpret_cast<const uint2*>(lo + dim);
           ql[s][0] = x.x;
           ql[s][1] = x.y;
@@ -722,15 +725,21 @@ kv_attend_kernel(Side sk, Side sv, int pages, int page_shift, Work wk, QueryOut 
             shared_bytes<KD::UB>(st + kat[un] + (i * group + e * 8 * KD::row),
                                  &kw[e][un * KD::UB / 4]);
         s[i][0] = s[i][1] = s[i][2] = s[i][3] = 0.f;
+        float more[3][4] = {};
 #pragma unroll
         for (int k = 0; k < KS; ++k) {
           uint32_t a0, a1, a2, a3, c0 = 0, c1 = 0, c2 = 0, c3 = 0;
           decode_key<KB, KLO>(kw[0], k, kbase, a0, a2, c0, c2);
           decode_key<KB, KLO>(kw[1], k, kbase, a1, a3, c1, c3);
-          mma16816(s[i], a0, a1, a2, a3, qh[k][0], qh[k][1]);
-          if constexpr (QLO) mma16816(s[i], a0, a1, a2, a3, ql[k][0], ql[k][1]);
-          if constexpr (KLO) mma16816(s[i], c0, c1, c2, c3, qh[k][0], qh[k][1]);
+          mma16816(KLO && k % 2 ? more[0] : s[i], a0, a1, a2, a3, qh[k][0], qh[k][1]);
+          if constexpr (KLO) {
+            mma16816(more[1], a0, a1, a2, a3, ql[k][0], ql[k][1]);
+            mma16816(more[2], c0, c1, c2, c3, qh[k][0], qh[k][1]);
+          }
         }
+        if constexpr (KLO)
+#pragma unroll
+          for (int e = 0; e < 4; ++e) s[i][e] += more[0][e] + (more[1][e] + more[2][e]);
       }
       float mx0 = -FLT_MAX, mx1 = -FLT_MAX, vmx = 0.f, vn[MT][2];
 #pragma unroll
@@ -758,7 +767,7 @@ kv_attend_kernel(Side sk, Side sv, int pages, int page_shift, Work wk, QueryOut 
 #pragma unroll
         for (int e = 0; e < 2; ++e) {
           const float x = s[i][2 * e], y = s[i][2 * e + 1];
-          if (PREC >= 2 && scores) {
+          if (KLO && scores) {
             const int tok = base + 16 * i + tok_k + 8 * e;
             if (tok < t1) {
               float* to = scores +
@@ -817,7 +826,7 @@ kv_attend_kernel(Side sk, Side sv, int pages, int page_shift, Work wk, QueryOut 
           const float x = p0 * w, y = p1 * w;
           const uint32_t hi = pack_half2(x, y);
           ph[i][e] = transpose8(hi);
-          if constexpr (QLO) {
+          if constexpr (VLO) {
             const float2 f = unpack_half2(hi);
             pl[i][e] = transpose8(pack_half2(x - f.x, y - f.y));
           }
@@ -838,9 +847,16 @@ kv_attend_kernel(Side sk, Side sv, int pages, int page_shift, Work wk, QueryOut 
           decode_value<VB, VLO>(vw[2], vw[3], m, vbase, a2, a3, c2, c3);
 #pragma unroll
           for (int z = 0; z < 2; ++z) {
-            mma16816(o[m + z], a0[z], a1[z], a2[z], a3[z], ph[i][0], ph[i][1]);
-            if constexpr (QLO) mma16816(o[m + z], a0[z], a1[z], a2[z], a3[z], pl[i][0], pl[i][1]);
-            if constexpr (VLO) mma16816(o[m + z], c0[z], c1[z], c2[z], c3[z], ph[i][0], ph[i][1]);
+            if constexpr (VLO) {
+              float sum[4] = {};
+              mma16816(sum, a0[z], a1[z], a2[z], a3[z], pl[i][0], pl[i][1]);
+              mma16816(sum, c0[z], c1[z], c2[z], c3[z], ph[i][0], ph[i][1]);
+              mma16816(sum, a0[z], a1[z], a2[z], a3[z], ph[i][0], ph[i][1]);
+#pragma unroll
+              for (int e = 0; e < 4; ++e) o[m + z][e] += sum[e];
+            } else {
+              mma16816(o[m + z], a0[z], a1[z], a2[z], a3[z], ph[i][0], ph[i][1]);
+            }
           }
         }
       }
@@ -1099,8 +1115,7 @@ int with_prec(int prec, F f) {
   switch (prec) {
     case 0: return f.template operator()<D, KB, VB, 0>();
     case 1: return f.template operator()<D, KB, VB, 1>();
-    case 2: return f.template operator()<D, KB, VB, 2>();
-    default: return f.template operator()<D, KB, VB, 3>();
+    default: return f.template operator()<D, KB, VB, 2>();
   }
 }
 template <int D, int KB, class F>
@@ -1194,7 +1209,7 @@ int pq_kv_attend(const pq_kv_cache* cache, const void* q, int dtype, int64_t q_s
     return fail(PQ_ERR_WORKSPACE, "pq_kv_attend needs %zu workspace bytes, got %zu", p.bytes,
                 ws_bytes);
   const cudaStream_t st = (cudaStream_t)stream;
-  const int prec = dtype == PQ_KV_F32 ? 3 : (lse || accumulate) ? 2 : dtype == PQ_KV_F16 ? 1 : 0;
+  const int prec = dtype != PQ_KV_BF16 ? 2 : lse || accumulate ? 1 : 0;
   kv::Work wk;
   wk.table = table;
   wk.table_stride = table_stride;

@@ -359,7 +359,7 @@ __device__ __noinline__ uint32_t exact_code(const T* x, float den, const float* 
 // flags; where(from, n, ...) gives the row, column and divisor of lane `from`'s
 // flag n; patch(n, code) is called on the lane that had the flag.
 template <class T, int BITS, class Where, class Patch>
-__device__ __forceinline__ void recompute(uint32_t near, const Codec& cd, const float* s_bounds,
+__device__ __forceinline__ void recompute(uint32_t near, const float* R, const float* s_bounds,
                                           int d, bool vec, Where where, Patch patch) {
   const int lane = threadIdx.x & 31;
   uint32_t pend = __ballot_sync(0xffffffffu, near != 0u);
@@ -379,7 +379,7 @@ __device__ __forceinline__ void recompute(uint32_t near, const Codec& cd, const 
     float den;
     where(max(mine, 0), n, x, col, den);
     const uint32_t code =
-        exact_code<T, BITS>(x, den, cd.R + (int64_t)col * d, s_bounds, d, vec, mine >= 0);
+        exact_code<T, BITS>(x, den, R + (int64_t)col * d, s_bounds, d, vec, mine >= 0);
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
       const uint32_t c = __shfl_sync(0xffffffffu, code, 8 * i);
@@ -390,6 +390,26 @@ __device__ __forceinline__ void recompute(uint32_t near, const Codec& cd, const 
     }
     if (!pend) pend = __ballot_sync(0xffffffffu, near != 0u);
   }
+}
+
+// The same for 32 coordinates (from col0 on) of each lane's row at x, out of line: the
+// caller keeps its registers for what happens often.
+template <class T, int BITS>
+__device__ __noinline__ void recompute_row(uint32_t near, uint32_t* packed, const T* x, float den,
+                                           int col0, const float* R, const float* s_bounds, int d,
+                                           bool vec) {
+  recompute<T, BITS>(
+      near, R, s_bounds, d, vec,
+      [&](int from, int k, const T*& row, int& col, float& dn) {
+        row = reinterpret_cast<const T*>(
+            __shfl_sync(0xffffffffu, reinterpret_cast<unsigned long long>(x), from));
+        col = min(col0 + k, d - 1);
+        dn = __shfl_sync(0xffffffffu, den, from);
+      },
+      [&](int k, uint32_t code) {
+        const int bit = k * BITS, shift = (bit & 24) + 8 - BITS - (bit & 7);
+        packed[bit >> 5] = (packed[bit >> 5] & ~(((1u << BITS) - 1u) << shift)) | code << shift;
+      });
 }
 
 // A quarter of a row, from x on (the row's coordinate k0): D / 4 elements.
@@ -557,7 +577,7 @@ __device__ __forceinline__ void append_few(const AppendArgs& a, uint32_t* s_cell
     }
   }
   recompute<T, BITS>(
-      near, cd, s_bounds, d, is_v ? a.v_vec : a.k_vec,
+      near, cd.R, s_bounds, d, is_v ? a.v_vec : a.k_vec,
       [&](int from, int n, const T*& x, int& col, float& dn) {
         const uint32_t r = min(row0 + (from >> 2) + 8 * (n >> 3), rows - 1);
         x = src + (int64_t)(r / heads) * sn + (r % heads) * sh;
@@ -882,22 +902,16 @@ __device__ __forceinline__ void append_many(const AppendArgs& a, uint8_t* smem, 
             ++i;
           }
         }
-        if (__any_sync(0xffffffffu, near != 0u))
-          recompute<T, BITS>(
-              near, cd, s_bounds, d, is_v ? a.v_vec : a.k_vec,
-              [&](int from, int k, const T*& x, int& col, float& dn) {
-                const uint32_t r = min(tile * 128 + q * 32 + from, rows - 1);
-                x = src + (int64_t)(r / heads) * sn + (r % heads) * sh;
-                col = min(col0 + k, d - 1);
-                dn = __shfl_sync(0xffffffffu, den, from);
-              },
-              [&](int k, uint32_t code) {
-                const int bit = k * BITS, shift = (bit & 24) + 8 - BITS - (bit & 7);
+        if (__any_sync(0xffffffffu, near != 0u)) {
+          uint32_t codes[BITS];
 #pragma unroll
-                for (int w = 0; w < BITS; ++w)
-                  if (w == bit >> 5)
-                    packed[w] = (packed[w] & ~(((1u << BITS) - 1u) << shift)) | code << shift;
-              });
+          for (int w = 0; w < BITS; ++w) codes[w] = packed[w];
+          const uint32_t r = min(row, rows - 1);
+          recompute_row<T, BITS>(near, codes, src + (int64_t)(r / heads) * sn + (r % heads) * sh,
+                                 den, col0, cd.R, s_bounds, d, is_v ? a.v_vec : a.k_vec);
+#pragma unroll
+          for (int w = 0; w < BITS; ++w) packed[w] = codes[w];
+        }
         if (at >= 0) {
           const int off = col0 * BITS / 8;
           if constexpr (BITS == 2) {
@@ -983,8 +997,9 @@ __global__ void __launch_bounds__(kManyThreads, 1) kv_append_kernel(AppendArgs a
 
 template <class T, int D>
 int launch_append(const AppendArgs& a, cudaStream_t st) {
-  // Few rows (two waves of blocks of 16, 12 us at D = 128 next to 20 us of one
-  // tile's way through the other kernel): the planes from L2.
+  // Few rows, one wave of blocks of 16 on either side of the cache: R's planes from
+  // L2 (bf16, D = 128, 4 bits: 256 rows in 9.8 us next to 14.9 by the other kernel,
+  // 2368 in 10.3 next to 15.4; 4736 would take 17.9).
   if (a.rows <= 16u * num_sms()) {
     using S = FewShape<T, D>;
     kv_append_few_kernel<T, D>

@@ -471,11 +471,11 @@ struct AttendShape {
   static constexpr int fit(int mt) { return room / (2 * stage_of(mt)) / 2 * 2; }
   // Registers allow 16 warps up to D = 128, fewer where operands come hi + lo
   // or the output is wider.
-  static constexpr int most = D == 64 ? (PREC == 0 ? 16 : 12)
-                              : D == 128 ? (PREC == 0 ? 16 : 10) : (PREC == 0 ? 10 : 8);
-  // Steps of 32 tokens (two independent chains of products) where at least 10
-  // warps then fit, else of 16.
-  static constexpr int MT = D <= 128 && fit(2) >= 10 ? 2 : 1;
+  static constexpr int most = D <= 128 ? (PREC == 0 ? 16 : 12) : (PREC == 0 ? 10 : 8);
+  // A warp's step is two groups of 16 tokens at D = 64, one above.  (4 bits, f16, 64
+  // heads' sequences of 0 to 32768 tokens at D = 64: 42 us next to 45 with one; at
+  // D = 128, bf16, 0 to 16384 tokens: 36.7 with one next to 37.5.)
+  static constexpr int MT = D == 64 ? 2 : 1;
   static constexpr int stage = stage_of(MT);
   static constexpr int warps = fit(MT) < most ? fit(MT) : most;
   static constexpr int threads = 32 * warps;
@@ -945,15 +945,15 @@ kv_join_kernel(Parts parts, Work wk, int workers, int d, int page_size,
   const float vscale = ldexpf(1.f / kWeightScale, -*exponent);
   pdl_next();
   // (The kernel before lets this one in after the queries' kernel has ended: what
-  // that one left can be read before the wait for the partial results.)
+  // that one left, in L2, can be read before the wait for the partial results.)
   Turn<D> turn;
   turn.ahead(R, d, j, part);
   const int len = clamp_length(wk.lengths[b], wk.table_width, page_size);
-  const int nu = wk.units_of(len), total = wk.first[wk.batch];
+  const int nu = wk.units_of(len), total = __ldcg(wk.first + wk.batch);
   int w0 = 0, nw = 0;
   if (nu) {
     const int n = min(workers, total);
-    const int64_t u0 = wk.first[b] + (int64_t)seg_in * nu;
+    const int64_t u0 = __ldcg(wk.first + b) + (int64_t)seg_in * nu;
     w0 = worker_of(u0 + wk.empty, n, total);
     nw = worker_of(u0 + nu - 1, n, total) - w0 + 1;
   }

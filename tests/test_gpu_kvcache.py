@@ -447,6 +447,21 @@ def test_attend_strides(gpu):
     check_attention(out, lse, ref, rlse, sizes, torch.bfloat16, 64)
 
 
+@pytest.mark.parametrize("dtype,d,bits,heads,lengths", [("f16", 242, 2, 3, (4000, 37)), ("f16", 64, 8, 8, (1700,)),
+                                                        ("f16", 128, 4, 2, (9, 300)), ("f32", 167, 4, 4, (3500,)),
+                                                        ("f32", 64, 8, 8, (30000,)), ("f32", 128, 2, 3, (1633, 5))])
+def test_attend_whole_error(gpu, dtype, d, bits, heads, lengths):
+    """The error over all outputs.  f16: the output's own rounding, at most 2^-11 of an element and 0.42 times that in
+    the mean, leaves no room for another of 11 bits (tokens share the centroids, so theirs would not average).  f32:
+    three roundings (2^-24) of scores in units of log 2, of up to 11 here, 2^-22 of an exponential and of each pair of
+    factors: 2^-19 if all had one sign, and no drift over thousands of sums."""
+    c = Case(d, bits, bits, heads=heads, lengths=lengths, page_size=64, dtype=dtype)
+    q = torch.tensor(1.5 * c.rng.standard_normal((len(lengths), heads * 2, d))).to(c.dtype)
+    out = c.cache.attend(q.cuda(), *c.on_gpu()).double().cpu().numpy()
+    ref, _, _ = O.attend(c.ref, c.kc, c.vc, q.double().numpy(), c.table, c.lengths, 1 / math.sqrt(d), False)
+    assert np.sqrt(((out - ref) ** 2).sum() / (ref ** 2).sum()) <= (2.0 ** -11 if dtype == "f16" else 2.0 ** -19)
+
+
 @pytest.mark.parametrize("dtype", ["f32", "f16", "bf16"])
 @pytest.mark.parametrize("group", [1, 3, 8, 11])
 def test_accumulate(gpu, dtype, group):
@@ -521,6 +536,19 @@ def test_evict_long(gpu):
     new = c.cache.evict(*c.on_gpu(), 9000, recent=500, sinks=4)
     np.testing.assert_array_equal(new.cpu().numpy(), O.evict(c.ref, c.table, c.lengths, 9000, 500, 4))
     c.check_pool()
+
+
+@pytest.mark.parametrize("prompt", [False, True])
+def test_evict_many_rows(gpu, prompt):
+    """More heads than clusters fit on the device, of lengths that one block's shared memory just holds, and a longer one."""
+    c = Case(16, 2, 2, heads=57, lengths=(9000, 7000), page_size=256)
+    w = c.rng.random((2, 57, 9000), np.float32) if prompt else None
+    for n in (9000, 5000):
+        c.lengths[0] = n
+        new = c.cache.evict(*c.on_gpu(), 4500, recent=300, sinks=4, weights=None if w is None else torch.tensor(w).cuda())
+        np.testing.assert_array_equal(new.cpu().numpy(), O.evict(c.ref, c.table, c.lengths, 4500, 300, 4, w))
+        c.lengths = new.cpu().numpy()
+        c.check_pool()
 
 
 def test_evict_bad_pages(gpu):

@@ -10,12 +10,14 @@
 // each other, and what does not have to move stays: at a constant budget a step
 // moves as many rows as it evicts.
 //
-// A sequence and head is one block, or a cluster of eight when tables have room
-// for more than 4096 tokens: each block keeps the keys of an eighth of the
-// tokens in shared memory (up to kKeep; beyond that they are read again), counts
-// go to the first block's histogram through distributed shared memory.  One
-// pass over weights and positions; bound by the latency of some eight cluster
-// barriers (65536 tokens, 48 heads: DRAM time is 2 us).
+// A sequence and head is one block or a cluster of eight, whose blocks have an
+// eighth of the tokens each and add their counts to the first one's histogram
+// through distributed shared memory.  A block keeps its tokens' keys in shared
+// memory (up to kKeep; beyond that weights and positions are read again).
+//
+// Bound by latency: of some eight barriers and, in one block, of the passes over
+// the keys.  48 heads of 65536 tokens with a cluster each take 56 us, of which
+// weights and the table are 2 us at DRAM's rate; the moves take 33 us more.
 #include <cooperative_groups.h>
 
 #include "kv.cuh"
@@ -447,8 +449,13 @@ int pq_kv_evict(const pq_kv_cache* cache, const int32_t* table, int64_t table_st
   const cudaStream_t st = (cudaStream_t)stream;
   const int rows = batch * c.heads;
   const int64_t width = (int64_t)table_width * c.page_size;
-  rc = width <= 4096 ? kv::launch_select<1>(a, rows, width, st)
-                     : kv::launch_select<8>(a, rows, width, st);
+  // A cluster for long rows, unless there are more than fit at once (three blocks
+  // an SM) and a block can keep all keys.  One block next to a cluster, us:
+  //   8 rows of 4096 tokens 18.6, 15.4; of 16384 50, 20; 48 rows of 4096 19.5, 23.6;
+  //   of 8192 28, 26; of 16384 50, 30; 128 rows of 8192 28, 60; of 16384 51, 70;
+  //   of 65536 438, 149; 512 rows of 8192 65, 214; of 32768 485, 366
+  const bool apart = width > kv::kKeep || (width > 4096 && rows * 8 <= 3 * num_sms());
+  rc = apart ? kv::launch_select<8>(a, rows, width, st) : kv::launch_select<1>(a, rows, width, st);
   if (rc) return rc;
   if (a.list_width) {
     const int64_t per = (a.list_width + 255) / 256;

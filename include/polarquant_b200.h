@@ -348,16 +348,17 @@ int pq_pack_codes(const uint8_t* codes, int64_t n, int d, int bits, uint8_t* out
  * A slot is page * page_size + offset.  A sequence is a row of a page table
  * (int32, table_width entries, row stride table_stride) and a length: its
  * token i lies in page table[i / page_size] at offset i % page_size, for every
- * head.  Entries behind the length are not read; table_width * page_size is at most
- * 2^30.  Lengths are taken as at most
- * table_width * page_size and at least 0; a token on a page outside
- * [0, pages) is not there (attention passes over it, nothing is written).
+ * head.  Entries behind the length are not read; table_width * page_size is at
+ * most 2^30.  Lengths are taken as at most table_width * page_size and at
+ * least 0; a token on a page outside [0, pages) is not there (attention passes
+ * over it, nothing is written).
  * Calls that write a page (append, evict, attend with `accumulate`) are
  * ordered by the caller against others that use it.
  *
  * d <= 256; k_bits and v_bits are 2, 4 or 8, on their own; page_size is a
  * power of two, 16 .. 1024; a pool has fewer than 2^32 rows; the arrays are
- * 16-byte aligned, and ldb is a row's packed bytes rounded up to 16.  dtype: 0 = f32, 1 = f16, 2 = bf16.
+ * 16-byte aligned, and ldb is a row's packed bytes rounded up to 16.  dtype:
+ * 0 = f32, 1 = f16, 2 = bf16.  Vectors are finite and of norms below 2^100.
  * The descriptor and its fields' sizes are host memory, read during the call.
  * ------------------------------------------------------------------------- */
 #define PQ_KV_F32 0
@@ -428,7 +429,7 @@ int pq_kv_attend(const pq_kv_cache* cache, const void* q, int dtype, int64_t q_s
  * each, at least the lengths) the tokens are a prompt's: token i has position
  * i and that weight, and the kept ones' positions and weights are written.
  * new_lengths: [batch], min(length, budget).  A page may be in one sequence
- * only. */
+ * only; batch * heads is below 65536. */
 size_t pq_kv_evict_workspace_bytes(const pq_kv_cache* cache, int batch, int table_width,
                                    int budget);
 int pq_kv_evict(const pq_kv_cache* cache, const int32_t* table, int64_t table_stride,

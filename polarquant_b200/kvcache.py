@@ -268,7 +268,8 @@ class KVCache:
         their sequences, which ``evict`` goes by.  weights: (n, heads) float32,
         the accumulated attention they start with (0 by default).
 
-        A row's norm and codes are Quantizer.encode's; vectors must be finite."""
+        A row's norm and codes are Quantizer.encode's; vectors must be finite,
+        and of norms below 2^100 for attend."""
         n = self._slots(slots)
         shape = (n, self.heads, self.d)
         code = self._vectors("k", k, shape)
@@ -333,7 +334,9 @@ class KVCache:
         Returns (sequences, query heads, d) of q's type; with return_lse also
         the natural logarithm of each softmax's sum, (sequences, query heads)
         float32, by which the result can be joined with attention over tokens
-        held elsewhere.  A sequence of length 0 gives 0 and -inf.
+        held elsewhere.  A sequence of length 0 gives 0 and -inf; tokens on
+        pages outside the pool are passed over, and lengths above what the
+        table has room for are taken as that.
 
         accumulate=True adds each token's softmax weight, summed over the query
         heads of its key-value head, to ``weights``, which ``evict`` goes by.
@@ -378,7 +381,7 @@ class KVCache:
         positions and weights are written to the cache.
 
         A page must belong to one sequence only: a shared prefix is copied, or
-        left out of the table, before."""
+        left out of the table, before.  sequences * heads is below 65536."""
         batch, table_width = self._sequences(table, lengths)
         for name, x in (("budget", budget), ("recent", recent), ("sinks", sinks)):
             if int(x) != x or not 0 <= x < 1 << 31:

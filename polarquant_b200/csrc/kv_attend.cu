@@ -10,8 +10,8 @@
 //  1. kv_query_kernel turns the queries (f32), splits each into f16 hi + lo
 //     planes of a power-of-two scale and one block sums up the sequences' units
 //     of work.
-//  2. kv_attend_kernel: persistent blocks take equal runs of units (a unit: 8
-//     warps' steps of one key-value head and up to eight of its query heads),
+//  2. kv_attend_kernel: persistent blocks take equal runs of units (a unit: one
+//     step of all warps of one key-value head and up to eight of its query heads),
 //     so ragged batches and single long sequences fill the GPU alike.  One pass
 //     with running maximum and sum; a block leaves one partial result for every
 //     head that its run touches.
@@ -32,10 +32,13 @@
 // pairs), from a table with a copy for each lane (at 2 bits each lane of half a
 // warp): no bank conflicts, and the address is one dp4a.
 //
-// What bounds it: at 4 bits and d = 128 a token and head is 136 bytes, 128
-// lookups of the 32 a cycle that an SM's shared memory gives, 160 byte
-// permutes of 64 a cycle and 16 matrix instructions of 0.46 a cycle; at HBM
-// rate that is 67 %, 50 % and 36 % of these.
+// What bounds it: issued instructions and shared memory.  At 4 bits and d = 128
+// sixteen tokens of a head are 2.2 KB and some 340 instructions, 64 of them lookups
+// (an SM's shared memory does one a cycle) and 16 matrix products.  16 sequences of 0 to 32768 tokens, 8 heads, 32 query heads, bf16:
+// the kernel 75 us, 3.4 TB/s of rows (the call 82, a copy's rate 40); issue slots
+// 65 % taken, shared memory 64 %, the matrix pipe 21 %.  tcgen05 would have the
+// decoded rows written to shared memory, which is twice the traffic of the
+// lookups.
 //
 // Roundings.  Centroids and queries are taken times powers of two that put the
 // largest at 2^13; f16 hi has 11 bits, hi + lo 22.  Softmax weights times value

@@ -355,6 +355,16 @@ __device__ __noinline__ uint32_t exact_code(const T* x, float den, const float* 
   return code;
 }
 
+// Replaces a stored row's code (of a word whose other codes may be replaced at the
+// same time).
+template <int BITS>
+__device__ __forceinline__ void replace_code(uint8_t* row, int col, uint32_t code) {
+  const int bit = col * BITS, shift = (bit & 24) + 8 - BITS - (bit & 7);
+  uint32_t* word = reinterpret_cast<uint32_t*>(row) + (bit >> 5);
+  atomicAnd(word, ~(((1u << BITS) - 1u) << shift));
+  atomicOr(word, code << shift);
+}
+
 // Replaces the codes of flagged coordinates, four at a time.  `near`: the lane's
 // flags; where(from, n, ...) gives the row, column and divisor of lane `from`'s
 // flag n; patch(n, code) is called on the lane that had the flag.
@@ -392,24 +402,23 @@ __device__ __forceinline__ void recompute(uint32_t near, const float* R, const f
   }
 }
 
-// The same for 32 coordinates (from col0 on) of each lane's row at x, out of line: the
-// caller keeps its registers for what happens often.
+// The same for coordinates of each lane's row at x whose codes are stored already
+// (at `to`): flags left[32 * i] for the 32 coordinates from col0 + 32 * i on.
 template <class T, int BITS>
-__device__ __noinline__ void recompute_row(uint32_t near, uint32_t* packed, const T* x, float den,
-                                           int col0, const float* R, const float* s_bounds, int d,
-                                           bool vec) {
-  recompute<T, BITS>(
-      near, R, s_bounds, d, vec,
-      [&](int from, int k, const T*& row, int& col, float& dn) {
-        row = reinterpret_cast<const T*>(
-            __shfl_sync(0xffffffffu, reinterpret_cast<unsigned long long>(x), from));
-        col = min(col0 + k, d - 1);
-        dn = __shfl_sync(0xffffffffu, den, from);
-      },
-      [&](int k, uint32_t code) {
-        const int bit = k * BITS, shift = (bit & 24) + 8 - BITS - (bit & 7);
-        packed[bit >> 5] = (packed[bit >> 5] & ~(((1u << BITS) - 1u) << shift)) | code << shift;
-      });
+__device__ __noinline__ void recompute_stored(const uint32_t* left, int chunks, const T* x,
+                                              float den, int col0, const float* R,
+                                              const float* s_bounds, int d, bool vec, uint8_t* to) {
+#pragma unroll 1
+  for (int i = 0; i < chunks; ++i, col0 += 32)
+    recompute<T, BITS>(
+        left[32 * i], R, s_bounds, d, vec,
+        [&](int from, int k, const T*& row, int& col, float& dn) {
+          row = reinterpret_cast<const T*>(
+              __shfl_sync(0xffffffffu, reinterpret_cast<unsigned long long>(x), from));
+          col = min(col0 + k, d - 1);
+          dn = __shfl_sync(0xffffffffu, den, from);
+        },
+        [&](int k, uint32_t code) { replace_code<BITS>(to, col0 + k, code); });
 }
 
 // A quarter of a row, from x on (the row's coordinate k0): D / 4 elements.
@@ -666,12 +675,14 @@ struct ManyShape {
   static constexpr int a_bytes = planes * kblocks * 128 * 128;
   static constexpr int b_bytes = 2 * kblocks * cols * 128;
   static constexpr int buffers = D <= 64 || (D == 128 && !wide) ? 2 : 1;
+  // (8 * 2 * cols: flags of what does not fit the list, eight warps' cols / 2 words.)
   // Coordinates to recompute that a block lists, and the tiles it takes in a
   // launch: about half to three quarters of the list at 8 bits and normal data.
   static constexpr int listed = D <= 128 ? 2048 : 1024;
   static constexpr int most_tiles = D <= 128 ? 24 : 8;
   static constexpr int tmem = cols < 16 ? 32 : 2 * cols;
-  static constexpr int smem = 1024 + b_bytes + buffers * a_bytes + 4 * kCellWords + 1024 + 9 * listed;
+  static constexpr int smem = 1024 + b_bytes + buffers * a_bytes + 4 * kCellWords + 1024 + 9 * listed +
+                              8 * 2 * cols;
 };
 constexpr int kCodeWarps = 8, kLoadWarps = 16;
 constexpr int kManyThreads = 32 * (kCodeWarps + kLoadWarps);
@@ -823,6 +834,9 @@ __device__ __forceinline__ void append_many(const AppendArgs& a, uint8_t* smem, 
     const int q = warp & 3, half = warp >> 2;
     const Coder<BITS> coder(cd, s_cell);
     constexpr float band = band_of(S::kblocks * 4 * (S::wide ? 3 : 2), BITS);
+    // Flags behind the list's end: chunks of 32 columns, a word a lane.
+    constexpr int chunks = S::cols / 64;
+    uint32_t* s_left = reinterpret_cast<uint32_t*>(l_col + S::listed) + warp * (S::cols / 2);
     uint32_t n = 0;
     auto place = [&](uint32_t tile) {
       const uint32_t r = tile * 128 + q * 32 + lane;
@@ -840,6 +854,7 @@ __device__ __forceinline__ void append_many(const AppendArgs& a, uint8_t* smem, 
       next = place(tile + gridDim.x);
       if (half == 0 && part == 0 && at >= 0) a.write_token(sd, is_v, row, at, norm);
       uint8_t* to = sd.rows + at * sd.ldb;
+      uint32_t over = 0;
 #pragma unroll 1
       for (int c = half * (S::cols / 2); c < (half + 1) * (S::cols / 2); c += 32) {
         uint32_t v[32];
@@ -849,6 +864,7 @@ __device__ __forceinline__ void append_many(const AppendArgs& a, uint8_t* smem, 
         const int col0 = part * S::cols + c, left = d - col0;
         if (left <= 0) {
           // Columns behind the row's end: zeros up to its padded length.
+          s_left[(c % (S::cols / 2)) + lane] = 0u;
           const int off = col0 * BITS / 8;
           if (at >= 0)
             for (int j = off; j < min(off + 4 * BITS, (int)sd.ldb); j += 4)
@@ -888,8 +904,9 @@ __device__ __forceinline__ void append_many(const AppendArgs& a, uint8_t* smem, 
             packed[w] &= __byte_perm(m, 0u, 0x0123);
           }
         }
-        // Coordinates next to a boundary go to the list; behind its end (a batch of
-        // zero vectors, say) they are recomputed at once.
+        // Coordinates next to a boundary go to the list.  Those behind its end (of many
+        // equal rows, say) are recomputed after the tile: in this loop the call would
+        // cost it 460 bytes of spilled registers.
         if (near) {
           const int cnt = __popc(near);
           int i = atomicAdd(s_listed, cnt);
@@ -902,16 +919,8 @@ __device__ __forceinline__ void append_many(const AppendArgs& a, uint8_t* smem, 
             ++i;
           }
         }
-        if (__any_sync(0xffffffffu, near != 0u)) {
-          uint32_t codes[BITS];
-#pragma unroll
-          for (int w = 0; w < BITS; ++w) codes[w] = packed[w];
-          const uint32_t r = min(row, rows - 1);
-          recompute_row<T, BITS>(near, codes, src + (int64_t)(r / heads) * sn + (r % heads) * sh,
-                                 den, col0, cd.R, s_bounds, d, is_v ? a.v_vec : a.k_vec);
-#pragma unroll
-          for (int w = 0; w < BITS; ++w) packed[w] = codes[w];
-        }
+        s_left[(c % (S::cols / 2)) + lane] = near;
+        over |= near;
         if (at >= 0) {
           const int off = col0 * BITS / 8;
           if constexpr (BITS == 2) {
@@ -928,6 +937,13 @@ __device__ __forceinline__ void append_many(const AppendArgs& a, uint8_t* smem, 
       tc::tc_fence_before();
       __syncwarp();
       if (lane == 0) tc::mbar_arrive(TEMPTY + 8 * acc);
+      if (__any_sync(0xffffffffu, over != 0u)) {
+        const uint32_t r = min(row, rows - 1);
+        recompute_stored<T, BITS>(s_left + lane, chunks,
+                                  src + (int64_t)(r / heads) * sn + (r % heads) * sh, den,
+                                  part * S::cols + half * (S::cols / 2), cd.R, s_bounds, d,
+                                  is_v ? a.v_vec : a.k_vec, to);
+      }
     }
   }
 
@@ -945,10 +961,7 @@ __device__ __forceinline__ void append_many(const AppendArgs& a, uint8_t* smem, 
         src + (int64_t)(r / heads) * sn + (r % heads) * sh, l_den[e], cd.R + (int64_t)col * d,
         s_bounds, d, is_v ? a.v_vec : a.k_vec, valid);
     if (valid && (lane & 7) == 0) {
-      const int bit = col * BITS, shift = (bit & 24) + 8 - BITS - (bit & 7);
-      uint32_t* word = reinterpret_cast<uint32_t*>(sd.rows + a.place(r) * sd.ldb) + (bit >> 5);
-      atomicAnd(word, ~(((1u << BITS) - 1u) << shift));
-      atomicOr(word, code << shift);
+      replace_code<BITS>(sd.rows + a.place(r) * sd.ldb, col, code);
     }
   }
 }

@@ -284,6 +284,28 @@ def test_append_of_zero_vectors_and_boundary_values(gpu):
     check_rows(cache, (c, c), k, v, slots)
 
 
+@pytest.mark.parametrize("dtype,d,bits", [("bf16", 128, 8), ("f16", 256, 4), ("f32", 128, 2), ("bf16", 64, 8), ("f32", 256, 8),
+                                          ("bf16", 80, 4)])
+def test_append_of_equal_rows_on_boundaries(gpu, dtype, d, bits):
+    """Many equal rows, the boundaries next to their own coordinates: a block's list is full after a few of them."""
+    R = codec(d, 4)[1][0]
+    rng = np.random.default_rng(d + bits)
+    x = torch.tensor(rng.standard_normal((2, d))).to(TYPES[dtype])
+    u = x.float().numpy()
+    u = u / np.sqrt((u.astype(np.float64) ** 2).sum(-1, keepdims=True)).astype(np.float32)
+    y = np.sort((u.astype(np.float64) @ R.astype(np.float64).T).ravel())
+    levels = 1 << bits
+    bounds = np.concatenate([y, np.linspace(y[-1] + 0.01, y[-1] + 0.5, levels)]) if len(y) < levels - 1 else y
+    bounds = np.sort(rng.permutation(bounds)[: levels - 1]).astype(np.float32)
+    c = (R, bounds, np.linspace(-1, 1, levels, dtype=np.float32))
+    n, heads = 400, 8
+    cache = KVCache(KVCodec(*c), heads=heads, pages=n // 16, page_size=16)
+    k, v = (r.expand(n, heads, d).contiguous().cuda() for r in x)
+    slots = torch.arange(n, device="cuda")
+    cache.append(k, v, slots, torch.zeros(n, dtype=torch.int32, device="cuda"))
+    check_rows(cache, (c, c), k, v, slots)
+
+
 def test_append_in_several_launches(gpu):
     """More rows than one launch of the append of many rows takes."""
     q, c = codec(64, 8)

@@ -16,8 +16,8 @@
 // memory (up to kKeep; beyond that weights and positions are read again).
 //
 // Bound by latency: of some eight barriers and, in one block, of the passes over
-// the keys.  48 heads of 65536 tokens with a cluster each take 56 us, of which
-// weights and the table are 2 us at DRAM's rate; the moves take 33 us more.
+// the keys.  48 heads of 65536 tokens with a cluster each take 56 us, 8 of them 35
+// us, of which weights and the table are 2 us at DRAM's rate.
 #include <cooperative_groups.h>
 
 #include "kv.cuh"

@@ -131,6 +131,13 @@ __global__ void __launch_bounds__(kEvictThreads, 3) kv_select_kernel(EvictArgs a
       }
     return;
   }
+  // Nothing stays, nothing is written, and no block of the cluster needs another:
+  // what follows reaches into the others' shared memory only behind a barrier of
+  // the cluster, and the radix passes, which have them, are for budgets above 0.
+  if (a.budget == 0) {
+    if (rank == 0 && tid == 0) a.counts[row] = 0;
+    return;
+  }
 
   // The largest position.
   int64_t recent_from = (int64_t)(len - 1) - a.recent;
@@ -185,7 +192,7 @@ __global__ void __launch_bounds__(kEvictThreads, 3) kv_select_kernel(EvictArgs a
   uint32_t prefix = 0, mask = 0;
   int need = a.budget;
 #pragma unroll 1
-  for (int pass = 0; pass < 3 && a.budget > 0; ++pass) {
+  for (int pass = 0; pass < 3; ++pass) {
     const int shift = pass == 0 ? 21 : pass == 1 ? 10 : 0, bits = pass == 2 ? 10 : 11;
     for (int i = tid; i < kBins; i += kEvictThreads) s_hist[i] = 0;
     sync();
@@ -236,8 +243,7 @@ __global__ void __launch_bounds__(kEvictThreads, 3) kv_select_kernel(EvictArgs a
   const int run = (end - begin + kEvictThreads - 1) / kEvictThreads;
   const int from = min(begin + tid * run, end), to = min(from + run, end);
   int ties = 0;
-  if (budget > 0)
-    for (int t = from; t < to; ++t) ties += key(t) == prefix;
+  for (int t = from; t < to; ++t) ties += key(t) == prefix;
   int total;
   int tie = block_scan(ties, s_warp, total);
   if constexpr (CL > 1) {
@@ -247,7 +253,7 @@ __global__ void __launch_bounds__(kEvictThreads, 3) kv_select_kernel(EvictArgs a
     for (int r = 0; r < rank; ++r) tie += s_rank[0][r];
   }
   auto stays = [&](uint32_t k, int& tie) {
-    if (budget == 0 || k < prefix) return false;
+    if (k < prefix) return false;
     return k > prefix || tie++ < need;
   };
   int holes_n = 0, movers_n = 0, tie1 = tie;

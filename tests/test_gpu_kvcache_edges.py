@@ -1,0 +1,38 @@
+"""The key-value cache where it could go wrong.
+
+The plain cases, and the helper that holds a cache next to its oracle, are in test_gpu_kvcache.py.
+"""
+import numpy as np
+import pytest
+import torch
+
+from oracle import kv_oracle as O
+from test_gpu_kvcache import Case
+
+pytestmark = pytest.mark.gpu
+
+
+def check_evict(c, budget, recent=0, sinks=0, w=None):
+    new = c.cache.evict(*c.on_gpu(), budget, recent=recent, sinks=sinks, weights=None if w is None else torch.tensor(w).cuda())
+    np.testing.assert_array_equal(new.cpu().numpy(), O.evict(c.ref, c.table, c.lengths, budget, recent, sinks, w))
+    c.check_pool()
+
+
+# -- eviction ------------------------------------------------------------------------------------------------------------
+
+@pytest.mark.parametrize("prompt", [False, True])
+@pytest.mark.parametrize("lengths", [(5000, 3), (17000, 0, 9000)])
+def test_evict_to_nothing(gpu, lengths, prompt):
+    """A budget of 0 for rows that a cluster of blocks takes: everything goes, and nothing is written."""
+    c = Case(16, 2, 2, heads=2, lengths=lengths, page_size=256)
+    w = c.rng.random((len(lengths), 2, max(lengths)), np.float32) if prompt else None
+    for recent, sinks in ((0, 0), (100, 4)):
+        check_evict(c, 0, recent, sinks, w)
+
+
+@pytest.mark.parametrize("prompt", [False, True])
+def test_evict_very_long(gpu, prompt):
+    """More tokens than the shared memory of a cluster's eight blocks holds the weights of (16384 each)."""
+    c = Case(16, 2, 2, heads=1, lengths=(150001, 140000), page_size=1024)
+    w = c.rng.random((2, 1, 150001), np.float32) if prompt else None
+    check_evict(c, 70000, 500, 4, w)

@@ -93,9 +93,8 @@ def evict(cache, table, lengths, budget, recent=0, sinks=0, prompt=None):
             kept = np.ones(length, bool)
             if length > budget:
                 safe = (pos < sinks) | (pos.astype(np.int64) > int(pos.max()) - recent)
-                key = np.where(safe, np.inf, w.astype(np.float64))
-                nan = np.isnan(key)
-                order = np.lexsort((np.arange(length), -np.where(nan, 0, key), nan))
+                nan = np.isnan(w)
+                order = np.lexsort((np.arange(length), -np.where(nan | safe, 0, w), nan & ~safe, ~safe))
                 kept[:] = False
                 kept[order[:budget]] = True
             source = np.arange(min(length, budget))

@@ -60,9 +60,9 @@ struct EvictArgs {
   }
 };
 
-// Monotone in the weight; -0 as 0, NaN below everything; protected as +inf.
+// Monotone in the weight; -0 as 0, NaN below everything, protected above +inf.
 __device__ __forceinline__ uint32_t weight_key(float w, bool safe) {
-  if (safe) return 0xff800000u;
+  if (safe) return 0xffffffffu;
   if (isnan(w)) return 0u;
   const uint32_t u = __float_as_uint(w == 0.f ? 0.f : w);
   return (u >> 31) ? ~u : (u | 0x80000000u);

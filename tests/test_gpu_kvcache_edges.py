@@ -36,3 +36,20 @@ def test_evict_very_long(gpu, prompt):
     c = Case(16, 2, 2, heads=1, lengths=(150001, 140000), page_size=1024)
     w = c.rng.random((2, 1, 150001), np.float32) if prompt else None
     check_evict(c, 70000, 500, 4, w)
+
+
+@pytest.mark.parametrize("prompt", [False, True])
+def test_evict_infinite_weights(gpu, prompt):
+    """Protected tokens come before any weight, the infinite ones too, however many there are and wherever they lie."""
+    c = Case(32, 4, 4, heads=3, lengths=(200,), page_size=16)
+    w = c.rng.random((1, 3, 200), np.float32)
+    w[0, 0, :150] = np.inf
+    w[0, 1, 20:60] = np.inf
+    w[0, 2] = np.inf
+    w[0, 2, 190:] = np.nan
+    if not prompt:
+        pg, off, _ = O.sequence(c.ref, c.table[0], 200)
+        for h in range(3):
+            c.ref["weights"][pg, h, off] = w[0, h]
+        c.cache.weights.copy_(torch.tensor(c.ref["weights"]))
+    check_evict(c, 50, 12, 3, w if prompt else None)

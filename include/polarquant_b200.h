@@ -424,7 +424,9 @@ int pq_kv_attend(const pq_kv_cache* cache, const void* q, int dtype, int64_t q_s
  * of a position below `sinks` or among the last `recent` positions first, then
  * the heaviest, ties to the lowest slot (a NaN weight counts as the lightest).
  * Kept tokens behind the budget move into the places of evicted ones before
- * it, the first into the first; all others stay where they are.  With
+ * it, the first into the first; all others stay where they are.  A token on a
+ * page outside the pool is not kept, and its place before the budget is not
+ * filled (as many fewer tokens stay).  With
  * prompt_weights ([batch][heads], strides in elements, prompt_width tokens
  * each, at least the lengths) the tokens are a prompt's: token i has position
  * i and that weight, and the kept ones' positions and weights are written.

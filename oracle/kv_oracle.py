@@ -85,20 +85,21 @@ def evict(cache, table, lengths, budget, recent=0, sinks=0, prompt=None):
     for b, length in enumerate(lengths):
         length = max(0, min(int(length), len(table[b]) * page))
         new.append(min(length, budget))
-        pg, off = np.asarray(table[b])[np.arange(length) // page], np.arange(length) % page
+        pg, off, tok = sequence(cache, table[b], length)  # the tokens that are there
         for h in range(heads):
             at = (pg, h, off)
-            w = (cache["weights"][at] if prompt is None else prompt[b, h, :length]).astype(np.float32).copy()
-            pos = cache["positions"][at].copy() if prompt is None else np.arange(length, dtype=np.int32)
-            kept = np.ones(length, bool)
-            if length > budget:
-                safe = (pos < sinks) | (pos.astype(np.int64) > int(pos.max()) - recent)
+            w = (cache["weights"][at] if prompt is None else prompt[b, h, tok]).astype(np.float32).copy()
+            pos = cache["positions"][at].copy() if prompt is None else tok.astype(np.int32)
+            first = tok < budget  # places that the kept tokens take
+            source = np.arange(first.sum())
+            if length > budget and len(source):
+                last = int(pos.max()) if prompt is None else length - 1
+                safe = (pos < sinks) | (pos.astype(np.int64) > last - recent)
                 nan = np.isnan(w)
-                order = np.lexsort((np.arange(length), -np.where(nan | safe, 0, w), nan & ~safe, ~safe))
-                kept[:] = False
-                kept[order[:budget]] = True
-            source = np.arange(min(length, budget))
-            source[~kept[:budget][:len(source)]] = np.flatnonzero(kept[budget:]) + budget if length > budget else 0
+                order = np.lexsort((tok, -np.where(nan | safe, 0, w), nan & ~safe, ~safe))
+                kept = np.zeros(len(tok), bool)
+                kept[order[:len(source)]] = True
+                source[~kept[first]] = np.flatnonzero(kept & ~first)
             to, fr = (pg[:len(source)], h, off[:len(source)]), (pg[source], h, off[source])
             for name in ("k_codes", "v_codes", "k_norms", "v_norms"):
                 cache[name][to] = cache[name][fr].copy()

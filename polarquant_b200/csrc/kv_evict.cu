@@ -4,11 +4,12 @@
 // descending, slot ascending) stay.  A radix selection on a monotone 32-bit key
 // of the weight (11, 11 and 10 bits) finds the key of the last one that stays
 // and how many of its equals do; then the evicted tokens before the budget
-// (holes) and the kept ones behind it (movers), equally many, are listed in slot
-// order and kv_move_kernel copies the j-th mover to the j-th hole.  Sources lie
-// behind the budget and destinations before it, so the copies do not depend on
-// each other, and what does not have to move stays: at a constant budget a step
-// moves as many rows as it evicts.
+// (holes) and the kept ones behind it (movers), equally many (tokens on pages
+// outside the pool are neither), are listed in slot order and kv_move_kernel
+// copies the j-th mover to the j-th hole.  Sources lie behind the budget and
+// destinations before it, so the copies do not depend on each other, and what
+// does not have to move stays: at a constant budget a step moves as many rows as
+// it evicts.
 //
 // A sequence and head is one block or a cluster of eight, whose blocks have an
 // eighth of the tokens each and add their counts to the first one's histogram
@@ -61,9 +62,10 @@ struct EvictArgs {
 };
 
 // Monotone in the weight; -0 as 0, NaN below everything, protected above +inf.
+// (0 is the key of a token on a page outside the pool.)
 __device__ __forceinline__ uint32_t weight_key(float w, bool safe) {
   if (safe) return 0xffffffffu;
-  if (isnan(w)) return 0u;
+  if (isnan(w)) return 1u;
   const uint32_t u = __float_as_uint(w == 0.f ? 0.f : w);
   return (u >> 31) ? ~u : (u | 0x80000000u);
 }
@@ -97,7 +99,7 @@ __device__ __forceinline__ int block_scan(int x, int* s_warp, int& total) {
 template <int CL>
 __global__ void __launch_bounds__(kEvictThreads, 3) kv_select_kernel(EvictArgs a) {
   extern __shared__ uint32_t s_key[];
-  __shared__ int s_hist[kBins], s_warp[32], s_rank[3][CL], s_max, s_digit, s_left;
+  __shared__ int s_hist[kBins], s_warp[32], s_rank[3][CL], s_max, s_digit, s_left, s_missing;
   auto cluster = cg::this_cluster();
   const int rank = CL > 1 ? (int)cluster.block_rank() : 0;
   const int row = blockIdx.x / CL, b = row / a.heads, h = row % a.heads, tid = threadIdx.x;
@@ -188,17 +190,26 @@ __global__ void __launch_bounds__(kEvictThreads, 3) kv_select_kernel(EvictArgs a
     return i < kKeep ? s_key[i + (i >> 5)] : read_key(t);
   };
 
-  // The key of the last token that stays, and how many of its equals do.
+  // The key of the last token that stays, and how many of its equals do.  A token
+  // on a page outside the pool cannot stay, and one before the budget is a place
+  // that no other can take: as many fewer stay.
   uint32_t prefix = 0, mask = 0;
   int need = a.budget;
 #pragma unroll 1
   for (int pass = 0; pass < 3; ++pass) {
     const int shift = pass == 0 ? 21 : pass == 1 ? 10 : 0, bits = pass == 2 ? 10 : 11;
     for (int i = tid; i < kBins; i += kEvictThreads) s_hist[i] = 0;
+    if (pass == 0 && tid == 0) s_missing = 0;
     sync();
+    int missing = 0;
     for (int t = begin + tid; t < end; t += kEvictThreads) {
       const uint32_t k = key(t);
+      missing += k == 0u && t < a.budget;
       if ((k & mask) == prefix) atomicAdd(&s_hist[(k >> shift) & ((1u << bits) - 1u)], 1);
+    }
+    if (pass == 0) {
+      missing = __reduce_add_sync(0xffffffffu, missing);
+      if ((tid & 31) == 0 && missing) atomicAdd(of(&s_missing, 0), missing);
     }
     if constexpr (CL > 1) {
       __syncthreads();
@@ -210,6 +221,12 @@ __global__ void __launch_bounds__(kEvictThreads, 3) kv_select_kernel(EvictArgs a
     }
     sync();
     if (rank == 0) {
+      if (pass == 0) need -= s_missing;
+      if (need == 0 && tid == 0)  // no place at all: no key is above the last digits
+        for (int r = 0; r < CL; ++r) {
+          *of(&s_digit, r) = (1 << bits) - 1;
+          *of(&s_left, r) = 0;
+        }
       // Four bins a thread from the highest down: where the count reaches `need`.
       constexpr int each = kBins / kEvictThreads;
       int c[each], sum = 0, total;
@@ -258,8 +275,9 @@ __global__ void __launch_bounds__(kEvictThreads, 3) kv_select_kernel(EvictArgs a
   };
   int holes_n = 0, movers_n = 0, tie1 = tie;
   for (int t = from; t < to; ++t) {
-    const bool kept = stays(key(t), tie1);
-    holes_n += t < budget && !kept;
+    const uint32_t k = key(t);
+    const bool kept = stays(k, tie1);
+    holes_n += t < budget && !kept && k;
     movers_n += t >= budget && kept;
   }
   // (counts of a block are below 2^30: two scans, as one word holds only one)
@@ -287,8 +305,9 @@ __global__ void __launch_bounds__(kEvictThreads, 3) kv_select_kernel(EvictArgs a
   int32_t* holes = a.lists + (int64_t)row * 2 * a.list_width;
   int32_t* movers = holes + a.list_width;
   for (int t = from; t < to; ++t) {
-    const bool kept = stays(key(t), tie);
-    if (t < budget && !kept) holes[at_hole++] = t;
+    const uint32_t k = key(t);
+    const bool kept = stays(k, tie);
+    if (t < budget && !kept && k) holes[at_hole++] = t;
     if (t >= budget && kept) movers[at_mover++] = t;
   }
   if (given && begin < budget) {

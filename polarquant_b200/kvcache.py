@@ -373,7 +373,9 @@ class KVCache:
         ones of the largest accumulated ``weights``, ties to the lowest slot.
         Tokens kept from behind the budget take the places of evicted ones
         before it, in order; the others stay where they are.  Returns the new
-        lengths, (sequences,) int32; pages behind them are free.
+        lengths, (sequences,) int32; pages behind them are free.  Tokens on pages
+        outside the pool are not there: none is kept, and none is moved onto such
+        a page, so that fewer than `budget` are left where the table has one.
 
         weights: (sequences, heads, tokens) float32 for prompts whose attention
         was computed elsewhere: token i has position i and this weight (the

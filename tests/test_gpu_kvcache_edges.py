@@ -53,3 +53,23 @@ def test_evict_infinite_weights(gpu, prompt):
             c.ref["weights"][pg, h, off] = w[0, h]
         c.cache.weights.copy_(torch.tensor(c.ref["weights"]))
     check_evict(c, 50, 12, 3, w if prompt else None)
+
+
+@pytest.mark.parametrize("prompt", [False, True])
+@pytest.mark.parametrize("bad", [(1,), (0, 1, 2), (8,), (1, 8, 9), (0, 1, 2, 3, 4, 5, 6, 7, 8, 9), ()])
+@pytest.mark.parametrize("budget", [48, 40, 1])
+def test_evict_missing_pages(gpu, bad, budget, prompt):
+    """Pages outside the pool: their tokens are not there to be kept, and no kept token is moved to where it would be lost."""
+    c = Case(32, 4, 4, heads=2, lengths=(160, 150), page_size=16)
+    for i, p in enumerate(bad):
+        c.table[0, p] = (-1, c.pages, 2 ** 31 - 1)[i % 3]
+    w = c.rng.random((2, 2, 160), np.float32) if prompt else None
+    check_evict(c, budget, 9, 2, w)
+
+
+def test_evict_missing_pages_of_long_rows(gpu):
+    """The same where a cluster of blocks takes a row, with pages missing in the shares of several of them."""
+    c = Case(16, 2, 2, heads=2, lengths=(20000,), page_size=64)
+    c.table[0, [0, 3, 40, 41, 42, 100, 200, 250, 312]] = -1
+    check_evict(c, 9000, 700, 4)
+    check_evict(c, 8999)

@@ -43,15 +43,19 @@
 // Roundings.  Centroids and queries are taken times powers of two that put the
 // largest at 2^13; f16 hi has 11 bits, hi + lo 22.  Softmax weights times value
 // norms (relative to a power of two near the largest so far) are rounded to
-// f16 for the product.  Precision levels (PREC):
-//   0 (bf16 out): hi alone everywhere: errors of 2^-12 next to the output's 2^-9
-//   1 (bf16 out; lse or accumulated weights, in f32, too): scores hi + lo
-//   2 (f16 or f32 out): values and their weights hi + lo as well.  (f16 with
-//     the centroids' hi alone had up to 3.4 times the error of the output's own
-//     rounding: all tokens share the few centroids' errors, nothing averages.)
+// f16 for the product.
+//   Scores are products of hi + lo for every type: what a score is off by, its
+//   softmax weight is off by, times the score, so that 11 bits lose 0.4 % of a
+//   weight at |q||k| / sqrt(d) = 100 and bf16 outputs were off by 1.2 times their
+//   own rounding at scores of 200, 1.6 times at 900.
+//   Values and their weights are hi alone for bf16 outputs: errors of 2^-12 in the
+//   mean next to the output's 2^-9, whatever the values and scores.
+//   For f16 and f32 outputs (FINE) they are hi + lo as well.  (f16 with the
+//   centroids' hi alone had up to 3.4 times the error of the output's own
+//   rounding: all tokens share the few centroids' errors, nothing averages.)
 // Maxima, sums and accumulators are f32.  The tensor cores' sums are cut off, not
-// rounded, and a chain of them drifts: at levels 1 and 2 scores are four sums put
-// together in f32, at 2 every group's values are added to the output in f32.
+// rounded, and a chain of them drifts: scores are four sums put together in f32,
+// and FINE adds every group's values to the output in f32.
 #include <float.h>
 
 #include "kv.cuh"
@@ -174,9 +178,10 @@ __device__ __forceinline__ int value_piece(int n) {
 
 // Decoding.  A side's table has 256 entries of 128 bytes, a copy of the entry's
 // word for every lane (2 bits: of its two words for every lane of half a warp);
-// keys' first, values' behind them, then (2 and 4 bits, hi + lo) both lo tables.
+// keys' first, values' behind them, then the lo tables of the sides that have one
+// (2 and 4 bits; at 8 an entry holds both parts): keys', then with FINE values'.
 // `base` is the lane's place in entry 0 as a shared-memory address; one dp4a adds
-// 128 times a byte of the packed word to it.
+// 128 times a byte of the packed word to it.  AT: where the table lies from there.
 constexpr uint32_t kTableBytes = 32768;
 
 template <int BITS>
@@ -184,27 +189,29 @@ __device__ __forceinline__ uint32_t lane_place(int lane) {
   return BITS == 2 ? (lane & 15) * 8 : lane * 4;
 }
 
-template <int LO>
+template <int AT>
 __device__ __forceinline__ uint32_t lookup(uint32_t base, uint32_t w, int byte) {
   const uint32_t at = __dp4a(w, 128u << (8 * byte), base);
   uint32_t x;
-  asm("ld.shared.b32 %0, [%1+%2];" : "=r"(x) : "r"(at), "n"(LO * 2 * (int)kTableBytes));
+  asm("ld.shared.b32 %0, [%1+%2];" : "=r"(x) : "r"(at), "n"(AT));
   return x;
 }
 
-template <int LO>
+template <int AT>
 __device__ __forceinline__ uint2 lookup2(uint32_t base, uint32_t w, int byte) {
   const uint32_t at = __dp4a(w, 128u << (8 * byte), base);
   uint2 x;
   asm("ld.shared.v2.b32 {%0,%1}, [%2+%3];"
       : "=r"(x.x), "=r"(x.y)
-      : "r"(at), "n"(LO * 2 * (int)kTableBytes));
+      : "r"(at), "n"(AT));
   return x;
 }
 
 // The four codes that a lane gives to one K step: pairs a (first operand
 // register) and b (third), hi and lo.
-template <int BITS, bool LO, int W>
+constexpr int kKeyLo = 2 * (int)kTableBytes;
+
+template <int BITS, int W>
 __device__ __forceinline__ void decode_key(const uint32_t (&w)[W], int s, uint32_t base,
                                            uint32_t& ah, uint32_t& bh, uint32_t& al, uint32_t& bl) {
   if constexpr (BITS == 4) {
@@ -212,35 +219,29 @@ __device__ __forceinline__ void decode_key(const uint32_t (&w)[W], int s, uint32
     const int b = (s & 1) * 2;
     ah = lookup<0>(base, x, b);
     bh = lookup<0>(base, x, b + 1);
-    if constexpr (LO) {
-      al = lookup<1>(base, x, b);
-      bl = lookup<1>(base, x, b + 1);
-    }
+    al = lookup<kKeyLo>(base, x, b);
+    bl = lookup<kKeyLo>(base, x, b + 1);
   } else if constexpr (BITS == 8) {
     const uint32_t x = w[s];
     const uint32_t e0 = lookup<0>(base, x, 0), e1 = lookup<0>(base, x, 1);
     const uint32_t e2 = lookup<0>(base, x, 2), e3 = lookup<0>(base, x, 3);
     ah = __byte_perm(e0, e1, 0x5410);
     bh = __byte_perm(e2, e3, 0x5410);
-    if constexpr (LO) {
-      al = __byte_perm(e0, e1, 0x7632);
-      bl = __byte_perm(e2, e3, 0x7632);
-    }
+    al = __byte_perm(e0, e1, 0x7632);
+    bl = __byte_perm(e2, e3, 0x7632);
   } else {
     const uint2 e = lookup2<0>(base, w[s >> 2], s & 3);
     ah = e.x;
     bh = e.y;
-    if constexpr (LO) {
-      const uint2 f = lookup2<1>(base, w[s >> 2], s & 3);
-      al = f.x;
-      bl = f.y;
-    }
+    const uint2 f = lookup2<kKeyLo>(base, w[s >> 2], s & 3);
+    al = f.x;
+    bl = f.y;
   }
 }
 
 // Codes 2m, 2m + 1 (and 2m + 2, 2m + 3) of two tokens' rows: of each code the pair
-// (x's, y's), even ones in `e`, odd ones in `o`.
-template <int BITS, bool LO, int W>
+// (x's, y's), even ones in `e`, odd ones in `o`.  LO: with lo parts, their table AT.
+template <int BITS, bool LO, int AT, int W>
 __device__ __forceinline__ void decode_value(const uint32_t (&x)[W], const uint32_t (&y)[W], int m,
                                              uint32_t base, uint32_t (&eh)[2], uint32_t (&oh)[2],
                                              uint32_t (&el)[2], uint32_t (&ol)[2]) {
@@ -252,7 +253,7 @@ __device__ __forceinline__ void decode_value(const uint32_t (&x)[W], const uint3
       eh[i] = __byte_perm(p, q, 0x5410);
       oh[i] = __byte_perm(p, q, 0x7632);
       if constexpr (LO) {
-        const uint32_t r = lookup<1>(base, x[n >> 2], n & 3), t = lookup<1>(base, y[n >> 2], n & 3);
+        const uint32_t r = lookup<AT>(base, x[n >> 2], n & 3), t = lookup<AT>(base, y[n >> 2], n & 3);
         el[i] = __byte_perm(r, t, 0x5410);
         ol[i] = __byte_perm(r, t, 0x7632);
       }
@@ -278,7 +279,7 @@ __device__ __forceinline__ void decode_value(const uint32_t (&x)[W], const uint3
     eh[1] = __byte_perm(p.y, q.y, 0x5410);
     oh[1] = __byte_perm(p.y, q.y, 0x7632);
     if constexpr (LO) {
-      const uint2 r = lookup2<1>(base, x[n >> 2], n & 3), t = lookup2<1>(base, y[n >> 2], n & 3);
+      const uint2 r = lookup2<AT>(base, x[n >> 2], n & 3), t = lookup2<AT>(base, y[n >> 2], n & 3);
       el[0] = __byte_perm(r.x, t.x, 0x5410);
       ol[0] = __byte_perm(r.x, t.x, 0x7632);
       el[1] = __byte_perm(r.y, t.y, 0x5410);
@@ -456,11 +457,10 @@ struct Parts {
   float2* ml;  // [slot][8]: maximum (log2), sum
 };
 
-template <int D, int KB, int VB, int PREC>
+template <int D, int KB, int VB, bool FINE>
 struct AttendShape {
-  // (8-bit entries hold both parts)
-  static constexpr bool lo_tables = (PREC >= 1 && KB != 8) || (PREC == 2 && VB != 8);
-  static constexpr int table_bytes = (lo_tables ? 4 : 2) * (int)kTableBytes;
+  static constexpr bool k_lo = KB != 8, v_lo = FINE && VB != 8;  // sides with a lo table
+  static constexpr int table_bytes = (2 + k_lo + v_lo) * (int)kTableBytes;
   static constexpr int ostride = D + 8;  // of a partial result's head in shared memory
   // A warp has two stages, a step's rows and norms each; a stage also holds the
   // warp's partial result at a segment's end, while the next segment's first
@@ -472,9 +472,8 @@ struct AttendShape {
   }
   static constexpr int room = 224 * 1024 - table_bytes;
   static constexpr int fit(int mt) { return room / (2 * stage_of(mt)) / 2 * 2; }
-  // Registers allow 16 warps up to D = 128, fewer where operands come hi + lo
-  // or the output is wider.
-  static constexpr int most = D <= 128 ? (PREC == 0 ? 16 : 12) : (PREC == 0 ? 10 : 8);
+  // Registers allow 12 warps up to D = 128 and 8 above.
+  static constexpr int most = D <= 128 ? 12 : 8;
   // A warp's step is two groups of 16 tokens at D = 64, one above.  (4 bits, f16, 64
   // heads' sequences of 0 to 32768 tokens at D = 64: 42 us next to 45 with one; at
   // D = 128, bf16, 0 to 16384 tokens: 36.7 with one next to 37.5.)
@@ -486,13 +485,13 @@ struct AttendShape {
   static constexpr int smem = table_bytes + 2 * warps * stage;
 };
 
-template <int D, int KB, int VB, int PREC>
-__global__ void __launch_bounds__(AttendShape<D, KB, VB, PREC>::threads, 1)
+template <int D, int KB, int VB, bool FINE>
+__global__ void __launch_bounds__(AttendShape<D, KB, VB, FINE>::threads, 1)
 kv_attend_kernel(Side sk, Side sv, int pages, int page_shift, Work wk, QueryOut qo, Parts parts,
                  float* __restrict__ scores, int64_t score_width) {
-  using Shape = AttendShape<D, KB, VB, PREC>;
+  using Shape = AttendShape<D, KB, VB, FINE>;
   constexpr int MT = Shape::MT, NW = Shape::warps;
-  constexpr bool KLO = PREC >= 1, VLO = PREC >= 2;
+  constexpr int VLO_AT = (Shape::k_lo ? 2 : 1) * (int)kTableBytes;  // from the values' table
   using KD = Deal<D, KB, 4>;
   using VD = Deal<D, VB, 8>;
   constexpr int KS = D / 16;  // K steps of a score, and pairs of coordinates of a value
@@ -504,18 +503,16 @@ kv_attend_kernel(Side sk, Side sv, int pages, int page_shift, Work wk, QueryOut 
   // Tables, from the codec's entries (set-up data: not written by the kernel
   // before).  A thread copies an entry to the 32 lanes' places.
 #pragma unroll
-  for (int side = 0; side < 2; ++side) {
-    const Codec& c = side ? sv.c : sk.c;
+  for (int table = 0; table < Shape::table_bytes / (int)kTableBytes; ++table) {
+    const bool lo = table >= 2, value = table == 1 || (lo && (!Shape::k_lo || table == 3));
+    const Codec& c = value ? sv.c : sk.c;
+    for (int n = tid; n < 256; n += Shape::threads) {
+      const uint2 e = c.pairs[(lo ? 256 : 0) + n];
+      const uint4 v = make_uint4(e.x, e.y, e.x, e.y);
 #pragma unroll
-    for (int part = 0; part < (Shape::lo_tables ? 2 : 1); ++part)
-      for (int n = tid; n < 256; n += Shape::threads) {
-        const uint2 e = c.pairs[part * 256 + n];
-        const uint4 v = make_uint4(e.x, e.y, e.x, e.y);
-#pragma unroll
-        for (int i = 0; i < 8; ++i)
-          *reinterpret_cast<uint4*>(smem + (2 * part + side) * kTableBytes + n * 128 +
-                                    ((i + n) & 7) * 16) = v;
-      }
+      for (int i = 0; i < 8; ++i)
+        *reinterpret_cast<uint4*>(smem + table * kTableBytes + n * 128 + ((i + n) & 7) * 16) = v;
+    }
   }
   const uint32_t table0 = (uint32_t)__cvta_generic_to_shared(smem);
   const uint32_t kbase = table0 + lane_place<KB>(lane);
@@ -667,7 +664,7 @@ kv_attend_kernel(Side sk, Side sv, int pages, int page_shift, Work wk, QueryOut 
     }
 
     // The queries as B operands: lane (g, t) holds head g.
-    uint32_t qh[KS][2], ql[KLO ? KS : 1][2];
+    uint32_t qh[KS][2], ql[KS][2];
     {
       const __half* hi = qo.hi + ((int64_t)seg.seg * kHeadsPer + g) * D;
       const __half* lo = qo.lo + ((int64_t)seg.seg * kHeadsPer + g) * D;
@@ -677,11 +674,9 @@ kv_attend_kernel(Side sk, Side sv, int pages, int page_shift, Work wk, QueryOut 
         uint2 x = *reinterpret_cast<const uint2*>(hi + dim);
         qh[s][0] = x.x;
         qh[s][1] = x.y;
-        if constexpr (KLO) {
-          x = *reinterpret_cast<const uint2*>(lo + dim);
-          ql[s][0] = x.x;
-          ql[s][1] = x.y;
-        }
+        x = *reinterpret_cast<const uint2*>(lo + dim);
+        ql[s][0] = x.x;
+        ql[s][1] = x.y;
       }
     }
     const float f0 = qo.factor[(int64_t)seg.seg * kHeadsPer + 2 * t];
@@ -731,18 +726,15 @@ kv_attend_kernel(Side sk, Side sv, int pages, int page_shift, Work wk, QueryOut 
         float more[3][4] = {};
 #pragma unroll
         for (int k = 0; k < KS; ++k) {
-          uint32_t a0, a1, a2, a3, c0 = 0, c1 = 0, c2 = 0, c3 = 0;
-          decode_key<KB, KLO>(kw[0], k, kbase, a0, a2, c0, c2);
-          decode_key<KB, KLO>(kw[1], k, kbase, a1, a3, c1, c3);
-          mma16816(KLO && k % 2 ? more[0] : s[i], a0, a1, a2, a3, qh[k][0], qh[k][1]);
-          if constexpr (KLO) {
-            mma16816(more[1], a0, a1, a2, a3, ql[k][0], ql[k][1]);
-            mma16816(more[2], c0, c1, c2, c3, qh[k][0], qh[k][1]);
-          }
+          uint32_t a0, a1, a2, a3, c0, c1, c2, c3;
+          decode_key<KB>(kw[0], k, kbase, a0, a2, c0, c2);
+          decode_key<KB>(kw[1], k, kbase, a1, a3, c1, c3);
+          mma16816(k % 2 ? more[0] : s[i], a0, a1, a2, a3, qh[k][0], qh[k][1]);
+          mma16816(more[1], a0, a1, a2, a3, ql[k][0], ql[k][1]);
+          mma16816(more[2], c0, c1, c2, c3, qh[k][0], qh[k][1]);
         }
-        if constexpr (KLO)
 #pragma unroll
-          for (int e = 0; e < 4; ++e) s[i][e] += more[0][e] + (more[1][e] + more[2][e]);
+        for (int e = 0; e < 4; ++e) s[i][e] += more[0][e] + (more[1][e] + more[2][e]);
       }
       float mx0 = -FLT_MAX, mx1 = -FLT_MAX, vmx = 0.f, vn[MT][2];
 #pragma unroll
@@ -770,7 +762,7 @@ kv_attend_kernel(Side sk, Side sv, int pages, int page_shift, Work wk, QueryOut 
 #pragma unroll
         for (int e = 0; e < 2; ++e) {
           const float x = s[i][2 * e], y = s[i][2 * e + 1];
-          if (KLO && scores) {
+          if (scores) {
             const int tok = base + 16 * i + tok_k + 8 * e;
             if (tok < t1) {
               float* to = scores +
@@ -829,7 +821,7 @@ kv_attend_kernel(Side sk, Side sv, int pages, int page_shift, Work wk, QueryOut 
           const float x = p0 * w, y = p1 * w;
           const uint32_t hi = pack_half2(x, y);
           ph[i][e] = transpose8(hi);
-          if constexpr (VLO) {
+          if constexpr (FINE) {
             const float2 f = unpack_half2(hi);
             pl[i][e] = transpose8(pack_half2(x - f.x, y - f.y));
           }
@@ -846,11 +838,11 @@ kv_attend_kernel(Side sk, Side sv, int pages, int page_shift, Work wk, QueryOut 
 #pragma unroll
         for (int m = 0; m < KS; m += 2) {
           uint32_t a0[2], a1[2], a2[2], a3[2], c0[2], c1[2], c2[2], c3[2];
-          decode_value<VB, VLO>(vw[0], vw[1], m, vbase, a0, a1, c0, c1);
-          decode_value<VB, VLO>(vw[2], vw[3], m, vbase, a2, a3, c2, c3);
+          decode_value<VB, FINE, VLO_AT>(vw[0], vw[1], m, vbase, a0, a1, c0, c1);
+          decode_value<VB, FINE, VLO_AT>(vw[2], vw[3], m, vbase, a2, a3, c2, c3);
 #pragma unroll
           for (int z = 0; z < 2; ++z) {
-            if constexpr (VLO) {
+            if constexpr (FINE) {
               float sum[4] = {};
               mma16816(sum, a0[z], a1[z], a2[z], a3[z], pl[i][0], pl[i][1]);
               mma16816(sum, c0[z], c1[z], c2[z], c3[z], ph[i][0], ph[i][1]);
@@ -1099,14 +1091,14 @@ inline int launch_pdl(void (*kernel)(KArgs...), dim3 grid, int threads, size_t s
   return PQ_OK;
 }
 
-template <int D, int KB, int VB, int PREC>
+template <int D, int KB, int VB, bool FINE>
 int launch_attend(const pq_kv_cache& c, Work wk, const AttendPlan& p, int workers,
                   cudaStream_t st) {
-  using Shape = AttendShape<D, KB, VB, PREC>;
-  auto kern = kv_attend_kernel<D, KB, VB, PREC>;
+  using Shape = AttendShape<D, KB, VB, FINE>;
+  auto kern = kv_attend_kernel<D, KB, VB, FINE>;
   const int page_shift = page_shift_of(c);
   static_assert(Shape::warps >= 4 && Shape::unit >= kLeastUnit, "too little shared memory");
-  const int rc = allow_smem<kv_attend_kernel<D, KB, VB, PREC>>(Shape::smem);
+  const int rc = allow_smem<kv_attend_kernel<D, KB, VB, FINE>>(Shape::smem);
   if (rc) return rc;
   return launch_pdl(kern, dim3(workers), Shape::threads, Shape::smem, st, true, side_k(c),
                     side_v(c), c.pages, page_shift, wk, p.q, p.parts, p.scores, p.width);
@@ -1114,33 +1106,29 @@ int launch_attend(const pq_kv_cache& c, Work wk, const AttendPlan& p, int worker
 
 // Calls f with the kernel's template arguments.
 template <int D, int KB, int VB, class F>
-int with_prec(int prec, F f) {
-  switch (prec) {
-    case 0: return f.template operator()<D, KB, VB, 0>();
-    case 1: return f.template operator()<D, KB, VB, 1>();
-    default: return f.template operator()<D, KB, VB, 2>();
-  }
+int with_fine(bool fine, F f) {
+  return fine ? f.template operator()<D, KB, VB, true>() : f.template operator()<D, KB, VB, false>();
 }
 template <int D, int KB, class F>
-int with_v(int vb, int prec, F f) {
-  return vb == 2 ? with_prec<D, KB, 2>(prec, f)
-                 : vb == 4 ? with_prec<D, KB, 4>(prec, f) : with_prec<D, KB, 8>(prec, f);
+int with_v(int vb, bool fine, F f) {
+  return vb == 2 ? with_fine<D, KB, 2>(fine, f)
+                 : vb == 4 ? with_fine<D, KB, 4>(fine, f) : with_fine<D, KB, 8>(fine, f);
 }
 template <int D, class F>
-int with_k(int kb, int vb, int prec, F f) {
-  return kb == 2 ? with_v<D, 2>(vb, prec, f)
-                 : kb == 4 ? with_v<D, 4>(vb, prec, f) : with_v<D, 8>(vb, prec, f);
+int with_k(int kb, int vb, bool fine, F f) {
+  return kb == 2 ? with_v<D, 2>(vb, fine, f)
+                 : kb == 4 ? with_v<D, 4>(vb, fine, f) : with_v<D, 8>(vb, fine, f);
 }
 template <class F>
-int with_shape(int D, int kb, int vb, int prec, F f) {
-  return D == 64 ? with_k<64>(kb, vb, prec, f)
-                 : D == 128 ? with_k<128>(kb, vb, prec, f) : with_k<256>(kb, vb, prec, f);
+int with_shape(int D, int kb, int vb, bool fine, F f) {
+  return D == 64 ? with_k<64>(kb, vb, fine, f)
+                 : D == 128 ? with_k<128>(kb, vb, fine, f) : with_k<256>(kb, vb, fine, f);
 }
 
 struct UnitOf {
-  template <int D, int KB, int VB, int PREC>
+  template <int D, int KB, int VB, bool FINE>
   int operator()() const {
-    return AttendShape<D, KB, VB, PREC>::unit;
+    return AttendShape<D, KB, VB, FINE>::unit;
   }
 };
 struct LaunchAttend {
@@ -1149,9 +1137,9 @@ struct LaunchAttend {
   const AttendPlan& p;
   int workers;
   cudaStream_t st;
-  template <int D, int KB, int VB, int PREC>
+  template <int D, int KB, int VB, bool FINE>
   int operator()() const {
-    return launch_attend<D, KB, VB, PREC>(c, wk, p, workers, st);
+    return launch_attend<D, KB, VB, FINE>(c, wk, p, workers, st);
   }
 };
 
@@ -1212,7 +1200,7 @@ int pq_kv_attend(const pq_kv_cache* cache, const void* q, int dtype, int64_t q_s
     return fail(PQ_ERR_WORKSPACE, "pq_kv_attend needs %zu workspace bytes, got %zu", p.bytes,
                 ws_bytes);
   const cudaStream_t st = (cudaStream_t)stream;
-  const int prec = dtype != PQ_KV_BF16 ? 2 : lse || accumulate ? 1 : 0;
+  const bool fine = dtype != PQ_KV_BF16;
   kv::Work wk;
   wk.table = table;
   wk.table_stride = table_stride;
@@ -1223,7 +1211,7 @@ int pq_kv_attend(const pq_kv_cache* cache, const void* q, int dtype, int64_t q_s
   wk.group = q_heads / c.heads;
   wk.blocks = p.blocks;
   wk.first = p.first;
-  wk.unit = kv::with_shape(p.D, c.k_bits, c.v_bits, prec, kv::UnitOf{});
+  wk.unit = kv::with_shape(p.D, c.k_bits, c.v_bits, fine, kv::UnitOf{});
   wk.empty = (kv::kSegmentCost + wk.unit - 1) / wk.unit;
   const int workers = p.workers;
   PQ_KV_DISPATCH_T(dtype, {
@@ -1233,7 +1221,7 @@ int pq_kv_attend(const pq_kv_cache* cache, const void* q, int dtype, int64_t q_s
                          : kv::launch_query<T_, 256>(c, q, q_stride_b, q_stride_h, scale, wk, p, st);
   });
   if (rc) return rc;
-  rc = kv::with_shape(p.D, c.k_bits, c.v_bits, prec, kv::LaunchAttend{c, wk, p, workers, st});
+  rc = kv::with_shape(p.D, c.k_bits, c.v_bits, fine, kv::LaunchAttend{c, wk, p, workers, st});
   if (rc) return rc;
   PQ_KV_DISPATCH_T(dtype, {
     rc = p.D == 64 ? kv::launch_join<T_, 64>(c, wk, p, workers, out, lse, accumulate, st)

@@ -42,7 +42,7 @@
 //
 // Roundings.  Centroids and queries are taken times powers of two that put the
 // largest at 2^13; f16 hi has 11 bits, hi + lo 22.  Softmax weights times value
-// norms (relative to a power of two near the largest so far) are rounded to
+// norms (times a scale that follows the largest product so far) are rounded to
 // f16 for the product.
 //   Scores are products of hi + lo for every type: what a score is off by, its
 //   softmax weight is off by, times the score, so that 11 bits lose 0.4 % of a
@@ -69,12 +69,16 @@ constexpr int kLeastUnit = 64;     // tokens of the smallest unit of any shape
 constexpr int kSegmentCost = 768;  // what taking up a segment costs, in tokens
 constexpr float kLog2e = 1.4426950408889634f;
 constexpr float kLn2 = 0.6931471805599453f;
-// Softmax weights relative to the running maximum reach 2^3 before that follows,
-// value norms 2^2 of their reference before it does, and their product is taken
-// times 2^10: at most 2^15 in f16, with 11 bits down to 2^-24 of the largest.
+// Softmax weights relative to the running maximum of the scores reach 2^3 before
+// that follows.  A value's weight, that times its norm, is held relative to a
+// reference of its own for each query head, near the largest such product so far:
+// a long value that is not attended to takes no bits from the others.  It is taken
+// times 2^10 and reaches 2^5 of its reference before that follows: at most 2^15 in
+// f16, with 11 bits down to 2^-23 of the largest.
 constexpr float kRescale = 3.f;
-constexpr float kNormRoom = 4.f;
 constexpr float kWeightScale = 1024.f;
+constexpr float kMostWeight = 32768.f;
+constexpr float kMostUp = 0x1p100f;  // (products below 2^-90 lose bits)
 
 __device__ __forceinline__ void pdl_wait() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
 __device__ __forceinline__ void pdl_next() {
@@ -453,7 +457,7 @@ kv_query_kernel(const T* __restrict__ q, int64_t sb, int64_t sh, int d, int page
 }
 
 struct Parts {
-  float* o;    // [slot][8][D]
+  float* o;    // [slot][8][D], times 2^(exponent of the values' centroids - 14)
   float2* ml;  // [slot][8]: maximum (log2), sum
 };
 
@@ -496,7 +500,7 @@ kv_attend_kernel(Side sk, Side sv, int pages, int page_shift, Work wk, QueryOut 
   using VD = Deal<D, VB, 8>;
   constexpr int KS = D / 16;  // K steps of a score, and pairs of coordinates of a value
   extern __shared__ __align__(128) uint8_t smem[];
-  __shared__ float s_m[NW][kHeadsPer], s_l[NW][kHeadsPer], s_f[NW][kHeadsPer], s_v[NW];
+  __shared__ float s_m[NW][kHeadsPer], s_l[NW][kHeadsPer], s_f[NW][kHeadsPer];
   __shared__ int s_b;
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, g = lane >> 2, t = lane & 3;
 
@@ -687,7 +691,7 @@ kv_attend_kernel(Side sk, Side sv, int pages, int page_shift, Work wk, QueryOut 
 #pragma unroll
     for (int m = 0; m < KS; ++m) o[m][0] = o[m][1] = o[m][2] = o[m][3] = 0.f;
     float m0 = -FLT_MAX, m1 = -FLT_MAX, l0 = 0.f, l1 = 0.f;
-    float vinv = 0.f, vlim = 0.f, vref = 0.f;  // value norms are taken times vinv = 2^10 / vref
+    float up0 = kMostUp, up1 = kMostUp;  // what value weights are taken times
 
 #pragma unroll 1
     for (; base < t1; base += stride) {
@@ -736,7 +740,7 @@ kv_attend_kernel(Side sk, Side sv, int pages, int page_shift, Work wk, QueryOut 
 #pragma unroll
         for (int e = 0; e < 4; ++e) s[i][e] += more[0][e] + (more[1][e] + more[2][e]);
       }
-      float mx0 = -FLT_MAX, mx1 = -FLT_MAX, vmx = 0.f, vn[MT][2];
+      float mx0 = -FLT_MAX, mx1 = -FLT_MAX, vn[MT][2];
 #pragma unroll
       for (int i = 0; i < MT; ++i)
 #pragma unroll
@@ -774,32 +778,9 @@ kv_attend_kernel(Side sk, Side sv, int pages, int page_shift, Work wk, QueryOut 
           }
           mx0 = fmaxf(mx0, x);
           mx1 = fmaxf(mx1, y);
-          vmx = fmaxf(vmx, vn[i][e]);
         }
 
-      if (__any_sync(0xffffffffu, mx0 > m0 + kRescale || mx1 > m1 + kRescale || vmx > vlim)) {
-#pragma unroll
-        for (int w = 4; w < 32; w <<= 1) {
-          mx0 = fmaxf(mx0, __shfl_xor_sync(0xffffffffu, mx0, w));
-          mx1 = fmaxf(mx1, __shfl_xor_sync(0xffffffffu, mx1, w));
-          vmx = fmaxf(vmx, __shfl_xor_sync(0xffffffffu, vmx, w));
-        }
-        mx0 = fmaxf(mx0, m0);
-        mx1 = fmaxf(mx1, m1);
-        float e0 = ex2(m0 - mx0), e1 = ex2(m1 - mx1);
-        m0 = mx0;
-        m1 = mx1;
-        l0 *= e0;
-        l1 *= e1;
-        if (vmx > vlim) {
-          const int ex = vmx < INFINITY ? max(-100, min(100, ilogbf(vmx) + 1)) : 100;
-          const float now = ldexpf(1.f, ex);
-          e0 *= vref / now;
-          e1 *= vref / now;
-          vref = now;
-          vinv = kWeightScale / now;
-          vlim = kNormRoom * now;
-        }
+      auto scale_output = [&](float e0, float e1) {
 #pragma unroll
         for (int m = 0; m < KS; ++m) {
           o[m][0] *= e0;
@@ -807,9 +788,30 @@ kv_attend_kernel(Side sk, Side sv, int pages, int page_shift, Work wk, QueryOut 
           o[m][2] *= e0;
           o[m][3] *= e1;
         }
+      };
+      if (__any_sync(0xffffffffu, mx0 > m0 + kRescale || mx1 > m1 + kRescale)) {
+#pragma unroll
+        for (int w = 4; w < 32; w <<= 1) {
+          mx0 = fmaxf(mx0, __shfl_xor_sync(0xffffffffu, mx0, w));
+          mx1 = fmaxf(mx1, __shfl_xor_sync(0xffffffffu, mx1, w));
+        }
+        mx0 = fmaxf(mx0, m0);
+        mx1 = fmaxf(mx1, m1);
+        l0 *= ex2(m0 - mx0);
+        l1 *= ex2(m1 - mx1);
+        // Products so far count for as much less: that much larger is their scale.
+        up0 *= ex2(mx0 - m0);
+        up1 *= ex2(mx1 - m1);
+        if (up0 > kMostUp || up1 > kMostUp) {
+          scale_output(up0 > kMostUp ? kMostUp / up0 : 1.f, up1 > kMostUp ? kMostUp / up1 : 1.f);
+          up0 = fminf(up0, kMostUp);
+          up1 = fminf(up1, kMostUp);
+        }
+        m0 = mx0;
+        m1 = mx1;
       }
-      // P^T as B operands: tokens of rows 2t, 2t + 1 (and + 8), head g.
-      uint32_t ph[MT][2], pl[MT][2];
+      // Softmax weights times value norms, in place of the scores.
+      float y0 = 0.f, y1 = 0.f;
 #pragma unroll
       for (int i = 0; i < MT; ++i)
 #pragma unroll
@@ -817,8 +819,34 @@ kv_attend_kernel(Side sk, Side sv, int pages, int page_shift, Work wk, QueryOut 
           const float p0 = ex2(s[i][2 * e] - m0), p1 = ex2(s[i][2 * e + 1] - m1);
           l0 += p0;
           l1 += p1;
-          const float w = vn[i][e] * vinv;
-          const float x = p0 * w, y = p1 * w;
+          s[i][2 * e] = p0 * vn[i][e];
+          s[i][2 * e + 1] = p1 * vn[i][e];
+          y0 = fmaxf(y0, s[i][2 * e]);
+          y1 = fmaxf(y1, s[i][2 * e + 1]);
+        }
+      if (__any_sync(0xffffffffu, y0 * up0 > kMostWeight || y1 * up1 > kMostWeight)) {
+#pragma unroll
+        for (int w = 4; w < 32; w <<= 1) {
+          y0 = fmaxf(y0, __shfl_xor_sync(0xffffffffu, y0, w));
+          y1 = fmaxf(y1, __shfl_xor_sync(0xffffffffu, y1, w));
+        }
+        // (a power of two: the largest product comes below kWeightScale)
+        auto follow = [](float y, float up) {
+          return y * up > kMostWeight
+                     ? ldexpf(kWeightScale, -min(ilogbf(fminf(y, FLT_MAX)) + 1, 110)) : up;
+        };
+        const float n0 = follow(y0, up0), n1 = follow(y1, up1);
+        scale_output(n0 / up0, n1 / up1);
+        up0 = n0;
+        up1 = n1;
+      }
+      // P^T as B operands: tokens of rows 2t, 2t + 1 (and + 8), head g.
+      uint32_t ph[MT][2], pl[MT][2];
+#pragma unroll
+      for (int i = 0; i < MT; ++i)
+#pragma unroll
+        for (int e = 0; e < 2; ++e) {
+          const float x = s[i][2 * e] * up0, y = s[i][2 * e + 1] * up1;
           const uint32_t hi = pack_half2(x, y);
           ph[i][e] = transpose8(hi);
           if constexpr (FINE) {
@@ -875,10 +903,12 @@ kv_attend_kernel(Side sk, Side sv, int pages, int page_shift, Work wk, QueryOut 
       s_m[warp][2 * t + 1] = m1;
       s_l[warp][2 * t] = l0;
       s_l[warp][2 * t + 1] = l1;
+      // (2^-14 for the centroids' scale: sums of values of norms up to 2^100 fit f32)
+      s_f[warp][2 * t] = 0x1p-14f / up0;
+      s_f[warp][2 * t + 1] = 0x1p-14f / up1;
     }
     const int active = min(NW, (t1 - seg.t0 + 16 * MT - 1) / (16 * MT));
     uint8_t* own = smem + Shape::table_bytes + (warp * 2 + (p ^ 1)) * Shape::stage;
-    if (lane == 0) s_v[warp] = vref;
     __shared__ const float* s_part[NW];
     if (lane == 0) s_part[warp] = reinterpret_cast<const float*>(own);
     if (warp < active) {
@@ -903,7 +933,7 @@ kv_attend_kernel(Side sk, Side sv, int pages, int page_shift, Work wk, QueryOut 
       float l = in ? s_l[lane][hd] * f : 0.f;
 #pragma unroll
       for (int w = 16; w > 0; w >>= 1) l += __shfl_xor_sync(0xffffffffu, l, w);
-      if (in) s_f[lane][hd] = f * s_v[lane];
+      if (in) s_f[lane][hd] *= f;
       if (lane == 0) parts.ml[slot * kHeadsPer + hd] = make_float2(mm, l);
     }
     __syncthreads();
@@ -937,7 +967,7 @@ kv_join_kernel(Parts parts, Work wk, int workers, int d, int page_size,
   const int b = seg / per, seg_in = seg % per, h = seg_in / wk.blocks, hb = seg_in % wk.blocks;
   const int ng = min(kHeadsPer, wk.group - hb * kHeadsPer);
   const int64_t row0 = ((int64_t)b * wk.heads + h) * wk.group + hb * kHeadsPer;
-  const float vscale = ldexpf(1.f / kWeightScale, -*exponent);
+  const float vscale = ldexpf(0x1p14f, -*exponent);
   pdl_next();
   // (The kernel before lets this one in after the queries' kernel has ended: what
   // that one left, in L2, can be read before the wait for the partial results.)

@@ -171,3 +171,118 @@ def test_graph_accumulates(gpu):
         assert (err <= more * (np.expm1(2 * ds.max()) + 2.0 ** -20) + 2.0 ** -23 * c.ref["weights"]).all()
         c.ref["weights"] = c.cache.weights.cpu().numpy()
     c.check_pool()
+
+
+def with_norms(c, b, tokens, norms, side="v"):
+    """Sets the stored norms of a sequence's tokens, for every head."""
+    t = np.array(tokens)
+    pg, off = c.table[b, t // c.page], t % c.page
+    c.ref[side + "_norms"][pg, :, off] = np.asarray(norms, np.float32)[:, None]
+    getattr(c.cache, side + "_norms").copy_(torch.tensor(c.ref[side + "_norms"]))
+
+
+def check_weighted(c, q):
+    """The outputs' error by the sum of p_j |v_j|, what was attended to, and not by the largest value."""
+    d, scale = c.d, 1 / math.sqrt(c.d)
+    ref = O.attend(c.ref, c.kc, c.vc, q.double().numpy(), c.table, c.lengths, scale)[0]
+    size, score = np.zeros(ref.shape[:2]), np.zeros(ref.shape[:2])
+    for b, h in np.ndindex(*size.shape):
+        pg, off, _ = O.sequence(c.ref, c.table[b], c.lengths[b])
+        at = (pg, h // (ref.shape[1] // c.heads), off)
+        k = c.kc[2].astype(np.float64)[c.ref["k_codes"][at]] * c.ref["k_norms"][at].astype(np.float64)[:, None]
+        v = c.vc[2].astype(np.float64)[c.ref["v_codes"][at]] * c.ref["v_norms"][at].astype(np.float64)[:, None]
+        turned = c.kc[0].astype(np.float64) @ q[b, h].double().numpy()
+        p = scale * (k @ turned)
+        p = np.exp(p - p.max())
+        size[b, h] = (p / p.sum() * np.sqrt((v ** 2).sum(-1))).sum()
+        score[b, h] = scale * (np.abs(k) @ np.abs(turned))[p > 2.0 ** -60].max()  # of tokens that have weight
+    out = c.cache.attend(q.cuda(), *c.on_gpu()).double().cpu().numpy()
+    ds = score * (2.0 ** -22 + (2 * d + 16) * 2.0 ** -24)
+    half = 2.0 ** -11 if c.dtype == torch.bfloat16 else 2.0 ** -22
+    # weights off by their score's error, a rounding and an exponential (2^-22); values by a centroid's rounding; sums in f32
+    bound = size * (np.expm1(2 * ds) + 2 * half + (4 * d + 64) * 2.0 ** -24)
+    bound = bound + np.sqrt((ref ** 2).sum(-1)) * torch.finfo(c.dtype).eps / 2 + math.sqrt(d) * torch.finfo(c.dtype).tiny
+    off = np.sqrt(((out - ref) ** 2).sum(-1))
+    assert np.isfinite(out).all()
+    assert (off <= bound).all(), (off / bound).max()
+
+
+@pytest.mark.parametrize("dtype", ["f32", "f16", "bf16"])
+@pytest.mark.parametrize("d,k_bits,v_bits", [(64, 4, 4), (128, 4, 2), (256, 2, 8)])
+@pytest.mark.parametrize("log_norm", [12, 24, 30, 60, 99])
+@pytest.mark.parametrize("first", [True, False])
+def test_attend_unattended_large_value(gpu, d, k_bits, v_bits, dtype, log_norm, first):
+    """Tokens without weight whose values are up to 2^99 times as long as the others', before and behind those: nothing is
+    left of them, and nothing is lost of the others."""
+    c = Case(d, k_bits, v_bits, heads=1, lengths=(300, 40), dtype=dtype, page_size=64)
+    q = torch.zeros(2, 2, d)
+    q[:, :, 0] = 30.0
+    for b, n in enumerate(c.lengths):
+        k = 0.3 * torch.tensor(c.rng.standard_normal((n, 1, d))).float()
+        lost = [0, 1, 17] if first else [n - 1, n - 5]
+        k[lost] = 0
+        k[lost, :, 0] = -130 * math.sqrt(d) / 30  # a score of -130 or, of two bits, -110: weights below 2^-150
+        c.append(c.slots(b, range(n)), np.arange(n, dtype=np.int32), k=k.to(c.dtype))
+        with_norms(c, b, lost, np.full(len(lost), 2.0 ** log_norm))
+    check_weighted(c, q.to(c.dtype))
+
+
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
+def test_attend_heads_of_different_tokens(gpu, dtype):
+    """Two queries on one key head, one at values 2^40 times as long as the other's."""
+    c = Case(64, 4, 4, heads=1, lengths=(400,), dtype=dtype, page_size=64)
+    k = 0.2 * torch.tensor(c.rng.standard_normal((400, 1, 64))).float()
+    k[:, :, 0] = torch.where(torch.arange(400) % 2 == 0, 20.0, -20.0)[:, None]
+    c.append(c.slots(0, range(400)), np.arange(400, dtype=np.int32), k=k.to(c.dtype))
+    with_norms(c, 0, range(400), np.where(np.arange(400) % 2 == 0, 2.0 ** -20, 2.0 ** 20) * np.exp(0.3 * c.rng.standard_normal(400)))
+    q = torch.zeros(1, 2, 64)
+    q[:, 0, 0], q[:, 1, 0] = 30.0, -30.0
+    check_weighted(c, q.to(c.dtype))
+
+
+@pytest.mark.parametrize("dtype", ["f32", "f16", "bf16"])
+def test_attend_values_of_length_zero(gpu, dtype):
+    """The token with all the weight has a value of 0, others' weights are 2^-40 of it; and all values 0."""
+    c = Case(64, 4, 4, heads=1, lengths=(100, 30), dtype=dtype, page_size=32)
+    q = torch.zeros(2, 2, 64)
+    q[:, :, 0] = 16.0
+    for b, n in enumerate(c.lengths):
+        k = 0.1 * torch.tensor(c.rng.standard_normal((n, 1, 64))).float()
+        k[3] = 0
+        k[3, :, 0] = 14.0
+        c.append(c.slots(b, range(n)), np.arange(n, dtype=np.int32), k=k.to(c.dtype))
+        with_norms(c, b, range(n), np.where(np.arange(n) == 3, 0.0, 2.0 ** 30 if dtype != "f16" else 2.0 ** 34))
+    check_weighted(c, q.to(c.dtype))
+    with_norms(c, 1, range(30), np.zeros(30))
+    check_weighted(c, q.to(c.dtype))
+
+
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
+@pytest.mark.parametrize("log_norm", [99.9, -60.0])
+def test_attend_values_of_extreme_lengths(gpu, dtype, log_norm):
+    """Many tokens of one value near the largest length (a sum over them before the division by the weights' would
+    overflow), and far below 1."""
+    c = Case(64, 4, 4, heads=2, lengths=(500, 64, 3), dtype=dtype, page_size=64)
+    for b, n in enumerate(c.lengths):
+        v = torch.tensor(c.rng.standard_normal((1, 2, 64))).to(c.dtype).expand(n, 2, 64).contiguous()
+        c.append(c.slots(b, range(n)), np.arange(n, dtype=np.int32), v=v)
+        with_norms(c, b, range(n), np.full(n, 2.0 ** log_norm))
+    check_weighted(c, torch.tensor(0.1 * c.rng.standard_normal((3, 4, 64))).to(c.dtype))
+
+
+@pytest.mark.parametrize("dtype", ["f32", "f16", "bf16"])
+@pytest.mark.parametrize("rising", [True, False])
+def test_attend_scores_against_norms(gpu, dtype, rising):
+    """Scores rise (fall) over the tokens as values get shorter (longer), so that the running maxima of the scores and of
+    the products with the values come from different tokens all along."""
+    n = 700
+    c = Case(64, 4, 4, heads=1, lengths=(n,), dtype=dtype, page_size=64)
+    t = np.arange(n) / n
+    t = t if rising else t[::-1]
+    k = 0.1 * torch.tensor(c.rng.standard_normal((n, 1, 64))).float()
+    k[:, 0, 0] = torch.tensor(10.0 * t.copy()).float()
+    c.append(c.slots(0, range(n)), np.arange(n, dtype=np.int32), k=k.to(c.dtype))
+    with_norms(c, 0, range(n), 2.0 ** (-28 * t) * 2.0 ** 14)
+    q = torch.zeros(1, 2, 64)
+    q[:, 0, 0], q[:, 1, 0] = 16.0, 2.0
+    check_weighted(c, q.to(c.dtype))

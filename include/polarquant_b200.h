@@ -385,8 +385,10 @@ typedef struct pq_kv_cache {
   int32_t v_bits;
 } pq_kv_cache;
 
-/* Lays out one side's tables once: rotation R (d x d f32), boundaries
- * (2^bits - 1 f32, ascending) and centroids (2^bits f32), all on the device. */
+/* Lays out one side's tables once: rotation R (d x d f32, orthonormal rows),
+ * boundaries (2^bits - 1 f32, ascending) and centroids (2^bits f32, finite), all
+ * on the device.  (None of that is checked here: other matrices' codes are not
+ * those of the exact product, and entries of 4 or more overflow.) */
 size_t pq_kv_codec_bytes(int d, int bits);
 int pq_kv_prepare_codec(const float* R, const float* boundaries, const float* centroids, int d,
                         int bits, void* codec, size_t codec_bytes, void* stream);

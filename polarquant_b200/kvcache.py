@@ -36,7 +36,8 @@ DTYPES = {torch.float32: 0, torch.float16: 1, torch.bfloat16: 2}
 class KVCodec:
     """One side's tables (rotation, boundaries, centroids) on a device.
 
-    rotation: (d, d); boundaries: (2^bits - 1,) ascending; centroids:
+    rotation: (d, d), orthonormal rows (to 1e-2 in every entry of R R^T, so one
+    rounded to bf16 is taken); boundaries: (2^bits - 1,) ascending; centroids:
     (2^bits,); arrays or tensors.  bits is 2, 4 or 8 and d at most 256."""
 
     def __init__(self, rotation, boundaries, centroids, device: Optional[torch.device] = None):
@@ -63,6 +64,11 @@ class KVCodec:
             raise ValueError("boundaries must ascend")
         if not bool(self.rotation.isfinite().all() & self.centroids.isfinite().all()):
             raise ValueError("rotation and centroids must be finite")
+        # Codes are exact within a bound on sums of rows of length 1, and R^T turns back.
+        r = self.rotation.cpu().double().numpy()
+        off = np.abs(r @ r.T - np.eye(self.d)).max()
+        if not off <= 1e-2:
+            raise ValueError(f"rotation's rows must be orthonormal (an entry of R R^T is off by {off:.3g})")
         nbytes = _lib.query("pq_kv_codec_bytes", self.d, self.bits)
         self.tables = workspace(nbytes, self.device)
         with torch.cuda.device(self.device):

@@ -9,7 +9,8 @@ import pytest
 import torch
 
 from oracle import kv_oracle as O
-from test_gpu_kvcache import Case
+from polarquant_b200 import KVCache, KVCodec
+from test_gpu_kvcache import Case, codec
 
 pytestmark = pytest.mark.gpu
 
@@ -286,3 +287,18 @@ def test_attend_scores_against_norms(gpu, dtype, rising):
     q = torch.zeros(1, 2, 64)
     q[:, 0, 0], q[:, 1, 0] = 16.0, 2.0
     check_weighted(c, q.to(c.dtype))
+
+
+# -- codecs and reads ----------------------------------------------------------------------------------------------------
+
+def test_codec_refuses_what_is_no_rotation(gpu):
+    """Codes are exact, and read turns vectors back, for rotations (and reflections) alone."""
+    _, (R, bounds, cent) = codec(64, 4)
+    skew = R.copy()
+    skew[3] = skew[4]
+    for bad in (2 * R, 5 * np.eye(64), skew, np.zeros((64, 64)), np.full((64, 64), 1e20), R + 0.01):
+        with pytest.raises(ValueError, match="rotation"):
+            KVCodec(bad, bounds, cent)
+    for good in (R, np.eye(64)[::-1], torch.tensor(R, device="cuda").bfloat16()):
+        KVCodec(good, bounds, cent)
+    KVCodec(np.array([[-1.0]]), bounds, cent)

@@ -57,9 +57,10 @@ class KVCodec:
         if tuple(np.shape(boundaries)) != (levels - 1,):
             raise ValueError(f"boundaries must hold {levels - 1} values, got "
                              f"{tuple(np.shape(boundaries))}")
-        self.rotation = to_device_f32(rotation, self.device)
-        self.boundaries = to_device_f32(boundaries, self.device)
-        self.centroids = to_device_f32(centroids, self.device)
+        # (copies: what was given may be used for something else afterwards)
+        self.rotation = to_device_f32(rotation, self.device).clone()
+        self.boundaries = to_device_f32(boundaries, self.device).clone()
+        self.centroids = to_device_f32(centroids, self.device).clone()
         if not bool((self.boundaries[1:] >= self.boundaries[:-1]).all()):
             raise ValueError("boundaries must ascend")
         if not bool(self.rotation.isfinite().all() & self.centroids.isfinite().all()):

@@ -302,3 +302,18 @@ def test_codec_refuses_what_is_no_rotation(gpu):
     for good in (R, np.eye(64)[::-1], torch.tensor(R, device="cuda").bfloat16()):
         KVCodec(good, bounds, cent)
     KVCodec(np.array([[-1.0]]), bounds, cent)
+
+
+def test_codec_keeps_its_own_tables(gpu):
+    """A tensor that a codec was made of can be used for something else afterwards."""
+    _, (R, bounds, cent) = codec(64, 4)
+    given = [torch.tensor(x, device="cuda") for x in (R, bounds, cent)]
+    cache = KVCache(KVCodec(*given), heads=1, pages=1, page_size=16)
+    x = torch.randn(16, 1, 64, device="cuda")
+    slots = torch.arange(16, device="cuda")
+    cache.append(x, x, slots, slots.int())
+    before = cache.read(slots)
+    for t in given:
+        t.zero_()
+    for a, b in zip(cache.read(slots), before):
+        assert torch.equal(a, b)

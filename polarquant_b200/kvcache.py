@@ -29,6 +29,7 @@ from .device import ptr, require_cuda, row_stride, stream_ptr, to_device_f32, wo
 
 MAX_D = 256
 BITS = (2, 4, 8)
+TURN_ROWS = 131072  # the encoder's chunk: a call of no more rows stays on the caller's stream
 PAGE_SIZES = (16, 32, 64, 128, 256, 512, 1024)
 DTYPES = {torch.float32: 0, torch.float16: 1, torch.bfloat16: 2}
 
@@ -314,20 +315,25 @@ class KVCache:
         return k, v
 
     def _unrotate(self, x: torch.Tensor, codec: KVCodec) -> torch.Tensor:
-        """x @ R for every vector, by the encoder's rotation kernel on R^T."""
+        """x @ R for every vector, by the encoder's rotation kernel on R^T.
+
+        In chunks of TURN_ROWS: calls of more rows are spread over streams that all
+        encoders of the process share, which a capture would keep for itself."""
         rows = x.shape[0] * self.heads
         if not rows:
             return x
+        y, size = torch.empty_like(x), self.d * x.element_size()
         with torch.cuda.device(self.device):
             st = stream_ptr(self.device)
             nb = _lib.query("pq_rotation_planes_bytes", self.d)
             planes = workspace(nb, self.device)
             turned = codec.rotation.t().contiguous()
             _lib.call("pq_prepare_rotation", ptr(turned), self.d, ptr(planes), nb, st)
-            ws = workspace(_lib.query("pq_encode_workspace_bytes", rows, self.d), self.device)
-            y = torch.empty_like(x)
-            _lib.call("pq_rotate_tc", ptr(x), rows, self.d, ptr(planes), ptr(y), ptr(ws),
-                      ws.numel(), st)
+            ws = workspace(_lib.query("pq_encode_workspace_bytes", min(rows, TURN_ROWS), self.d),
+                           self.device)
+            for at in range(0, rows, TURN_ROWS):
+                _lib.call("pq_rotate_tc", x.data_ptr() + at * size, min(TURN_ROWS, rows - at), self.d,
+                          ptr(planes), y.data_ptr() + at * size, ptr(ws), ws.numel(), st)
         return y
 
     def attend(self, q: torch.Tensor, table: torch.Tensor, lengths: torch.Tensor, *,

@@ -317,3 +317,48 @@ def test_codec_keeps_its_own_tables(gpu):
         t.zero_()
     for a, b in zip(cache.read(slots), before):
         assert torch.equal(a, b)
+
+
+def test_read_under_capture(gpu):
+    """Reads of few and of very many rows are captured, and replayed on new contents; the many run while another stream
+    turns as many rows by the encoder, in the same process and outside of the capture."""
+    from polarquant_b200 import _lib
+    from polarquant_b200.device import ptr, stream_ptr
+    n, heads, d = 70000, 2, 16  # 140000 rows
+    q, tables = codec(d, 4)
+    cache = KVCache(q, heads=heads, pages=-(-n // 256), page_size=256)
+    slots = torch.randperm(cache.pages * 256, device="cuda")[:n]
+    few = slots[:33].clone()
+    position = torch.zeros(n, dtype=torch.int32, device="cuda")
+    x = [torch.randn(n, heads, d, device="cuda") for _ in range(2)]
+    cache.append(x[0], x[0], slots, position)
+    want = [cache.read(s, dtype=t) for s, t in ((slots, torch.float32), (few, torch.bfloat16))]
+    # the encoder's own call, all of its buffers ready
+    R = torch.tensor(tables[0], device="cuda").contiguous()
+    nb = _lib.query("pq_rotation_planes_bytes", d)
+    planes = torch.empty(nb, dtype=torch.uint8, device="cuda")
+    _lib.call("pq_prepare_rotation", ptr(R), d, ptr(planes), nb, stream_ptr())
+    ws = torch.empty(_lib.query("pq_encode_workspace_bytes", n * heads, d), dtype=torch.uint8, device="cuda")
+    y = torch.empty_like(x[0])
+    torch.cuda.synchronize()
+    other = torch.cuda.Stream()
+    turn = lambda: _lib.call("pq_rotate_tc", ptr(x[0]), n * heads, d, ptr(planes), ptr(y), ptr(ws), ws.numel(),  # noqa: E731
+                             stream_ptr())
+    g = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(g, capture_error_mode="relaxed"):
+        got = [cache.read(slots), cache.read(few, dtype=torch.bfloat16)]
+        with torch.cuda.stream(other):
+            turn()
+    other.synchronize()
+    for new in x[::-1]:
+        cache.append(new, new, slots, position)
+        g.replay()
+        if new is x[0]:
+            for a, b in zip(got, want):
+                assert torch.equal(a[0], b[0]) and torch.equal(a[1], b[1])
+        for a, (s, t) in zip(got, ((slots, torch.float32), (few, torch.bfloat16))):
+            for z, eager in zip(a, cache.read(s, dtype=t)):
+                assert torch.equal(z, eager)
+    # the other stream's: factors of 22 bits, sums of d products in f32
+    off = (y.view(-1, d).double() - x[0].view(-1, d).double() @ R.double().T).abs()
+    assert (off <= (d + 2) * 2.0 ** -22 * x[0].view(-1, d).double().norm(dim=-1, keepdim=True)).all()

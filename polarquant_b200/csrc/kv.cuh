@@ -6,6 +6,7 @@
 #include <atomic>
 
 #include "common.cuh"
+#include "context.cuh"
 
 namespace pqb {
 namespace kv {
@@ -125,18 +126,19 @@ inline int check_sequences(const int32_t* table, int table_width, const int32_t*
   return PQ_OK;
 }
 
-// Lets a kernel take more than 48 KB of dynamic shared memory, once on each
-// device (the runtime's call costs 1 us; a device's number above 63 asks anew).
-// K is the kernel itself, so that each has a mask of its own.
+// Lets a kernel take more than 48 KB of dynamic shared memory, once in each
+// context of a device (the runtime's call costs 1 us; a device's number above 63
+// asks anew).  K is the kernel itself, so that each has ids of its own.
 template <auto K>
 inline int allow_smem(int bytes) {
-  static std::atomic<uint64_t> done{0};
+  static std::atomic<unsigned long long> done[64];
   int dev = 0;
   PQ_CUDA_TRY(cudaGetDevice(&dev));
-  const uint64_t bit = dev < 64 ? 1ull << dev : 0ull;
-  if (done.load(std::memory_order_relaxed) & bit) return PQ_OK;
+  const unsigned long long id = current_ctx_id();
+  if (id && dev < 64 && done[dev].load(std::memory_order_relaxed) == id) return PQ_OK;
   PQ_CUDA_TRY(cudaFuncSetAttribute(K, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes));
-  done.fetch_or(bit, std::memory_order_relaxed);
+  // (the call above made the context current, where there was none)
+  if (dev < 64) done[dev].store(current_ctx_id(), std::memory_order_relaxed);
   return PQ_OK;
 }
 

@@ -14,11 +14,10 @@
 // call.  Calls whose work overlaps on the GPU (different streams, or host
 // threads racing) therefore race on the array and must be serialised by the
 // caller.
-#include <cuda.h>
-
 #include <mutex>
 
 #include "common.cuh"
+#include "context.cuh"
 
 namespace pqb {
 
@@ -31,40 +30,10 @@ static __device__ __align__(256) unsigned char g_noalloc_scratch[kNoAllocScratch
 // current, once per device and context: the cached address is dropped when
 // the device's current context is no longer the one it was taken in (after a
 // cudaDeviceReset the primary context is re-created and the array may live at
-// another address).  The context id comes from the driver (cuCtxGetCurrent,
-// cuCtxGetId), reached through cudaGetDriverEntryPoint.
+// another address).
 static void* g_noalloc_addr[256];
 static unsigned long long g_noalloc_ctx[256];
 static std::mutex g_noalloc_mu;
-
-typedef CUresult (*PfnCtxGetCurrent)(CUcontext*);
-typedef CUresult (*PfnCtxGetId)(CUcontext, unsigned long long*);
-
-// Id of the calling thread's current context, 0 when there is none (or the
-// driver cannot say).
-static unsigned long long current_ctx_id() {
-  static PfnCtxGetCurrent get_current = nullptr;
-  static PfnCtxGetId get_id = nullptr;
-  static bool looked_up = false;
-  if (!looked_up) {
-    void* p = nullptr;
-    cudaDriverEntryPointQueryResult q;
-    if (cudaGetDriverEntryPoint("cuCtxGetCurrent", &p, cudaEnableDefault, &q) == cudaSuccess &&
-        q == cudaDriverEntryPointSuccess)
-      get_current = reinterpret_cast<PfnCtxGetCurrent>(p);
-    p = nullptr;
-    if (cudaGetDriverEntryPoint("cuCtxGetId", &p, cudaEnableDefault, &q) == cudaSuccess &&
-        q == cudaDriverEntryPointSuccess)
-      get_id = reinterpret_cast<PfnCtxGetId>(p);
-    looked_up = true;
-  }
-  if (!get_current || !get_id) return 0;
-  CUcontext ctx = nullptr;
-  unsigned long long id = 0;
-  if (get_current(&ctx) != CUDA_SUCCESS || ctx == nullptr) return 0;
-  if (get_id(ctx, &id) != CUDA_SUCCESS) return 0;
-  return id;
-}
 
 static int noalloc_scratch(void** out) {
   int dev = 0;

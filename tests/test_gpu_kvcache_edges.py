@@ -3,6 +3,9 @@
 The plain cases, and the helper that holds a cache next to its oracle, are in test_gpu_kvcache.py.
 """
 import math
+import os
+import subprocess
+import sys
 
 import numpy as np
 import pytest
@@ -362,3 +365,64 @@ def test_read_under_capture(gpu):
     # the other stream's: factors of 22 bits, sums of d products in f32
     off = (y.view(-1, d).double() - x[0].view(-1, d).double() @ R.double().T).abs()
     assert (off <= (d + 2) * 2.0 ** -22 * x[0].view(-1, d).double().norm(dim=-1, keepdim=True)).all()
+
+
+CONTEXTS = """
+import ctypes, sys
+sys.path.insert(0, {root!r})
+import torch
+from polarquant_b200 import _lib
+rt = ctypes.CDLL("libcudart.so.12")  # torch's, loaded with it
+
+def ok(code):
+    assert code == 0, code
+
+def device(values):
+    p = ctypes.c_void_p()
+    data = bytes(values)
+    ok(rt.cudaMalloc(ctypes.byref(p), ctypes.c_size_t(len(data))))
+    ok(rt.cudaMemcpy(p, data, ctypes.c_size_t(len(data)), 1))
+    return p.value
+
+def f32(*x):
+    return bytes((ctypes.c_float * len(x))(*x))
+
+def i32(*x):
+    return bytes((ctypes.c_int32 * len(x))(*x))
+
+d, page, pages, n = 64, 16, 320, 5000
+for turn in range(2):
+    eye = device(f32(*[float(i == j) for i in range(d) for j in range(d)]))
+    bounds, cent = device(f32(-0.1, 0.0, 0.1)), device(f32(-0.2, -0.05, 0.05, 0.2))
+    size = _lib.query("pq_kv_codec_bytes", d, 2)
+    codec = device(size)
+    _lib.call("pq_kv_prepare_codec", eye, bounds, cent, d, 2, codec, size, None)
+    rows, norms = (device(pages * page * 16) for _ in range(2)), (device(f32(*[1.0] * (pages * page))) for _ in range(2))
+    (kr, vr), (kn, vn) = rows, norms
+    c = _lib.KVCacheDesc(k_rows=kr, v_rows=vr, k_norms=kn, v_norms=vn, positions=device(i32(*range(pages * page))),
+                         weights=device(f32(*[float(i % 7) for i in range(pages * page)])), k_codec=codec, v_codec=codec,
+                         k_ldb=16, v_ldb=16, pages=pages, heads=1, page_size=page, d=d, k_bits=2, v_bits=2)
+    ref = ctypes.byref(c)
+    table, lengths, slots = device(i32(*range(pages))), device(i32(n)), device(bytes((ctypes.c_int64 * n)(*range(n))))
+    x, out = device(n * d * 4), device(d * 4)
+    # an append of many rows, attention and an eviction: kernels of more than 48 KB of shared memory
+    _lib.call("pq_kv_append", ref, x, x, 0, n, d, d, d, d, slots, device(i32(*range(n))), None, None)
+    size = _lib.query("pq_kv_attend_workspace_bytes", ref, 1, 1, pages, 0)
+    _lib.call("pq_kv_attend", ref, x, 0, d, d, table, pages, pages, lengths, 1, 1, 1.0, out, None, 0, device(size), size, None)
+    new = device(4)
+    size = _lib.query("pq_kv_evict_workspace_bytes", ref, 1, pages, 4999)
+    _lib.call("pq_kv_evict", ref, table, pages, pages, lengths, 1, 4999, 0, 0, None, 0, 0, 0, new, device(size), size, None)
+    left = ctypes.c_int32()
+    ok(rt.cudaMemcpy(ctypes.byref(left), ctypes.c_void_p(new), ctypes.c_size_t(4), 2))
+    assert left.value == 4999
+    if turn == 0:
+        ok(rt.cudaDeviceReset())
+print("both contexts")
+"""
+
+
+def test_context_made_anew(gpu):
+    """What a kernel is allowed in a context ends with it: calls go on in the next one."""
+    root = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
+    r = subprocess.run([sys.executable, "-c", CONTEXTS.format(root=root)], capture_output=True, text=True, timeout=240)
+    assert r.returncode == 0 and "both contexts" in r.stdout, r.stderr

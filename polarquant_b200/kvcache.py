@@ -59,9 +59,9 @@ class KVCodec:
             raise ValueError(f"boundaries must hold {levels - 1} values, got "
                              f"{tuple(np.shape(boundaries))}")
         # (copies: what was given may be used for something else afterwards)
-        self.rotation = to_device_f32(rotation, self.device).clone()
-        self.boundaries = to_device_f32(boundaries, self.device).clone()
-        self.centroids = to_device_f32(centroids, self.device).clone()
+        self.rotation = to_device_f32(rotation, self.device).detach().clone()
+        self.boundaries = to_device_f32(boundaries, self.device).detach().clone()
+        self.centroids = to_device_f32(centroids, self.device).detach().clone()
         if not bool((self.boundaries[1:] >= self.boundaries[:-1]).all()):
             raise ValueError("boundaries must ascend")
         if not bool(self.rotation.isfinite().all() & self.centroids.isfinite().all()):

@@ -322,6 +322,19 @@ def test_codec_keeps_its_own_tables(gpu):
         assert torch.equal(a, b)
 
 
+def test_codec_of_parameters(gpu):
+    """Tables that require a gradient are constants to a codec."""
+    _, tables = codec(64, 4)
+    x = torch.randn(16, 1, 64, device="cuda")
+    slots = torch.arange(16, device="cuda")
+    got = []
+    for t in (tables, [torch.nn.Parameter(torch.tensor(t, device="cuda")) for t in tables]):
+        cache = KVCache(KVCodec(*t), heads=1, pages=1, page_size=16)
+        cache.append(x, x, slots, slots.int())
+        got.append(cache.read(slots)[0])
+    assert not got[1].requires_grad and torch.equal(*got)
+
+
 def test_read_under_capture(gpu):
     """Reads of few and of very many rows are captured, and replayed on new contents; the many run while another stream
     turns as many rows by the encoder, in the same process and outside of the capture."""

@@ -364,8 +364,10 @@ class KVCache:
         code = self._vectors("q", q, (batch, hq, self.d))
         if scale is None:
             scale = self._scale
-        elif not math.isfinite(scale):
-            raise ValueError(f"scale must be finite, got {scale}")
+        else:
+            scale = float(scale)
+            if not math.isfinite(scale):
+                raise ValueError(f"scale must be finite, got {scale}")
         out = q.new_empty((batch, hq, self.d))
         lse = self.weights.new_empty((batch, hq)) if return_lse else None
         if batch:

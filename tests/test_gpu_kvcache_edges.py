@@ -335,6 +335,20 @@ def test_codec_of_parameters(gpu):
     assert not got[1].requires_grad and torch.equal(*got)
 
 
+def test_scale_of_any_number(gpu):
+    q, _ = codec(64, 4)
+    cache = KVCache(q, heads=1, pages=1, page_size=16)
+    x = torch.randn(16, 1, 64, device="cuda")
+    slots = torch.arange(16, device="cuda")
+    cache.append(x, x, slots, slots.int())
+    table, lengths = torch.zeros(1, 1, dtype=torch.int32, device="cuda"), torch.tensor([16], dtype=torch.int32, device="cuda")
+    got = [cache.attend(x[:1], table, lengths, scale=s) for s in (2.0, 2, np.float32(2), np.float64(2), torch.tensor(2.0))]
+    assert all(torch.equal(t, got[0]) for t in got)
+    for bad in (np.float32("inf"), torch.tensor(math.nan)):
+        with pytest.raises(ValueError, match="scale"):
+            cache.attend(x[:1], table, lengths, scale=bad)
+
+
 def test_read_under_capture(gpu):
     """Reads of few and of very many rows are captured, and replayed on new contents; the many run while another stream
     turns as many rows by the encoder, in the same process and outside of the capture."""

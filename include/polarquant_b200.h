@@ -432,8 +432,8 @@ int pq_kv_attend(const pq_kv_cache* cache, const void* q, int dtype, int64_t q_s
  * prompt_weights ([batch][heads], strides in elements, prompt_width tokens
  * each, at least the lengths) the tokens are a prompt's: token i has position
  * i and that weight, and the kept ones' positions and weights are written.
- * new_lengths: [batch], min(length, budget).  A page may be in one sequence
- * only; batch * heads is below 65536. */
+ * new_lengths: [batch], min(length, budget), not in the place of lengths.  A page
+ * may be in one sequence only; batch * heads is below 65536. */
 size_t pq_kv_evict_workspace_bytes(const pq_kv_cache* cache, int batch, int table_width,
                                    int budget);
 int pq_kv_evict(const pq_kv_cache* cache, const int32_t* table, int64_t table_stride,

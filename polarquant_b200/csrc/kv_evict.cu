@@ -452,6 +452,8 @@ int pq_kv_evict(const pq_kv_cache* cache, const int32_t* table, int64_t table_st
   if (!ws || ws_bytes < need)
     return fail(PQ_ERR_WORKSPACE, "pq_kv_evict needs %zu workspace bytes, got %zu", need,
                 ws_bytes);
+  PQ_CHECK_ARG(new_lengths + batch <= lengths || lengths + batch <= new_lengths,
+               "new_lengths must not overlap lengths");
   a.sk = kv::side_k(c);
   a.sv = kv::side_v(c);
   a.heads = c.heads;

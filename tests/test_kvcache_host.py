@@ -139,3 +139,11 @@ def test_oracle_evicts_by_weight():
 def test_types_and_sizes_are_the_headers():
     from polarquant_b200 import _lib
     assert ctypes.sizeof(_lib.KVCacheDesc) == 8 * 8 + 2 * 8 + 6 * 4
+
+
+@pytest.mark.parametrize("lengths,new,batch", [(4096, 4096, 1), (4096, 4100, 2), (4100, 4096, 2), (4096, 4096 + 4 * 9, 10)])
+def test_evict_refuses_new_lengths_over_lengths(lib, lengths, new, batch):
+    """Blocks of one sequence's heads read its length while one of them writes the new one."""
+    c = ctypes.byref(desc())
+    assert lib.pq_kv_evict(c, 16, 4, 4, lengths, batch, 5, 0, 0, 0, 0, 0, 0, new, 1 << 16, 1 << 30, None) == -1
+    assert b"overlap" in lib.pq_last_error()

@@ -414,7 +414,9 @@ int pq_kv_read(const pq_kv_cache* cache, const int64_t* slots, int64_t n, void* 
  * the same dtype; lse (or NULL) [batch][q_heads] f32, the natural logarithm of
  * the softmax's sum.  A sequence without tokens gives 0 and -inf.  accumulate:
  * adds every token's softmax weights, summed over its head's query heads, to
- * `weights`. */
+ * `weights`; the workspace then has 4 bytes for every query head and token that
+ * the table has room for.  Scores come from factors of 22 bits and f32 sums;
+ * values and their weights have 22 bits, with dtype bf16 11. */
 size_t pq_kv_attend_workspace_bytes(const pq_kv_cache* cache, int batch, int q_heads,
                                     int table_width, int accumulate);
 int pq_kv_attend(const pq_kv_cache* cache, const void* q, int dtype, int64_t q_stride_b,

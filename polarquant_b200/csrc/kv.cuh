@@ -179,12 +179,6 @@ __device__ __forceinline__ __nv_bfloat16 from_f32<__nv_bfloat16>(float x) {
     }                                     \
   } while (0)
 
-// Code j of a packed row (first code in the highest bits of a byte).
-__device__ __forceinline__ uint32_t code_at(const uint8_t* row, int j, int bits) {
-  const uint32_t bit = (uint32_t)j * (uint32_t)bits;
-  return (row[bit >> 3] >> (8 - bits - (int)(bit & 7u))) & ((1u << bits) - 1u);
-}
-
 __device__ __forceinline__ int clamp_length(int len, int table_width, int page_size) {
   return max(0, min(len, table_width * page_size));
 }

@@ -33,12 +33,13 @@
 // warp): no bank conflicts, and the address is one dp4a.
 //
 // What bounds it: issued instructions and shared memory.  At 4 bits and d = 128
-// sixteen tokens of a head are 2.2 KB and some 340 instructions, 64 of them lookups
-// (an SM's shared memory does one a cycle) and 16 matrix products.  16 sequences of 0 to 32768 tokens, 8 heads, 32 query heads, bf16:
-// the kernel 75 us, 3.4 TB/s of rows (the call 82, a copy's rate 40); issue slots
-// 65 % taken, shared memory 64 %, the matrix pipe 21 %.  tcgen05 would have the
-// decoded rows written to shared memory, which is twice the traffic of the
-// lookups.
+// sixteen tokens of a head are 2.2 KB and, for bf16 outputs, some 470 instructions,
+// 96 of them lookups (an SM's shared memory does one a cycle) and 32 matrix products.
+// 16 sequences of 0 to 32768 tokens, 8 heads, 32 query heads, bf16: the kernel
+// 100 us, 2.6 TB/s of rows (the call 106, a copy's rate 40); issue slots 57 % taken,
+// shared memory 63 %, the matrix pipe 31 %, three warps a scheduler.  tcgen05 would
+// relieve the matrix pipe, which is not the limit, and have the decoded rows, four
+// times the codes for each of hi and lo, written to shared or tensor memory first.
 //
 // Roundings.  Centroids and queries are taken times powers of two that put the
 // largest at 2^13; f16 hi has 11 bits, hi + lo 22.  Softmax weights times value
@@ -476,11 +477,14 @@ struct AttendShape {
   }
   static constexpr int room = 224 * 1024 - table_bytes;
   static constexpr int fit(int mt) { return room / (2 * stage_of(mt)) / 2 * 2; }
-  // Registers allow 12 warps up to D = 128 and 8 above.
+  // Registers allow 12 warps up to D = 128 (16 of bf16 outputs spill: 113 us instead
+  // of 100 of the case above) and 8 at D = 256, where shared memory leaves 8, 6 or 4
+  // warps beside two, three or four tables.
   static constexpr int most = D <= 128 ? 12 : 8;
-  // A warp's step is two groups of 16 tokens at D = 64, one above.  (4 bits, f16, 64
-  // heads' sequences of 0 to 32768 tokens at D = 64: 42 us next to 45 with one; at
-  // D = 128, bf16, 0 to 16384 tokens: 36.7 with one next to 37.5.)
+  // A warp's step is two groups of 16 tokens at D = 64, one above.  (4 bits, bf16, 16
+  // sequences of 0 to 32768 tokens, 8 heads of 4 query heads, D = 64: 65 us next to 71
+  // with one; at D = 128, 0 to 16384 tokens: 67 with one next to 66 with two, which
+  // needs as many registers more as spill with hi + lo values; 8 + 4 bits 52 and 52.)
   static constexpr int MT = D == 64 ? 2 : 1;
   static constexpr int stage = stage_of(MT);
   static constexpr int warps = fit(MT) < most ? fit(MT) : most;

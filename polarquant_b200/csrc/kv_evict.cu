@@ -16,9 +16,12 @@
 // through distributed shared memory.  A block keeps its tokens' keys in shared
 // memory (up to kKeep; beyond that weights and positions are read again).
 //
-// Bound by latency: of some eight barriers and, in one block, of the passes over
-// the keys.  48 heads of 65536 tokens with a cluster each take 56 us, 8 of them 35
-// us, of which weights and the table are 2 us at DRAM's rate.
+// Bound by latency, of passes and barriers alike: 48 heads of 0 to 65536 tokens with
+// a cluster each take 44 us, of which weights and the table are 2 us at DRAM's rate;
+// 47 % of the issue slots are taken, and of the 13 cycles between a warp's
+// instructions loads from memory take 2.7, barriers 2.5 and fixed latencies 2.3.
+// Eight heads of 65536 tokens, moves included, take 34 us, of 131072 52; beyond that
+// keys no longer fit the cluster's shared memory and are read again: 262144 188 us.
 #include <cooperative_groups.h>
 
 #include "kv.cuh"
@@ -95,7 +98,7 @@ __device__ __forceinline__ int block_scan(int x, int* s_warp, int& total) {
 }
 
 // (Three blocks an SM: with registers for one, 48 clusters of eight took turns,
-// 70 us instead of 42.)
+// 70 us instead of 44.)
 template <int CL>
 __global__ void __launch_bounds__(kEvictThreads, 3) kv_select_kernel(EvictArgs a) {
   extern __shared__ uint32_t s_key[];

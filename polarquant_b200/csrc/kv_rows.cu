@@ -645,12 +645,15 @@ kv_append_few_kernel(AppendArgs a) {
 // lane per row, code, pack and store it.  The three run on different tiles.
 //
 // Bound by the two ends' instructions and the waits between them: 196608 rows of
-// either side, bf16, d = 128, 4 bits, take 104 us, 1.2 TB/s of 6.4; 45 % of the
-// issue slots, 30 % of the ALUs and 10 % of the tensor pipe are taken.
+// either side, bf16, d = 128, 4 bits, take 101 us, 1.3 TB/s of 6.4; 50 % of the
+// issue slots, 34 % of the ALUs and 12 % of the tensor pipe are taken.  768 threads
+// leave 80 registers each, and all but the 16-bit kernels of D = 64 spill (268 bytes
+// of stores a thread here, 1000 at D = 256): the longest waits are for local memory
+// and rows alike (long scoreboard 4.8 of 11 cycles between a warp's instructions).
 // ---------------------------------------------------------------------------
 
 // tc::mbar_wait that sleeps: the waiting warps would otherwise issue as many
-// instructions as the working ones (10 us of 104).
+// instructions as the working ones (10 us).
 __device__ __forceinline__ bool wait(uint32_t bar, uint32_t parity, volatile int* abort, int err) {
   if (tc::mbar_try_wait(bar, parity)) return true;
   const long long t0 = clock64();
@@ -676,12 +679,12 @@ struct ManyShape {
   static constexpr int a_bytes = planes * kblocks * 128 * 128;
   static constexpr int b_bytes = 2 * kblocks * cols * 128;
   static constexpr int buffers = D <= 64 || (D == 128 && !wide) ? 2 : 1;
-  // (8 * 2 * cols: flags of what does not fit the list, eight warps' cols / 2 words.)
   // Coordinates to recompute that a block lists, and the tiles it takes in a
   // launch: about half to three quarters of the list at 8 bits and normal data.
   static constexpr int listed = D <= 128 ? 2048 : 1024;
   static constexpr int most_tiles = D <= 128 ? 24 : 8;
-  static constexpr int tmem = cols < 16 ? 32 : 2 * cols;
+  static constexpr int tmem = 2 * cols;
+  // (8 * 2 * cols: flags of what does not fit the list, eight warps' cols / 2 words.)
   static constexpr int smem = 1024 + b_bytes + buffers * a_bytes + 4 * kCellWords + 1024 + 9 * listed +
                               8 * 2 * cols;
 };
@@ -1038,11 +1041,13 @@ int launch_append(const AppendArgs& a, cudaStream_t st) {
 // ---------------------------------------------------------------------------
 // Read: norm * centroid[code], rounded once.
 //
-// A lane takes 16 codes of a row; a warp 32 such pieces of one token.  Bound by
-// the bytes written (2 x 196608 rows of d = 128, 4 bits, to bf16: 32 us, 4.0 TB/s
-// of codes read and vectors written); the lookups are from tables with a copy for each lane (or
-// each pair of lanes half a warp apart, for 64-bit entries): an f32 centroid at
-// 8 bits, both of a byte's at 4, both of a nibble's at 2.
+// A lane takes 16 codes of a row; a warp 32 such pieces of one token.  2 x 196608
+// rows of d = 128, 4 bits, to bf16: 33 us, 4.0 TB/s of codes read and vectors written,
+// 0.62 of a copy's rate.  Bound by the wait for codes, of which a warp has one task's
+// on the way (long scoreboard 6.5 of 18 cycles between a warp's instructions), and by
+// instructions (58 % of the issue slots).  The lookups are from tables with a copy
+// for each lane (or each pair of lanes half a warp apart, for 64-bit entries): an
+// f32 centroid at 8 bits, both of a byte's at 4, both of a nibble's at 2.
 // ---------------------------------------------------------------------------
 
 struct ReadArgs {

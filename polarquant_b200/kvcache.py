@@ -39,7 +39,10 @@ class KVCodec:
 
     rotation: (d, d), orthonormal rows (to 1e-2 in every entry of R R^T, so one
     rounded to bf16 is taken); boundaries: (2^bits - 1,) ascending; centroids:
-    (2^bits,); arrays or tensors.  bits is 2, 4 or 8 and d at most 256."""
+    (2^bits,); arrays or tensors.  bits is 2, 4 or 8 and d at most 256.
+
+    Making one checks and lays out the tables and waits for the device: once for
+    a model's rotation, not once a cache or a step."""
 
     def __init__(self, rotation, boundaries, centroids, device: Optional[torch.device] = None):
         if device is None:
@@ -354,7 +357,12 @@ class KVCache:
         accumulate=True adds each token's softmax weight, summed over the query
         heads of its key-value head, to ``weights``, which ``evict`` goes by.
         (The sum of several sequences that share a page is taken in no fixed
-        order.)"""
+        order.)  It takes 4 bytes of workspace for every query head and token that
+        the table has room for, whatever the lengths: cut a wide table to the
+        pages that the longest sequence needs.
+
+        Scores are as exact as f32 allows for every type; values and their
+        weights have 22 bits, for bfloat16 outputs 11."""
         batch, width = self._sequences(table, lengths)
         if not isinstance(q, torch.Tensor) or q.dim() != 3:
             raise ValueError("q must be a (sequences, query heads, d) tensor")
@@ -395,10 +403,12 @@ class KVCache:
         weights: (sequences, heads, tokens) float32 for prompts whose attention
         was computed elsewhere: token i has position i and this weight (the
         column sums of the prompt's attention, say), and the kept tokens'
-        positions and weights are written to the cache.
+        positions and weights are written to the cache.  A sequence longer than
+        that is taken as that long.
 
         A page must belong to one sequence only: a shared prefix is copied, or
-        left out of the table, before.  sequences * heads is below 65536."""
+        left out of the table, before.  sequences * heads is below 65536.  (Wide
+        tables get the kernel for long sequences: cut them as for ``attend``.)"""
         batch, table_width = self._sequences(table, lengths)
         for name, x in (("budget", budget), ("recent", recent), ("sinks", sinks)):
             if int(x) != x or not 0 <= x < 1 << 31:

@@ -358,7 +358,8 @@ int pq_pack_codes(const uint8_t* codes, int64_t n, int d, int bits, uint8_t* out
  * d <= 256; k_bits and v_bits are 2, 4 or 8, on their own; page_size is a
  * power of two, 16 .. 1024; a pool has fewer than 2^32 rows; the arrays are
  * 16-byte aligned, and ldb is a row's packed bytes rounded up to 16.  dtype:
- * 0 = f32, 1 = f16, 2 = bf16.  Vectors are finite and of norms below 2^100.
+ * 0 = f32, 1 = f16, 2 = bf16.  Vectors are finite and of norms below 2^100
+ * (values shorter than 2^-90 lose bits in attention).
  * The descriptor and its fields' sizes are host memory, read during the call.
  * ------------------------------------------------------------------------- */
 #define PQ_KV_F32 0

@@ -398,7 +398,8 @@ class KVCache:
         before it, in order; the others stay where they are.  Returns the new
         lengths, (sequences,) int32; pages behind them are free.  Tokens on pages
         outside the pool are not there: none is kept, and none is moved onto such
-        a page, so that fewer than `budget` are left where the table has one.
+        a page, so that fewer than `budget` are left where the table has one (the
+        new length counts such places).
 
         weights: (sequences, heads, tokens) float32 for prompts whose attention
         was computed elsewhere: token i has position i and this weight (the
